@@ -77,6 +77,27 @@ class ModelDesc(ctypes.Structure):
                 ("tok_embd", c_void_p), ("output_norm", c_void_p), ("layers", POINTER(LayerDesc))]
 
 
+class PagesDesc(ctypes.Structure):
+    """sllm_gfx950_pages_desc."""
+    _fields_ = [("n_layer", c_int32), ("n_head_kv", c_int32), ("head_dim", c_int32), ("page_tokens", c_int32),
+                ("n_pages", c_int32), ("dtype", c_int32), ("mem", c_void_p)]
+
+
+class PromptDesc(ctypes.Structure):
+    """sllm_gfx950_prompt_desc."""
+    _fields_ = [("dtype", c_int32), ("n_head", c_int32), ("n_head_kv", c_int32), ("head_dim", c_int32),
+                ("n_seq", c_int32), ("q_len", c_void_p), ("k_len", c_void_p)]
+
+
+class PromptIO(ctypes.Structure):
+    """sllm_gfx950_prompt_io."""
+    _fields_ = [("q", c_void_p), ("k", c_void_p), ("v", c_void_p), ("out", c_void_p), ("scale", c_float)] + \
+               [(n, c_size_t) for n in ("q_tok", "q_head", "k_tok", "k_head", "v_tok", "v_head", "out_tok", "out_head")]
+
+
+# element types of a cache and of attention's rows (sllm_gfx950_attn.h)
+DTYPES = {"float32": 0, "float16": 1, "bfloat16": 2}
+
 # Every function the C ABI exports: name -> (restype, argtypes).
 PROTOTYPES = {
     "sllm_gfx950_open": (c_int, [c_int]),
@@ -157,6 +178,27 @@ PROTOTYPES = {
     "sllm_gfx950_ctx_set_graph": (c_int, [c_void_p, c_int]),
     "sllm_gfx950_trace_dots": (c_size_t, [c_void_p]),
     "sllm_gfx950_ctx_trace": (c_int, [c_void_p, c_void_p, c_void_p]),
+    "sllm_gfx950_pages_bytes": (c_size_t, [POINTER(PagesDesc)]),
+    "sllm_gfx950_pages_new": (c_int, [POINTER(PagesDesc), POINTER(c_void_p)]),
+    "sllm_gfx950_pages_free": (None, [c_void_p]),
+    "sllm_gfx950_pages_mem": (c_void_p, [c_void_p]),
+    "sllm_gfx950_pages_in_use": (c_int32, [c_void_p]),
+    "sllm_gfx950_seq_new": (c_int, [c_void_p, POINTER(c_int32)]),
+    "sllm_gfx950_seq_fork": (c_int, [c_void_p, c_int32, c_int32, c_int32, c_void_p]),
+    "sllm_gfx950_seq_copy": (c_int, [c_void_p, c_void_p, c_int32, c_void_p]),
+    "sllm_gfx950_seq_truncate": (c_int, [c_void_p, c_int32, c_int32]),
+    "sllm_gfx950_seq_free": (c_int, [c_void_p, c_void_p, c_int32]),
+    "sllm_gfx950_seq_len": (c_int32, [c_void_p, c_int32]),
+    "sllm_gfx950_seq_tables": (c_int32, [c_void_p, c_void_p, c_int32, c_void_p, c_int32]),
+    "sllm_gfx950_pages_compact": (c_int, [c_void_p, POINTER(c_int32)]),
+    "sllm_gfx950_batch_create": (c_int, [c_void_p, c_void_p, c_void_p, c_int32, c_int32, c_int32, POINTER(c_void_p)]),
+    "sllm_gfx950_batch_destroy": (None, [c_void_p]),
+    "sllm_gfx950_batch_rows": (c_int32, [c_void_p]),
+    "sllm_gfx950_batch_store": (c_int, [c_void_p, c_int32, c_void_p, c_size_t, c_void_p, c_size_t]),
+    "sllm_gfx950_batch_attend": (c_int, [c_void_p, c_int32, c_void_p, c_size_t, c_float, c_void_p, c_size_t]),
+    "sllm_gfx950_prompt_create": (c_int, [POINTER(PromptDesc), POINTER(c_void_p)]),
+    "sllm_gfx950_prompt_attend": (c_int, [c_void_p, POINTER(PromptIO)]),
+    "sllm_gfx950_prompt_destroy": (None, [c_void_p]),
 }
 
 SYNTH_PROTOTYPES = {
@@ -632,3 +674,167 @@ class DeviceDecoder:
         if getattr(self, "m", None):
             lib().sllm_gfx950_model_free(self.m)
             self.m = None
+
+
+# ---------------------------------------------------------------------------
+# attention for many sequences
+# ---------------------------------------------------------------------------
+
+def _ints(v):
+    return np.ascontiguousarray(v, np.int32)
+
+
+class PagedCache:
+    """sllm_gfx950_pages: n_pages pages of page_tokens positions for many
+    sequences, in `mem` (device memory of pages_bytes) or its own."""
+
+    def __init__(self, dev, n_layer, n_head_kv, head_dim, page_tokens, n_pages, dtype="float32", mem=None):
+        self.dev, self.p = dev, None
+        self.desc = PagesDesc(n_layer, n_head_kv, head_dim, page_tokens, n_pages, DTYPES[dtype], mem)
+        self.dtype = dtype
+        p = c_void_p()
+        check(lib().sllm_gfx950_pages_new(ctypes.byref(self.desc), ctypes.byref(p)), "pages_new")
+        self.p = p
+
+    @property
+    def nbytes(self):
+        return lib().sllm_gfx950_pages_bytes(ctypes.byref(self.desc))
+
+    @property
+    def mem(self):
+        return lib().sllm_gfx950_pages_mem(self.p)
+
+    def in_use(self):
+        return lib().sllm_gfx950_pages_in_use(self.p)
+
+    def new(self):
+        s = c_int32()
+        check(lib().sllm_gfx950_seq_new(self.p, ctypes.byref(s)), "seq_new")
+        return s.value
+
+    def fork(self, src, n_tokens, n=1):
+        """n sequences that go on from the first n_tokens positions of src."""
+        out = (c_int32 * max(n, 1))()
+        check(lib().sllm_gfx950_seq_fork(self.p, src, n_tokens, n, out), "seq_fork")
+        return out[:n]
+
+    def copy(self, seqs):
+        """A sequence with pages of its own for each of seqs."""
+        n = len(seqs)
+        out = (c_int32 * max(n, 1))()
+        check(lib().sllm_gfx950_seq_copy(self.p, (c_int32 * max(n, 1))(*seqs), n, out), "seq_copy")
+        return out[:n]
+
+    def truncate(self, seq, n_tokens):
+        check(lib().sllm_gfx950_seq_truncate(self.p, seq, n_tokens), "seq_truncate")
+
+    def free(self, seqs):
+        n = len(seqs)
+        check(lib().sllm_gfx950_seq_free(self.p, (c_int32 * max(n, 1))(*seqs), n), "seq_free")
+
+    def length(self, seq):
+        n = lib().sllm_gfx950_seq_len(self.p, seq)
+        check(min(n, 0), "seq_len")
+        return n
+
+    def table(self, seq):
+        """A sequence's page numbers (int32)."""
+        one = (c_int32 * 1)(seq)
+        n = lib().sllm_gfx950_seq_tables(self.p, one, 1, None, 0)
+        check(min(n, 0), "seq_tables")
+        out = np.empty(n, np.int32)
+        check(min(lib().sllm_gfx950_seq_tables(self.p, one, 1, ptr(out) if n else None, n), 0), "seq_tables")
+        return out
+
+    def tables(self, seqs):
+        """The page numbers of sequences that have equally many (int32[n][pages])."""
+        n = len(seqs)
+        ids = (c_int32 * max(n, 1))(*seqs)
+        total = lib().sllm_gfx950_seq_tables(self.p, ids, n, None, 0)
+        check(min(total, 0), "seq_tables")
+        out = np.empty(total, np.int32)
+        check(min(lib().sllm_gfx950_seq_tables(self.p, ids, n, ptr(out) if total else None, total), 0), "seq_tables")
+        return out.reshape(n, -1) if n else out.reshape(0, 0)
+
+    def compact(self):
+        """Move the pages in use to the front; how many were moved."""
+        n = c_int32()
+        check(lib().sllm_gfx950_pages_compact(self.p, ctypes.byref(n)), "pages_compact")
+        return n.value
+
+    def batch(self, seqs, n_new, n_head, act=None):
+        """A step: n_new[i] new positions for sequence seqs[i] (Batch)."""
+        return Batch(self, seqs, n_new, n_head, act or self.dtype)
+
+    def close(self):
+        if self.p:
+            lib().sllm_gfx950_pages_free(self.p)
+            self.p = None
+
+    def __del__(self):
+        if getattr(self, "p", None) and _lib is not None:
+            self.close()
+
+
+class Batch:
+    """sllm_gfx950_batch: a step's new positions, stored and attended to layer by
+    layer. Pointers are device addresses; strides are in elements, 0: packed."""
+
+    def __init__(self, cache, seqs, n_new, n_head, act):
+        self.b, self.cache = None, cache
+        ids, new = _ints(seqs), _ints(n_new)
+        if ids.shape != new.shape or ids.ndim != 1:
+            raise ValueError("batch: one count of new positions for each sequence")
+        b = c_void_p()
+        check(lib().sllm_gfx950_batch_create(cache.p, ptr(ids) if ids.size else None, ptr(new) if new.size else None,
+                                             ids.size, n_head, DTYPES[act], ctypes.byref(b)), "batch_create")
+        self.b = b
+
+    @property
+    def rows(self):
+        return lib().sllm_gfx950_batch_rows(self.b)
+
+    def store(self, layer, k, v, k_stride=0, v_stride=0):
+        check(lib().sllm_gfx950_batch_store(self.b, layer, k, k_stride, v, v_stride), "batch_store")
+
+    def attend(self, layer, q, out, scale, q_stride=0, out_stride=0):
+        check(lib().sllm_gfx950_batch_attend(self.b, layer, q, q_stride, scale, out, out_stride), "batch_attend")
+
+    def close(self):
+        if self.b:
+            lib().sllm_gfx950_batch_destroy(self.b)
+            self.b = None
+
+    def __del__(self):
+        if getattr(self, "b", None) and _lib is not None:
+            self.close()
+
+
+class PromptAttention:
+    """sllm_gfx950_prompt: causal attention over packed sequences of q_len[i]
+    query rows and k_len[i] key rows (None: as many)."""
+
+    def __init__(self, dev, dtype, n_head, n_head_kv, head_dim, q_len, k_len=None):
+        self.dev, self.p = dev, None
+        q, k = _ints(q_len), None if k_len is None else _ints(k_len)
+        if q.ndim != 1 or (k is not None and k.shape != q.shape):
+            raise ValueError("prompt: one key length for each query length")
+        d = PromptDesc(DTYPES[dtype], n_head, n_head_kv, head_dim, q.size, ptr(q) if q.size else None,
+                       None if k is None or not k.size else ptr(k))
+        p = c_void_p()
+        check(lib().sllm_gfx950_prompt_create(ctypes.byref(d), ctypes.byref(p)), "prompt_create")
+        self.p = p
+
+    def run(self, q, k, v, out, scale, q_strides=(0, 0), k_strides=(0, 0), v_strides=(0, 0), out_strides=(0, 0)):
+        """Device addresses; strides (token, head) in elements, (0, 0): packed."""
+        io = PromptIO(q, k, v, out, scale, *q_strides, *k_strides, *v_strides, *out_strides)
+        check(lib().sllm_gfx950_prompt_attend(self.p, ctypes.byref(io)), "prompt_attend")
+
+    def close(self):
+        if self.p:
+            lib().sllm_gfx950_prompt_destroy(self.p)
+            self.p = None
+
+    def __del__(self):
+        if getattr(self, "p", None) and _lib is not None:
+            self.close()

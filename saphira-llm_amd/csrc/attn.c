@@ -1,0 +1,1108 @@
+/*
+ * attn.c -- the paged cache, a step's batch and the prompt plan of
+ * sllm_gfx950_attn.h: host side of attn_kernels.hip.
+ *
+ * Which pages a sequence holds is known here alone, so every page number that a
+ * kernel reads comes from a table built and checked here. A batch lays out the
+ * step once: the sequences' page tables, the runs of pages that several of them
+ * share, and which workgroup takes which rows against which keys.
+ */
+#define _POSIX_C_SOURCE 200809L
+
+#include "shim_internal.h"
+#include "attn_layout.h"
+
+#include <saphira_amd/sllm_gfx950_attn.h>
+
+#include <math.h>
+#include <pthread.h>
+#include <stdlib.h>
+#include <string.h>
+
+#define ATT_NEED_OPEN()                                                                  \
+    do {                                                                                 \
+        if (!sllm_shim_is_open()) return sllm_shim_fail(SLLM_GFX950_ERR_NO_DEVICE, "library not open"); \
+    } while (0)
+
+#define FAIL_ARG(...)   sllm_shim_fail(SLLM_GFX950_ERR_ARG, __VA_ARGS__)
+#define FAIL_NOMEM(...) sllm_shim_fail(SLLM_GFX950_ERR_NOMEM, __VA_ARGS__)
+
+#define LOG2E 1.44269504088896340736
+
+static uint32_t type_size(int32_t dtype) { return dtype == SLLM_GFX950_F32 ? 4u : 2u; }
+static int bad_type(int32_t dtype) { return dtype != SLLM_GFX950_F32 && dtype != SLLM_GFX950_F16 && dtype != SLLM_GFX950_BF16; }
+
+/* the kernels' instances for rows and a cache of these types (shim_internal.h), or -1 */
+static int type_pair(int32_t act, int32_t cache) {
+    if (act == cache) return act == SLLM_GFX950_F32 ? 0 : act == SLLM_GFX950_F16 ? 2 : 3;
+    return act == SLLM_GFX950_F32 && cache == SLLM_GFX950_F16 ? 1 : -1;
+}
+
+static int bad_heads(int32_t n_head, int32_t n_head_kv, int32_t head_dim) {
+    return n_head_kv < 1 || n_head < n_head_kv || n_head > SLLM_GFX950_ATTN_MAX_HEADS || n_head % n_head_kv != 0 ||
+           head_dim < 8 || head_dim > SLLM_GFX950_ATTN_MAX_HEAD_DIM || head_dim % 8 != 0;
+}
+
+static int misaligned(const void *p) { return ((uintptr_t) p & 15u) != 0; }
+
+/* ------------------------------------------------------------------ */
+/* the cache                                                           */
+/* ------------------------------------------------------------------ */
+
+typedef struct sequence {
+    int32_t  used, len;
+    int32_t  n_pages, cap;
+    int32_t *page;
+    uint32_t mark;                   /* the call that named it last (pool's stamp) */
+} sequence;
+
+/* a batch's device memory and the pinned memory its tables are sent from; kept
+ * by the cache for the next batch (`sent`: the copy out of `pin` is done) */
+typedef struct buffer {
+    uint8_t   *dev, *pin;
+    size_t     dev_bytes, pin_bytes;
+    hipEvent_t sent;
+} buffer;
+
+#define KEPT_BUFFERS 4
+
+struct sllm_gfx950_pages {
+    pthread_mutex_t mtx;
+    sllm_gfx950_pages_desc d;
+    uint8_t   *mem;
+    int        own_mem, gone;        /* gone: freed, batches still open */
+    uint64_t   page_bytes, layer_bytes;
+    uint32_t   page_shift, block_bytes, row_bytes;
+    /* who holds a page: sequences, and open batches */
+    int32_t   *refs, *holds;
+    int32_t    n_free, low;          /* low: no free page below it */
+    sequence  *seq;
+    int32_t    n_seq, cap_seq, low_seq;
+    uint32_t   stamp;
+    int32_t    open;                 /* batches */
+    buffer     kept[KEPT_BUFFERS];
+    int        n_kept;
+};
+
+static uint64_t desc_page_bytes(const sllm_gfx950_pages_desc *d) {
+    return (uint64_t) d->n_layer * 2u * (uint64_t) d->n_head_kv * (uint64_t) d->page_tokens * (uint64_t) d->head_dim * type_size(d->dtype);
+}
+
+static int bad_desc(const sllm_gfx950_pages_desc *d) {
+    return d == NULL || bad_type(d->dtype) || bad_heads(d->n_head_kv, d->n_head_kv, d->head_dim) || d->n_layer < 1 ||
+           d->n_layer > 65536 || d->page_tokens < 16 || d->page_tokens > 1024 || (d->page_tokens & (d->page_tokens - 1)) != 0 ||
+           d->n_pages < 1 || d->n_pages > (1 << 28) || desc_page_bytes(d) > 1ull << 32;
+}
+
+size_t sllm_gfx950_pages_bytes(const sllm_gfx950_pages_desc *d) {
+    return bad_desc(d) ? 0 : (size_t) (desc_page_bytes(d) * (uint64_t) d->n_pages);
+}
+
+int sllm_gfx950_pages_new(const sllm_gfx950_pages_desc *d, sllm_gfx950_pages **out) {
+    ATT_NEED_OPEN();
+    if (out == NULL) return FAIL_ARG("pages_new: NULL out");
+    *out = NULL;
+    if (bad_desc(d)) return FAIL_ARG("pages_new: sizes, page length or type outside what a cache takes");
+    if (misaligned(d->mem)) return FAIL_ARG("pages_new: mem is not 16-byte aligned");
+    sllm_gfx950_pages *p = calloc(1, sizeof *p);
+    int32_t *counts = calloc((size_t) d->n_pages * 2, sizeof *counts);
+    if (p == NULL || counts == NULL) {
+        free(p);
+        free(counts);
+        return FAIL_NOMEM("pages_new: %d pages", d->n_pages);
+    }
+    p->d = *d;
+    p->refs = counts;
+    p->holds = counts + d->n_pages;
+    p->n_free = d->n_pages;
+    p->page_bytes = desc_page_bytes(d);
+    p->layer_bytes = p->page_bytes / (uint64_t) d->n_layer;
+    p->row_bytes = (uint32_t) d->head_dim * type_size(d->dtype);
+    p->block_bytes = (uint32_t) d->page_tokens * p->row_bytes;
+    while ((1 << p->page_shift) < d->page_tokens) ++p->page_shift;
+    p->mem = d->mem;
+    if (p->mem == NULL) {
+        const hipError_t e = hipMalloc((void **) &p->mem, (size_t) (p->page_bytes * (uint64_t) d->n_pages));
+        if (e != hipSuccess) {
+            free(p);
+            free(counts);
+            return sllm_shim_hip_fail(e, "hipMalloc(pages)");
+        }
+        p->own_mem = 1;
+    }
+    pthread_mutex_init(&p->mtx, NULL);
+    *out = p;
+    return SLLM_GFX950_OK;
+}
+
+static void buffer_drop(buffer *b) {
+    if (b->dev) hipFree(b->dev);
+    if (b->pin) hipHostFree(b->pin);
+    if (b->sent) hipEventDestroy(b->sent);
+    memset(b, 0, sizeof *b);
+}
+
+static void pages_drop(sllm_gfx950_pages *p) {
+    if (sllm_shim_is_open()) hipStreamSynchronize(sllm_shim_stream());
+    for (int i = 0; i < p->n_kept; ++i) buffer_drop(&p->kept[i]);
+    if (p->own_mem) hipFree(p->mem);
+    for (int32_t i = 0; i < p->n_seq; ++i) free(p->seq[i].page);
+    free(p->seq);
+    free(p->refs);
+    pthread_mutex_destroy(&p->mtx);
+    free(p);
+}
+
+void sllm_gfx950_pages_free(sllm_gfx950_pages *p) {
+    if (p == NULL) return;
+    pthread_mutex_lock(&p->mtx);
+    p->gone = 1;
+    const int32_t open = p->open;
+    pthread_mutex_unlock(&p->mtx);
+    if (open == 0) pages_drop(p);
+}
+
+void *sllm_gfx950_pages_mem(const sllm_gfx950_pages *p) { return p ? p->mem : NULL; }
+int32_t sllm_gfx950_pages_in_use(const sllm_gfx950_pages *p) { return p ? p->d.n_pages - p->n_free : 0; }
+
+/* (the cache's lock is held by everything below that takes or gives pages) */
+
+static int32_t take_page(sllm_gfx950_pages *p) {         /* (n_free > 0) */
+    while (p->refs[p->low] != 0 || p->holds[p->low] != 0) ++p->low;
+    --p->n_free;
+    p->refs[p->low] = 1;
+    return p->low++;
+}
+
+static void maybe_free(sllm_gfx950_pages *p, int32_t page) {
+    if (p->refs[page] != 0 || p->holds[page] != 0) return;
+    ++p->n_free;
+    if (page < p->low) p->low = page;
+}
+
+static void give_page(sllm_gfx950_pages *p, int32_t page) {
+    --p->refs[page];
+    maybe_free(p, page);
+}
+
+static sequence *find(sllm_gfx950_pages *p, int32_t s) {
+    return s >= 0 && s < p->n_seq && p->seq[s].used ? &p->seq[s] : NULL;
+}
+
+static int32_t pages_for(const sllm_gfx950_pages *p, int32_t len) {
+    return (int32_t) (((uint32_t) len + (1u << p->page_shift) - 1u) >> p->page_shift);
+}
+
+static int reserve(sequence *s, int32_t n) {             /* room for n page numbers; 0: no memory */
+    if (n <= s->cap) return 1;
+    int32_t cap = s->cap < 16 ? 16 : s->cap;
+    while (cap < n) cap += cap / 2;
+    int32_t *page = realloc(s->page, (size_t) cap * sizeof *page);
+    if (page == NULL) return 0;
+    s->page = page;
+    s->cap = cap;
+    return 1;
+}
+
+/* n empty sequences into ids; 0: no memory (none is made) */
+static int new_sequences(sllm_gfx950_pages *p, int32_t n, int32_t *ids) {
+    int32_t at = p->low_seq, got = 0;
+    while (got < n) {
+        while (at < p->n_seq && p->seq[at].used) ++at;
+        if (at == p->cap_seq) {
+            const int32_t cap = p->cap_seq ? p->cap_seq * 2 : 64;
+            sequence *seq = cap > SLLM_GFX950_ATTN_MAX_SEQS ? NULL : realloc(p->seq, (size_t) cap * sizeof *seq);
+            if (seq == NULL) break;
+            memset(seq + p->cap_seq, 0, (size_t) (cap - p->cap_seq) * sizeof *seq);
+            p->seq = seq;
+            p->cap_seq = cap;
+        }
+        if (at == p->n_seq) ++p->n_seq;
+        p->seq[at].used = 1;
+        p->seq[at].len = p->seq[at].n_pages = 0;
+        ids[got++] = at;
+    }
+    if (got < n) {
+        while (got-- > 0) p->seq[ids[got]].used = 0;
+        return 0;
+    }
+    p->low_seq = at + 1;
+    return 1;
+}
+
+static void end_sequence(sllm_gfx950_pages *p, int32_t id) {
+    sequence *s = &p->seq[id];
+    for (int32_t i = 0; i < s->n_pages; ++i) give_page(p, s->page[i]);
+    s->used = s->len = s->n_pages = 0;
+    if (id < p->low_seq) p->low_seq = id;
+}
+
+/* copies of pages, in as few launches as they fit */
+typedef struct copies {
+    const sllm_gfx950_pages *p;
+    att_copy_args a;
+    uint32_t most;                   /* rows of the pair with the most */
+    int      st;
+} copies;
+
+static void copies_start(copies *c, const sllm_gfx950_pages *p) {
+    c->p = p;
+    c->a.mem = p->mem;
+    c->a.page_bytes = p->page_bytes;
+    c->a.block_bytes = p->block_bytes;
+    c->a.row_bytes = p->row_bytes;
+    c->a.n_blocks = (uint32_t) (p->page_bytes / p->block_bytes);
+    c->a.n_pairs = c->most = 0;
+    c->st = SLLM_GFX950_OK;
+}
+
+static int copies_flush(copies *c) {
+    if (c->st == SLLM_GFX950_OK && c->a.n_pairs > 0) {
+        const uint64_t chunks = (uint64_t) c->most * c->a.row_bytes / 16u * c->a.n_blocks;
+        void *args[] = { &c->a };
+        c->st = sllm_shim_launch(sllm_shim_attn_function(SLLM_ATTN_COPY),
+                                 (uint32_t) ((chunks + ATT_COPY_CHUNKS - 1) / ATT_COPY_CHUNKS), c->a.n_pairs, ATT_THREADS, 0, args);
+    }
+    c->a.n_pairs = c->most = 0;
+    return c->st;
+}
+
+static void copies_add(copies *c, int32_t src, int32_t dst, int32_t rows) {
+    if (c->a.n_pairs == ATT_PAIRS) copies_flush(c);
+    c->a.pair[c->a.n_pairs++] = (att_pair) { (uint32_t) src, (uint32_t) dst, (uint32_t) rows };
+    if ((uint32_t) rows > c->most) c->most = (uint32_t) rows;
+}
+
+int sllm_gfx950_seq_new(sllm_gfx950_pages *p, int32_t *seq) {
+    ATT_NEED_OPEN();
+    if (p == NULL || seq == NULL) return FAIL_ARG("seq_new: NULL");
+    pthread_mutex_lock(&p->mtx);
+    const int ok = new_sequences(p, 1, seq);
+    pthread_mutex_unlock(&p->mtx);
+    return ok ? SLLM_GFX950_OK : FAIL_NOMEM("seq_new: no room for another sequence");
+}
+
+int sllm_gfx950_seq_fork(sllm_gfx950_pages *p, int32_t src, int32_t n_tokens, int32_t n, int32_t *seqs) {
+    ATT_NEED_OPEN();
+    if (p == NULL || n < 0 || (n > 0 && seqs == NULL)) return FAIL_ARG("seq_fork: NULL or a count below 0");
+    if (n > SLLM_GFX950_ATTN_MAX_SEQS) return FAIL_ARG("seq_fork: %d copies", n);
+    pthread_mutex_lock(&p->mtx);
+    int st = SLLM_GFX950_OK;
+    const sequence *s = find(p, src);
+    if (s == NULL) st = FAIL_ARG("seq_fork: no sequence %d", src);
+    else if (n_tokens < 0 || n_tokens > s->len) st = FAIL_ARG("seq_fork: %d of %d positions", n_tokens, s->len);
+    const int32_t whole = n_tokens >> p->page_shift, rows = n_tokens & (p->d.page_tokens - 1);
+    if (st == SLLM_GFX950_OK && rows && n > p->n_free) st = FAIL_NOMEM("seq_fork: %d pages wanted, %d free", n, p->n_free);
+    if (st == SLLM_GFX950_OK && !new_sequences(p, n, seqs)) st = FAIL_NOMEM("seq_fork: no room for %d sequences", n);
+    int32_t got = 0;
+    if (st == SLLM_GFX950_OK) {
+        copies c;
+        copies_start(&c, p);
+        for (; got < n && st == SLLM_GFX950_OK; ++got) {
+            s = &p->seq[src];                            /* (new_sequences may have moved them) */
+            sequence *f = &p->seq[seqs[got]];
+            if (!reserve(f, whole + 1)) { st = FAIL_NOMEM("seq_fork: page table"); break; }
+            if (whole > 0) memcpy(f->page, s->page, (size_t) whole * sizeof *f->page);
+            for (int32_t i = 0; i < whole; ++i) ++p->refs[f->page[i]];
+            f->n_pages = whole;
+            f->len = n_tokens;
+            if (rows) {
+                const int32_t to = take_page(p);
+                f->page[f->n_pages++] = to;
+                copies_add(&c, s->page[whole], to, rows);
+            }
+        }
+        if (st == SLLM_GFX950_OK) st = copies_flush(&c);
+        if (st != SLLM_GFX950_OK) for (int32_t i = 0; i < n; ++i) end_sequence(p, seqs[i]);
+    }
+    pthread_mutex_unlock(&p->mtx);
+    return st;
+}
+
+int sllm_gfx950_seq_copy(sllm_gfx950_pages *p, const int32_t *src, int32_t n, int32_t *seqs) {
+    ATT_NEED_OPEN();
+    if (p == NULL || n < 0 || (n > 0 && (src == NULL || seqs == NULL))) return FAIL_ARG("seq_copy: NULL or a count below 0");
+    if (n > SLLM_GFX950_ATTN_MAX_SEQS) return FAIL_ARG("seq_copy: %d copies", n);
+    int32_t *ids = malloc((size_t) (n ? n : 1) * sizeof *ids);      /* (src and seqs may be one array) */
+    if (ids == NULL) return FAIL_NOMEM("seq_copy: %d sequences", n);
+    pthread_mutex_lock(&p->mtx);
+    int st = SLLM_GFX950_OK;
+    int64_t want = 0;
+    for (int32_t i = 0; i < n && st == SLLM_GFX950_OK; ++i) {
+        const sequence *s = find(p, src[i]);
+        if (s == NULL) st = FAIL_ARG("seq_copy: no sequence %d", src[i]);
+        else want += s->n_pages;
+    }
+    if (st == SLLM_GFX950_OK && want > p->n_free) st = FAIL_NOMEM("seq_copy: %lld pages wanted, %d free", (long long) want, p->n_free);
+    if (st == SLLM_GFX950_OK && !new_sequences(p, n, ids)) st = FAIL_NOMEM("seq_copy: no room for %d sequences", n);
+    if (st == SLLM_GFX950_OK) {
+        copies c;
+        copies_start(&c, p);
+        for (int32_t i = 0; i < n && st == SLLM_GFX950_OK; ++i) {
+            const sequence *s = &p->seq[src[i]];
+            sequence *f = &p->seq[ids[i]];
+            if (!reserve(f, s->n_pages)) { st = FAIL_NOMEM("seq_copy: page table"); break; }
+            for (int32_t j = 0; j < s->n_pages; ++j) {
+                f->page[f->n_pages++] = take_page(p);
+                const int32_t left = s->len - (j << p->page_shift);
+                copies_add(&c, s->page[j], f->page[j], left < p->d.page_tokens ? left : p->d.page_tokens);
+            }
+            f->len = s->len;
+        }
+        if (st == SLLM_GFX950_OK) st = copies_flush(&c);
+        if (st == SLLM_GFX950_OK) memcpy(seqs, ids, (size_t) n * sizeof *ids);
+        else for (int32_t i = 0; i < n; ++i) end_sequence(p, ids[i]);
+    }
+    pthread_mutex_unlock(&p->mtx);
+    free(ids);
+    return st;
+}
+
+int sllm_gfx950_seq_truncate(sllm_gfx950_pages *p, int32_t seq, int32_t n_tokens) {
+    ATT_NEED_OPEN();
+    if (p == NULL) return FAIL_ARG("seq_truncate: NULL");
+    pthread_mutex_lock(&p->mtx);
+    int st = SLLM_GFX950_OK;
+    sequence *s = find(p, seq);
+    if (s == NULL) st = FAIL_ARG("seq_truncate: no sequence %d", seq);
+    else if (n_tokens < 0 || n_tokens > s->len) st = FAIL_ARG("seq_truncate: %d of %d positions", n_tokens, s->len);
+    else {
+        const int32_t keep = pages_for(p, n_tokens);
+        while (s->n_pages > keep) give_page(p, s->page[--s->n_pages]);
+        s->len = n_tokens;
+    }
+    pthread_mutex_unlock(&p->mtx);
+    return st;
+}
+
+/* every one of n sequences there and named once (p->stamp is this call's) */
+static int check_names(sllm_gfx950_pages *p, const int32_t *seqs, int32_t n, const char *who) {
+    ++p->stamp;
+    for (int32_t i = 0; i < n; ++i) {
+        sequence *s = find(p, seqs[i]);
+        if (s == NULL) return FAIL_ARG("%s: no sequence %d", who, seqs[i]);
+        if (s->mark == p->stamp) return FAIL_ARG("%s: sequence %d twice", who, seqs[i]);
+        s->mark = p->stamp;
+    }
+    return SLLM_GFX950_OK;
+}
+
+int sllm_gfx950_seq_free(sllm_gfx950_pages *p, const int32_t *seqs, int32_t n) {
+    ATT_NEED_OPEN();
+    if (p == NULL || n < 0 || (n > 0 && seqs == NULL)) return FAIL_ARG("seq_free: NULL or a count below 0");
+    pthread_mutex_lock(&p->mtx);
+    const int st = check_names(p, seqs, n, "seq_free");
+    for (int32_t i = 0; i < n && st == SLLM_GFX950_OK; ++i) end_sequence(p, seqs[i]);
+    pthread_mutex_unlock(&p->mtx);
+    return st;
+}
+
+int32_t sllm_gfx950_seq_len(sllm_gfx950_pages *p, int32_t seq) {
+    ATT_NEED_OPEN();
+    if (p == NULL) return FAIL_ARG("seq_len: NULL");
+    pthread_mutex_lock(&p->mtx);
+    const sequence *s = find(p, seq);
+    const int32_t len = s ? s->len : FAIL_ARG("seq_len: no sequence %d", seq);
+    pthread_mutex_unlock(&p->mtx);
+    return len;
+}
+
+int32_t sllm_gfx950_seq_tables(sllm_gfx950_pages *p, const int32_t *seqs, int32_t n, int32_t *pages, int32_t cap) {
+    ATT_NEED_OPEN();
+    if (p == NULL || n < 0 || (n > 0 && seqs == NULL) || cap < 0 || (cap > 0 && pages == NULL)) return FAIL_ARG("seq_tables: NULL or a count below 0");
+    pthread_mutex_lock(&p->mtx);
+    int64_t total = 0;
+    for (int32_t i = 0; i < n && total >= 0; ++i) {
+        const sequence *s = find(p, seqs[i]);
+        total = s ? total + s->n_pages : FAIL_ARG("seq_tables: no sequence %d", seqs[i]);
+    }
+    if (total > INT32_MAX) total = FAIL_ARG("seq_tables: too many pages");
+    if (total >= 0 && total <= cap) {
+        for (int32_t i = 0; i < n; ++i) {
+            const sequence *s = &p->seq[seqs[i]];
+            if (s->n_pages > 0) memcpy(pages, s->page, (size_t) s->n_pages * sizeof *pages);
+            pages += s->n_pages;
+        }
+    }
+    pthread_mutex_unlock(&p->mtx);
+    return (int32_t) total;
+}
+
+int sllm_gfx950_pages_compact(sllm_gfx950_pages *p, int32_t *n_moved) {
+    ATT_NEED_OPEN();
+    if (n_moved) *n_moved = 0;
+    if (p == NULL) return FAIL_ARG("pages_compact: NULL");
+    pthread_mutex_lock(&p->mtx);
+    int st = SLLM_GFX950_OK;
+    const int32_t n_used = p->d.n_pages - p->n_free;
+    /* where each page above n_used goes */
+    int32_t *to = NULL, moved = 0;
+    if (p->open > 0) st = FAIL_ARG("pages_compact: %d batches are open", p->open);
+    else if ((to = malloc((size_t) p->d.n_pages * sizeof *to)) == NULL) st = FAIL_NOMEM("pages_compact: %d pages", p->d.n_pages);
+    if (st == SLLM_GFX950_OK) {
+        copies c;
+        copies_start(&c, p);
+        int32_t hole = 0;
+        for (int32_t i = n_used; i < p->d.n_pages; ++i) {
+            if (p->refs[i] == 0) continue;
+            while (p->refs[hole] != 0) ++hole;           /* (as many holes below n_used as pages above it) */
+            to[i] = hole++;
+            ++moved;
+            copies_add(&c, i, to[i], p->d.page_tokens);
+        }
+        st = copies_flush(&c);
+    }
+    if (st == SLLM_GFX950_OK && moved > 0) {
+        for (int32_t i = 0; i < p->n_seq; ++i) {
+            sequence *s = &p->seq[i];
+            for (int32_t j = 0; j < s->n_pages; ++j) if (s->page[j] >= n_used) s->page[j] = to[s->page[j]];
+        }
+        for (int32_t i = n_used; i < p->d.n_pages; ++i) {
+            if (p->refs[i] == 0) continue;
+            p->refs[to[i]] = p->refs[i];
+            p->refs[i] = 0;
+        }
+        p->low = n_used;
+    }
+    free(to);
+    pthread_mutex_unlock(&p->mtx);
+    if (st == SLLM_GFX950_OK && n_moved) *n_moved = moved;
+    return st;
+}
+
+/* ------------------------------------------------------------------ */
+/* a batch                                                             */
+/* ------------------------------------------------------------------ */
+
+enum { FEW, SOME, ROWS, N_MODES };
+
+/* workgroups of a launch: their threads fit 32 bits */
+#define MAX_ITEMS ((size_t) 1 << 23)
+
+typedef struct items { att_item *v; size_t n, cap; } items;
+
+static att_item *items_add(items *x) {
+    if (x->n == x->cap) {
+        const size_t cap = x->cap ? x->cap * 2 : 256;
+        att_item *v = realloc(x->v, cap * sizeof *v);
+        if (v == NULL) return NULL;
+        x->v = v;
+        x->cap = cap;
+    }
+    return &x->v[x->n++];
+}
+
+struct sllm_gfx950_batch {
+    sllm_gfx950_pages *p;
+    int32_t   n_head, pair;
+    uint32_t  n_tok;
+    uint32_t  n_items[N_MODES];
+    int       join;                  /* a row has partial results */
+    buffer    buf;
+    size_t    off_items[N_MODES], off_tables, off_list, off_tok_seq, off_seqs, off_segs, off_part_o, off_part_ml;
+    int32_t  *held;                  /* the pages it holds */
+    int32_t   n_held;
+};
+
+/* a run of keys and the tokens of the sequences that read it (order[lo .. hi)) */
+typedef struct segment {
+    int32_t  lo, hi;
+    int32_t  page0, n_keys;          /* from page page0 of each of their tables */
+    uint32_t n_tok, list, part0, n_split;
+    int      mode;
+} segment;
+
+typedef struct plan {
+    const sllm_gfx950_pages *p;
+    const int32_t *seqs, *n_new;
+    int32_t  *order, n_order;        /* sequences with new tokens, like tables side by side */
+    int32_t  *common;                /* whole pages that order[i] shares with order[i - 1] */
+    uint32_t *tok0, *table;          /* of sequence i: its first row, where its page numbers start */
+    segment  *seg;
+    int32_t   n_seg;
+    uint32_t  n_list;
+} plan;
+
+/* fewer shared keys than this are read by each sequence for itself: a segment
+ * of their own costs a row a partial result more */
+#define MIN_SHARED 128
+
+/* The runs of order[lo .. hi), which share their pages below `from`. At most two
+ * per sequence: one of its own, and one at each place where it parts from its
+ * neighbour. */
+static void find_segments(plan *x, int32_t lo, int32_t hi, int32_t from) {
+    while (hi - lo > 1) {
+        int32_t common = INT32_MAX;
+        for (int32_t i = lo + 1; i < hi; ++i) if (x->common[i] < common) common = x->common[i];
+        if (((int64_t) (common - from) << x->p->page_shift) >= MIN_SHARED) {
+            segment *s = &x->seg[x->n_seg++];
+            *s = (segment) { .lo = lo, .hi = hi, .page0 = from, .n_keys = (common - from) << x->p->page_shift };
+            from = common;
+        }
+        /* the groups that go on together beyond `common`: the largest in this
+         * loop, so that calls go no deeper than the logarithm of their number */
+        int32_t big_lo = lo, big_hi = lo, start = lo;
+        for (int32_t i = lo + 1; i <= hi; ++i) {
+            if (i < hi && x->common[i] != common) continue;
+            if (i - start > big_hi - big_lo) {
+                big_lo = start;
+                big_hi = i;
+            }
+            start = i;
+        }
+        start = lo;
+        for (int32_t i = lo + 1; i <= hi; ++i) {
+            if (i < hi && x->common[i] != common) continue;
+            if (start != big_lo) find_segments(x, start, i, from);
+            start = i;
+        }
+        lo = big_lo;
+        hi = big_hi;
+    }
+    const sequence *s = &x->p->seq[x->seqs[x->order[lo]]];
+    x->seg[x->n_seg++] = (segment) { .lo = lo, .hi = hi, .page0 = from, .n_keys = s->len - (from << x->p->page_shift) };
+}
+
+static __thread const plan *g_sort;                      /* for qsort */
+
+static int by_table(const void *a, const void *b) {
+    const int32_t ia = *(const int32_t *) a, ib = *(const int32_t *) b;
+    const sequence *s = &g_sort->p->seq[g_sort->seqs[ia]], *t = &g_sort->p->seq[g_sort->seqs[ib]];
+    const int32_t n = s->n_pages < t->n_pages ? s->n_pages : t->n_pages;
+    for (int32_t i = 0; i < n; ++i) if (s->page[i] != t->page[i]) return s->page[i] < t->page[i] ? -1 : 1;
+    return ia < ib ? -1 : ia > ib;
+}
+
+static int mode_of(uint32_t rows) { return rows <= ATT_FEW_ROWS ? FEW : rows <= ATT_SOME_ROWS ? SOME : ROWS; }
+
+/*
+ * A split's keys: as many as give every CU two workgroups over the whole
+ * step, a multiple of SPLIT_KEYS and at least LEAST_SPLIT. Shorter ones would
+ * cost more in partial results than the idle CUs they fill.
+ */
+#define SPLIT_KEYS  128u
+#define LEAST_SPLIT 256u
+
+static uint32_t split_keys(const plan *x, uint32_t group, uint32_t n_head_kv) {
+    uint64_t work = 0;
+    for (int32_t i = 0; i < x->n_seg; ++i) {
+        const segment *s = &x->seg[i];
+        const uint64_t tiles = s->mode == ROWS ? ((uint64_t) s->n_tok * group + ATT_ROWS - 1) / ATT_ROWS : 1;
+        work += tiles * (uint64_t) s->n_keys * n_head_kv;
+    }
+    const uint64_t wgs = 2u * (uint64_t) sllm_shim_cu();
+    uint64_t keys = (work + wgs - 1) / wgs;
+    if (keys < LEAST_SPLIT) keys = LEAST_SPLIT;
+    keys = (keys + SPLIT_KEYS - 1) / SPLIT_KEYS * SPLIT_KEYS;
+    return keys > (1u << 30) ? 1u << 30 : (uint32_t) keys;
+}
+
+static size_t align256(size_t x) { return (x + 255) & ~(size_t) 255; }
+
+static int buffer_get(sllm_gfx950_pages *p, buffer *b, size_t dev_bytes, size_t pin_bytes) {
+    memset(b, 0, sizeof *b);
+    for (int i = 0; i < p->n_kept; ++i) {
+        if (p->kept[i].dev_bytes >= dev_bytes && p->kept[i].pin_bytes >= pin_bytes) {
+            *b = p->kept[i];
+            p->kept[i] = p->kept[--p->n_kept];
+            const hipError_t e = hipEventSynchronize(b->sent);
+            if (e == hipSuccess) return SLLM_GFX950_OK;
+            buffer_drop(b);
+            return sllm_shim_hip_fail(e, "hipEventSynchronize(batch)");
+        }
+    }
+    /* a quarter more than asked for: the next steps' tables are a little longer */
+    dev_bytes += dev_bytes / 4;
+    pin_bytes += pin_bytes / 4;
+    hipError_t e = hipMalloc((void **) &b->dev, dev_bytes);
+    const char *what = "hipMalloc(batch)";
+    if (e == hipSuccess) { e = hipHostMalloc((void **) &b->pin, pin_bytes, hipHostMallocDefault); what = "hipHostMalloc(batch)"; }
+    if (e == hipSuccess) { e = hipEventCreateWithFlags(&b->sent, hipEventDisableTiming); what = "hipEventCreate(batch)"; }
+    b->dev_bytes = dev_bytes;
+    b->pin_bytes = pin_bytes;
+    if (e == hipSuccess) return SLLM_GFX950_OK;
+    buffer_drop(b);
+    return sllm_shim_hip_fail(e, what);
+}
+
+static void buffer_put(sllm_gfx950_pages *p, buffer *b) {
+    if (b->dev == NULL) return;
+    if (p->n_kept == KEPT_BUFFERS) {                     /* the smallest goes */
+        int least = 0;
+        for (int i = 1; i < p->n_kept; ++i) if (p->kept[i].dev_bytes < p->kept[least].dev_bytes) least = i;
+        if (p->kept[least].dev_bytes < b->dev_bytes) {
+            const buffer t = p->kept[least];
+            p->kept[least] = *b;
+            *b = t;
+        }
+        if (sllm_shim_is_open()) hipStreamSynchronize(sllm_shim_stream());
+        buffer_drop(b);
+        return;
+    }
+    p->kept[p->n_kept++] = *b;
+    memset(b, 0, sizeof *b);
+}
+
+/* The step's segments, work items and tables into the batch's buffer. */
+static int lay_out(sllm_gfx950_batch *b, plan *x, int32_t n, const int32_t *len0) {
+    sllm_gfx950_pages *p = b->p;
+    const uint32_t kv = (uint32_t) p->d.n_head_kv, group = (uint32_t) b->n_head / kv;
+    const uint32_t hd_pad = p->d.head_dim <= 64 ? 64 : 128;
+    items it[N_MODES] = { { 0 } };
+    int st = SLLM_GFX950_OK;
+
+    /* like tables side by side, and how far each goes with the one before it:
+     * in whole pages of positions that were there before the step */
+    for (int32_t i = 0; i < n; ++i) if (x->n_new[i] > 0) x->order[x->n_order++] = i;
+    g_sort = x;
+    qsort(x->order, (size_t) x->n_order, sizeof *x->order, by_table);
+    for (int32_t i = 1; i < x->n_order; ++i) {
+        const int32_t ia = x->order[i - 1], ib = x->order[i];
+        const sequence *s = &p->seq[x->seqs[ia]], *t = &p->seq[x->seqs[ib]];
+        int32_t most = (len0[ia] < len0[ib] ? len0[ia] : len0[ib]) >> p->page_shift, c = 0;
+        while (c < most && s->page[c] == t->page[c]) ++c;
+        x->common[i] = c;
+    }
+    if (x->n_order > 0) find_segments(x, 0, x->n_order, 0);
+    uint64_t n_list = 0;
+    for (int32_t i = 0; i < x->n_seg; ++i) {
+        segment *s = &x->seg[i];
+        for (int32_t j = s->lo; j < s->hi; ++j) s->n_tok += (uint32_t) x->n_new[x->order[j]];
+        s->list = ATT_TOKENS;
+        if (s->hi - s->lo > 1) { s->list = (uint32_t) n_list; n_list += s->n_tok; }
+        s->mode = mode_of(s->n_tok * group);
+    }
+    /* segments of each sequence, and those with one part alone */
+    uint32_t *seg_count = calloc((size_t) n + 1, sizeof *seg_count), *seg_at = calloc((size_t) n + 1, sizeof *seg_at);
+    uint8_t *alone = calloc((size_t) n + 1, 1);
+    if (seg_count == NULL || seg_at == NULL || alone == NULL) { st = FAIL_NOMEM("batch_create: tables"); goto out; }
+    const uint32_t split = split_keys(x, group, kv);
+    uint64_t n_part = 0, n_segs = 0, n_pages = 0;
+    for (int32_t i = 0; i < x->n_seg; ++i) {
+        segment *s = &x->seg[i];
+        s->n_split = ((uint32_t) s->n_keys + split - 1) / split;
+        for (int32_t j = s->lo; j < s->hi; ++j) ++seg_count[x->order[j]];
+    }
+    for (int32_t i = 0; i < x->n_seg; ++i) {
+        segment *s = &x->seg[i];
+        const int32_t q = x->order[s->lo];
+        alone[q] = s->hi - s->lo == 1 && seg_count[q] == 1 && s->n_split == 1;
+        if (alone[q]) { seg_count[q] = 0; continue; }
+        s->part0 = (uint32_t) n_part;
+        n_part += (uint64_t) kv * s->n_split * s->n_tok * group;
+        if (n_part > 0xfffffff0ull) { st = FAIL_ARG("batch_create: too many rows and splits"); goto out; }
+    }
+    for (int32_t i = 0; i < n; ++i) {
+        seg_at[i] = (uint32_t) n_segs;
+        n_segs += seg_count[i];
+        seg_count[i] = 0;
+        n_pages += (uint64_t) p->seq[x->seqs[i]].n_pages;
+    }
+    b->join = n_part > 0;
+
+    /* the work, longest first within a mode's launch */
+    for (int32_t i = 0; i < x->n_seg && st == SLLM_GFX950_OK; ++i) {
+        const segment *s = &x->seg[i];
+        const int32_t q = x->order[s->lo];
+        const uint32_t rows = s->n_tok * group, tile = s->mode == ROWS ? ATT_ROWS : ATT_SOME_ROWS;
+        const int own = s->hi - s->lo == 1;
+        const int32_t vis0 = own ? len0[q] - (s->page0 << p->page_shift) + 1 : ATT_SEE_ALL;
+        for (uint32_t k = 0; k < s->n_split && st == SLLM_GFX950_OK; ++k) {
+            for (uint32_t r = 0; r < rows && st == SLLM_GFX950_OK; r += tile) {
+                const uint32_t nr = rows - r < tile ? rows - r : tile;
+                const uint64_t sees = (uint64_t) vis0 + (r + nr - 1) / group;
+                uint32_t key0 = k * split, key1 = (uint32_t) s->n_keys < key0 + split ? (uint32_t) s->n_keys : key0 + split;
+                if (key1 > sees) key1 = (uint32_t) sees;
+                for (uint32_t h = 0; h < kv; ++h) {
+                    att_item *a = items_add(&it[s->mode]);
+                    if (a == NULL) { st = FAIL_NOMEM("batch_create: work items"); break; }
+                    *a = (att_item) { r, nr, own ? x->tok0[q] : 0, s->list, vis0, key0, key1,
+                                      x->table[q] + (uint32_t) s->page0, h,
+                                      alone[q] ? ATT_DIRECT : s->part0 + (h * s->n_split + k) * rows + r };
+                }
+            }
+        }
+    }
+    for (int m = 0; m < N_MODES && st == SLLM_GFX950_OK; ++m) if (it[m].n > MAX_ITEMS) st = FAIL_ARG("batch_create: too much work for a launch");
+    if (st != SLLM_GFX950_OK) goto out;
+
+    size_t at = 0;
+    for (int m = 0; m < N_MODES; ++m) {
+        b->n_items[m] = (uint32_t) it[m].n;
+        b->off_items[m] = at;
+        at = align256(at + it[m].n * sizeof(att_item));
+    }
+    b->off_tables = at;  at = align256(at + n_pages * 4);
+    b->off_list = at;    at = align256(at + n_list * 4);
+    b->off_tok_seq = at; at = align256(at + (size_t) b->n_tok * 4);
+    b->off_seqs = at;    at = align256(at + (size_t) n * sizeof(att_seq));
+    b->off_segs = at;    at = align256(at + n_segs * sizeof(att_seg));
+    const size_t sent = at;
+    b->off_part_ml = at; at = align256(at + n_part * 8);
+    b->off_part_o = at;  at = align256(at + n_part * hd_pad * 4);
+    if ((st = buffer_get(p, &b->buf, at + 256, sent + 256)) != SLLM_GFX950_OK) goto out;
+
+    uint8_t *to = b->buf.pin;
+    for (int m = 0; m < N_MODES; ++m) if (it[m].n) memcpy(to + b->off_items[m], it[m].v, it[m].n * sizeof(att_item));
+    uint32_t *tables = (uint32_t *) (to + b->off_tables), *list = (uint32_t *) (to + b->off_list);
+    uint32_t *tok_seq = (uint32_t *) (to + b->off_tok_seq);
+    att_seq *seqs = (att_seq *) (to + b->off_seqs);
+    att_seg *segs = (att_seg *) (to + b->off_segs);
+    for (int32_t i = 0; i < n; ++i) {
+        const sequence *s = &p->seq[x->seqs[i]];
+        if (s->n_pages > 0) memcpy(tables + x->table[i], s->page, (size_t) s->n_pages * 4);
+        for (int32_t t = 0; t < x->n_new[i]; ++t) tok_seq[x->tok0[i] + (uint32_t) t] = (uint32_t) i;
+        seqs[i] = (att_seq) { x->tok0[i], (uint32_t) x->n_new[i], x->table[i], (uint32_t) len0[i], seg_at[i], 0 };
+    }
+    for (int32_t i = 0; i < x->n_seg; ++i) {
+        const segment *s = &x->seg[i];
+        uint32_t t = 0;
+        for (int32_t j = s->lo; j < s->hi; ++j) {
+            const int32_t q = x->order[j];
+            if (!alone[q]) segs[seqs[q].seg0 + seqs[q].n_seg++] = (att_seg) { s->part0, s->n_tok * group, s->n_split, t * group };
+            for (int32_t k = 0; k < x->n_new[q] && s->list != ATT_TOKENS; ++k) list[s->list + t + (uint32_t) k] = x->tok0[q] + (uint32_t) k;
+            t += (uint32_t) x->n_new[q];
+        }
+    }
+    if (sent > 0) {
+        hipError_t e = hipMemcpyAsync(b->buf.dev, b->buf.pin, sent, hipMemcpyHostToDevice, sllm_shim_stream());
+        if (e == hipSuccess) e = hipEventRecord(b->buf.sent, sllm_shim_stream());
+        if (e != hipSuccess) {
+            hipStreamSynchronize(sllm_shim_stream());
+            buffer_drop(&b->buf);
+            st = sllm_shim_hip_fail(e, "batch_create");
+        }
+    }
+out:
+    for (int m = 0; m < N_MODES; ++m) free(it[m].v);
+    free(seg_count);
+    free(seg_at);
+    free(alone);
+    return st;
+}
+
+int sllm_gfx950_batch_create(sllm_gfx950_pages *p, const int32_t *seqs, const int32_t *n_new, int32_t n, int32_t n_head,
+                             int32_t act_dtype, sllm_gfx950_batch **out) {
+    ATT_NEED_OPEN();
+    if (out == NULL) return FAIL_ARG("batch_create: NULL out");
+    *out = NULL;
+    if (p == NULL || n < 0 || n > SLLM_GFX950_ATTN_MAX_SEQS || (n > 0 && (seqs == NULL || n_new == NULL))) {
+        return FAIL_ARG("batch_create: NULL, or %d sequences", n);
+    }
+    if (bad_heads(n_head, p->d.n_head_kv, p->d.head_dim)) return FAIL_ARG("batch_create: %d query heads over %d", n_head, p->d.n_head_kv);
+    const int pair = bad_type(act_dtype) ? -1 : type_pair(act_dtype, p->d.dtype);
+    if (pair < 0) return FAIL_ARG("batch_create: rows of type %d over a cache of type %d", act_dtype, p->d.dtype);
+
+    const size_t n1 = (size_t) n + 1;
+    sllm_gfx950_batch *b = calloc(1, sizeof *b);
+    int32_t *work = malloc(n1 * 5 * sizeof *work);
+    uint32_t *uwork = malloc(n1 * 2 * sizeof *uwork);
+    segment *seg = calloc(n1 * 2, sizeof *seg);
+    plan x = { .p = p, .seqs = seqs, .n_new = n_new, .seg = seg };
+    int st = SLLM_GFX950_OK;
+    if (b == NULL || work == NULL || uwork == NULL || seg == NULL) {
+        st = FAIL_NOMEM("batch_create: %d sequences", n);
+        goto out;
+    }
+    int32_t *len0 = work, *pages0 = work + n1, *last0 = work + 2 * n1;
+    x.order = work + 3 * n1;
+    x.common = work + 4 * n1;
+    x.tok0 = uwork;
+    x.table = uwork + n1;
+    b->p = p;
+    b->n_head = n_head;
+    b->pair = pair;
+
+    pthread_mutex_lock(&p->mtx);
+    int64_t want = 0, tokens = 0, held = 0;
+    st = check_names(p, seqs, n, "batch_create");
+    for (int32_t i = 0; i < n && st == SLLM_GFX950_OK; ++i) {
+        sequence *s = &p->seq[seqs[i]];
+        if (n_new[i] < 0 || (int64_t) s->len + n_new[i] > SLLM_GFX950_ATTN_MAX_LEN) {
+            st = FAIL_ARG("batch_create: %d new positions for sequence %d of %d", n_new[i], seqs[i], s->len);
+            break;
+        }
+        const int32_t pages = pages_for(p, s->len + n_new[i]);
+        const int own_last = s->len % p->d.page_tokens == 0 || p->refs[s->page[s->n_pages - 1]] == 1 || n_new[i] == 0;
+        want += pages - s->n_pages + !own_last;
+        x.tok0[i] = (uint32_t) tokens;
+        x.table[i] = (uint32_t) held;
+        tokens += n_new[i];
+        held += pages;
+        len0[i] = s->len;
+        pages0[i] = s->n_pages;
+        last0[i] = own_last ? -1 : s->page[s->n_pages - 1];
+        if (tokens > SLLM_GFX950_ATTN_MAX_TOKENS || held > INT32_MAX) st = FAIL_ARG("batch_create: too many new positions or pages");
+        else if (!reserve(s, pages)) st = FAIL_NOMEM("batch_create: page table");
+    }
+    if (st == SLLM_GFX950_OK && tokens * n_head > SLLM_GFX950_ATTN_MAX_ROWS) st = FAIL_ARG("batch_create: too many rows");
+    if (st == SLLM_GFX950_OK && want > p->n_free) st = FAIL_NOMEM("batch_create: %lld pages wanted, %d free", (long long) want, p->n_free);
+    if (st == SLLM_GFX950_OK && (b->held = malloc((size_t) (held ? held : 1) * sizeof *b->held)) == NULL) st = FAIL_NOMEM("batch_create: pages held");
+    if (st == SLLM_GFX950_OK) {
+        copies c;
+        copies_start(&c, p);
+        b->n_tok = (uint32_t) tokens;
+        for (int32_t i = 0; i < n; ++i) {
+            sequence *s = &p->seq[seqs[i]];
+            if (last0[i] >= 0) {                         /* it would write into a page that others hold */
+                s->page[s->n_pages - 1] = take_page(p);
+                copies_add(&c, last0[i], s->page[s->n_pages - 1], s->len % p->d.page_tokens);
+            }
+            s->len += n_new[i];
+            const int32_t pages = pages_for(p, s->len);
+            while (s->n_pages < pages) s->page[s->n_pages++] = take_page(p);
+        }
+        st = copies_flush(&c);
+        if (st == SLLM_GFX950_OK) st = lay_out(b, &x, n, len0);
+        for (int32_t i = 0; i < n; ++i) {
+            sequence *s = &p->seq[seqs[i]];
+            if (st != SLLM_GFX950_OK) {                  /* as it was */
+                while (s->n_pages > pages0[i]) give_page(p, s->page[--s->n_pages]);
+                if (last0[i] >= 0) {
+                    give_page(p, s->page[s->n_pages - 1]);
+                    s->page[s->n_pages - 1] = last0[i];
+                }
+                s->len = len0[i];
+                continue;
+            }
+            if (last0[i] >= 0) give_page(p, last0[i]);
+            for (int32_t j = 0; j < s->n_pages; ++j) {
+                ++p->holds[s->page[j]];
+                b->held[b->n_held++] = s->page[j];
+            }
+        }
+        if (st == SLLM_GFX950_OK) ++p->open;
+    }
+    pthread_mutex_unlock(&p->mtx);
+out:
+    free(work);
+    free(uwork);
+    free(seg);
+    if (st != SLLM_GFX950_OK) {
+        if (b != NULL) free(b->held);
+        free(b);
+        return st;
+    }
+    *out = b;
+    return SLLM_GFX950_OK;
+}
+
+void sllm_gfx950_batch_destroy(sllm_gfx950_batch *b) {
+    if (b == NULL) return;
+    sllm_gfx950_pages *p = b->p;
+    pthread_mutex_lock(&p->mtx);
+    for (int32_t i = 0; i < b->n_held; ++i) {
+        --p->holds[b->held[i]];
+        maybe_free(p, b->held[i]);
+    }
+    buffer_put(p, &b->buf);
+    const int last = --p->open == 0 && p->gone;
+    pthread_mutex_unlock(&p->mtx);
+    if (last) pages_drop(p);
+    free(b->held);
+    free(b);
+}
+
+int32_t sllm_gfx950_batch_rows(const sllm_gfx950_batch *b) { return b ? (int32_t) b->n_tok : 0; }
+
+/* bytes between a tensor's rows of `width` elements; 0: not what a call takes */
+static uint64_t row_bytes(size_t stride, uint64_t width, uint32_t size) {
+    if (stride == 0) stride = (size_t) width;
+    if (stride > (1u << 28) || stride < width || stride * size % 16u != 0) return 0;
+    return (uint64_t) stride * size;
+}
+
+int sllm_gfx950_batch_store(sllm_gfx950_batch *b, int32_t layer, const void *k, size_t k_stride, const void *v, size_t v_stride) {
+    ATT_NEED_OPEN();
+    if (b == NULL) return FAIL_ARG("batch_store: NULL");
+    sllm_gfx950_pages *p = b->p;
+    if (layer < 0 || layer >= p->d.n_layer) return FAIL_ARG("batch_store: layer %d of %d", layer, p->d.n_layer);
+    const uint32_t kv = (uint32_t) p->d.n_head_kv, hd = (uint32_t) p->d.head_dim, size = b->pair <= 1 ? 4u : 2u;
+    const uint64_t kt = row_bytes(k_stride, (uint64_t) kv * hd, size), vt = row_bytes(v_stride, (uint64_t) kv * hd, size);
+    if (kt == 0 || vt == 0) return FAIL_ARG("batch_store: stride");
+    if (b->n_tok == 0) return SLLM_GFX950_OK;
+    if (k == NULL || v == NULL || misaligned(k) || misaligned(v)) return FAIL_ARG("batch_store: NULL or misaligned rows");
+    uint8_t *layer_mem = p->mem + (uint64_t) layer * p->layer_bytes;
+    att_store_args a = { k, v, layer_mem, layer_mem + (uint64_t) kv * p->block_bytes,
+                         (const uint32_t *) (b->buf.dev + b->off_tables), (const uint32_t *) (b->buf.dev + b->off_tok_seq),
+                         (const att_seq *) (b->buf.dev + b->off_seqs), kt, vt, p->page_bytes, p->page_shift, hd, kv, b->n_tok };
+    void *args[] = { &a };
+    const uint64_t threads = (uint64_t) b->n_tok * (hd / 8u);
+    return sllm_shim_launch(sllm_shim_attn_function(SLLM_ATTN_STORE + (b->pair < 2 ? b->pair : 2)),
+                            (uint32_t) ((threads + ATT_THREADS - 1) / ATT_THREADS), 2u * kv, ATT_THREADS, 0, args);
+}
+
+static int bad_scale(float scale) { return !(scale > 0.0f) || isinf(scale); }
+
+int sllm_gfx950_batch_attend(sllm_gfx950_batch *b, int32_t layer, const void *q, size_t q_stride, float scale, void *out,
+                             size_t out_stride) {
+    ATT_NEED_OPEN();
+    if (b == NULL) return FAIL_ARG("batch_attend: NULL");
+    sllm_gfx950_pages *p = b->p;
+    if (layer < 0 || layer >= p->d.n_layer) return FAIL_ARG("batch_attend: layer %d of %d", layer, p->d.n_layer);
+    const uint32_t kv = (uint32_t) p->d.n_head_kv, hd = (uint32_t) p->d.head_dim, size = b->pair <= 1 ? 4u : 2u;
+    const uint64_t qt = row_bytes(q_stride, (uint64_t) b->n_head * hd, size), ot = row_bytes(out_stride, (uint64_t) b->n_head * hd, size);
+    if (qt == 0 || ot == 0) return FAIL_ARG("batch_attend: stride");
+    if (bad_scale(scale)) return FAIL_ARG("batch_attend: scale %g", (double) scale);
+    if (b->n_tok == 0) return SLLM_GFX950_OK;
+    if (q == NULL || out == NULL || misaligned(q) || misaligned(out)) return FAIL_ARG("batch_attend: NULL or misaligned rows");
+    const uint32_t wide = hd > 64, group = (uint32_t) b->n_head / kv;
+    uint8_t *dev = b->buf.dev;
+    const uint8_t *layer_mem = p->mem + (uint64_t) layer * p->layer_bytes;
+    att_args a = { .q = q, .out = out, .k = layer_mem, .v = layer_mem + (uint64_t) kv * p->block_bytes,
+                   .tables = (const uint32_t *) (dev + b->off_tables), .list = (const uint32_t *) (dev + b->off_list),
+                   .part_o = (float *) (dev + b->off_part_o), .part_ml = (float *) (dev + b->off_part_ml),
+                   .q_tok = qt, .q_head = (uint64_t) hd * size, .out_tok = ot, .out_head = (uint64_t) hd * size,
+                   .page_bytes = p->page_bytes, .page_shift = p->page_shift, .hd = hd, .group = group,
+                   .c = (float) ((double) scale * LOG2E) };
+    /* the partial results are one set of memory: a call's launches stay together */
+    pthread_mutex_lock(&p->mtx);
+    int st = SLLM_GFX950_OK;
+    for (int m = 0; m < N_MODES && st == SLLM_GFX950_OK; ++m) {
+        a.items = (const att_item *) (dev + b->off_items[m]);
+        a.n_items = b->n_items[m];
+        void *args[] = { &a };
+        st = sllm_shim_launch(sllm_shim_attn_function(SLLM_ATTN_ATTEND + (b->pair * 2 + (int) wide) * 3 + m), a.n_items, 1, ATT_THREADS, 0, args);
+    }
+    if (st == SLLM_GFX950_OK && b->join) {
+        att_join_args j = { out, a.part_o, a.part_ml, (const uint32_t *) (dev + b->off_tok_seq), (const att_seq *) (dev + b->off_seqs),
+                            (const att_seg *) (dev + b->off_segs), ot, hd, wide ? 128 : 64, group, (uint32_t) b->n_head, b->n_tok, 0 };
+        void *args[] = { &j };
+        const uint64_t waves = (uint64_t) b->n_tok * (uint64_t) b->n_head;
+        st = sllm_shim_launch(sllm_shim_attn_function(SLLM_ATTN_JOIN + (b->pair < 2 ? 0 : b->pair - 1)),
+                              (uint32_t) ((waves + ATT_THREADS / 64 - 1) / (ATT_THREADS / 64)), 1, ATT_THREADS, 0, args);
+    }
+    pthread_mutex_unlock(&p->mtx);
+    return st;
+}
+
+/* ------------------------------------------------------------------ */
+/* whole prompts                                                       */
+/* ------------------------------------------------------------------ */
+
+struct sllm_gfx950_prompt {
+    int32_t  dtype, n_head, n_head_kv, head_dim;
+    uint64_t n_q, n_k;               /* rows */
+    uint32_t n_items;
+    att_item *items;                 /* device */
+};
+
+static int longest_first(const void *a, const void *b) {
+    const att_item *x = a, *y = b;
+    if (x->key1 != y->key1) return x->key1 > y->key1 ? -1 : 1;
+    if (x->kv != y->kv) return x->kv < y->kv ? -1 : 1;
+    if (x->head != y->head) return x->head < y->head ? -1 : 1;
+    return x->row0 < y->row0 ? -1 : x->row0 > y->row0;
+}
+
+int sllm_gfx950_prompt_create(const sllm_gfx950_prompt_desc *d, sllm_gfx950_prompt **out) {
+    ATT_NEED_OPEN();
+    if (out == NULL) return FAIL_ARG("prompt_create: NULL out");
+    *out = NULL;
+    if (d == NULL || bad_type(d->dtype) || bad_heads(d->n_head, d->n_head_kv, d->head_dim) || d->n_seq < 0 ||
+        d->n_seq > SLLM_GFX950_ATTN_MAX_SEQS || (d->n_seq > 0 && d->q_len == NULL)) {
+        return FAIL_ARG("prompt_create: type, heads, head dimension or sequences outside what a plan takes");
+    }
+    sllm_gfx950_prompt *p = calloc(1, sizeof *p);
+    items it = { 0 };
+    int st = SLLM_GFX950_OK;
+    if (p == NULL) return FAIL_NOMEM("prompt_create");
+    p->dtype = d->dtype;
+    p->n_head = d->n_head;
+    p->n_head_kv = d->n_head_kv;
+    p->head_dim = d->head_dim;
+    const uint32_t group = (uint32_t) (d->n_head / d->n_head_kv);
+    for (int32_t i = 0; i < d->n_seq && st == SLLM_GFX950_OK; ++i) {
+        const int32_t nq = d->q_len[i], nk = d->k_len ? d->k_len[i] : nq;
+        if (nq < 0 || nk < 0 || p->n_q + (uint64_t) nq > SLLM_GFX950_ATTN_MAX_TOKENS || p->n_k + (uint64_t) nk > SLLM_GFX950_ATTN_MAX_TOKENS) {
+            st = FAIL_ARG("prompt_create: sequence %d of %d and %d rows, or too many", i, nq, nk);
+            break;
+        }
+        const uint32_t rows = (uint32_t) nq * group;
+        for (uint32_t r = 0; r < rows && st == SLLM_GFX950_OK; r += ATT_ROWS) {
+            const uint32_t n = rows - r < ATT_ROWS ? rows - r : ATT_ROWS;
+            const int32_t last = (int32_t) ((r + n - 1) / group) + nk - nq + 1;    /* keys that the last row sees */
+            for (int32_t h = 0; h < d->n_head_kv; ++h) {
+                att_item *a = items_add(&it);
+                if (a == NULL) { st = FAIL_NOMEM("prompt_create: work items"); break; }
+                *a = (att_item) { r, n, (uint32_t) p->n_q, ATT_TOKENS, nk - nq + 1, 0, last > 0 ? (uint32_t) last : 0,
+                                  (uint32_t) p->n_k, (uint32_t) h, ATT_DIRECT };
+            }
+        }
+        p->n_q += (uint64_t) nq;
+        p->n_k += (uint64_t) nk;
+        if (st == SLLM_GFX950_OK && it.n > MAX_ITEMS) st = FAIL_ARG("prompt_create: too many rows");
+    }
+    if (st == SLLM_GFX950_OK && it.n > 0) {
+        qsort(it.v, it.n, sizeof *it.v, longest_first);
+        p->n_items = (uint32_t) it.n;
+        hipError_t e = hipMalloc((void **) &p->items, it.n * sizeof *it.v);
+        if (e != hipSuccess) { p->items = NULL; st = sllm_shim_hip_fail(e, "hipMalloc(prompt plan)"); }
+        else {
+            e = hipMemcpyAsync(p->items, it.v, it.n * sizeof *it.v, hipMemcpyHostToDevice, sllm_shim_stream());
+            if (e == hipSuccess) e = hipStreamSynchronize(sllm_shim_stream());
+            if (e != hipSuccess) st = sllm_shim_hip_fail(e, "prompt_create");
+        }
+    }
+    free(it.v);
+    if (st != SLLM_GFX950_OK) {
+        if (p->items) hipFree(p->items);
+        free(p);
+        return st;
+    }
+    *out = p;
+    return SLLM_GFX950_OK;
+}
+
+void sllm_gfx950_prompt_destroy(sllm_gfx950_prompt *p) {
+    if (p == NULL) return;
+    if (p->items) {
+        if (sllm_shim_is_open()) hipStreamSynchronize(sllm_shim_stream());
+        hipFree(p->items);
+    }
+    free(p);
+}
+
+/* A tensor [n][heads][hd] with strides tok and head in elements, 0 and 0: packed.
+ * Bytes into *t and *h and how far it reaches into *extent; 0: not what a call takes. */
+static int strides(size_t tok, size_t head, uint64_t heads, uint64_t hd, uint64_t n, uint32_t size, uint64_t *t, uint64_t *h,
+                   uint64_t *extent) {
+    if (tok == 0 && head == 0) {
+        tok = (size_t) (heads * hd);
+        head = (size_t) hd;
+    }
+    if (tok > (1u << 28) || (uint64_t) head > 1ull << 40 || tok * size % 16u != 0 || head * size % 16u != 0) return 0;
+    *t = (uint64_t) tok * size;
+    *h = (uint64_t) head * size;
+    *extent = n == 0 ? 0 : (n - 1) * *t + (heads - 1) * *h + hd * size;
+    return 1;
+}
+
+int sllm_gfx950_prompt_attend(sllm_gfx950_prompt *p, const sllm_gfx950_prompt_io *io) {
+    ATT_NEED_OPEN();
+    if (p == NULL || io == NULL) return FAIL_ARG("prompt_attend: NULL");
+    if (bad_scale(io->scale)) return FAIL_ARG("prompt_attend: scale %g", (double) io->scale);
+    const uint32_t size = type_size(p->dtype), hd = (uint32_t) p->head_dim;
+    att_args a = { .q = io->q, .out = io->out, .k = io->k, .v = io->v, .items = p->items, .hd = hd,
+                   .group = (uint32_t) (p->n_head / p->n_head_kv), .n_items = p->n_items, .c = (float) ((double) io->scale * LOG2E) };
+    uint64_t qx, kx, vx, ox;
+    if (!strides(io->q_tok, io->q_head, (uint64_t) p->n_head, hd, p->n_q, size, &a.q_tok, &a.q_head, &qx) ||
+        !strides(io->k_tok, io->k_head, (uint64_t) p->n_head_kv, hd, p->n_k, size, &a.k_tok, &a.k_head, &kx) ||
+        !strides(io->v_tok, io->v_head, (uint64_t) p->n_head_kv, hd, p->n_k, size, &a.v_tok, &a.v_head, &vx) ||
+        !strides(io->out_tok, io->out_head, (uint64_t) p->n_head, hd, p->n_q, size, &a.out_tok, &a.out_head, &ox)) {
+        return FAIL_ARG("prompt_attend: strides");
+    }
+    /* rows of out apart: heads within a token, or tokens within a head */
+    const uint64_t row = (uint64_t) hd * size;
+    const int by_tok = a.out_head >= row && (p->n_q <= 1 || a.out_tok >= (uint64_t) (p->n_head - 1) * a.out_head + row);
+    const int by_head = a.out_tok >= row && (p->n_head == 1 || a.out_head >= (p->n_q ? (p->n_q - 1) : 0) * a.out_tok + row);
+    if (!by_tok && !by_head) return FAIL_ARG("prompt_attend: rows of out overlap");
+    if (p->n_items == 0) return SLLM_GFX950_OK;
+    if (io->q == NULL || io->out == NULL || misaligned(io->q) || misaligned(io->k) || misaligned(io->v) || misaligned(io->out) ||
+        (p->n_k > 0 && (io->k == NULL || io->v == NULL))) {
+        return FAIL_ARG("prompt_attend: NULL or misaligned rows");
+    }
+    const int type = p->dtype == SLLM_GFX950_F32 ? 0 : p->dtype == SLLM_GFX950_F16 ? 1 : 2;
+    void *args[] = { &a };
+    return sllm_shim_launch(sllm_shim_attn_function(SLLM_ATTN_PROMPT + type * 2 + (hd > 64)), p->n_items, 1, ATT_THREADS, 0, args);
+}

@@ -1,0 +1,647 @@
+// attn_kernels.hip -- attention over a paged cache and over packed prompts, and
+// the cache's copies (sllm_gfx950_attn.h), for gfx950.
+//
+// Attention of a row: out = sum_j p_j v_j / sum_j p_j, p_j = 2^(c (s_j - m)),
+// s_j = q . k_j, c = scale log2(e), m a running maximum of s. One pass over the
+// keys: m, the sum l and the sums of p v are carried in f32 registers and scaled
+// down when a larger s comes.
+//
+// A row is a query token and one of the query heads of a KV head, so that the
+// heads that share keys share the tile that holds them. The scores are formed
+// as S^T = K Q^T with 16 x 16 matrix instructions: a lane then holds scores of
+// one row (lane % 16) for four keys (4 (lane / 16) + i), which is the operand
+// layout that O^T += V^T P^T wants, so p never leaves its lane; only a tile's
+// maximum crosses lanes.
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+#include "attn_layout.h"
+
+namespace {
+
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+
+// Pointers read from memory or built from integers are generic to the compiler
+// and would be accessed with flat instructions, which count against the LDS
+// counter too: these name the address space.
+#define GLOBAL __attribute__((address_space(1)))
+#define G_CAST(T, p) ((GLOBAL T *) (p))
+#define LDS_PTR(p) ((__attribute__((address_space(3))) void *) (p))
+
+constexpr int WAVES = 4;
+
+// what keys past the end and dimensions past head_dim are read from
+__device__ __attribute__((aligned(16))) uint32_t att_zeros[4];
+
+template <int N> __device__ __forceinline__ void wait_vmem() {   // s_waitcnt vmcnt(N), the other counters untouched
+    static_assert(N >= 0 && N < 64, "vmcnt");
+    __builtin_amdgcn_s_waitcnt((N & 15) | ((N >> 4) << 14) | (7 << 4) | (15 << 8));
+}
+
+__device__ __forceinline__ uint32_t uniform(uint32_t x) { return (uint32_t) __builtin_amdgcn_readfirstlane((int) x); }
+
+// over the four lanes that hold a row (lane, lane ^ 16, lane ^ 32, lane ^ 48)
+__device__ __forceinline__ float row_max(float x) {
+    u32x2 r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    x = fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+    r = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+__device__ __forceinline__ float row_sum(float x) {
+    u32x2 r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    x = __uint_as_float(r[0]) + __uint_as_float(r[1]);
+    r = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
+
+template <typename T> struct vec8 { typedef T type __attribute__((ext_vector_type(8))); };
+template <typename T> struct vec4 { typedef T type __attribute__((ext_vector_type(4))); };
+
+__device__ __forceinline__ f32x4 mfma(vec8<_Float16>::type a, vec8<_Float16>::type b, f32x4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
+}
+__device__ __forceinline__ f32x4 mfma(vec8<__bf16>::type a, vec8<__bf16>::type b, f32x4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
+}
+__device__ __forceinline__ f32x4 mfma(float a, float b, f32x4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x4f32(a, b, c, 0, 0, 0);
+}
+
+constexpr float LOWEST = -3.402823466e38f;
+
+// ---------------------------------------------------------------------------
+// attention
+// ---------------------------------------------------------------------------
+
+// Keys of a tile and what it takes in LDS. A tile holds its keys' rows of D
+// values, then its values' rows, 16-byte pieces of a row swapped about by the
+// row (ksw, vsw) so that the lanes of one read fall into different banks.
+template <typename T, int D, bool KEYS> struct tile {
+    static constexpr bool WIDE = sizeof(T) == 4;
+    static constexpr int KT = (KEYS ? 32 : 64) / (WIDE ? 2 : 1);
+    static constexpr int ROWB = D * (int) sizeof(T);
+    static constexpr int CH = ROWB / 16;
+    static constexpr int HALF = KT * ROWB;
+    static constexpr int BYTES = 2 * HALF;
+    static constexpr int STAGES = 2;
+    static constexpr int LDS = BYTES * STAGES * (KEYS ? WAVES : 1);
+    static __device__ __forceinline__ uint32_t ksw(uint32_t r) { return !WIDE && CH == 16 ? r & 15u : r & 7u; }
+    static __device__ __forceinline__ uint32_t vsw(uint32_t r) {
+        if (WIDE) return (CH == 32 ? (r >> 2) & 7u : (r >> 2) & 3u) << 2;
+        return (CH == 16 ? r & 7u : (r >> 1) & 3u) << 1;
+    }
+};
+
+// A: the type of q and out. T: of the keys and values. D: head_dim, padded. A
+// wave has NT tiles of 16 rows. KEYS: the waves take the item's tiles in turn,
+// all for the same rows, and their results are joined in LDS; else each wave
+// has rows of its own and all share a tile. PAGED: keys are found by page.
+template <typename A, typename T, int D, int NT, bool KEYS, bool PAGED>
+struct attention {
+    typedef tile<T, D, KEYS> L;
+    static constexpr bool WIDE = L::WIDE;
+    static constexpr bool SPLIT = !WIDE && sizeof(A) == 4;       // f32 rows against f16 keys
+    static constexpr int KT = L::KT;
+    static constexpr int KS = KT / 16;                           // 16-key subtiles
+    static constexpr int DT = D / 16;
+    static constexpr int QC = D * (int) sizeof(T) / 64;          // 16-byte pieces of a row that a lane holds
+    static constexpr int GROUP = KEYS ? (KT < 16 ? KT : 16) : KT / WAVES;   // rows that one address serves: within a page
+    static constexpr int GROUPS = (KEYS ? KT : KT / WAVES) / GROUP;
+    static constexpr int RPI = 1024 / L::ROWB;                   // rows of a copy instruction
+    typedef typename vec8<T>::type t8;
+
+    const att_args &a;
+    const att_item it;
+    uint8_t *S;
+    uint32_t lane, wave, g, li;
+
+    // rows: lane li of row tile nt
+    int lim[NT];                    // keys the row sees
+    float c[NT];
+    float m[NT], l[NT];
+    f32x4 o[DT][NT];
+    // a lane's pieces of q: 8 values (SPLIT: and what rounding left of them), or 4 f32
+    t8 qf[WIDE ? 1 : NT][WIDE ? 1 : QC], ql[SPLIT ? NT : 1][SPLIT ? QC : 1];
+    f32x4 qw[WIDE ? NT : 1][WIDE ? QC : 1];
+    int lim_min, lim_max;           // of the wave's rows
+
+    __device__ __forceinline__ uint32_t row_of(int nt) const {
+        return min((KEYS ? 0u : wave * (16u * NT)) + 16u * (uint32_t) nt + li, it.n_rows - 1u);
+    }
+    __device__ __forceinline__ uint32_t token(uint32_t t) const {
+        return it.list == ATT_TOKENS ? it.tok0 + t : *G_CAST(const uint32_t, a.list + it.list + t);
+    }
+    __device__ __forceinline__ int limit(uint32_t t) const {     // (vis0 + t, at most the range's end)
+        return min((int) it.key1, it.vis0 + (int) t);
+    }
+
+    __device__ __forceinline__ void load_q() {
+        const uint32_t first = KEYS ? 0u : wave * (16u * NT);
+        lim_min = limit((it.row0 + min(first, it.n_rows - 1u)) / a.group);
+        lim_max = limit((it.row0 + min(first + 16u * NT, it.n_rows) - 1u) / a.group);
+        lim_min = (int) uniform((uint32_t) lim_min);
+        lim_max = (int) uniform((uint32_t) lim_max);
+        if (first >= it.n_rows) lim_max = 0;                     // a wave without rows
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+            const uint32_t r = it.row0 + row_of(nt), t = r / a.group, h = it.head * a.group + r % a.group;
+            lim[nt] = limit(t);
+            const uint8_t *src = (const uint8_t *) a.q + token(t) * a.q_tok + h * a.q_head;
+            c[nt] = a.c;
+            if constexpr (WIDE) {
+#pragma unroll
+                for (int s = 0; s < QC; ++s) {
+                    const uint32_t d = 4u * (4u * s + g);
+                    qw[nt][s] = d < a.hd ? *G_CAST(const f32x4, src + d * 4u) : (f32x4) { 0, 0, 0, 0 };
+                }
+            } else if constexpr (!SPLIT) {
+#pragma unroll
+                for (int s = 0; s < QC; ++s) {
+                    const uint32_t d = 8u * (4u * s + g);
+                    const u32x4 v = d < a.hd ? *G_CAST(const u32x4, src + d * 2u) : (u32x4) { 0, 0, 0, 0 };
+                    qf[nt][s] = __builtin_bit_cast(t8, v);
+                }
+            } else {
+                // f32 queries as the sum of two f16 values: 22 bits of each. The row is
+                // first scaled by a power of two to a largest magnitude of 1..2, so that
+                // neither part leaves f16's range; c takes the power back.
+                f32x4 x[QC][2];
+                float top = 0.0f;
+#pragma unroll
+                for (int s = 0; s < QC; ++s) {
+                    const uint32_t d = 8u * (4u * s + g);
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) {
+                        x[s][i] = d < a.hd ? *G_CAST(const f32x4, src + d * 4u + 16u * i) : (f32x4) { 0, 0, 0, 0 };
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) top = fmaxf(top, fabsf(x[s][i][e]));
+                    }
+                }
+                top = row_max(top);
+                const int e2 = min(max((int) (__float_as_uint(top) >> 23) - 127, -100), 100);
+                const float down = __uint_as_float((uint32_t) (127 - e2) << 23);
+                c[nt] = a.c * __uint_as_float((uint32_t) (127 + e2) << 23);
+#pragma unroll
+                for (int s = 0; s < QC; ++s) {
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) {
+                        const float f = x[s][e >> 2][e & 3] * down;
+                        const T hi = (T) f;
+                        qf[nt][s][e] = hi;
+                        ql[nt][s][e] = (T) (f - (float) hi);
+                    }
+                }
+            }
+        }
+    }
+
+    // Copy a tile's keys and values into `to` (this wave's rows of it).
+    __device__ __forceinline__ void issue(uint32_t t, uint8_t *to) const {
+        const uint8_t *zero = (const uint8_t *) att_zeros;
+        const uint32_t rowk = PAGED ? a.hd * (uint32_t) sizeof(T) : (uint32_t) a.k_tok;
+        const uint32_t rowv = PAGED ? rowk : (uint32_t) a.v_tok;
+#pragma unroll
+        for (int gr = 0; gr < GROUPS; ++gr) {
+            const uint32_t r0 = (KEYS ? 0u : wave * (uint32_t) GROUP) + (uint32_t) gr * GROUP;      // row in the tile
+            const uint32_t key = t * KT + r0;
+            const uint8_t *kb, *vb;
+            if constexpr (PAGED) {
+                const uint32_t at = min(key, it.key1 - 1u);
+                const uint32_t page = uniform(*G_CAST(const uint32_t, a.tables + it.kv + (at >> a.page_shift)));
+                const uint64_t off = page * a.page_bytes + ((uint64_t) (it.head << a.page_shift) + (at & ((1u << a.page_shift) - 1u) & ~(uint32_t) (GROUP - 1))) * rowk;
+                kb = a.k + off;
+                vb = a.v + off;
+            } else {
+                kb = a.k + (uint64_t) (it.kv + key) * a.k_tok + it.head * a.k_head;
+                vb = a.v + (uint64_t) (it.kv + key) * a.v_tok + it.head * a.v_head;
+            }
+#pragma unroll
+            for (int j = 0; j < GROUP / RPI; ++j) {
+                const uint32_t rg = (uint32_t) j * RPI + lane / L::CH, r = r0 + rg, ch = lane % L::CH;
+                const uint32_t ck = ch ^ L::ksw(r), cv = ch ^ L::vsw(r);
+                const bool in = t * KT + r < it.key1;
+                const uint8_t *ks = in && ck * 16u < a.hd * (uint32_t) sizeof(T) ? kb + (uint64_t) rg * rowk + ck * 16u : zero;
+                const uint8_t *vs = in && cv * 16u < a.hd * (uint32_t) sizeof(T) ? vb + (uint64_t) rg * rowv + cv * 16u : zero;
+                uint8_t *dst = to + (r0 + (uint32_t) j * RPI) * L::ROWB;
+                __builtin_amdgcn_global_load_lds((const void *) ks, LDS_PTR(dst), 16, 0, 0);
+                __builtin_amdgcn_global_load_lds((const void *) vs, LDS_PTR(dst + L::HALF), 16, 0, 0);
+            }
+        }
+    }
+
+    // A value of the tile that is infinite or NaN.
+    __device__ __forceinline__ static bool odd(float x) { return (__float_as_uint(x) & 0x7f800000u) == 0x7f800000u; }
+
+    // One tile: scores, the maximum, p, and the products with the values.
+    // SEEN: every row sees every key of it. CAREFUL: an infinite or NaN value must
+    // not reach rows that do not see its key (0 times it is NaN): such values
+    // are left out of the products and added to the rows that see them.
+    template <bool SEEN, bool CAREFUL>
+    __device__ __forceinline__ void step(uint32_t t, const uint8_t *tl) {
+        f32x4 s[KS][NT];
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks) {
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) s[ks][nt] = (f32x4) { 0, 0, 0, 0 };
+            const uint32_t r = 16u * ks + li;
+            const uint8_t *row = tl + r * L::ROWB;
+#pragma unroll
+            for (int q = 0; q < QC; ++q) {
+                const uint8_t *src = row + (((4u * q + g) ^ L::ksw(r)) * 16u);
+                if constexpr (WIDE) {
+                    const f32x4 kf = *reinterpret_cast<const f32x4 *>(src);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+#pragma unroll
+                        for (int nt = 0; nt < NT; ++nt) s[ks][nt] = mfma(kf[e], qw[nt][q][e], s[ks][nt]);
+                    }
+                } else {
+                    const t8 kf = *reinterpret_cast<const t8 *>(src);
+#pragma unroll
+                    for (int nt = 0; nt < NT; ++nt) s[ks][nt] = mfma(kf, qf[nt][q], s[ks][nt]);
+                    if constexpr (SPLIT) {
+#pragma unroll
+                        for (int nt = 0; nt < NT; ++nt) s[ks][nt] = mfma(kf, ql[nt][q], s[ks][nt]);
+                    }
+                }
+            }
+        }
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+            float top = m[nt];
+#pragma unroll
+            for (int ks = 0; ks < KS; ++ks) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    if (!SEEN) s[ks][nt][i] = (int) (t * KT + 16u * ks + 4u * g + i) < lim[nt] ? s[ks][nt][i] : -INFINITY;
+                    top = fmaxf(top, s[ks][nt][i]);
+                }
+            }
+            top = row_max(top);
+            if (__any(top > m[nt])) {
+                const float f = __builtin_amdgcn_exp2f((m[nt] - top) * c[nt]);
+                m[nt] = top;
+                l[nt] *= f;
+#pragma unroll
+                for (int dt = 0; dt < DT; ++dt) o[dt][nt] *= f;
+            }
+            // m is at least the lowest float, so a masked -inf gives 2^-inf = 0 and never inf - inf
+            const float mc = fmaxf(m[nt] * c[nt], LOWEST);
+            float sum = 0.0f;
+#pragma unroll
+            for (int ks = 0; ks < KS; ++ks) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    s[ks][nt][i] = __builtin_amdgcn_exp2f(fmaf(s[ks][nt][i], c[nt], -mc));
+                    sum += s[ks][nt][i];
+                }
+            }
+            l[nt] += sum;
+        }
+        const uint8_t *tv = tl + L::HALF;
+        if constexpr (WIDE) {
+#pragma unroll
+            for (int ks = 0; ks < KS; ++ks) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const uint32_t r = 16u * ks + 4u * g + i;
+#pragma unroll
+                    for (int dt = 0; dt < DT; ++dt) {
+                        const uint32_t ch = (4u * dt + (li >> 2)) ^ L::vsw(r);
+                        float vf = *reinterpret_cast<const float *>(tv + r * L::ROWB + ch * 16u + (li & 3u) * 4u);
+                        if (CAREFUL) vf = odd(vf) ? 0.0f : vf;
+#pragma unroll
+                        for (int nt = 0; nt < NT; ++nt) o[dt][nt] = mfma(vf, s[ks][nt][i], o[dt][nt]);
+                    }
+                }
+            }
+        } else {
+            // 32 keys at a time: a lane's operand holds keys 4 g + 0..3 of both 16-key subtiles
+#pragma unroll
+            for (int u = 0; u < KS / 2; ++u) {
+                t8 p[NT], pl[SPLIT ? NT : 1];
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) {
+                        const float f = s[2 * u + (e >> 2)][nt][e & 3];
+                        p[nt][e] = (T) f;
+                        if constexpr (SPLIT) pl[nt][e] = (T) (f - (float) p[nt][e]);
+                    }
+                }
+#pragma unroll
+                for (int dt = 0; dt < DT; ++dt) {
+                    s16x4 h[2];
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) {
+                        const uint32_t r = 32u * u + 16u * i + 4u * g + (li >> 2);
+                        const uint32_t ch = (2u * dt + ((li >> 1) & 1u)) ^ L::vsw(r);
+                        h[i] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                            (__attribute__((address_space(3))) s16x4 *) (tv + r * L::ROWB + ch * 16u + (li & 1u) * 8u));
+                    }
+                    t8 vf = __builtin_bit_cast(t8, __builtin_shufflevector(h[0], h[1], 0, 1, 2, 3, 4, 5, 6, 7));
+                    if (CAREFUL) {
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) vf[e] = odd((float) vf[e]) ? (T) 0.0f : vf[e];
+                    }
+#pragma unroll
+                    for (int nt = 0; nt < NT; ++nt) {
+                        o[dt][nt] = mfma(vf, p[nt], o[dt][nt]);
+                        if constexpr (SPLIT) o[dt][nt] = mfma(vf, pl[nt], o[dt][nt]);
+                    }
+                }
+            }
+        }
+        if (CAREFUL) {
+            for (uint32_t r = 0; r < (uint32_t) KT; ++r) {
+                const uint8_t *row = tv + r * L::ROWB;
+#pragma unroll
+                for (int dt = 0; dt < DT; ++dt) {
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const uint32_t by = (16u * dt + 4u * g + i) * (uint32_t) sizeof(T);
+                        const float v = (float) *reinterpret_cast<const T *>(row + ((by >> 4) ^ L::vsw(r)) * 16u + (by & 15u));
+#pragma unroll
+                        for (int nt = 0; nt < NT; ++nt) {
+                            if (odd(v) && (int) (t * KT + r) < lim[nt]) o[dt][nt][i] += v;
+                        }
+                    }
+                }
+            }
+        }
+    }
+
+    template <bool CAREFUL>
+    __device__ __forceinline__ void tile_step(uint32_t t, const uint8_t *tl) {
+        if ((int) (t * KT) >= lim_max) return;                   // none of the wave's rows sees it
+        if ((int) (t * KT + KT) <= lim_min) step<true, false>(t, tl);
+        else step<false, CAREFUL>(t, tl);
+    }
+
+    template <bool CAREFUL>
+    __device__ __forceinline__ void pass() {
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+            m[nt] = LOWEST;
+            l[nt] = 0.0f;
+#pragma unroll
+            for (int dt = 0; dt < DT; ++dt) o[dt][nt] = (f32x4) { 0, 0, 0, 0 };
+        }
+        // key0 is a tile's first key
+        const uint32_t t1 = (it.key1 + KT - 1u) / KT;
+        constexpr uint32_t STEP = KEYS ? WAVES : 1;
+        uint32_t t = it.key0 / KT + (KEYS ? wave : 0u);
+        uint8_t *buf = S + (KEYS ? wave * (uint32_t) (L::BYTES * L::STAGES) : 0u);
+        if (it.key0 >= it.key1) return;
+        if (t < t1) issue(t, buf);
+        for (uint32_t n = 0; t < t1; t += STEP, ++n) {
+            wait_vmem<0>();
+            __builtin_amdgcn_s_waitcnt(0xC07F);                  // this wave's reads of the other stage are done
+            if (!KEYS) __builtin_amdgcn_s_barrier();
+            __builtin_amdgcn_sched_barrier(0);
+            if (t + STEP < t1) issue(t + STEP, buf + ((n + 1u) & 1u) * L::BYTES);
+            __builtin_amdgcn_sched_barrier(0);
+            tile_step<CAREFUL>(t, buf + (n & 1u) * L::BYTES);
+        }
+    }
+
+    __device__ __forceinline__ bool has_odd() const {
+        bool bad = false;
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+            for (int dt = 0; dt < DT; ++dt) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) bad |= odd(o[dt][nt][i]);
+            }
+        }
+        return bad;
+    }
+
+    // four of a row's results, from dimension d on
+    __device__ __forceinline__ void put(uint32_t row, uint32_t d, f32x4 x) const {
+        if (d >= a.hd) return;
+        const uint32_t r = it.row0 + row, t = r / a.group, h = it.head * a.group + r % a.group;
+        uint8_t *dst = (uint8_t *) a.out + token(t) * a.out_tok + h * a.out_head + d * sizeof(A);
+        if constexpr (sizeof(A) == 4) {
+            *G_CAST(f32x4, dst) = x;
+        } else {
+            typename vec4<A>::type y;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) y[i] = (A) x[i];
+            *G_CAST(u32x2, dst) = __builtin_bit_cast(u32x2, y);
+        }
+    }
+    __device__ __forceinline__ void finish(uint32_t row, uint32_t d, f32x4 x, float mc, float sum, bool sees) const {
+        if (it.part == ATT_DIRECT) {
+            put(row, d, sees ? x / sum : (f32x4) { 0, 0, 0, 0 });
+        } else {
+            const uint64_t at = it.part + row;
+            *G_CAST(f32x4, a.part_o + at * D + d) = x;
+            if (d == 0) {
+                a.part_ml[2 * at] = mc;
+                a.part_ml[2 * at + 1] = sum;
+            }
+        }
+    }
+
+    __device__ __forceinline__ void run() {
+        load_q();
+        pass<false>();
+        // 0 x inf in a key that a row does not see: only then is anything not finite
+        // that need not be, and only then is the pass made again
+        if (KEYS) {
+            if (__any(has_odd())) pass<true>();
+        } else {
+            if (__syncthreads_or(has_odd())) pass<true>();
+        }
+        float mc[NT];
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+            l[nt] = row_sum(l[nt]);
+            mc[nt] = fmaxf(m[nt] * c[nt], LOWEST);
+        }
+        if constexpr (!KEYS) {
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) {
+                const uint32_t row = wave * (16u * NT) + 16u * nt + li;
+                if (row < it.n_rows) {
+#pragma unroll
+                    for (int dt = 0; dt < DT; ++dt) finish(row, 16u * dt + 4u * g, o[dt][nt], mc[nt], l[nt], lim[nt] > 0);
+                }
+            }
+        } else {
+            // the waves' results side by side in LDS: [wave][row][D], then (m, l)
+            __syncthreads();
+            float *so = reinterpret_cast<float *>(S);
+            float *sm = so + WAVES * 16 * NT * D;
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) {
+                const uint32_t row = wave * (16u * NT) + 16u * nt + li;
+#pragma unroll
+                for (int dt = 0; dt < DT; ++dt) *reinterpret_cast<f32x4 *>(so + row * D + 16 * dt + 4 * g) = o[dt][nt];
+                if (g == 0) {
+                    sm[2 * row] = mc[nt];
+                    sm[2 * row + 1] = l[nt];
+                }
+            }
+            __syncthreads();
+            for (uint32_t i = threadIdx.x; i < it.n_rows * (D / 4); i += ATT_THREADS) {
+                const uint32_t row = i / (D / 4), d = 4u * (i % (D / 4));
+                float top = LOWEST, sum = 0.0f, ml[WAVES][2];
+#pragma unroll
+                for (int w = 0; w < WAVES; ++w) {
+                    ml[w][0] = sm[2 * (w * 16 * NT + row)];
+                    ml[w][1] = sm[2 * (w * 16 * NT + row) + 1];
+                    top = fmaxf(top, ml[w][0]);
+                }
+                f32x4 x = { 0, 0, 0, 0 };
+#pragma unroll
+                for (int w = 0; w < WAVES; ++w) {
+                    const float f = __builtin_amdgcn_exp2f(ml[w][0] - top);
+                    sum += f * ml[w][1];
+                    x += f * *reinterpret_cast<const f32x4 *>(so + (w * 16 * NT + row) * D + d);
+                }
+                finish(row, d, x, top, sum, limit((it.row0 + row) / a.group) > 0);
+            }
+        }
+    }
+};
+
+template <typename A, typename T, int D, int NT, bool KEYS, bool PAGED>
+__device__ __forceinline__ void attend_body(const att_args &a) {
+    typedef attention<A, T, D, NT, KEYS, PAGED> att;
+    constexpr int JOIN = KEYS ? WAVES * 16 * NT * (D + 2) * 4 : 0;
+    __shared__ __attribute__((aligned(1024))) uint8_t S[att::L::LDS > JOIN ? att::L::LDS : JOIN];
+    const att_item it = a.items[blockIdx.x];
+    const uint32_t lane = threadIdx.x & 63u;
+    att x = { a, it, S, lane, uniform(threadIdx.x >> 6), lane >> 4, lane & 15u };
+    x.run();
+}
+
+}  // namespace
+
+#define ATTEND(name, A, T, D, NT, KEYS, PAGED, PER_CU)                                     \
+    extern "C" __global__ void __launch_bounds__(ATT_THREADS, PER_CU) name(const att_args a) { \
+        attend_body<A, T, D, NT, KEYS, PAGED>(a);                                          \
+    }
+#define ATTEND_PAGED(types, A, T)                                          \
+    ATTEND(sllm_k_attend_##types##_64_few, A, T, 64, 1, true, true, 1)     \
+    ATTEND(sllm_k_attend_##types##_64_some, A, T, 64, 2, true, true, 1)    \
+    ATTEND(sllm_k_attend_##types##_64_rows, A, T, 64, 2, false, true, 1)   \
+    ATTEND(sllm_k_attend_##types##_128_few, A, T, 128, 1, true, true, 1)   \
+    ATTEND(sllm_k_attend_##types##_128_some, A, T, 128, 2, true, true, 1)  \
+    ATTEND(sllm_k_attend_##types##_128_rows, A, T, 128, 2, false, true, 1)
+#define ATTEND_PROMPT(type, T)                                             \
+    ATTEND(sllm_k_prompt_##type##_64, T, T, 64, 2, false, false, 1)        \
+    ATTEND(sllm_k_prompt_##type##_128, T, T, 128, 2, false, false, 1)
+
+ATTEND_PAGED(f32, float, float)
+ATTEND_PAGED(f32f16, float, _Float16)
+ATTEND_PAGED(f16, _Float16, _Float16)
+ATTEND_PAGED(bf16, __bf16, __bf16)
+ATTEND_PROMPT(f32, float)
+ATTEND_PROMPT(f16, _Float16)
+ATTEND_PROMPT(bf16, __bf16)
+
+namespace {
+
+// The partial results of one row, a wave a row: out = sum_i 2^(m_i - M) o_i / sum_i 2^(m_i - M) l_i,
+// M the largest m_i, always in the same order.
+template <typename A>
+__device__ __forceinline__ void join_body(const att_join_args &a) {
+    const uint32_t lane = threadIdx.x & 63u;
+    const uint32_t id = uniform(blockIdx.x * (ATT_THREADS / 64) + (threadIdx.x >> 6));
+    if (id >= a.n_tok * a.n_head) return;
+    const uint32_t tok = id / a.n_head, h = id % a.n_head, kvh = h / a.group, hh = h % a.group;
+    const att_seq s = a.seqs[a.tok_seq[tok]];
+    if (s.n_seg == 0) return;                                    // written already
+    float top = LOWEST, sum = 0.0f, x0 = 0.0f, x1 = 0.0f;
+    const bool in = 2u * lane < a.hd;
+    for (uint32_t i = 0; i < s.n_seg; ++i) {
+        const att_seg sg = a.segs[s.seg0 + i];
+        const uint64_t row = sg.part0 + (uint64_t) kvh * sg.n_split * sg.n_rows + sg.row_off + (tok - s.tok0) * a.group + hh;
+        for (uint32_t k = 0; k < sg.n_split; ++k) {
+            const uint64_t at = row + (uint64_t) k * sg.n_rows;
+            const float m = a.part_ml[2 * at], l = a.part_ml[2 * at + 1];
+            const float x = in ? a.part_o[at * a.hd_pad + 2 * lane] : 0.0f;
+            const float y = in ? a.part_o[at * a.hd_pad + 2 * lane + 1] : 0.0f;
+            const float up = fmaxf(top, m), f = __builtin_amdgcn_exp2f(top - up), e = __builtin_amdgcn_exp2f(m - up);
+            top = up;
+            sum = sum * f + l * e;
+            x0 = x0 * f + x * e;
+            x1 = x1 * f + y * e;
+        }
+    }
+    if (in) {
+        A *dst = (A *) ((uint8_t *) a.out + tok * a.out_tok) + h * a.hd + 2 * lane;
+        dst[0] = (A) (x0 / sum);
+        dst[1] = (A) (x1 / sum);
+    }
+}
+
+// A step's rows into their pages: a thread for each eight values of a row,
+// blockIdx.y the KV head's keys or values.
+template <typename A, typename T>
+__device__ __forceinline__ void store_body(const att_store_args &a) {
+    const uint32_t per_row = a.hd / 8, id = blockIdx.x * ATT_THREADS + threadIdx.x;
+    const uint32_t tok = id / per_row, ch = id % per_row, h = blockIdx.y >> 1, kv = blockIdx.y & 1u;
+    if (tok >= a.n_tok) return;
+    const att_seq s = a.seqs[a.tok_seq[tok]];
+    const uint32_t pos = s.len0 + (tok - s.tok0), page = a.tables[s.table + (pos >> a.page_shift)];
+    const uint8_t *src = kv ? (const uint8_t *) a.v + tok * a.v_tok : (const uint8_t *) a.k + tok * a.k_tok;
+    src += (h * a.hd + 8u * ch) * sizeof(A);
+    uint8_t *dst = (kv ? a.cv : a.ck) + page * a.page_bytes +
+                   (((uint64_t) (h << a.page_shift) + (pos & ((1u << a.page_shift) - 1u))) * a.hd + 8u * ch) * sizeof(T);
+    if constexpr (sizeof(A) == sizeof(T)) {
+#pragma unroll
+        for (int i = 0; i < (int) sizeof(T) / 2; ++i) G_CAST(u32x4, dst)[i] = G_CAST(const u32x4, src)[i];
+    } else {
+        typename vec8<T>::type y;
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const f32x4 x = G_CAST(const f32x4, src)[i];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) y[4 * i + e] = (T) x[e];    // to nearest, ties to even
+        }
+        *G_CAST(u32x4, dst) = __builtin_bit_cast(u32x4, y);
+    }
+}
+
+}  // namespace
+
+#define JOIN(name, A) extern "C" __global__ void __launch_bounds__(ATT_THREADS) name(const att_join_args a) { join_body<A>(a); }
+#define STORE(name, A, T) extern "C" __global__ void __launch_bounds__(ATT_THREADS) name(const att_store_args a) { store_body<A, T>(a); }
+
+JOIN(sllm_k_attn_join_f32, float)
+JOIN(sllm_k_attn_join_f16, _Float16)
+JOIN(sllm_k_attn_join_bf16, __bf16)
+STORE(sllm_k_attn_store_f32, float, float)
+STORE(sllm_k_attn_store_f32f16, float, _Float16)
+STORE(sllm_k_attn_store_16, _Float16, _Float16)
+
+// Pages to pages: blockIdx.y a pair of them, ATT_COPY_CHUNKS 16-byte pieces of
+// what it holds a workgroup, all four of a thread's in flight together.
+extern "C" __global__ void __launch_bounds__(ATT_THREADS) sllm_k_attn_copy(const att_copy_args a) {
+    const att_pair p = a.pair[blockIdx.y];
+    const uint32_t per = p.rows * a.row_bytes / 16u, n = per * a.n_blocks;
+    const uint8_t *src = a.mem + p.src * a.page_bytes;
+    uint8_t *dst = a.mem + p.dst * a.page_bytes;
+    constexpr int UN = ATT_COPY_CHUNKS / ATT_THREADS;
+    u32x4 v[UN];
+    uint64_t at[UN];
+#pragma unroll
+    for (int i = 0; i < UN; ++i) {
+        const uint32_t x = blockIdx.x * ATT_COPY_CHUNKS + (uint32_t) i * ATT_THREADS + threadIdx.x;
+        at[i] = (uint64_t) (x / per) * a.block_bytes + (x % per) * 16u;
+        if (x < n) v[i] = *G_CAST(const u32x4, src + at[i]);
+    }
+#pragma unroll
+    for (int i = 0; i < UN; ++i) {
+        const uint32_t x = blockIdx.x * ATT_COPY_CHUNKS + (uint32_t) i * ATT_THREADS + threadIdx.x;
+        if (x < n) *G_CAST(u32x4, dst + at[i]) = v[i];
+    }
+}

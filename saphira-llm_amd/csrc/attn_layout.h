@@ -1,0 +1,107 @@
+/*
+ * attn_layout.h -- what attn.c hands to the kernels of attn_kernels.hip: the
+ * argument structs and the device tables, one definition for both sides.
+ */
+#ifndef SLLM_ATTN_LAYOUT_H
+#define SLLM_ATTN_LAYOUT_H
+
+#include <stdint.h>
+
+/* rows (query token x head of one KV head) that a workgroup takes: with the
+ * four waves on different rows, or on different keys of the same 16 or 32 */
+#define ATT_ROWS      128
+#define ATT_FEW_ROWS  16
+#define ATT_SOME_ROWS 32
+#define ATT_THREADS   256
+
+#define ATT_DIRECT    0xffffffffu    /* att_item.part: rows go to the output */
+#define ATT_TOKENS    0xffffffffu    /* att_item.list: tokens in order */
+#define ATT_SEE_ALL   (1 << 30)      /* att_item.vis0: every key of the range */
+
+/*
+ * One workgroup's share: rows row0 .. row0 + n_rows of a segment (a run of
+ * keys and the tokens that read it) against its keys key0 .. key1. Row r is
+ * token r / group and head r % group of KV head `head`; token t is row
+ * tok0 + t of the query tensor, or what list[list + t] names, and sees the
+ * keys below vis0 + t.
+ */
+typedef struct att_item {
+    uint32_t row0, n_rows, tok0, list;
+    int32_t  vis0;
+    uint32_t key0, key1;
+    uint32_t kv;            /* paged: where the segment's page numbers start; packed: the first key's row */
+    uint32_t head;
+    uint32_t part;          /* row of the partial results that row0's go to, or ATT_DIRECT */
+} att_item;
+
+typedef struct att_args {
+    const void     *q;
+    void           *out;
+    const uint8_t  *k, *v;           /* paged: the layer's keys and values in page 0 */
+    const uint32_t *tables;
+    const uint32_t *list;
+    const att_item *items;
+    float          *part_o;          /* [row][head_dim padded] sums of p v */
+    float          *part_ml;         /* [row][2]: the running maximum (log2) and the sum of p */
+    uint64_t        q_tok, q_head, out_tok, out_head;    /* bytes */
+    uint64_t        k_tok, k_head, v_tok, v_head;        /* bytes */
+    uint64_t        page_bytes;
+    uint32_t        page_shift, hd, group, n_items;
+    float           c;               /* scale * log2(e) */
+    uint32_t        pad;
+} att_args;
+
+/* the partial results of a token: those of n_split splits of a segment, whose
+ * rows are n_rows apart from split to split and n_split * n_rows from KV head
+ * to KV head */
+typedef struct att_seg {
+    uint32_t part0, n_rows, n_split, row_off;
+} att_seg;
+
+/* a sequence of a batch: its rows tok0 .. tok0 + n_new, where its page numbers
+ * start, its positions before the step, and its segments */
+typedef struct att_seq {
+    uint32_t tok0, n_new, table, len0, seg0, n_seg;
+} att_seq;
+
+typedef struct att_join_args {
+    void           *out;
+    const float    *part_o, *part_ml;
+    const uint32_t *tok_seq;         /* a token's sequence */
+    const att_seq  *seqs;
+    const att_seg  *segs;
+    uint64_t        out_tok;         /* bytes */
+    uint32_t        hd, hd_pad, group, n_head, n_tok, pad;
+} att_join_args;
+
+typedef struct att_store_args {
+    const void     *k, *v;
+    uint8_t        *ck, *cv;         /* the layer's keys and values in page 0 */
+    const uint32_t *tables, *tok_seq;
+    const att_seq  *seqs;
+    uint64_t        k_tok, v_tok;    /* bytes */
+    uint64_t        page_bytes;
+    uint32_t        page_shift, hd, n_head_kv, n_tok;
+} att_store_args;
+
+typedef struct att_pair { uint32_t src, dst, rows; } att_pair;
+#define ATT_PAIRS 320
+
+/* blocks of block_bytes (a KV head's keys or values of a page in one layer),
+ * of each the first rows * row_bytes */
+typedef struct att_copy_args {
+    uint8_t  *mem;
+    uint64_t  page_bytes;
+    uint32_t  block_bytes, row_bytes, n_blocks, n_pairs;
+    att_pair  pair[ATT_PAIRS];
+} att_copy_args;
+
+#define ATT_COPY_CHUNKS 1024u        /* 16-byte pieces a workgroup */
+
+#if defined(__cplusplus)
+static_assert(sizeof(att_item) == 40 && sizeof(att_args) == 168 && sizeof(att_copy_args) <= 4096, "attn_layout.h");
+#else
+_Static_assert(sizeof(att_item) == 40 && sizeof(att_args) == 168 && sizeof(att_copy_args) <= 4096, "attn_layout.h");
+#endif
+
+#endif /* SLLM_ATTN_LAYOUT_H */

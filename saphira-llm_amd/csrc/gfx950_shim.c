@@ -1,8 +1,8 @@
 /*
  * gfx950_shim.c -- the thin C11 shim between the host code and HIP.
  *
- * Loads the gfx950 code objects built from i2s_kernels.hip and
- * decode_kernels.hip (embedded in this library at build time) with
+ * Loads the gfx950 code objects built from i2s_kernels.hip,
+ * decode_kernels.hip and attn_kernels.hip (embedded in this library at build time) with
  * hipModuleLoadData, launches its entry points
  * with hipModuleLaunchKernel on one library-owned stream, and owns the device
  * buffers: registered weight tensors, per-call scratch and job tables.
@@ -54,6 +54,20 @@ __asm__(".section .rodata.sllm_gfx950_decode_object,\"a\",@progbits\n"
         ".globl sllm_gfx950_decode_object\n"
         "sllm_gfx950_decode_object:\n"
         ".incbin \"" SLLM_GFX950_DEC_HSACO "\"\n"
+        ".byte 0\n"
+        ".previous\n");
+
+#ifndef SLLM_GFX950_ATT_HSACO
+#error "SLLM_GFX950_ATT_HSACO must name the attention code object to embed"
+#endif
+
+extern const unsigned char sllm_gfx950_attn_object[];
+__asm__(".section .rodata.sllm_gfx950_attn_object,\"a\",@progbits\n"
+        ".balign 4096\n"
+        ".hidden sllm_gfx950_attn_object\n"
+        ".globl sllm_gfx950_attn_object\n"
+        "sllm_gfx950_attn_object:\n"
+        ".incbin \"" SLLM_GFX950_ATT_HSACO "\"\n"
         ".byte 0\n"
         ".previous\n");
 
@@ -119,7 +133,8 @@ static struct {
     int            cu;
     size_t         hbm;
     char           name[520];
-    hipModule_t    mod, dec_mod;
+    hipModule_t    mod, dec_mod, attn_mod;
+    hipFunction_t  k_attn[SLLM_ATTN_FUNCTIONS];
     hipFunction_t  k_quant, k_quant_list, k_quant_host, k_host_done;
     hipFunction_t  k_slab, k_wide;
     hipFunction_t  k_stream[N_LPR];
@@ -275,6 +290,19 @@ static int load_functions(void) {
     return SLLM_GFX950_OK;
 }
 
+static int load_attn_functions(void) {
+    static const char *const types[4] = { "f32", "f32f16", "f16", "bf16" }, *const rows[3] = { "few", "some", "rows" };
+    static const char *const rest[7] = { "join_f32", "join_f16", "join_bf16", "store_f32", "store_f32f16", "store_16", "copy" };
+    for (int i = 0; i < SLLM_ATTN_FUNCTIONS; ++i) {
+        char name[64];
+        if (i < SLLM_ATTN_PROMPT) snprintf(name, sizeof name, "sllm_k_attend_%s_%d_%s", types[i / 6], i / 3 % 2 ? 128 : 64, rows[i % 3]);
+        else if (i < SLLM_ATTN_JOIN) snprintf(name, sizeof name, "sllm_k_prompt_%s_%d", types[(i - SLLM_ATTN_PROMPT) / 2 ? (i - SLLM_ATTN_PROMPT) / 2 + 1 : 0], i % 2 ? 128 : 64);
+        else snprintf(name, sizeof name, "sllm_k_attn_%s", rest[i - SLLM_ATTN_JOIN]);
+        HIP_TRY(hipModuleGetFunction(&g.k_attn[i], g.attn_mod, name));
+    }
+    return SLLM_GFX950_OK;
+}
+
 int sllm_gfx950_open(int device) {
     pthread_mutex_lock(&g_mtx);
     int st = SLLM_GFX950_OK;
@@ -286,7 +314,7 @@ int sllm_gfx950_open(int device) {
         return st;
     }
     /* what has been created, for the unwind on failure */
-    int have_mod = 0, have_dec = 0, have_stream = 0, have_ev0 = 0, have_ev1 = 0;
+    int have_mod = 0, have_dec = 0, have_attn = 0, have_stream = 0, have_ev0 = 0, have_ev1 = 0;
     int count = 0;
     hipDeviceProp_t prop;
     hipError_t e = hipGetDeviceCount(&count);
@@ -319,6 +347,12 @@ int sllm_gfx950_open(int device) {
         goto unwind;
     }
     have_dec = 1;
+    if ((e = hipModuleLoadData(&g.attn_mod, sllm_gfx950_attn_object)) != hipSuccess) {
+        st = hip_fail(e, "hipModuleLoadData(attention)");
+        goto unwind;
+    }
+    have_attn = 1;
+    if ((st = load_attn_functions()) != SLLM_GFX950_OK) goto unwind;
     if ((e = hipStreamCreateWithFlags(&g.stream, hipStreamNonBlocking)) != hipSuccess) {
         st = hip_fail(e, "hipStreamCreateWithFlags");
         goto unwind;
@@ -353,6 +387,7 @@ unwind:
     if (have_ev1) hipEventDestroy(g.ev_stop);
     if (have_ev0) hipEventDestroy(g.ev_start);
     if (have_stream) hipStreamDestroy(g.stream);
+    if (have_attn) hipModuleUnload(g.attn_mod);
     if (have_dec) hipModuleUnload(g.dec_mod);
     if (have_mod) hipModuleUnload(g.mod);
     memset(&g, 0, sizeof g);
@@ -379,6 +414,7 @@ void sllm_gfx950_close(void) {
         hipEventDestroy(g.ev_start);
         hipEventDestroy(g.ev_stop);
         hipStreamDestroy(g.stream);
+        hipModuleUnload(g.attn_mod);
         hipModuleUnload(g.dec_mod);
         hipModuleUnload(g.mod);
         memset(&g, 0, sizeof g);
@@ -528,6 +564,8 @@ int sllm_shim_decode_function(const char *name, hipFunction_t *f) {
     HIP_TRY(hipModuleGetFunction(f, g.dec_mod, name));
     return SLLM_GFX950_OK;
 }
+
+hipFunction_t sllm_shim_attn_function(int i) { return g.k_attn[i]; }
 
 int sllm_shim_launch(hipFunction_t f, uint32_t gx, uint32_t gy, uint32_t block, uint32_t lds, void **args) {
     if (gx == 0 || gy == 0) return SLLM_GFX950_OK;
