@@ -226,7 +226,7 @@ static int new_sequences(sllm_gfx950_pages *p, int32_t n, int32_t *ids) {
         while (got-- > 0) p->seq[ids[got]].used = 0;
         return 0;
     }
-    p->low_seq = at + 1;
+    if (n > 0) p->low_seq = at + 1;
     return 1;
 }
 
