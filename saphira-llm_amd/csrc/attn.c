@@ -474,8 +474,6 @@ int sllm_gfx950_pages_compact(sllm_gfx950_pages *p, int32_t *n_moved) {
 /* a batch                                                             */
 /* ------------------------------------------------------------------ */
 
-enum { FEW, SOME, ROWS, N_MODES };
-
 /* workgroups of a launch: their threads fit 32 bits */
 #define MAX_ITEMS ((size_t) 1 << 23)
 
@@ -496,10 +494,10 @@ struct sllm_gfx950_batch {
     sllm_gfx950_pages *p;
     int32_t   n_head, pair;
     uint32_t  n_tok;
-    uint32_t  n_items[N_MODES];
+    uint32_t  n_items;
     int       join;                  /* a row has partial results */
     buffer    buf;
-    size_t    off_items[N_MODES], off_tables, off_list, off_tok_seq, off_seqs, off_segs, off_part_o, off_part_ml;
+    size_t    off_tables, off_list, off_toks, off_segs, off_part_o, off_part_ml;     /* (its items are at 0) */
     int32_t  *held;                  /* the pages it holds */
     int32_t   n_held;
 };
@@ -508,8 +506,8 @@ struct sllm_gfx950_batch {
 typedef struct segment {
     int32_t  lo, hi;
     int32_t  page0, n_keys;          /* from page page0 of each of their tables */
-    uint32_t n_tok, list, part0, n_split;
-    int      mode;
+    uint32_t n_tok, list, part0, n_split, split;
+    uint32_t mode;
 } segment;
 
 typedef struct plan {
@@ -573,21 +571,31 @@ static int by_table(const void *a, const void *b) {
     return ia < ib ? -1 : ia > ib;
 }
 
-static int mode_of(uint32_t rows) { return rows <= ATT_FEW_ROWS ? FEW : rows <= ATT_SOME_ROWS ? SOME : ROWS; }
+static uint32_t mode_of(uint32_t rows) { return rows <= ATT_FEW_ROWS ? ATT_FEW : rows <= ATT_SOME_ROWS ? ATT_SOME : ATT_MANY; }
+
+/* the dearest first */
+static int by_work(const void *a, const void *b) {
+    const att_item *x = a, *y = b;
+    if (x->mode != y->mode) return x->mode > y->mode ? -1 : 1;
+    const uint32_t n = x->key1 > x->key0 ? x->key1 - x->key0 : 0, m = y->key1 > y->key0 ? y->key1 - y->key0 : 0;
+    if (n != m) return n > m ? -1 : 1;
+    return x->part != y->part ? (x->part < y->part ? -1 : 1) : x->row0 != y->row0 ? (x->row0 < y->row0 ? -1 : 1) :
+           x->tok0 != y->tok0 ? (x->tok0 < y->tok0 ? -1 : 1) : x->head < y->head ? -1 : x->head > y->head;
+}
 
 /*
  * A split's keys: as many as give every CU two workgroups over the whole
  * step, a multiple of SPLIT_KEYS and at least LEAST_SPLIT. Shorter ones would
  * cost more in partial results than the idle CUs they fill.
  */
-#define SPLIT_KEYS  128u
-#define LEAST_SPLIT 256u
+#define SPLIT_KEYS  64u
+#define LEAST_SPLIT 128u
 
 static uint32_t split_keys(const plan *x, uint32_t group, uint32_t n_head_kv) {
     uint64_t work = 0;
     for (int32_t i = 0; i < x->n_seg; ++i) {
         const segment *s = &x->seg[i];
-        const uint64_t tiles = s->mode == ROWS ? ((uint64_t) s->n_tok * group + ATT_ROWS - 1) / ATT_ROWS : 1;
+        const uint64_t tiles = s->mode == ATT_MANY ? ((uint64_t) s->n_tok * group + ATT_ROWS - 1) / ATT_ROWS : 1;
         work += tiles * (uint64_t) s->n_keys * n_head_kv;
     }
     const uint64_t wgs = 2u * (uint64_t) sllm_shim_cu();
@@ -648,7 +656,7 @@ static int lay_out(sllm_gfx950_batch *b, plan *x, int32_t n, const int32_t *len0
     sllm_gfx950_pages *p = b->p;
     const uint32_t kv = (uint32_t) p->d.n_head_kv, group = (uint32_t) b->n_head / kv;
     const uint32_t hd_pad = p->d.head_dim <= 64 ? 64 : 128;
-    items it[N_MODES] = { { 0 } };
+    items it = { 0 };
     int st = SLLM_GFX950_OK;
 
     /* like tables side by side, and how far each goes with the one before it:
@@ -681,6 +689,9 @@ static int lay_out(sllm_gfx950_batch *b, plan *x, int32_t n, const int32_t *len0
     for (int32_t i = 0; i < x->n_seg; ++i) {
         segment *s = &x->seg[i];
         s->n_split = ((uint32_t) s->n_keys + split - 1) / split;
+        s->split = ((uint32_t) s->n_keys + s->n_split - 1) / s->n_split;        /* evenly */
+        s->split = (s->split + SPLIT_KEYS - 1) / SPLIT_KEYS * SPLIT_KEYS;
+        s->n_split = ((uint32_t) s->n_keys + s->split - 1) / s->split;
         for (int32_t j = s->lo; j < s->hi; ++j) ++seg_count[x->order[j]];
     }
     for (int32_t i = 0; i < x->n_seg; ++i) {
@@ -700,42 +711,38 @@ static int lay_out(sllm_gfx950_batch *b, plan *x, int32_t n, const int32_t *len0
     }
     b->join = n_part > 0;
 
-    /* the work, longest first within a mode's launch */
+    /* the work */
     for (int32_t i = 0; i < x->n_seg && st == SLLM_GFX950_OK; ++i) {
         const segment *s = &x->seg[i];
         const int32_t q = x->order[s->lo];
-        const uint32_t rows = s->n_tok * group, tile = s->mode == ROWS ? ATT_ROWS : ATT_SOME_ROWS;
+        const uint32_t rows = s->n_tok * group, tile = s->mode == ATT_MANY ? ATT_ROWS : ATT_SOME_ROWS;
         const int own = s->hi - s->lo == 1;
         const int32_t vis0 = own ? len0[q] - (s->page0 << p->page_shift) + 1 : ATT_SEE_ALL;
         for (uint32_t k = 0; k < s->n_split && st == SLLM_GFX950_OK; ++k) {
             for (uint32_t r = 0; r < rows && st == SLLM_GFX950_OK; r += tile) {
                 const uint32_t nr = rows - r < tile ? rows - r : tile;
                 const uint64_t sees = (uint64_t) vis0 + (r + nr - 1) / group;
-                uint32_t key0 = k * split, key1 = (uint32_t) s->n_keys < key0 + split ? (uint32_t) s->n_keys : key0 + split;
+                uint32_t key0 = k * s->split, key1 = (uint32_t) s->n_keys < key0 + s->split ? (uint32_t) s->n_keys : key0 + s->split;
                 if (key1 > sees) key1 = (uint32_t) sees;
                 for (uint32_t h = 0; h < kv; ++h) {
-                    att_item *a = items_add(&it[s->mode]);
+                    att_item *a = items_add(&it);
                     if (a == NULL) { st = FAIL_NOMEM("batch_create: work items"); break; }
                     *a = (att_item) { r, nr, own ? x->tok0[q] : 0, s->list, vis0, key0, key1,
                                       x->table[q] + (uint32_t) s->page0, h,
-                                      alone[q] ? ATT_DIRECT : s->part0 + (h * s->n_split + k) * rows + r };
+                                      alone[q] ? ATT_DIRECT : s->part0 + (h * s->n_split + k) * rows + r, s->mode, 0 };
                 }
             }
         }
     }
-    for (int m = 0; m < N_MODES && st == SLLM_GFX950_OK; ++m) if (it[m].n > MAX_ITEMS) st = FAIL_ARG("batch_create: too much work for a launch");
+    if (st == SLLM_GFX950_OK && it.n > MAX_ITEMS) st = FAIL_ARG("batch_create: too much work for a launch");
     if (st != SLLM_GFX950_OK) goto out;
+    if (it.n > 0) qsort(it.v, it.n, sizeof *it.v, by_work);
 
-    size_t at = 0;
-    for (int m = 0; m < N_MODES; ++m) {
-        b->n_items[m] = (uint32_t) it[m].n;
-        b->off_items[m] = at;
-        at = align256(at + it[m].n * sizeof(att_item));
-    }
+    b->n_items = (uint32_t) it.n;
+    size_t at = align256(it.n * sizeof(att_item));
     b->off_tables = at;  at = align256(at + n_pages * 4);
     b->off_list = at;    at = align256(at + n_list * 4);
-    b->off_tok_seq = at; at = align256(at + (size_t) b->n_tok * 4);
-    b->off_seqs = at;    at = align256(at + (size_t) n * sizeof(att_seq));
+    b->off_toks = at;    at = align256(at + (size_t) b->n_tok * sizeof(att_tok));
     b->off_segs = at;    at = align256(at + n_segs * sizeof(att_seg));
     const size_t sent = at;
     b->off_part_ml = at; at = align256(at + n_part * 8);
@@ -743,25 +750,25 @@ static int lay_out(sllm_gfx950_batch *b, plan *x, int32_t n, const int32_t *len0
     if ((st = buffer_get(p, &b->buf, at + 256, sent + 256)) != SLLM_GFX950_OK) goto out;
 
     uint8_t *to = b->buf.pin;
-    for (int m = 0; m < N_MODES; ++m) if (it[m].n) memcpy(to + b->off_items[m], it[m].v, it[m].n * sizeof(att_item));
+    if (it.n > 0) memcpy(to, it.v, it.n * sizeof(att_item));
     uint32_t *tables = (uint32_t *) (to + b->off_tables), *list = (uint32_t *) (to + b->off_list);
-    uint32_t *tok_seq = (uint32_t *) (to + b->off_tok_seq);
-    att_seq *seqs = (att_seq *) (to + b->off_seqs);
+    att_tok *toks = (att_tok *) (to + b->off_toks);
     att_seg *segs = (att_seg *) (to + b->off_segs);
-    for (int32_t i = 0; i < n; ++i) {
-        const sequence *s = &p->seq[x->seqs[i]];
-        if (s->n_pages > 0) memcpy(tables + x->table[i], s->page, (size_t) s->n_pages * 4);
-        for (int32_t t = 0; t < x->n_new[i]; ++t) tok_seq[x->tok0[i] + (uint32_t) t] = (uint32_t) i;
-        seqs[i] = (att_seq) { x->tok0[i], (uint32_t) x->n_new[i], x->table[i], (uint32_t) len0[i], seg_at[i], 0 };
-    }
     for (int32_t i = 0; i < x->n_seg; ++i) {
         const segment *s = &x->seg[i];
         uint32_t t = 0;
         for (int32_t j = s->lo; j < s->hi; ++j) {
             const int32_t q = x->order[j];
-            if (!alone[q]) segs[seqs[q].seg0 + seqs[q].n_seg++] = (att_seg) { s->part0, s->n_tok * group, s->n_split, t * group };
+            if (!alone[q]) segs[seg_at[q] + seg_count[q]++] = (att_seg) { s->part0, s->n_tok * group, s->n_split, t * group };
             for (int32_t k = 0; k < x->n_new[q] && s->list != ATT_TOKENS; ++k) list[s->list + t + (uint32_t) k] = x->tok0[q] + (uint32_t) k;
             t += (uint32_t) x->n_new[q];
+        }
+    }
+    for (int32_t i = 0; i < n; ++i) {
+        const sequence *s = &p->seq[x->seqs[i]];
+        if (s->n_pages > 0) memcpy(tables + x->table[i], s->page, (size_t) s->n_pages * 4);
+        for (int32_t t = 0; t < x->n_new[i]; ++t) {
+            toks[x->tok0[i] + (uint32_t) t] = (att_tok) { x->table[i], (uint32_t) (len0[i] + t), seg_at[i], seg_count[i], (uint32_t) t, { 0 } };
         }
     }
     if (sent > 0) {
@@ -774,7 +781,7 @@ static int lay_out(sllm_gfx950_batch *b, plan *x, int32_t n, const int32_t *len0
         }
     }
 out:
-    for (int m = 0; m < N_MODES; ++m) free(it[m].v);
+    free(it.v);
     free(seg_count);
     free(seg_at);
     free(alone);
@@ -924,8 +931,7 @@ int sllm_gfx950_batch_store(sllm_gfx950_batch *b, int32_t layer, const void *k, 
     if (k == NULL || v == NULL || misaligned(k) || misaligned(v)) return FAIL_ARG("batch_store: NULL or misaligned rows");
     uint8_t *layer_mem = p->mem + (uint64_t) layer * p->layer_bytes;
     att_store_args a = { k, v, layer_mem, layer_mem + (uint64_t) kv * p->block_bytes,
-                         (const uint32_t *) (b->buf.dev + b->off_tables), (const uint32_t *) (b->buf.dev + b->off_tok_seq),
-                         (const att_seq *) (b->buf.dev + b->off_seqs), kt, vt, p->page_bytes, p->page_shift, hd, kv, b->n_tok };
+                         (const uint32_t *) (b->buf.dev + b->off_tables), (const att_tok *) (b->buf.dev + b->off_toks), kt, vt, p->page_bytes, p->page_shift, hd, kv, b->n_tok };
     void *args[] = { &a };
     const uint64_t threads = (uint64_t) b->n_tok * (hd / 8u);
     return sllm_shim_launch(sllm_shim_attn_function(SLLM_ATTN_STORE + (b->pair < 2 ? b->pair : 2)),
@@ -950,7 +956,7 @@ int sllm_gfx950_batch_attend(sllm_gfx950_batch *b, int32_t layer, const void *q,
     uint8_t *dev = b->buf.dev;
     const uint8_t *layer_mem = p->mem + (uint64_t) layer * p->layer_bytes;
     att_args a = { .q = q, .out = out, .k = layer_mem, .v = layer_mem + (uint64_t) kv * p->block_bytes,
-                   .tables = (const uint32_t *) (dev + b->off_tables), .list = (const uint32_t *) (dev + b->off_list),
+                   .items = (const att_item *) dev, .n_items = b->n_items, .tables = (const uint32_t *) (dev + b->off_tables), .list = (const uint32_t *) (dev + b->off_list),
                    .part_o = (float *) (dev + b->off_part_o), .part_ml = (float *) (dev + b->off_part_ml),
                    .q_tok = qt, .q_head = (uint64_t) hd * size, .out_tok = ot, .out_head = (uint64_t) hd * size,
                    .page_bytes = p->page_bytes, .page_shift = p->page_shift, .hd = hd, .group = group,
@@ -958,19 +964,14 @@ int sllm_gfx950_batch_attend(sllm_gfx950_batch *b, int32_t layer, const void *q,
     /* the partial results are one set of memory: a call's launches stay together */
     pthread_mutex_lock(&p->mtx);
     int st = SLLM_GFX950_OK;
-    for (int m = 0; m < N_MODES && st == SLLM_GFX950_OK; ++m) {
-        a.items = (const att_item *) (dev + b->off_items[m]);
-        a.n_items = b->n_items[m];
-        void *args[] = { &a };
-        st = sllm_shim_launch(sllm_shim_attn_function(SLLM_ATTN_ATTEND + (b->pair * 2 + (int) wide) * 3 + m), a.n_items, 1, ATT_THREADS, 0, args);
-    }
+    void *args[] = { &a };
+    st = sllm_shim_launch(sllm_shim_attn_function(SLLM_ATTN_ATTEND + b->pair * 2 + (int) wide), a.n_items, 1, ATT_THREADS, 0, args);
     if (st == SLLM_GFX950_OK && b->join) {
-        att_join_args j = { out, a.part_o, a.part_ml, (const uint32_t *) (dev + b->off_tok_seq), (const att_seq *) (dev + b->off_seqs),
-                            (const att_seg *) (dev + b->off_segs), ot, hd, wide ? 128 : 64, group, (uint32_t) b->n_head, b->n_tok, 0 };
-        void *args[] = { &j };
-        const uint64_t waves = (uint64_t) b->n_tok * (uint64_t) b->n_head;
-        st = sllm_shim_launch(sllm_shim_attn_function(SLLM_ATTN_JOIN + (b->pair < 2 ? 0 : b->pair - 1)),
-                              (uint32_t) ((waves + ATT_THREADS / 64 - 1) / (ATT_THREADS / 64)), 1, ATT_THREADS, 0, args);
+        att_join_args j = { out, a.part_o, a.part_ml, (const att_tok *) (dev + b->off_toks), (const att_seg *) (dev + b->off_segs), ot,
+                            hd, group };
+        void *jargs[] = { &j };
+        st = sllm_shim_launch(sllm_shim_attn_function(SLLM_ATTN_JOIN + (b->pair < 2 ? 0 : b->pair - 1) * 2 + (int) wide),
+                              b->n_tok, (uint32_t) b->n_head, ATT_THREADS, 0, jargs);
     }
     pthread_mutex_unlock(&p->mtx);
     return st;
@@ -1026,7 +1027,7 @@ int sllm_gfx950_prompt_create(const sllm_gfx950_prompt_desc *d, sllm_gfx950_prom
                 att_item *a = items_add(&it);
                 if (a == NULL) { st = FAIL_NOMEM("prompt_create: work items"); break; }
                 *a = (att_item) { r, n, (uint32_t) p->n_q, ATT_TOKENS, nk - nq + 1, 0, last > 0 ? (uint32_t) last : 0,
-                                  (uint32_t) p->n_k, (uint32_t) h, ATT_DIRECT };
+                                  (uint32_t) p->n_k, (uint32_t) h, ATT_DIRECT, ATT_MANY, 0 };
             }
         }
         p->n_q += (uint64_t) nq;
@@ -1071,7 +1072,7 @@ static int strides(size_t tok, size_t head, uint64_t heads, uint64_t hd, uint64_
         tok = (size_t) (heads * hd);
         head = (size_t) hd;
     }
-    if (tok > (1u << 28) || (uint64_t) head > 1ull << 40 || tok * size % 16u != 0 || head * size % 16u != 0) return 0;
+    if (tok > (1u << 25) || (uint64_t) head > 1ull << 40 || tok * size % 16u != 0 || head * size % 16u != 0) return 0;
     *t = (uint64_t) tok * size;
     *h = (uint64_t) head * size;
     *extent = n == 0 ? 0 : (n - 1) * *t + (heads - 1) * *h + hd * size;

@@ -29,12 +29,12 @@ typedef short s16x4 __attribute__((ext_vector_type(4)));
 // counter too: these name the address space.
 #define GLOBAL __attribute__((address_space(1)))
 #define G_CAST(T, p) ((GLOBAL T *) (p))
+// Tables that no kernel writes: with an address that is the same for the whole
+// wave these are scalar loads, which do not queue behind the tiles' copies.
+#define C_CAST(T, p) ((__attribute__((address_space(4))) const T *) (p))
 #define LDS_PTR(p) ((__attribute__((address_space(3))) void *) (p))
 
 constexpr int WAVES = 4;
-
-// what keys past the end and dimensions past head_dim are read from
-__device__ __attribute__((aligned(16))) uint32_t att_zeros[4];
 
 template <int N> __device__ __forceinline__ void wait_vmem() {   // s_waitcnt vmcnt(N), the other counters untouched
     static_assert(N >= 0 && N < 64, "vmcnt");
@@ -86,7 +86,7 @@ template <typename T, int D, bool KEYS> struct tile {
     static constexpr int CH = ROWB / 16;
     static constexpr int HALF = KT * ROWB;
     static constexpr int BYTES = 2 * HALF;
-    static constexpr int STAGES = 2;
+    static constexpr int STAGES = KEYS ? 1 : 2;
     static constexpr int LDS = BYTES * STAGES * (KEYS ? WAVES : 1);
     static __device__ __forceinline__ uint32_t ksw(uint32_t r) { return !WIDE && CH == 16 ? r & 15u : r & 7u; }
     static __device__ __forceinline__ uint32_t vsw(uint32_t r) {
@@ -113,10 +113,40 @@ struct attention {
     static constexpr int RPI = 1024 / L::ROWB;                   // rows of a copy instruction
     typedef typename vec8<T>::type t8;
 
+    static constexpr int COPIES = GROUP / RPI;                   // instructions of a group, for keys and for values
+    static constexpr int DA = WIDE ? 4 : 2;                      // 16-byte pieces of 16 dimensions
+
     const att_args &a;
     const att_item it;
     uint8_t *S;
     uint32_t lane, wave, g, li;
+
+    // What a lane adds to a tile's place in LDS, once for all tiles. Keys: row li of a
+    // 16-key subtile, piece 4 q + g; the row's swap is the same in every subtile.
+    // Values: dimension tile 0 of row 4 g (16 bits: 4 g + li / 4, of the transposing
+    // read; f32: 4 g + i, a row further each); dimension tile dt is at ^ dt * 16 DA.
+    uint32_t koff[QC], voff;
+    // a lane's place in the rows that a copy instruction fills, or past any end where
+    // the row has no such piece
+    uint32_t kcopy[COPIES], vcopy[COPIES];
+
+    __device__ __forceinline__ void places() {
+#pragma unroll
+        for (int q = 0; q < QC; ++q) koff[q] = li * L::ROWB + (((4u * q + g) ^ L::ksw(li)) * 16u);
+        const uint32_t r = WIDE ? 4u * g : 4u * g + (li >> 2);
+        voff = L::HALF + r * L::ROWB + (WIDE ? ((li >> 2) ^ L::vsw(r)) * 16u + (li & 3u) * 4u
+                                             : (((li >> 1) & 1u) ^ L::vsw(r)) * 16u + (li & 1u) * 8u);
+        const uint32_t rowk = PAGED ? a.hd * (uint32_t) sizeof(T) : (uint32_t) a.k_tok;
+        const uint32_t rowv = PAGED ? rowk : (uint32_t) a.v_tok;
+#pragma unroll
+        for (int j = 0; j < COPIES; ++j) {
+            const uint32_t rg = (uint32_t) j * RPI + lane / L::CH, ch = lane % L::CH;
+            const uint32_t rt = (KEYS ? 0u : wave * (uint32_t) GROUP) + rg;        // (groups are 16 rows apart: the same swaps)
+            const uint32_t ck = (ch ^ L::ksw(rt)) * 16u, cv = (ch ^ L::vsw(rt)) * 16u;
+            kcopy[j] = ck < a.hd * (uint32_t) sizeof(T) ? rg * rowk + ck : 0xfffffff0u;
+            vcopy[j] = cv < a.hd * (uint32_t) sizeof(T) ? rg * rowv + cv : 0xfffffff0u;
+        }
+    }
 
     // rows: lane li of row tile nt
     int lim[NT];                    // keys the row sees
@@ -198,37 +228,35 @@ struct attention {
         }
     }
 
-    // Copy a tile's keys and values into `to` (this wave's rows of it).
-    __device__ __forceinline__ void issue(uint32_t t, uint8_t *to) const {
-        const uint8_t *zero = (const uint8_t *) att_zeros;
-        const uint32_t rowk = PAGED ? a.hd * (uint32_t) sizeof(T) : (uint32_t) a.k_tok;
-        const uint32_t rowv = PAGED ? rowk : (uint32_t) a.v_tok;
+    // Copy a tile's keys and values into the stage at `to` (this wave's rows of it),
+    // straight to LDS. The buffers end behind the range's last key: what lies past it,
+    // and past head_dim, arrives as zeros.
+    __device__ __forceinline__ void issue(uint32_t t, uint32_t to) const {
+        const uint32_t row = a.hd * (uint32_t) sizeof(T);
+        const uint32_t rowk = PAGED ? row : (uint32_t) a.k_tok, rowv = PAGED ? row : (uint32_t) a.v_tok;
 #pragma unroll
         for (int gr = 0; gr < GROUPS; ++gr) {
             const uint32_t r0 = (KEYS ? 0u : wave * (uint32_t) GROUP) + (uint32_t) gr * GROUP;      // row in the tile
             const uint32_t key = t * KT + r0;
+            const uint32_t n = key < it.key1 ? min(it.key1 - key, (uint32_t) GROUP) : 0u;
             const uint8_t *kb, *vb;
             if constexpr (PAGED) {
                 const uint32_t at = min(key, it.key1 - 1u);
-                const uint32_t page = uniform(*G_CAST(const uint32_t, a.tables + it.kv + (at >> a.page_shift)));
-                const uint64_t off = page * a.page_bytes + ((uint64_t) (it.head << a.page_shift) + (at & ((1u << a.page_shift) - 1u) & ~(uint32_t) (GROUP - 1))) * rowk;
+                const uint32_t page = *C_CAST(uint32_t, a.tables + it.kv + (at >> a.page_shift));
+                const uint64_t off = page * a.page_bytes + ((uint64_t) (it.head << a.page_shift) + (at & ((1u << a.page_shift) - 1u) & ~(uint32_t) (GROUP - 1))) * row;
                 kb = a.k + off;
                 vb = a.v + off;
             } else {
                 kb = a.k + (uint64_t) (it.kv + key) * a.k_tok + it.head * a.k_head;
                 vb = a.v + (uint64_t) (it.kv + key) * a.v_tok + it.head * a.v_head;
             }
+            const __amdgpu_buffer_rsrc_t rk = __builtin_amdgcn_make_buffer_rsrc((void *) kb, (short) 0, (int) uniform(n ? n * rowk - (rowk - row) : 0u), 0x00020000);
+            const __amdgpu_buffer_rsrc_t rv = __builtin_amdgcn_make_buffer_rsrc((void *) vb, (short) 0, (int) uniform(n ? n * rowv - (rowv - row) : 0u), 0x00020000);
+            uint8_t *dst = S + to + r0 * L::ROWB;
 #pragma unroll
-            for (int j = 0; j < GROUP / RPI; ++j) {
-                const uint32_t rg = (uint32_t) j * RPI + lane / L::CH, r = r0 + rg, ch = lane % L::CH;
-                const uint32_t ck = ch ^ L::ksw(r), cv = ch ^ L::vsw(r);
-                const bool in = t * KT + r < it.key1;
-                const uint8_t *ks = in && ck * 16u < a.hd * (uint32_t) sizeof(T) ? kb + (uint64_t) rg * rowk + ck * 16u : zero;
-                const uint8_t *vs = in && cv * 16u < a.hd * (uint32_t) sizeof(T) ? vb + (uint64_t) rg * rowv + cv * 16u : zero;
-                uint8_t *dst = to + (r0 + (uint32_t) j * RPI) * L::ROWB;
-                __builtin_amdgcn_global_load_lds((const void *) ks, LDS_PTR(dst), 16, 0, 0);
-                __builtin_amdgcn_global_load_lds((const void *) vs, LDS_PTR(dst + L::HALF), 16, 0, 0);
-            }
+            for (int j = 0; j < COPIES; ++j) __builtin_amdgcn_raw_ptr_buffer_load_lds(rk, LDS_PTR(dst + j * 1024), 16, kcopy[j], 0, 0, 0);
+#pragma unroll
+            for (int j = 0; j < COPIES; ++j) __builtin_amdgcn_raw_ptr_buffer_load_lds(rv, LDS_PTR(dst + L::HALF + j * 1024), 16, vcopy[j], 0, 0, 0);
         }
     }
 
@@ -240,26 +268,24 @@ struct attention {
     // not reach rows that do not see its key (0 times it is NaN): such values
     // are left out of the products and added to the rows that see them.
     template <bool SEEN, bool CAREFUL>
-    __device__ __forceinline__ void step(uint32_t t, const uint8_t *tl) {
+    __device__ __forceinline__ void step(uint32_t t, uint32_t tl) {
         f32x4 s[KS][NT];
 #pragma unroll
         for (int ks = 0; ks < KS; ++ks) {
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt) s[ks][nt] = (f32x4) { 0, 0, 0, 0 };
-            const uint32_t r = 16u * ks + li;
-            const uint8_t *row = tl + r * L::ROWB;
 #pragma unroll
             for (int q = 0; q < QC; ++q) {
-                const uint8_t *src = row + (((4u * q + g) ^ L::ksw(r)) * 16u);
+                const uint32_t src = tl + koff[q] + 16u * ks * L::ROWB;
                 if constexpr (WIDE) {
-                    const f32x4 kf = *reinterpret_cast<const f32x4 *>(src);
+                    const f32x4 kf = *reinterpret_cast<const f32x4 *>(S + src);
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
 #pragma unroll
                         for (int nt = 0; nt < NT; ++nt) s[ks][nt] = mfma(kf[e], qw[nt][q][e], s[ks][nt]);
                     }
                 } else {
-                    const t8 kf = *reinterpret_cast<const t8 *>(src);
+                    const t8 kf = *reinterpret_cast<const t8 *>(S + src);
 #pragma unroll
                     for (int nt = 0; nt < NT; ++nt) s[ks][nt] = mfma(kf, qf[nt][q], s[ks][nt]);
                     if constexpr (SPLIT) {
@@ -269,6 +295,7 @@ struct attention {
                 }
             }
         }
+        __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
             float top = m[nt];
@@ -301,17 +328,18 @@ struct attention {
             }
             l[nt] += sum;
         }
-        const uint8_t *tv = tl + L::HALF;
+        __builtin_amdgcn_sched_barrier(0);
         if constexpr (WIDE) {
 #pragma unroll
             for (int ks = 0; ks < KS; ++ks) {
+                __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                    const uint32_t r = 16u * ks + 4u * g + i;
 #pragma unroll
                     for (int dt = 0; dt < DT; ++dt) {
-                        const uint32_t ch = (4u * dt + (li >> 2)) ^ L::vsw(r);
-                        float vf = *reinterpret_cast<const float *>(tv + r * L::ROWB + ch * 16u + (li & 3u) * 4u);
+                        // (rows 16 further on have the swap of four 16-dimension tiles further, where rows are that long)
+                        const uint32_t at = (tl + voff) ^ (((uint32_t) dt ^ (L::CH == 32 ? 4u * (ks & 1) : 0u)) * 16u * DA);
+                        float vf = *reinterpret_cast<const float *>(S + at + (16u * ks + i) * L::ROWB);
                         if (CAREFUL) vf = odd(vf) ? 0.0f : vf;
 #pragma unroll
                         for (int nt = 0; nt < NT; ++nt) o[dt][nt] = mfma(vf, s[ks][nt][i], o[dt][nt]);
@@ -322,6 +350,7 @@ struct attention {
             // 32 keys at a time: a lane's operand holds keys 4 g + 0..3 of both 16-key subtiles
 #pragma unroll
             for (int u = 0; u < KS / 2; ++u) {
+                __builtin_amdgcn_sched_barrier(0);
                 t8 p[NT], pl[SPLIT ? NT : 1];
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt) {
@@ -337,10 +366,8 @@ struct attention {
                     s16x4 h[2];
 #pragma unroll
                     for (int i = 0; i < 2; ++i) {
-                        const uint32_t r = 32u * u + 16u * i + 4u * g + (li >> 2);
-                        const uint32_t ch = (2u * dt + ((li >> 1) & 1u)) ^ L::vsw(r);
-                        h[i] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-                            (__attribute__((address_space(3))) s16x4 *) (tv + r * L::ROWB + ch * 16u + (li & 1u) * 8u));
+                        const uint32_t at = ((tl + voff) ^ (uint32_t) dt * 16u * DA) + (32u * u + 16u * i) * L::ROWB;
+                        h[i] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4 *) (S + at));
                     }
                     t8 vf = __builtin_bit_cast(t8, __builtin_shufflevector(h[0], h[1], 0, 1, 2, 3, 4, 5, 6, 7));
                     if (CAREFUL) {
@@ -357,7 +384,7 @@ struct attention {
         }
         if (CAREFUL) {
             for (uint32_t r = 0; r < (uint32_t) KT; ++r) {
-                const uint8_t *row = tv + r * L::ROWB;
+                const uint8_t *row = S + tl + L::HALF + r * L::ROWB;
 #pragma unroll
                 for (int dt = 0; dt < DT; ++dt) {
 #pragma unroll
@@ -375,7 +402,7 @@ struct attention {
     }
 
     template <bool CAREFUL>
-    __device__ __forceinline__ void tile_step(uint32_t t, const uint8_t *tl) {
+    __device__ __forceinline__ void tile_step(uint32_t t, uint32_t tl) {
         if ((int) (t * KT) >= lim_max) return;                   // none of the wave's rows sees it
         if ((int) (t * KT + KT) <= lim_min) step<true, false>(t, tl);
         else step<false, CAREFUL>(t, tl);
@@ -394,9 +421,20 @@ struct attention {
         const uint32_t t1 = (it.key1 + KT - 1u) / KT;
         constexpr uint32_t STEP = KEYS ? WAVES : 1;
         uint32_t t = it.key0 / KT + (KEYS ? wave : 0u);
-        uint8_t *buf = S + (KEYS ? wave * (uint32_t) (L::BYTES * L::STAGES) : 0u);
+        const uint32_t buf = KEYS ? wave * (uint32_t) (L::BYTES * L::STAGES) : 0u;
         if (it.key0 >= it.key1) return;
         if (t < t1) issue(t, buf);
+        if constexpr (L::STAGES == 1) {
+            for (; t < t1; t += STEP) {
+                wait_vmem<0>();
+                __builtin_amdgcn_sched_barrier(0);
+                tile_step<CAREFUL>(t, buf);
+                __builtin_amdgcn_s_waitcnt(0xC07F);              // the tile is read
+                __builtin_amdgcn_sched_barrier(0);
+                if (t + STEP < t1) issue(t + STEP, buf);
+            }
+            return;
+        }
         for (uint32_t n = 0; t < t1; t += STEP, ++n) {
             wait_vmem<0>();
             __builtin_amdgcn_s_waitcnt(0xC07F);                  // this wave's reads of the other stage are done
@@ -449,6 +487,7 @@ struct attention {
     }
 
     __device__ __forceinline__ void run() {
+        places();
         load_q();
         pass<false>();
         // 0 x inf in a key that a row does not see: only then is anything not finite
@@ -512,75 +551,126 @@ struct attention {
 };
 
 template <typename A, typename T, int D, int NT, bool KEYS, bool PAGED>
-__device__ __forceinline__ void attend_body(const att_args &a) {
-    typedef attention<A, T, D, NT, KEYS, PAGED> att;
-    constexpr int JOIN = KEYS ? WAVES * 16 * NT * (D + 2) * 4 : 0;
-    __shared__ __attribute__((aligned(1024))) uint8_t S[att::L::LDS > JOIN ? att::L::LDS : JOIN];
-    const att_item it = a.items[blockIdx.x];
+__device__ __forceinline__ void attend_item(const att_args &a, const att_item &it, uint8_t *S) {
     const uint32_t lane = threadIdx.x & 63u;
-    att x = { a, it, S, lane, uniform(threadIdx.x >> 6), lane >> 4, lane & 15u };
+    attention<A, T, D, NT, KEYS, PAGED> x = { a, it, S, lane, uniform(threadIdx.x >> 6), lane >> 4, lane & 15u };
     x.run();
+}
+
+constexpr int max_of(int a, int b) { return a > b ? a : b; }
+
+__device__ __forceinline__ att_item item_of(const att_args &a) {
+    att_item it;
+    uint32_t w[sizeof(att_item) / 4];
+#pragma unroll
+    for (uint32_t i = 0; i < sizeof(att_item) / 4; ++i) w[i] = C_CAST(uint32_t, a.items + blockIdx.x)[i];
+    __builtin_memcpy(&it, w, sizeof it);
+    return it;
+}
+
+template <typename T, int D>
+__device__ __forceinline__ void prompt_body(const att_args &a) {
+    __shared__ __attribute__((aligned(1024))) uint8_t S[tile<T, D, false>::LDS];
+    attend_item<T, T, D, 2, false, false>(a, item_of(a), S);
+}
+
+template <typename A, typename T, int D>
+__device__ __forceinline__ void paged_body(const att_args &a) {
+    __shared__ __attribute__((aligned(1024))) uint8_t S[max_of(max_of(tile<T, D, false>::LDS, tile<T, D, true>::LDS), WAVES * 32 * (D + 2) * 4)];
+    const att_item it = item_of(a);
+    if (it.mode == ATT_FEW) attend_item<A, T, D, 1, true, true>(a, it, S);
+    else if (it.mode == ATT_SOME) attend_item<A, T, D, 2, true, true>(a, it, S);
+    else attend_item<A, T, D, 2, false, true>(a, it, S);
 }
 
 }  // namespace
 
-#define ATTEND(name, A, T, D, NT, KEYS, PAGED, PER_CU)                                     \
-    extern "C" __global__ void __launch_bounds__(ATT_THREADS, PER_CU) name(const att_args a) { \
-        attend_body<A, T, D, NT, KEYS, PAGED>(a);                                          \
-    }
-#define ATTEND_PAGED(types, A, T)                                          \
-    ATTEND(sllm_k_attend_##types##_64_few, A, T, 64, 1, true, true, 1)     \
-    ATTEND(sllm_k_attend_##types##_64_some, A, T, 64, 2, true, true, 1)    \
-    ATTEND(sllm_k_attend_##types##_64_rows, A, T, 64, 2, false, true, 1)   \
-    ATTEND(sllm_k_attend_##types##_128_few, A, T, 128, 1, true, true, 1)   \
-    ATTEND(sllm_k_attend_##types##_128_some, A, T, 128, 2, true, true, 1)  \
-    ATTEND(sllm_k_attend_##types##_128_rows, A, T, 128, 2, false, true, 1)
-#define ATTEND_PROMPT(type, T)                                             \
-    ATTEND(sllm_k_prompt_##type##_64, T, T, 64, 2, false, false, 1)        \
-    ATTEND(sllm_k_prompt_##type##_128, T, T, 128, 2, false, false, 1)
+#define PROMPT(name, T, D) extern "C" __global__ void __launch_bounds__(ATT_THREADS, 2) name(const att_args a) { prompt_body<T, D>(a); }
+#define PAGED(name, A, T, D) extern "C" __global__ void __launch_bounds__(ATT_THREADS, 2) name(const att_args a) { paged_body<A, T, D>(a); }
 
-ATTEND_PAGED(f32, float, float)
-ATTEND_PAGED(f32f16, float, _Float16)
-ATTEND_PAGED(f16, _Float16, _Float16)
-ATTEND_PAGED(bf16, __bf16, __bf16)
-ATTEND_PROMPT(f32, float)
-ATTEND_PROMPT(f16, _Float16)
-ATTEND_PROMPT(bf16, __bf16)
+PAGED(sllm_k_attend_f32_64, float, float, 64)
+PAGED(sllm_k_attend_f32_128, float, float, 128)
+PAGED(sllm_k_attend_f32f16_64, float, _Float16, 64)
+PAGED(sllm_k_attend_f32f16_128, float, _Float16, 128)
+PAGED(sllm_k_attend_f16_64, _Float16, _Float16, 64)
+PAGED(sllm_k_attend_f16_128, _Float16, _Float16, 128)
+PAGED(sllm_k_attend_bf16_64, __bf16, __bf16, 64)
+PAGED(sllm_k_attend_bf16_128, __bf16, __bf16, 128)
+PROMPT(sllm_k_prompt_f32_64, float, 64)
+PROMPT(sllm_k_prompt_f32_128, float, 128)
+PROMPT(sllm_k_prompt_f16_64, _Float16, 64)
+PROMPT(sllm_k_prompt_f16_128, _Float16, 128)
+PROMPT(sllm_k_prompt_bf16_64, __bf16, 64)
+PROMPT(sllm_k_prompt_bf16_128, __bf16, 128)
 
 namespace {
 
-// The partial results of one row, a wave a row: out = sum_i 2^(m_i - M) o_i / sum_i 2^(m_i - M) l_i,
-// M the largest m_i, always in the same order.
-template <typename A>
+// The partial results of one row, a workgroup a row: out = sum_i f_i o_i / sum_i f_i l_i
+// with f_i = 2^(m_i - M), M the largest m_i. The waves take every fourth split of a
+// segment and are added up in order, so the same call gives the same bits. What costs
+// is the chain of loads (token, segment, parts): a part's o, m and l are asked for
+// together, and several splits at once.
+template <typename A, int D>
 __device__ __forceinline__ void join_body(const att_join_args &a) {
-    const uint32_t lane = threadIdx.x & 63u;
-    const uint32_t id = uniform(blockIdx.x * (ATT_THREADS / 64) + (threadIdx.x >> 6));
-    if (id >= a.n_tok * a.n_head) return;
-    const uint32_t tok = id / a.n_head, h = id % a.n_head, kvh = h / a.group, hh = h % a.group;
-    const att_seq s = a.seqs[a.tok_seq[tok]];
-    if (s.n_seg == 0) return;                                    // written already
-    float top = LOWEST, sum = 0.0f, x0 = 0.0f, x1 = 0.0f;
-    const bool in = 2u * lane < a.hd;
-    for (uint32_t i = 0; i < s.n_seg; ++i) {
-        const att_seg sg = a.segs[s.seg0 + i];
-        const uint64_t row = sg.part0 + (uint64_t) kvh * sg.n_split * sg.n_rows + sg.row_off + (tok - s.tok0) * a.group + hh;
-        for (uint32_t k = 0; k < sg.n_split; ++k) {
-            const uint64_t at = row + (uint64_t) k * sg.n_rows;
-            const float m = a.part_ml[2 * at], l = a.part_ml[2 * at + 1];
-            const float x = in ? a.part_o[at * a.hd_pad + 2 * lane] : 0.0f;
-            const float y = in ? a.part_o[at * a.hd_pad + 2 * lane + 1] : 0.0f;
-            const float up = fmaxf(top, m), f = __builtin_amdgcn_exp2f(top - up), e = __builtin_amdgcn_exp2f(m - up);
+    constexpr int V = D / 64;
+    typedef float vec __attribute__((ext_vector_type(V)));
+    __shared__ float so[WAVES][D], sm[WAVES][2];
+    const uint32_t lane = threadIdx.x & 63u, wave = uniform(threadIdx.x >> 6);
+    const uint32_t tok = blockIdx.x, h = blockIdx.y, kvh = h / a.group, hh = h % a.group;
+    const uint32_t seg0 = C_CAST(uint32_t, &a.toks[tok].seg0)[0], n_seg = C_CAST(uint32_t, &a.toks[tok].n_seg)[0];
+    const uint32_t at = C_CAST(uint32_t, &a.toks[tok].t)[0] * a.group + hh;
+    if (n_seg == 0) return;                                      // written already
+    float top = LOWEST, sum = 0.0f, x[V] = {};
+    for (uint32_t i = 0; i < n_seg; ++i) {
+        const uint32_t part0 = C_CAST(uint32_t, &a.segs[seg0 + i].part0)[0], n_rows = C_CAST(uint32_t, &a.segs[seg0 + i].n_rows)[0];
+        const uint32_t n_split = C_CAST(uint32_t, &a.segs[seg0 + i].n_split)[0], off = C_CAST(uint32_t, &a.segs[seg0 + i].row_off)[0];
+        const uint64_t row = part0 + (uint64_t) kvh * n_split * n_rows + off + at;
+        constexpr int UN = 4;
+        for (uint32_t k = wave; k < n_split; k += WAVES * UN) {
+            float m[UN], l[UN];
+            vec o[UN];
+#pragma unroll
+            for (int u = 0; u < UN; ++u) {                       // (past the end: the last split again, with no weight)
+                const uint64_t r = row + (uint64_t) min(k + (uint32_t) u * WAVES, n_split - 1u) * n_rows;
+                m[u] = G_CAST(const float, a.part_ml)[2 * r];
+                l[u] = G_CAST(const float, a.part_ml)[2 * r + 1];
+                o[u] = *G_CAST(const vec, a.part_o + r * D + V * lane);
+            }
+            float up = top;
+#pragma unroll
+            for (int u = 0; u < UN; ++u) up = fmaxf(up, m[u]);
+            const float f = __builtin_amdgcn_exp2f(top - up);
             top = up;
-            sum = sum * f + l * e;
-            x0 = x0 * f + x * e;
-            x1 = x1 * f + y * e;
+            sum *= f;
+#pragma unroll
+            for (int v = 0; v < V; ++v) x[v] *= f;
+#pragma unroll
+            for (int u = 0; u < UN; ++u) {
+                if (k + (uint32_t) u * WAVES < n_split) {
+                    const float e = __builtin_amdgcn_exp2f(m[u] - up);
+                    sum = fmaf(l[u], e, sum);
+#pragma unroll
+                    for (int v = 0; v < V; ++v) x[v] = fmaf(o[u][v], e, x[v]);
+                }
+            }
         }
     }
-    if (in) {
-        A *dst = (A *) ((uint8_t *) a.out + tok * a.out_tok) + h * a.hd + 2 * lane;
-        dst[0] = (A) (x0 / sum);
-        dst[1] = (A) (x1 / sum);
+#pragma unroll
+    for (int v = 0; v < V; ++v) so[wave][V * lane + v] = x[v];
+    if (lane == 0) {
+        sm[wave][0] = top;
+        sm[wave][1] = sum;
     }
+    __syncthreads();
+    if (threadIdx.x >= a.hd) return;
+    float all = fmaxf(fmaxf(sm[0][0], sm[1][0]), fmaxf(sm[2][0], sm[3][0])), l = 0.0f, o = 0.0f;
+#pragma unroll
+    for (int w = 0; w < WAVES; ++w) {
+        const float e = __builtin_amdgcn_exp2f(sm[w][0] - all);
+        l = fmaf(sm[w][1], e, l);
+        o = fmaf(so[w][threadIdx.x], e, o);
+    }
+    *G_CAST(A, (uint8_t *) a.out + tok * a.out_tok + (uint64_t) (h * a.hd + threadIdx.x) * sizeof(A)) = (A) (o / l);
 }
 
 // A step's rows into their pages: a thread for each eight values of a row,
@@ -590,8 +680,7 @@ __device__ __forceinline__ void store_body(const att_store_args &a) {
     const uint32_t per_row = a.hd / 8, id = blockIdx.x * ATT_THREADS + threadIdx.x;
     const uint32_t tok = id / per_row, ch = id % per_row, h = blockIdx.y >> 1, kv = blockIdx.y & 1u;
     if (tok >= a.n_tok) return;
-    const att_seq s = a.seqs[a.tok_seq[tok]];
-    const uint32_t pos = s.len0 + (tok - s.tok0), page = a.tables[s.table + (pos >> a.page_shift)];
+    const uint32_t pos = a.toks[tok].pos, page = a.tables[a.toks[tok].table + (pos >> a.page_shift)];
     const uint8_t *src = kv ? (const uint8_t *) a.v + tok * a.v_tok : (const uint8_t *) a.k + tok * a.k_tok;
     src += (h * a.hd + 8u * ch) * sizeof(A);
     uint8_t *dst = (kv ? a.cv : a.ck) + page * a.page_bytes +
@@ -613,12 +702,15 @@ __device__ __forceinline__ void store_body(const att_store_args &a) {
 
 }  // namespace
 
-#define JOIN(name, A) extern "C" __global__ void __launch_bounds__(ATT_THREADS) name(const att_join_args a) { join_body<A>(a); }
+#define JOIN(name, A, D) extern "C" __global__ void __launch_bounds__(ATT_THREADS) name(const att_join_args a) { join_body<A, D>(a); }
 #define STORE(name, A, T) extern "C" __global__ void __launch_bounds__(ATT_THREADS) name(const att_store_args a) { store_body<A, T>(a); }
 
-JOIN(sllm_k_attn_join_f32, float)
-JOIN(sllm_k_attn_join_f16, _Float16)
-JOIN(sllm_k_attn_join_bf16, __bf16)
+JOIN(sllm_k_attn_join_f32_64, float, 64)
+JOIN(sllm_k_attn_join_f32_128, float, 128)
+JOIN(sllm_k_attn_join_f16_64, _Float16, 64)
+JOIN(sllm_k_attn_join_f16_128, _Float16, 128)
+JOIN(sllm_k_attn_join_bf16_64, __bf16, 64)
+JOIN(sllm_k_attn_join_bf16_128, __bf16, 128)
 STORE(sllm_k_attn_store_f32, float, float)
 STORE(sllm_k_attn_store_f32f16, float, _Float16)
 STORE(sllm_k_attn_store_16, _Float16, _Float16)

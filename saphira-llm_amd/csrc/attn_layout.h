@@ -13,6 +13,7 @@
 #define ATT_FEW_ROWS  16
 #define ATT_SOME_ROWS 32
 #define ATT_THREADS   256
+enum { ATT_FEW, ATT_SOME, ATT_MANY };
 
 #define ATT_DIRECT    0xffffffffu    /* att_item.part: rows go to the output */
 #define ATT_TOKENS    0xffffffffu    /* att_item.list: tokens in order */
@@ -32,6 +33,8 @@ typedef struct att_item {
     uint32_t kv;            /* paged: where the segment's page numbers start; packed: the first key's row */
     uint32_t head;
     uint32_t part;          /* row of the partial results that row0's go to, or ATT_DIRECT */
+    uint32_t mode;          /* ATT_FEW, ATT_SOME, ATT_MANY (prompts: unused) */
+    uint32_t pad;
 } att_item;
 
 typedef struct att_args {
@@ -58,27 +61,28 @@ typedef struct att_seg {
     uint32_t part0, n_rows, n_split, row_off;
 } att_seg;
 
-/* a sequence of a batch: its rows tok0 .. tok0 + n_new, where its page numbers
- * start, its positions before the step, and its segments */
-typedef struct att_seq {
-    uint32_t tok0, n_new, table, len0, seg0, n_seg;
-} att_seq;
+/* a new token of a batch: where its sequence's page numbers start and its
+ * position (the store); the segments of its sequence and its number in the step
+ * (the join; n_seg 0: its rows are in the output already) */
+typedef struct att_tok {
+    uint32_t table, pos, seg0, n_seg, t;
+    uint32_t pad[3];
+} att_tok;
 
 typedef struct att_join_args {
     void           *out;
     const float    *part_o, *part_ml;
-    const uint32_t *tok_seq;         /* a token's sequence */
-    const att_seq  *seqs;
+    const att_tok  *toks;
     const att_seg  *segs;
     uint64_t        out_tok;         /* bytes */
-    uint32_t        hd, hd_pad, group, n_head, n_tok, pad;
+    uint32_t        hd, group;
 } att_join_args;
 
 typedef struct att_store_args {
     const void     *k, *v;
     uint8_t        *ck, *cv;         /* the layer's keys and values in page 0 */
-    const uint32_t *tables, *tok_seq;
-    const att_seq  *seqs;
+    const uint32_t *tables;
+    const att_tok  *toks;
     uint64_t        k_tok, v_tok;    /* bytes */
     uint64_t        page_bytes;
     uint32_t        page_shift, hd, n_head_kv, n_tok;
@@ -99,9 +103,9 @@ typedef struct att_copy_args {
 #define ATT_COPY_CHUNKS 1024u        /* 16-byte pieces a workgroup */
 
 #if defined(__cplusplus)
-static_assert(sizeof(att_item) == 40 && sizeof(att_args) == 168 && sizeof(att_copy_args) <= 4096, "attn_layout.h");
+static_assert(sizeof(att_item) == 48 && sizeof(att_args) == 168 && sizeof(att_copy_args) <= 4096, "attn_layout.h");
 #else
-_Static_assert(sizeof(att_item) == 40 && sizeof(att_args) == 168 && sizeof(att_copy_args) <= 4096, "attn_layout.h");
+_Static_assert(sizeof(att_item) == 48 && sizeof(att_args) == 168 && sizeof(att_copy_args) <= 4096, "attn_layout.h");
 #endif
 
 #endif /* SLLM_ATTN_LAYOUT_H */

@@ -291,13 +291,15 @@ static int load_functions(void) {
 }
 
 static int load_attn_functions(void) {
-    static const char *const types[4] = { "f32", "f32f16", "f16", "bf16" }, *const rows[3] = { "few", "some", "rows" };
-    static const char *const rest[7] = { "join_f32", "join_f16", "join_bf16", "store_f32", "store_f32f16", "store_16", "copy" };
+    static const char *const types[4] = { "f32", "f32f16", "f16", "bf16" };
+    static const char *const rest[4] = { "store_f32", "store_f32f16", "store_16", "copy" };
     for (int i = 0; i < SLLM_ATTN_FUNCTIONS; ++i) {
         char name[64];
-        if (i < SLLM_ATTN_PROMPT) snprintf(name, sizeof name, "sllm_k_attend_%s_%d_%s", types[i / 6], i / 3 % 2 ? 128 : 64, rows[i % 3]);
-        else if (i < SLLM_ATTN_JOIN) snprintf(name, sizeof name, "sllm_k_prompt_%s_%d", types[(i - SLLM_ATTN_PROMPT) / 2 ? (i - SLLM_ATTN_PROMPT) / 2 + 1 : 0], i % 2 ? 128 : 64);
-        else snprintf(name, sizeof name, "sllm_k_attn_%s", rest[i - SLLM_ATTN_JOIN]);
+        const int of = i < SLLM_ATTN_PROMPT ? i : i < SLLM_ATTN_JOIN ? i - SLLM_ATTN_PROMPT : i - SLLM_ATTN_JOIN;
+        const int type = i < SLLM_ATTN_PROMPT ? of / 2 : of / 2 ? of / 2 + 1 : 0;        /* (rows of f32, f16, bf16) */
+        if (i >= SLLM_ATTN_STORE) snprintf(name, sizeof name, "sllm_k_attn_%s", rest[i - SLLM_ATTN_STORE]);
+        else snprintf(name, sizeof name, "sllm_k_%s_%s_%d", i < SLLM_ATTN_PROMPT ? "attend" : i < SLLM_ATTN_JOIN ? "prompt" : "attn_join",
+                      types[type], of % 2 ? 128 : 64);
         HIP_TRY(hipModuleGetFunction(&g.k_attn[i], g.attn_mod, name));
     }
     return SLLM_GFX950_OK;

@@ -64,15 +64,16 @@ SLLM_HIDDEN int         sllm_shim_fail(int status, const char *fmt, ...)
 SLLM_HIDDEN int         sllm_shim_hip_fail(hipError_t e, const char *what);
 /* an entry point of the decode code object */
 SLLM_HIDDEN int         sllm_shim_decode_function(const char *name, hipFunction_t *f);
-/* the attention code object's entry points (attn_kernels.hip), loaded by open:
+/* the attention code object's entry points (attn_kernels.hip), loaded by open,
+ * each for head_dim up to 64 and up to 128 (`wide`) where it depends on it:
  * attention over pages for (rows' type, cache's type) f32/f32, f32/f16,
- * f16/f16, bf16/bf16, head_dim up to 64 or 128, few / some / many rows;
- * prompts for f32, f16, bf16 and those head dimensions; the join of partial
- * results by the rows' type; the store for f32, f32 to f16, 16 bits; page copies */
+ * f16/f16, bf16/bf16; prompts, and the join of partial results, for rows of
+ * f32, f16, bf16; the store for f32, f32 to f16, 16 bits; page copies */
 enum {
-    SLLM_ATTN_ATTEND = 0,                        /* + (types * 2 + wide) * 3 + rows */
-    SLLM_ATTN_PROMPT = 24,                       /* + type * 2 + wide */
-    SLLM_ATTN_JOIN = 30, SLLM_ATTN_STORE = 33, SLLM_ATTN_COPY = 36, SLLM_ATTN_FUNCTIONS = 37
+    SLLM_ATTN_ATTEND = 0,                        /* + types * 2 + wide */
+    SLLM_ATTN_PROMPT = 8,                        /* + type * 2 + wide */
+    SLLM_ATTN_JOIN = 14,                         /* + type * 2 + wide */
+    SLLM_ATTN_STORE = 20, SLLM_ATTN_COPY = 23, SLLM_ATTN_FUNCTIONS = 24
 };
 SLLM_HIDDEN hipFunction_t sllm_shim_attn_function(int i);
 /* grid gx x gy of `block` threads on the library stream */

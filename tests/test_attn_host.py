@@ -371,19 +371,18 @@ def test_how_a_step_is_laid_out(amd, L):
         return got
 
     alone = c.new()
-    assert step([alone], [1]) == {"sllm_k_attend_f32_64_few": 2}                 # one part: straight to the output
+    assert step([alone], [1]) == {"sllm_k_attend_f32_64": 2}         # one part: straight to the output
     got = step([a], [1])
-    assert "sllm_k_attn_join_f32" in got and got["sllm_k_attend_f32_64_few"] % 2 == 0
+    assert "sllm_k_attn_join_f32_64" in got and got["sllm_k_attend_f32_64"] % 2 == 0
     counts = []
     for n in (8, 16):
         kids = c.fork(a, 1000, n)
         got = step(kids, [1] * n)
         # each has keys of its own from position 992 on, once for each KV head
-        assert got["sllm_k_attend_f32_64_few"] == 2 * n
-        counts.append(got.get("sllm_k_attend_f32_64_some", 0) + got.get("sllm_k_attend_f32_64_rows", 0))
+        counts.append(got["sllm_k_attend_f32_64"] - 2 * n)
+        assert L.sllm_gfx950_seq_free(c.p, I(*kids), n) == 0
     assert counts[0] == counts[1] > 0
-    # few, some and many rows
-    assert set(step([alone], [7])) == {"sllm_k_attend_f32_64_some"} and step([alone], [40]) == {"sllm_k_attend_f32_64_rows": 4}
+    assert step([alone], [40]) == {"sllm_k_attend_f32_64": 4}        # 160 rows of each KV head: two tiles
     L.sllm_gfx950_free(mem)
     c.close()
 
