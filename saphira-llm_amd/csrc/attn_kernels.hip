@@ -105,7 +105,7 @@ struct attention {
     static constexpr bool WIDE = L::WIDE;
     static constexpr bool SPLIT = !WIDE && sizeof(A) == 4;       // f32 rows against f16 keys
     static constexpr int KT = L::KT;
-    static constexpr int KS = KT / 16;                           // 16-key subtiles
+    static constexpr int KS = WIDE ? 1 : 2;                      // 16-key subtiles of a step
     static constexpr int DT = D / 16;
     static constexpr int QC = D * (int) sizeof(T) / 64;          // 16-byte pieces of a row that a lane holds
     static constexpr int GROUP = KEYS ? (KT < 16 ? KT : 16) : KT / WAVES;   // rows that one address serves: within a page
@@ -263,12 +263,13 @@ struct attention {
     // A value of the tile that is infinite or NaN.
     __device__ __forceinline__ static bool odd(float x) { return (__float_as_uint(x) & 0x7f800000u) == 0x7f800000u; }
 
-    // One tile: scores, the maximum, p, and the products with the values.
-    // SEEN: every row sees every key of it. CAREFUL: an infinite or NaN value must
-    // not reach rows that do not see its key (0 times it is NaN): such values
-    // are left out of the products and added to the rows that see them.
-    template <bool SEEN, bool CAREFUL>
-    __device__ __forceinline__ void step(uint32_t t, uint32_t tl) {
+    // 16 KS keys of a tile (its part `part`), from key `key` of the range, at `tl`: scores,
+    // the maximum, p, and the products with the values.
+    // CAREFUL: an infinite or NaN value must not reach rows that do not see its key
+    // (0 times it is NaN): such values are left out of the products and added to
+    // the rows that see them.
+    template <bool CAREFUL>
+    __device__ __forceinline__ void step(uint32_t key, uint32_t tl, uint32_t part) {
         f32x4 s[KS][NT];
 #pragma unroll
         for (int ks = 0; ks < KS; ++ks) {
@@ -296,16 +297,24 @@ struct attention {
             }
         }
         __builtin_amdgcn_sched_barrier(0);
+        // (a branch around the scores alone: two copies of the products would each keep the sums in registers of their own)
+        if ((int) (key + 16u * KS) > lim_min) {
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+                for (int ks = 0; ks < KS; ++ks) {
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) s[ks][nt][i] = (int) (key + 16u * ks + 4u * g + i) < lim[nt] ? s[ks][nt][i] : -INFINITY;
+                }
+            }
+        }
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
             float top = m[nt];
 #pragma unroll
             for (int ks = 0; ks < KS; ++ks) {
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    if (!SEEN) s[ks][nt][i] = (int) (t * KT + 16u * ks + 4u * g + i) < lim[nt] ? s[ks][nt][i] : -INFINITY;
-                    top = fmaxf(top, s[ks][nt][i]);
-                }
+                for (int i = 0; i < 4; ++i) top = fmaxf(top, s[ks][nt][i]);
             }
             top = row_max(top);
             if (__any(top > m[nt])) {
@@ -337,8 +346,8 @@ struct attention {
                 for (int i = 0; i < 4; ++i) {
 #pragma unroll
                     for (int dt = 0; dt < DT; ++dt) {
-                        // (rows 16 further on have the swap of four 16-dimension tiles further, where rows are that long)
-                        const uint32_t at = (tl + voff) ^ (((uint32_t) dt ^ (L::CH == 32 ? 4u * (ks & 1) : 0u)) * 16u * DA);
+                        // (16 rows further on have the swap of four 16-dimension tiles further, where rows are that long)
+                        const uint32_t at = (tl + voff) ^ (((uint32_t) dt ^ (L::CH == 32 ? 4u * (part & 1u) : 0u)) * 16u * DA);
                         float vf = *reinterpret_cast<const float *>(S + at + (16u * ks + i) * L::ROWB);
                         if (CAREFUL) vf = odd(vf) ? 0.0f : vf;
 #pragma unroll
@@ -383,17 +392,17 @@ struct attention {
             }
         }
         if (CAREFUL) {
-            for (uint32_t r = 0; r < (uint32_t) KT; ++r) {
+            for (uint32_t r = 0; r < 16u * KS; ++r) {
                 const uint8_t *row = S + tl + L::HALF + r * L::ROWB;
 #pragma unroll
                 for (int dt = 0; dt < DT; ++dt) {
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
                         const uint32_t by = (16u * dt + 4u * g + i) * (uint32_t) sizeof(T);
-                        const float v = (float) *reinterpret_cast<const T *>(row + ((by >> 4) ^ L::vsw(r)) * 16u + (by & 15u));
+                        const float v = (float) *reinterpret_cast<const T *>(row + ((by >> 4) ^ L::vsw(16u * KS * part + r)) * 16u + (by & 15u));
 #pragma unroll
                         for (int nt = 0; nt < NT; ++nt) {
-                            if (odd(v) && (int) (t * KT + r) < lim[nt]) o[dt][nt][i] += v;
+                            if (odd(v) && (int) (key + r) < lim[nt]) o[dt][nt][i] += v;
                         }
                     }
                 }
@@ -403,9 +412,8 @@ struct attention {
 
     template <bool CAREFUL>
     __device__ __forceinline__ void tile_step(uint32_t t, uint32_t tl) {
-        if ((int) (t * KT) >= lim_max) return;                   // none of the wave's rows sees it
-        if ((int) (t * KT + KT) <= lim_min) step<true, false>(t, tl);
-        else step<false, CAREFUL>(t, tl);
+#pragma unroll
+        for (int h = 0; h < KT / (16 * KS); ++h) step<CAREFUL>(t * KT + 16u * KS * h, tl + 16u * KS * h * L::ROWB, h);
     }
 
     template <bool CAREFUL>
