@@ -573,36 +573,58 @@ static int by_table(const void *a, const void *b) {
 
 static uint32_t mode_of(uint32_t rows) { return rows <= ATT_FEW_ROWS ? ATT_FEW : rows <= ATT_SOME_ROWS ? ATT_SOME : ATT_MANY; }
 
-/* the dearest first */
-static int by_work(const void *a, const void *b) {
-    const att_item *x = a, *y = b;
-    if (x->mode != y->mode) return x->mode > y->mode ? -1 : 1;
-    const uint32_t n = x->key1 > x->key0 ? x->key1 - x->key0 : 0, m = y->key1 > y->key0 ? y->key1 - y->key0 : 0;
-    if (n != m) return n > m ? -1 : 1;
-    return x->part != y->part ? (x->part < y->part ? -1 : 1) : x->row0 != y->row0 ? (x->row0 < y->row0 ? -1 : 1) :
-           x->tok0 != y->tok0 ? (x->tok0 < y->tok0 ? -1 : 1) : x->head < y->head ? -1 : x->head > y->head;
+/*
+ * A split's keys. Few rows: the work is cut so that 25/32 of the CUs have a
+ * workgroup each, or where that makes splits of over LONG_SPLIT keys, so that
+ * all have two, which the memory wants; but never below what one step of the
+ * four waves takes. Many rows: 25/32 of the CUs, at least 128 keys: their
+ * partial results weigh more. Measured with head_dim 128 over splits of 64 to
+ * 2048 keys (us, at the rule and at the best of them): one sequence of 8192
+ * positions, bf16 12.1 / 12.0, 64 of about 1000 28.0 / 26.9, 8 of 4096 to 65536
+ * 62.8 / 62.8; 64 behind 4096 shared ones 22.8 / 22.5, behind 16384 36.4 / 36.1.
+ */
+#define SPLIT_KEYS 64u
+#define LONG_SPLIT 512u
+
+static uint32_t seg_tiles(const segment *s, uint32_t group) {
+    const uint32_t tile = s->mode == ATT_MANY ? ATT_ROWS : ATT_SOME_ROWS;
+    return (s->n_tok * group + tile - 1) / tile;
 }
 
-/*
- * A split's keys: as many as give every CU two workgroups over the whole
- * step, a multiple of SPLIT_KEYS and at least LEAST_SPLIT. Shorter ones would
- * cost more in partial results than the idle CUs they fill.
- */
-#define SPLIT_KEYS  64u
-#define LEAST_SPLIT 128u
-
-static uint32_t split_keys(const plan *x, uint32_t group, uint32_t n_head_kv) {
+static uint32_t split_keys(const plan *x, uint32_t group, uint32_t n_head_kv, int many, uint32_t step) {
     uint64_t work = 0;
     for (int32_t i = 0; i < x->n_seg; ++i) {
         const segment *s = &x->seg[i];
-        const uint64_t tiles = s->mode == ATT_MANY ? ((uint64_t) s->n_tok * group + ATT_ROWS - 1) / ATT_ROWS : 1;
-        work += tiles * (uint64_t) s->n_keys * n_head_kv;
+        if ((s->mode == ATT_MANY) == many) work += (uint64_t) seg_tiles(s, group) * (uint64_t) s->n_keys * n_head_kv;
     }
-    const uint64_t wgs = 2u * (uint64_t) sllm_shim_cu();
-    uint64_t keys = (work + wgs - 1) / wgs;
-    if (keys < LEAST_SPLIT) keys = LEAST_SPLIT;
+    const uint64_t cu = (uint64_t) sllm_shim_cu();
+    uint64_t keys = work / (cu * 25 / 32 + 1) + 1;
+    if (!many && keys > LONG_SPLIT) {
+        keys = work / (2 * cu) * 17 / 16;                /* (more than an even share: splits are not all of one length) */
+        if (keys < LONG_SPLIT) keys = LONG_SPLIT;
+    }
+    const uint64_t least = many ? 128 : 4 * step;
+    if (keys < least) keys = least;
     keys = (keys + SPLIT_KEYS - 1) / SPLIT_KEYS * SPLIT_KEYS;
-    return keys > (1u << 30) ? 1u << 30 : (uint32_t) keys;
+    return keys > (1u << 28) ? 1u << 28 : (uint32_t) keys;
+}
+
+static uint64_t item_keys(const att_item *a) { return a->key1 > a->key0 ? a->key1 - a->key0 : 0; }
+
+/* Workgroups start in this order: many rows first, then the longest, so that what
+ * starts last is short. (Giving each XCD, workgroup i % 8, sequences of its own, so
+ * that its L2 holds their keys, gained 2 % for 24 prompts of up to 2048 rows, but its
+ * uneven ends lost 13 % for four and 40 % for 64 sequences behind a shared prefix.) */
+static int by_work(const void *a, const void *b) {
+    const att_item *x = a, *y = b;
+    if (x->mode != y->mode) return x->mode > y->mode ? -1 : 1;
+    if (item_keys(x) != item_keys(y)) return item_keys(x) > item_keys(y) ? -1 : 1;
+    return x->pad < y->pad ? -1 : x->pad > y->pad;       /* (the order they came in) */
+}
+
+static void order_work(items *x) {
+    for (size_t i = 0; i < x->n; ++i) x->v[i].pad = (uint32_t) i;
+    if (x->n > 0) qsort(x->v, x->n, sizeof *x->v, by_work);
 }
 
 static size_t align256(size_t x) { return (x + 255) & ~(size_t) 255; }
@@ -684,11 +706,12 @@ static int lay_out(sllm_gfx950_batch *b, plan *x, int32_t n, const int32_t *len0
     uint32_t *seg_count = calloc((size_t) n + 1, sizeof *seg_count), *seg_at = calloc((size_t) n + 1, sizeof *seg_at);
     uint8_t *alone = calloc((size_t) n + 1, 1);
     if (seg_count == NULL || seg_at == NULL || alone == NULL) { st = FAIL_NOMEM("batch_create: tables"); goto out; }
-    const uint32_t split = split_keys(x, group, kv);
+    const uint32_t step = p->d.dtype == SLLM_GFX950_F32 ? 16 : 32;
+    const uint32_t split[2] = { split_keys(x, group, kv, 0, step), split_keys(x, group, kv, 1, step) };
     uint64_t n_part = 0, n_segs = 0, n_pages = 0;
     for (int32_t i = 0; i < x->n_seg; ++i) {
         segment *s = &x->seg[i];
-        s->n_split = ((uint32_t) s->n_keys + split - 1) / split;
+        s->n_split = ((uint32_t) s->n_keys + split[s->mode == ATT_MANY] - 1) / split[s->mode == ATT_MANY];
         s->split = ((uint32_t) s->n_keys + s->n_split - 1) / s->n_split;        /* evenly */
         s->split = (s->split + SPLIT_KEYS - 1) / SPLIT_KEYS * SPLIT_KEYS;
         s->n_split = ((uint32_t) s->n_keys + s->split - 1) / s->split;
@@ -718,25 +741,23 @@ static int lay_out(sllm_gfx950_batch *b, plan *x, int32_t n, const int32_t *len0
         const uint32_t rows = s->n_tok * group, tile = s->mode == ATT_MANY ? ATT_ROWS : ATT_SOME_ROWS;
         const int own = s->hi - s->lo == 1;
         const int32_t vis0 = own ? len0[q] - (s->page0 << p->page_shift) + 1 : ATT_SEE_ALL;
-        for (uint32_t k = 0; k < s->n_split && st == SLLM_GFX950_OK; ++k) {
-            for (uint32_t r = 0; r < rows && st == SLLM_GFX950_OK; r += tile) {
+        for (uint32_t hk = 0; hk < kv * s->n_split && st == SLLM_GFX950_OK; ++hk) {
+            const uint32_t h = hk / s->n_split, k = hk % s->n_split, key0 = k * s->split;
+            for (uint32_t r = 0; r < rows; r += tile) {
                 const uint32_t nr = rows - r < tile ? rows - r : tile;
                 const uint64_t sees = (uint64_t) vis0 + (r + nr - 1) / group;
-                uint32_t key0 = k * s->split, key1 = (uint32_t) s->n_keys < key0 + s->split ? (uint32_t) s->n_keys : key0 + s->split;
+                uint32_t key1 = (uint32_t) s->n_keys < key0 + s->split ? (uint32_t) s->n_keys : key0 + s->split;
                 if (key1 > sees) key1 = (uint32_t) sees;
-                for (uint32_t h = 0; h < kv; ++h) {
-                    att_item *a = items_add(&it);
-                    if (a == NULL) { st = FAIL_NOMEM("batch_create: work items"); break; }
-                    *a = (att_item) { r, nr, own ? x->tok0[q] : 0, s->list, vis0, key0, key1,
-                                      x->table[q] + (uint32_t) s->page0, h,
-                                      alone[q] ? ATT_DIRECT : s->part0 + (h * s->n_split + k) * rows + r, s->mode, 0 };
-                }
+                att_item *a = items_add(&it);
+                if (a == NULL) { st = FAIL_NOMEM("batch_create: work items"); break; }
+                *a = (att_item) { r, nr, own ? x->tok0[q] : 0, s->list, vis0, key0, key1, x->table[q] + (uint32_t) s->page0, h,
+                                  alone[q] ? ATT_DIRECT : s->part0 + hk * rows + r, s->mode, 0 };
             }
         }
     }
     if (st == SLLM_GFX950_OK && it.n > MAX_ITEMS) st = FAIL_ARG("batch_create: too much work for a launch");
     if (st != SLLM_GFX950_OK) goto out;
-    if (it.n > 0) qsort(it.v, it.n, sizeof *it.v, by_work);
+    order_work(&it);
 
     b->n_items = (uint32_t) it.n;
     size_t at = align256(it.n * sizeof(att_item));
@@ -988,14 +1009,6 @@ struct sllm_gfx950_prompt {
     att_item *items;                 /* device */
 };
 
-static int longest_first(const void *a, const void *b) {
-    const att_item *x = a, *y = b;
-    if (x->key1 != y->key1) return x->key1 > y->key1 ? -1 : 1;
-    if (x->kv != y->kv) return x->kv < y->kv ? -1 : 1;
-    if (x->head != y->head) return x->head < y->head ? -1 : 1;
-    return x->row0 < y->row0 ? -1 : x->row0 > y->row0;
-}
-
 int sllm_gfx950_prompt_create(const sllm_gfx950_prompt_desc *d, sllm_gfx950_prompt **out) {
     ATT_NEED_OPEN();
     if (out == NULL) return FAIL_ARG("prompt_create: NULL out");
@@ -1020,10 +1033,10 @@ int sllm_gfx950_prompt_create(const sllm_gfx950_prompt_desc *d, sllm_gfx950_prom
             break;
         }
         const uint32_t rows = (uint32_t) nq * group;
-        for (uint32_t r = 0; r < rows && st == SLLM_GFX950_OK; r += ATT_ROWS) {
-            const uint32_t n = rows - r < ATT_ROWS ? rows - r : ATT_ROWS;
-            const int32_t last = (int32_t) ((r + n - 1) / group) + nk - nq + 1;    /* keys that the last row sees */
-            for (int32_t h = 0; h < d->n_head_kv; ++h) {
+        for (int32_t h = 0; h < d->n_head_kv && st == SLLM_GFX950_OK; ++h) {
+            for (uint32_t r = 0; r < rows; r += ATT_ROWS) {
+                const uint32_t n = rows - r < ATT_ROWS ? rows - r : ATT_ROWS;
+                const int32_t last = (int32_t) ((r + n - 1) / group) + nk - nq + 1;    /* keys that the last row sees */
                 att_item *a = items_add(&it);
                 if (a == NULL) { st = FAIL_NOMEM("prompt_create: work items"); break; }
                 *a = (att_item) { r, n, (uint32_t) p->n_q, ATT_TOKENS, nk - nq + 1, 0, last > 0 ? (uint32_t) last : 0,
@@ -1035,7 +1048,7 @@ int sllm_gfx950_prompt_create(const sllm_gfx950_prompt_desc *d, sllm_gfx950_prom
         if (st == SLLM_GFX950_OK && it.n > MAX_ITEMS) st = FAIL_ARG("prompt_create: too many rows");
     }
     if (st == SLLM_GFX950_OK && it.n > 0) {
-        qsort(it.v, it.n, sizeof *it.v, longest_first);
+        order_work(&it);
         p->n_items = (uint32_t) it.n;
         hipError_t e = hipMalloc((void **) &p->items, it.n * sizeof *it.v);
         if (e != hipSuccess) { p->items = NULL; st = sllm_shim_hip_fail(e, "hipMalloc(prompt plan)"); }

@@ -35,6 +35,13 @@ typedef short s16x4 __attribute__((ext_vector_type(4)));
 #define LDS_PTR(p) ((__attribute__((address_space(3))) void *) (p))
 
 constexpr int WAVES = 4;
+#ifndef ILV_A
+#define ILV_A 4
+#define ILV_B 4
+#endif
+
+// what copies to LDS read in place of keys past the end and dimensions past head_dim
+__device__ __attribute__((aligned(16))) uint32_t att_zeros[4];
 
 template <int N> __device__ __forceinline__ void wait_vmem() {   // s_waitcnt vmcnt(N), the other counters untouched
     static_assert(N >= 0 && N < 64, "vmcnt");
@@ -76,17 +83,19 @@ constexpr float LOWEST = -3.402823466e38f;
 // attention
 // ---------------------------------------------------------------------------
 
-// Keys of a tile and what it takes in LDS. A tile holds its keys' rows of D
-// values, then its values' rows, 16-byte pieces of a row swapped about by the
-// row (ksw, vsw) so that the lanes of one read fall into different banks.
+// Keys of a tile and what it takes in LDS: its keys' rows of D values, then its
+// values' rows, 16-byte pieces of a row swapped about by the row (ksw, vsw) so
+// that the lanes of one read fall into different banks. KEYS: a wave's own tiles,
+// whose keys go to registers, so that a stage is its values alone.
 template <typename T, int D, bool KEYS> struct tile {
     static constexpr bool WIDE = sizeof(T) == 4;
-    static constexpr int KT = (KEYS ? 32 : 64) / (WIDE ? 2 : 1);
+    static constexpr int KT = WIDE ? 16 : 32;
     static constexpr int ROWB = D * (int) sizeof(T);
     static constexpr int CH = ROWB / 16;
     static constexpr int HALF = KT * ROWB;
-    static constexpr int BYTES = 2 * HALF;
-    static constexpr int STAGES = KEYS ? 1 : 2;
+    static constexpr int VALUES = KEYS ? 0 : HALF;               // where the values are
+    static constexpr int BYTES = VALUES + HALF;
+    static constexpr int STAGES = KEYS ? 1 : 4;
     static constexpr int LDS = BYTES * STAGES * (KEYS ? WAVES : 1);
     static __device__ __forceinline__ uint32_t ksw(uint32_t r) { return !WIDE && CH == 16 ? r & 15u : r & 7u; }
     static __device__ __forceinline__ uint32_t vsw(uint32_t r) {
@@ -105,7 +114,7 @@ struct attention {
     static constexpr bool WIDE = L::WIDE;
     static constexpr bool SPLIT = !WIDE && sizeof(A) == 4;       // f32 rows against f16 keys
     static constexpr int KT = L::KT;
-    static constexpr int KS = WIDE ? 1 : 2;                      // 16-key subtiles of a step
+    static constexpr int KS = KT / 16;                           // 16-key subtiles
     static constexpr int DT = D / 16;
     static constexpr int QC = D * (int) sizeof(T) / 64;          // 16-byte pieces of a row that a lane holds
     static constexpr int GROUP = KEYS ? (KT < 16 ? KT : 16) : KT / WAVES;   // rows that one address serves: within a page
@@ -114,7 +123,9 @@ struct attention {
     typedef typename vec8<T>::type t8;
 
     static constexpr int COPIES = GROUP / RPI;                   // instructions of a group, for keys and for values
+    static constexpr uint32_t PAST = 0xfffffff0u;                // a place past any end
     static constexpr int DA = WIDE ? 4 : 2;                      // 16-byte pieces of 16 dimensions
+    static constexpr int VM = 2 * COPIES;                        // a wave's copies for a tile (not KEYS)
 
     const att_args &a;
     const att_item it;
@@ -128,23 +139,33 @@ struct attention {
     uint32_t koff[QC], voff;
     // a lane's place in the rows that a copy instruction fills, or past any end where
     // the row has no such piece
-    uint32_t kcopy[COPIES], vcopy[COPIES];
+    // KEYS: keys are read as the products take them, and values are swapped when they
+    // are written to LDS, at vput.
+    uint32_t kcopy[KEYS ? QC : COPIES], vcopy[COPIES], vput[KEYS ? COPIES : 1];
 
     __device__ __forceinline__ void places() {
 #pragma unroll
-        for (int q = 0; q < QC; ++q) koff[q] = li * L::ROWB + (((4u * q + g) ^ L::ksw(li)) * 16u);
+        for (int q = 0; q < QC; ++q) {
+            if (!KEYS) koff[q] = li * L::ROWB + (((4u * q + g) ^ L::ksw(li)) * 16u);
+            else kcopy[q] = (4u * q + g) * 16u < a.hd * (uint32_t) sizeof(T) ? li * a.hd * (uint32_t) sizeof(T) + (4u * q + g) * 16u : PAST;
+        }
         const uint32_t r = WIDE ? 4u * g : 4u * g + (li >> 2);
-        voff = L::HALF + r * L::ROWB + (WIDE ? ((li >> 2) ^ L::vsw(r)) * 16u + (li & 3u) * 4u
+        voff = L::VALUES + r * L::ROWB + (WIDE ? ((li >> 2) ^ L::vsw(r)) * 16u + (li & 3u) * 4u
                                              : (((li >> 1) & 1u) ^ L::vsw(r)) * 16u + (li & 1u) * 8u);
         const uint32_t rowk = PAGED ? a.hd * (uint32_t) sizeof(T) : (uint32_t) a.k_tok;
         const uint32_t rowv = PAGED ? rowk : (uint32_t) a.v_tok;
 #pragma unroll
         for (int j = 0; j < COPIES; ++j) {
             const uint32_t rg = (uint32_t) j * RPI + lane / L::CH, ch = lane % L::CH;
-            const uint32_t rt = (KEYS ? 0u : wave * (uint32_t) GROUP) + rg;        // (groups are 16 rows apart: the same swaps)
+            if constexpr (KEYS) {                                // (16 rows further on: the same swap)
+                vcopy[j] = ch * 16u < rowv ? rg * rowv + ch * 16u : PAST;
+                vput[j] = rg * L::ROWB + (ch ^ L::vsw(rg)) * 16u;
+                continue;
+            }
+            const uint32_t rt = wave * (uint32_t) GROUP + rg;
             const uint32_t ck = (ch ^ L::ksw(rt)) * 16u, cv = (ch ^ L::vsw(rt)) * 16u;
-            kcopy[j] = ck < a.hd * (uint32_t) sizeof(T) ? rg * rowk + ck : 0xfffffff0u;
-            vcopy[j] = cv < a.hd * (uint32_t) sizeof(T) ? rg * rowv + cv : 0xfffffff0u;
+            if (!KEYS) kcopy[j] = ck < a.hd * (uint32_t) sizeof(T) ? rg * rowk + ck : PAST;
+            vcopy[j] = cv < a.hd * (uint32_t) sizeof(T) ? rg * rowv + cv : PAST;
         }
     }
 
@@ -228,178 +249,239 @@ struct attention {
         }
     }
 
-    // Copy a tile's keys and values into the stage at `to` (this wave's rows of it),
-    // straight to LDS. The buffers end behind the range's last key: what lies past it,
-    // and past head_dim, arrives as zeros.
+    // Where GROUP rows of keys and of values are, from `key` on (of which the rows below
+    // the range's end are read).
+    struct span { const uint8_t *k, *v; };
+    __device__ __forceinline__ span rows_at(uint32_t key) const {
+        if constexpr (PAGED) {
+            const uint32_t at = min(key, it.key1 - 1u);
+            const uint32_t page = *C_CAST(uint32_t, a.tables + it.kv + (at >> a.page_shift));
+            const uint64_t off = page * a.page_bytes + ((uint64_t) (it.head << a.page_shift) + (at & ((1u << a.page_shift) - 1u) & ~(uint32_t) (GROUP - 1))) * (a.hd * (uint32_t) sizeof(T));
+            return { a.k + off, a.v + off };
+        } else {
+            return { a.k + (uint64_t) (it.kv + key) * a.k_tok + it.head * a.k_head, a.v + (uint64_t) (it.kv + key) * a.v_tok + it.head * a.v_head };
+        }
+    }
+
+    // Copy rows straight to LDS at `to`. `whole`: all of them, of full length, are there;
+    // else those from `n` on and what is past head_dim arrive as zeros.
+    __device__ __forceinline__ void copy_rows(const uint8_t *from, const uint32_t (&place)[COPIES], uint32_t to, bool whole, uint32_t n) const {
+        if (whole) {
+#pragma unroll
+            for (int j = 0; j < COPIES; ++j) __builtin_amdgcn_global_load_lds((const void *) (from + place[j]), LDS_PTR(S + to + j * 1024), 16, 0, 0);
+        } else {
+#pragma unroll
+            for (int j = 0; j < COPIES; ++j) {
+                const bool in = (uint32_t) j * RPI + lane / L::CH < n && place[j] != PAST;
+                __builtin_amdgcn_global_load_lds((const void *) (in ? from + place[j] : (const uint8_t *) att_zeros), LDS_PTR(S + to + j * 1024), 16, 0, 0);
+            }
+        }
+    }
+    // rows of a group of tile row r0 that are below the range's end, and whether a tile's all are
+    __device__ __forceinline__ uint32_t rows_in(uint32_t key) const { return key < it.key1 ? min(it.key1 - key, (uint32_t) GROUP) : 0u; }
+    __device__ __forceinline__ bool is_whole(uint32_t t) const { return (t + 1u) * KT <= it.key1 && a.hd == D; }
+
+    // not KEYS: this wave's rows of a tile into the stage at `to`
     __device__ __forceinline__ void issue(uint32_t t, uint32_t to) const {
-        const uint32_t row = a.hd * (uint32_t) sizeof(T);
-        const uint32_t rowk = PAGED ? row : (uint32_t) a.k_tok, rowv = PAGED ? row : (uint32_t) a.v_tok;
+        const uint32_t r0 = wave * (uint32_t) GROUP;             // row in the tile
+        const span m = rows_at(t * KT + r0);
+        const bool whole = is_whole(t);
+        const uint32_t n = rows_in(t * KT + r0);
+        copy_rows(m.k, kcopy, to + r0 * L::ROWB, whole, n);
+        copy_rows(m.v, vcopy, to + L::VALUES + r0 * L::ROWB, whole, n);
+    }
+    // KEYS: a tile's keys, as the products take them, and its values, on their way in
+    // registers. What is past the end or past head_dim is zero.
+    struct load {
+        u32x4 k[KEYS ? KS : 1][KEYS ? QC : 1], v[KEYS ? GROUPS : 1][KEYS ? COPIES : 1];
+    };
+    struct span_of_tile { span m[GROUPS]; };
+    __device__ __forceinline__ span_of_tile spans(uint32_t t) const {
+        span_of_tile x;
+#pragma unroll
+        for (int gr = 0; gr < GROUPS; ++gr) x.m[gr] = rows_at(t * KT + (uint32_t) gr * GROUP);
+        return x;
+    }
+    __device__ __forceinline__ void fetch(load &x, const span_of_tile &at, uint32_t t) const {
+        __amdgpu_buffer_rsrc_t k[GROUPS], v[GROUPS];
 #pragma unroll
         for (int gr = 0; gr < GROUPS; ++gr) {
-            const uint32_t r0 = (KEYS ? 0u : wave * (uint32_t) GROUP) + (uint32_t) gr * GROUP;      // row in the tile
-            const uint32_t key = t * KT + r0;
-            const uint32_t n = key < it.key1 ? min(it.key1 - key, (uint32_t) GROUP) : 0u;
-            const uint8_t *kb, *vb;
-            if constexpr (PAGED) {
-                const uint32_t at = min(key, it.key1 - 1u);
-                const uint32_t page = *C_CAST(uint32_t, a.tables + it.kv + (at >> a.page_shift));
-                const uint64_t off = page * a.page_bytes + ((uint64_t) (it.head << a.page_shift) + (at & ((1u << a.page_shift) - 1u) & ~(uint32_t) (GROUP - 1))) * row;
-                kb = a.k + off;
-                vb = a.v + off;
-            } else {
-                kb = a.k + (uint64_t) (it.kv + key) * a.k_tok + it.head * a.k_head;
-                vb = a.v + (uint64_t) (it.kv + key) * a.v_tok + it.head * a.v_head;
-            }
-            const __amdgpu_buffer_rsrc_t rk = __builtin_amdgcn_make_buffer_rsrc((void *) kb, (short) 0, (int) uniform(n ? n * rowk - (rowk - row) : 0u), 0x00020000);
-            const __amdgpu_buffer_rsrc_t rv = __builtin_amdgcn_make_buffer_rsrc((void *) vb, (short) 0, (int) uniform(n ? n * rowv - (rowv - row) : 0u), 0x00020000);
-            uint8_t *dst = S + to + r0 * L::ROWB;
+            const int bytes = (int) uniform(rows_in(t * KT + (uint32_t) gr * GROUP) * (a.hd * (uint32_t) sizeof(T)));
+            k[gr] = __builtin_amdgcn_make_buffer_rsrc((void *) at.m[gr].k, (short) 0, bytes, 0x00020000);
+            v[gr] = __builtin_amdgcn_make_buffer_rsrc((void *) at.m[gr].v, (short) 0, bytes, 0x00020000);
+        }
+        // read once, and not kept (2: nontemporal): 64.9 -> 60.6 us for 8 sequences of 16384 positions, bf16
 #pragma unroll
-            for (int j = 0; j < COPIES; ++j) __builtin_amdgcn_raw_ptr_buffer_load_lds(rk, LDS_PTR(dst + j * 1024), 16, kcopy[j], 0, 0, 0);
+        for (int gr = 0; gr < GROUPS; ++gr) {
 #pragma unroll
-            for (int j = 0; j < COPIES; ++j) __builtin_amdgcn_raw_ptr_buffer_load_lds(rv, LDS_PTR(dst + L::HALF + j * 1024), 16, vcopy[j], 0, 0, 0);
+            for (int q = 0; q < QC; ++q) x.k[gr][q] = __builtin_amdgcn_raw_buffer_load_b128(k[gr], kcopy[q], 0, 2);
+        }
+#pragma unroll
+        for (int gr = 0; gr < GROUPS; ++gr) {
+#pragma unroll
+            for (int j = 0; j < COPIES; ++j) x.v[gr][j] = __builtin_amdgcn_raw_buffer_load_b128(v[gr], vcopy[j], 0, 2);
         }
     }
 
     // A value of the tile that is infinite or NaN.
     __device__ __forceinline__ static bool odd(float x) { return (__float_as_uint(x) & 0x7f800000u) == 0x7f800000u; }
 
-    // 16 KS keys of a tile (its part `part`), from key `key` of the range, at `tl`: scores,
-    // the maximum, p, and the products with the values.
-    // CAREFUL: an infinite or NaN value must not reach rows that do not see its key
-    // (0 times it is NaN): such values are left out of the products and added to
-    // the rows that see them.
-    template <bool CAREFUL>
-    __device__ __forceinline__ void step(uint32_t key, uint32_t tl, uint32_t part) {
-        f32x4 s[KS][NT];
+    typedef f32x4 scores[KS][NT];
+
+    __device__ __forceinline__ void score(f32x4 (&s)[NT], const u32x4 &piece, int q) const {
+        if constexpr (WIDE) {
+            const f32x4 kf = __builtin_bit_cast(f32x4, piece);
 #pragma unroll
-        for (int ks = 0; ks < KS; ++ks) {
+            for (int e = 0; e < 4; ++e) {
 #pragma unroll
-            for (int nt = 0; nt < NT; ++nt) s[ks][nt] = (f32x4) { 0, 0, 0, 0 };
+                for (int nt = 0; nt < NT; ++nt) s[nt] = mfma(kf[e], qw[nt][q][e], s[nt]);
+            }
+        } else {
+            const t8 kf = __builtin_bit_cast(t8, piece);
 #pragma unroll
-            for (int q = 0; q < QC; ++q) {
-                const uint32_t src = tl + koff[q] + 16u * ks * L::ROWB;
-                if constexpr (WIDE) {
-                    const f32x4 kf = *reinterpret_cast<const f32x4 *>(S + src);
+            for (int nt = 0; nt < NT; ++nt) s[nt] = mfma(kf, qf[nt][q], s[nt]);
+            if constexpr (SPLIT) {
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-#pragma unroll
-                        for (int nt = 0; nt < NT; ++nt) s[ks][nt] = mfma(kf[e], qw[nt][q][e], s[ks][nt]);
-                    }
-                } else {
-                    const t8 kf = *reinterpret_cast<const t8 *>(S + src);
-#pragma unroll
-                    for (int nt = 0; nt < NT; ++nt) s[ks][nt] = mfma(kf, qf[nt][q], s[ks][nt]);
-                    if constexpr (SPLIT) {
-#pragma unroll
-                        for (int nt = 0; nt < NT; ++nt) s[ks][nt] = mfma(kf, ql[nt][q], s[ks][nt]);
-                    }
-                }
+                for (int nt = 0; nt < NT; ++nt) s[nt] = mfma(kf, ql[nt][q], s[nt]);
             }
         }
-        __builtin_amdgcn_sched_barrier(0);
-        // (a branch around the scores alone: two copies of the products would each keep the sums in registers of their own)
-        if ((int) (key + 16u * KS) > lim_min) {
-#pragma unroll
-            for (int nt = 0; nt < NT; ++nt) {
-#pragma unroll
-                for (int ks = 0; ks < KS; ++ks) {
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) s[ks][nt][i] = (int) (key + 16u * ks + 4u * g + i) < lim[nt] ? s[ks][nt][i] : -INFINITY;
-                }
-            }
-        }
+    }
+
+    // keys that a row does not see, of the tile from `key` on (a branch around the scores
+    // alone: two copies of the products would each keep the sums in registers of their own)
+    __device__ __forceinline__ void mask(scores &s, uint32_t key) const {
+        if ((int) (key + KT) <= lim_min) return;
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
-            float top = m[nt];
 #pragma unroll
             for (int ks = 0; ks < KS; ++ks) {
 #pragma unroll
-                for (int i = 0; i < 4; ++i) top = fmaxf(top, s[ks][nt][i]);
+                for (int i = 0; i < 4; ++i) s[ks][nt][i] = (int) (key + 16u * ks + 4u * g + i) < lim[nt] ? s[ks][nt][i] : -INFINITY;
             }
-            top = row_max(top);
-            if (__any(top > m[nt])) {
-                const float f = __builtin_amdgcn_exp2f((m[nt] - top) * c[nt]);
-                m[nt] = top;
-                l[nt] *= f;
+        }
+    }
+
+    // p of a tile as the products take it: the cache's type (SPLIT: and what rounding to
+    // it left), or f32
+    struct probs {
+        t8 p[WIDE ? 1 : NT], rest[SPLIT ? NT : 1];
+        f32x4 w[WIDE ? NT : 1];
+    };
+
+    // s to p. The maximum moves only where a score is over it by 8 or more (as a power of
+    // two): until then p is at most 256, which costs no precision, and the sums need no
+    // scaling. Whether any did; then f is what the sums so far are to be scaled by.
+    __device__ __forceinline__ bool soften(const scores &s, probs &p, float (&f)[NT]) {
+        float top[NT];
+        bool over[NT], any = false;
 #pragma unroll
-                for (int dt = 0; dt < DT; ++dt) o[dt][nt] *= f;
+        for (int nt = 0; nt < NT; ++nt) {
+            top[nt] = m[nt];
+#pragma unroll
+            for (int ks = 0; ks < KS; ++ks) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) top[nt] = fmaxf(top[nt], s[ks][nt][i]);
             }
+            top[nt] = row_max(top[nt]);
+            over[nt] = (top[nt] - m[nt]) * c[nt] > 8.0f;             // (the row's own scores alone decide)
+            any |= over[nt];
+        }
+        const bool moved = __any(any);
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+            const float to = over[nt] ? top[nt] : m[nt];
+            f[nt] = __builtin_amdgcn_exp2f((m[nt] - to) * c[nt]);
+            m[nt] = to;
             // m is at least the lowest float, so a masked -inf gives 2^-inf = 0 and never inf - inf
-            const float mc = fmaxf(m[nt] * c[nt], LOWEST);
+            const float mc = fmaxf(to * c[nt], LOWEST);
             float sum = 0.0f;
 #pragma unroll
             for (int ks = 0; ks < KS; ++ks) {
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                    s[ks][nt][i] = __builtin_amdgcn_exp2f(fmaf(s[ks][nt][i], c[nt], -mc));
-                    sum += s[ks][nt][i];
+                    const float x = __builtin_amdgcn_exp2f(fmaf(s[ks][nt][i], c[nt], -mc));
+                    sum += x;
+                    if constexpr (WIDE) {
+                        p.w[nt][i] = x;
+                    } else {
+                        p.p[nt][4 * ks + i] = (T) x;
+                        if constexpr (SPLIT) p.rest[nt][4 * ks + i] = (T) (x - (float) p.p[nt][4 * ks + i]);
+                    }
                 }
             }
-            l[nt] += sum;
+            l[nt] = fmaf(l[nt], f[nt], sum);
         }
-        __builtin_amdgcn_sched_barrier(0);
+        return moved;
+    }
+
+    __device__ __forceinline__ void rescale(bool moved, const float (&f)[NT]) {
+        if (!moved) return;
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+            for (int dt = 0; dt < DT; ++dt) o[dt][nt] *= f[nt];
+        }
+    }
+
+    // A tile's values as the products take them: keys 4 g + 0..3 of each 16-key subtile, by
+    // a transposing read (16 bits); one key an instruction (f32: not held).
+    struct values { t8 v[WIDE ? 1 : DT]; };
+    __device__ __forceinline__ void values_of(values &x, uint32_t tl) const {
+        if constexpr (!WIDE) {
+#pragma unroll
+            for (int dt = 0; dt < DT; ++dt) {
+                s16x4 h[2];
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    const uint32_t at = ((tl + voff) ^ (uint32_t) dt * 16u * DA) + 16u * i * L::ROWB;
+                    h[i] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4 *) (S + at));
+                }
+                x.v[dt] = __builtin_bit_cast(t8, __builtin_shufflevector(h[0], h[1], 0, 1, 2, 3, 4, 5, 6, 7));
+            }
+        }
+    }
+
+    // O^T += V^T P^T for the tile at `tl`, from key `key` on.
+    // CAREFUL: an infinite or NaN value must not reach rows that do not see its key
+    // (0 times it is NaN): such values are left out of the products and added to
+    // the rows that see them.
+    template <bool CAREFUL>
+    __device__ __forceinline__ void products(const values &x, const probs &p, uint32_t key, uint32_t tl) {
         if constexpr (WIDE) {
 #pragma unroll
-            for (int ks = 0; ks < KS; ++ks) {
-                __builtin_amdgcn_sched_barrier(0);
+            for (int i = 0; i < 4; ++i) {
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
+                for (int dt = 0; dt < DT; ++dt) {
+                    float vf = *reinterpret_cast<const float *>(S + ((tl + voff) ^ (uint32_t) dt * 16u * DA) + i * L::ROWB);
+                    if (CAREFUL) vf = odd(vf) ? 0.0f : vf;
 #pragma unroll
-                    for (int dt = 0; dt < DT; ++dt) {
-                        // (16 rows further on have the swap of four 16-dimension tiles further, where rows are that long)
-                        const uint32_t at = (tl + voff) ^ (((uint32_t) dt ^ (L::CH == 32 ? 4u * (part & 1u) : 0u)) * 16u * DA);
-                        float vf = *reinterpret_cast<const float *>(S + at + (16u * ks + i) * L::ROWB);
-                        if (CAREFUL) vf = odd(vf) ? 0.0f : vf;
-#pragma unroll
-                        for (int nt = 0; nt < NT; ++nt) o[dt][nt] = mfma(vf, s[ks][nt][i], o[dt][nt]);
-                    }
+                    for (int nt = 0; nt < NT; ++nt) o[dt][nt] = mfma(vf, p.w[nt][i], o[dt][nt]);
                 }
             }
         } else {
-            // 32 keys at a time: a lane's operand holds keys 4 g + 0..3 of both 16-key subtiles
 #pragma unroll
-            for (int u = 0; u < KS / 2; ++u) {
-                __builtin_amdgcn_sched_barrier(0);
-                t8 p[NT], pl[SPLIT ? NT : 1];
+            for (int dt = 0; dt < DT; ++dt) {
+                t8 vf = x.v[dt];
+                if (CAREFUL) {
 #pragma unroll
-                for (int nt = 0; nt < NT; ++nt) {
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) {
-                        const float f = s[2 * u + (e >> 2)][nt][e & 3];
-                        p[nt][e] = (T) f;
-                        if constexpr (SPLIT) pl[nt][e] = (T) (f - (float) p[nt][e]);
-                    }
+                    for (int e = 0; e < 8; ++e) vf[e] = odd((float) vf[e]) ? (T) 0.0f : vf[e];
                 }
 #pragma unroll
-                for (int dt = 0; dt < DT; ++dt) {
-                    s16x4 h[2];
-#pragma unroll
-                    for (int i = 0; i < 2; ++i) {
-                        const uint32_t at = ((tl + voff) ^ (uint32_t) dt * 16u * DA) + (32u * u + 16u * i) * L::ROWB;
-                        h[i] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4 *) (S + at));
-                    }
-                    t8 vf = __builtin_bit_cast(t8, __builtin_shufflevector(h[0], h[1], 0, 1, 2, 3, 4, 5, 6, 7));
-                    if (CAREFUL) {
-#pragma unroll
-                        for (int e = 0; e < 8; ++e) vf[e] = odd((float) vf[e]) ? (T) 0.0f : vf[e];
-                    }
-#pragma unroll
-                    for (int nt = 0; nt < NT; ++nt) {
-                        o[dt][nt] = mfma(vf, p[nt], o[dt][nt]);
-                        if constexpr (SPLIT) o[dt][nt] = mfma(vf, pl[nt], o[dt][nt]);
-                    }
+                for (int nt = 0; nt < NT; ++nt) {
+                    o[dt][nt] = mfma(vf, p.p[nt], o[dt][nt]);
+                    if constexpr (SPLIT) o[dt][nt] = mfma(vf, p.rest[nt], o[dt][nt]);
                 }
             }
         }
         if (CAREFUL) {
-            for (uint32_t r = 0; r < 16u * KS; ++r) {
-                const uint8_t *row = S + tl + L::HALF + r * L::ROWB;
+            for (uint32_t r = 0; r < (uint32_t) KT; ++r) {
+                const uint8_t *row = S + tl + L::VALUES + r * L::ROWB;
 #pragma unroll
                 for (int dt = 0; dt < DT; ++dt) {
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
                         const uint32_t by = (16u * dt + 4u * g + i) * (uint32_t) sizeof(T);
-                        const float v = (float) *reinterpret_cast<const T *>(row + ((by >> 4) ^ L::vsw(16u * KS * part + r)) * 16u + (by & 15u));
+                        const float v = (float) *reinterpret_cast<const T *>(row + ((by >> 4) ^ L::vsw(r)) * 16u + (by & 15u));
 #pragma unroll
                         for (int nt = 0; nt < NT; ++nt) {
                             if (odd(v) && (int) (key + r) < lim[nt]) o[dt][nt][i] += v;
@@ -410,14 +492,80 @@ struct attention {
         }
     }
 
-    template <bool CAREFUL>
-    __device__ __forceinline__ void tile_step(uint32_t t, uint32_t tl) {
+    __device__ __forceinline__ void clear(scores &s) const {
 #pragma unroll
-        for (int h = 0; h < KT / (16 * KS); ++h) step<CAREFUL>(t * KT + 16u * KS * h, tl + 16u * KS * h * L::ROWB, h);
+        for (int ks = 0; ks < KS; ++ks) {
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) s[ks][nt] = (f32x4) { 0, 0, 0, 0 };
+        }
     }
 
+    // the first of the wave's tiles; key0 is a tile's first key
+    __device__ __forceinline__ uint32_t first_tile() const { return it.key0 / KT + (KEYS ? wave : 0u); }
+    static constexpr uint32_t STEP = KEYS ? WAVES : 1;
+    load x;                         // KEYS: the tile that is on its way
+
+    __device__ __forceinline__ uint32_t stage(uint32_t b) const { return (KEYS ? wave : b) * L::BYTES; }
+    // the first tiles set off
+    __device__ __forceinline__ void start() {
+        if (it.key0 >= it.key1) return;
+        const uint32_t t = first_tile();
+        if constexpr (KEYS) {
+            fetch(x, spans(t), t);
+        } else {
+            issue(t, stage(0));
+            issue(t + 1, stage(1));
+        }
+    }
+
+    // KEYS: tile t, in registers, which then take the next (two tiles on their way at a
+    // time were no faster: 58.8 us and 57.4 for 8 sequences of 16384 positions, bf16)
     template <bool CAREFUL>
-    __device__ __forceinline__ void pass() {
+    __device__ __forceinline__ void turn(uint32_t t) {
+        const uint32_t then = t + STEP;
+        const span_of_tile m = spans(then);                      // (past the end: the last page again)
+        scores s;
+        clear(s);
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks) {
+#pragma unroll
+            for (int q = 0; q < QC; ++q) score(s[ks], x.k[ks][q], q);
+        }
+#pragma unroll
+        for (int gr = 0; gr < GROUPS; ++gr) {
+#pragma unroll
+            for (int j = 0; j < COPIES; ++j) *reinterpret_cast<u32x4 *>(S + stage(0) + vput[j] + gr * GROUP * L::ROWB) = x.v[gr][j];
+        }
+        __builtin_amdgcn_sched_barrier(0);
+        if (then * KT < it.key1) fetch(x, m, then);
+        mask(s, t * KT);
+        probs p;
+        float f[NT];
+        rescale(soften(s, p, f), f);
+        __builtin_amdgcn_sched_barrier(0);
+        values v;
+        values_of(v, stage(0));
+        products<CAREFUL>(v, p, t * KT, stage(0));
+    }
+
+    __device__ __forceinline__ void scores_of(scores &s, uint32_t at) const {
+        clear(s);
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks) {
+#pragma unroll
+            for (int q = 0; q < QC; ++q) score(s[ks], *reinterpret_cast<const u32x4 *>(S + at + koff[q] + 16u * ks * L::ROWB), q);
+        }
+    }
+    // not KEYS: all but the last N of the wave's loads have arrived, and the other
+    // waves' have too; the stages read before are free
+    template <int N> __device__ __forceinline__ void meet() const {
+        wait_vmem<N>();
+        __builtin_amdgcn_s_waitcnt(0xC07F);
+        __builtin_amdgcn_s_barrier();
+        __builtin_amdgcn_sched_barrier(0);
+    }
+
+    __device__ __forceinline__ void begin() {
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
             m[nt] = LOWEST;
@@ -425,32 +573,103 @@ struct attention {
 #pragma unroll
             for (int dt = 0; dt < DT; ++dt) o[dt][nt] = (f32x4) { 0, 0, 0, 0 };
         }
-        // key0 is a tile's first key
-        const uint32_t t1 = (it.key1 + KT - 1u) / KT;
-        constexpr uint32_t STEP = KEYS ? WAVES : 1;
-        uint32_t t = it.key0 / KT + (KEYS ? wave : 0u);
-        const uint32_t buf = KEYS ? wave * (uint32_t) (L::BYTES * L::STAGES) : 0u;
-        if (it.key0 >= it.key1) return;
-        if (t < t1) issue(t, buf);
-        if constexpr (L::STAGES == 1) {
-            for (; t < t1; t += STEP) {
-                wait_vmem<0>();
-                __builtin_amdgcn_sched_barrier(0);
-                tile_step<CAREFUL>(t, buf);
-                __builtin_amdgcn_s_waitcnt(0xC07F);              // the tile is read
-                __builtin_amdgcn_sched_barrier(0);
-                if (t + STEP < t1) issue(t + STEP, buf);
-            }
-            return;
+    }
+
+    // The order of a loop iteration's instructions: the keys' reads, then each matrix
+    // instruction with its share of the vector ones and of the values' reads.
+    __device__ __forceinline__ static void interleave() {
+        constexpr int PER = (WIDE ? 4 : 1) * NT * (SPLIT ? 2 : 1);
+        constexpr int MS = KS * QC * PER, MP = DT * PER, DV = WIDE ? 4 * DT : 0;
+        __builtin_amdgcn_sched_group_barrier(0x100, KS * QC, 0);
+#pragma unroll
+        for (int i = 0; i < MS; ++i) {
+            __builtin_amdgcn_sched_group_barrier(0x8, 1, 0);
+            __builtin_amdgcn_sched_group_barrier(0x2, ILV_A, 0);
+            if (i < DV) __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
         }
-        for (uint32_t n = 0; t < t1; t += STEP, ++n) {
-            wait_vmem<0>();
-            __builtin_amdgcn_s_waitcnt(0xC07F);                  // this wave's reads of the other stage are done
-            if (!KEYS) __builtin_amdgcn_s_barrier();
-            __builtin_amdgcn_sched_barrier(0);
-            if (t + STEP < t1) issue(t + STEP, buf + ((n + 1u) & 1u) * L::BYTES);
-            __builtin_amdgcn_sched_barrier(0);
-            tile_step<CAREFUL>(t, buf + (n & 1u) * L::BYTES);
+#pragma unroll
+        for (int i = 0; i < MP; ++i) {
+            __builtin_amdgcn_sched_group_barrier(0x8, 1, 0);
+            __builtin_amdgcn_sched_group_barrier(0x2, ILV_B, 0);
+        }
+    }
+
+    // The keys of the range, once (start() went before). Not KEYS: three tiles are worked
+    // on at a time, the scores of one, p of the one before it and the products of the one
+    // before that, which do not wait for each other: the matrix unit and the vector unit
+    // both have work. A tile's copy is asked for two tiles ahead.
+    __device__ __forceinline__ void pass() {
+        begin();
+        if (it.key0 >= it.key1) return;
+        const uint32_t t1 = (it.key1 + KT - 1u) / KT;
+        uint32_t t = first_tile();
+        if constexpr (KEYS) {
+            for (; t < t1; t += STEP) turn<false>(t);
+        } else {
+            scores s, next;
+            probs p;
+            float f[NT];
+            meet<VM>();
+            issue(t + 2, stage(2));
+            scores_of(s, stage(0));
+            meet<VM>();
+            scores_of(next, stage(1));
+            mask(s, t * KT);
+            bool moved = soften(s, p, f);
+            uint32_t n = 1;                                      // tile t + n's scores are `next`
+            for (; t + n < t1; ++n) {
+                rescale(moved, f);
+                meet<0>();
+                // (the transposing reads before the copy: the compiler waits for copies to LDS before one)
+                values v;
+                values_of(v, stage((n - 1) & 3u));
+                __builtin_amdgcn_sched_barrier(0);
+                issue(t + n + 2, stage((n + 2) & 3u));
+#pragma unroll
+                for (int ks = 0; ks < KS; ++ks) {
+#pragma unroll
+                    for (int nt = 0; nt < NT; ++nt) s[ks][nt] = next[ks][nt];
+                }
+                mask(s, (t + n) * KT);
+                __builtin_amdgcn_sched_barrier(0);
+                probs q;
+                scores_of(next, stage((n + 1) & 3u));
+                products<false>(v, p, (t + n - 1) * KT, stage((n - 1) & 3u));
+                moved = soften(s, q, f);
+                p = q;
+                interleave();
+            }
+            rescale(moved, f);
+            wait_vmem<0>();                                      // nothing comes into LDS any more
+            values v;
+            values_of(v, stage((n - 1) & 3u));
+            products<false>(v, p, (t + n - 1) * KT, stage((n - 1) & 3u));
+        }
+    }
+
+    // The same with care, a tile after the other.
+    __device__ __forceinline__ void careful_pass() {
+        begin();
+        if (it.key0 >= it.key1) return;
+        const uint32_t t1 = (it.key1 + KT - 1u) / KT;
+        for (uint32_t t = first_tile(); t < t1; t += STEP) {
+            if constexpr (KEYS) {
+                fetch(x, spans(t), t);
+                turn<true>(t);
+            } else {
+                issue(t, stage(0));
+                meet<0>();
+                scores s;
+                probs p;
+                values v;
+                float f[NT];
+                scores_of(s, stage(0));
+                mask(s, t * KT);
+                rescale(soften(s, p, f), f);
+                values_of(v, stage(0));
+                products<true>(v, p, t * KT, stage(0));
+                meet<0>();
+            }
         }
     }
 
@@ -496,14 +715,19 @@ struct attention {
 
     __device__ __forceinline__ void run() {
         places();
+        start();                                                 // the first tile is on its way while q is read
         load_q();
-        pass<false>();
+        pass();
         // 0 x inf in a key that a row does not see: only then is anything not finite
         // that need not be, and only then is the pass made again
         if (KEYS) {
-            if (__any(has_odd())) pass<true>();
+            if (__any(has_odd())) careful_pass();
         } else {
-            if (__syncthreads_or(has_odd())) pass<true>();
+            uint32_t *votes = reinterpret_cast<uint32_t *>(S + L::LDS);
+            const bool bad = __any(has_odd());
+            if (lane == 0) votes[wave] = bad;
+            __syncthreads();
+            if ((votes[0] | votes[1] | votes[2] | votes[3]) != 0) careful_pass();
         }
         float mc[NT];
 #pragma unroll
@@ -565,6 +789,9 @@ __device__ __forceinline__ void attend_item(const att_args &a, const att_item &i
     x.run();
 }
 
+// One LDS variable a kernel: beside a second, the compiler waits for copies to the one
+// before it reads it anywhere.
+constexpr int VOTES = WAVES * 4;
 constexpr int max_of(int a, int b) { return a > b ? a : b; }
 
 __device__ __forceinline__ att_item item_of(const att_args &a) {
@@ -578,13 +805,13 @@ __device__ __forceinline__ att_item item_of(const att_args &a) {
 
 template <typename T, int D>
 __device__ __forceinline__ void prompt_body(const att_args &a) {
-    __shared__ __attribute__((aligned(1024))) uint8_t S[tile<T, D, false>::LDS];
+    __shared__ __attribute__((aligned(1024))) uint8_t S[tile<T, D, false>::LDS + VOTES];
     attend_item<T, T, D, 2, false, false>(a, item_of(a), S);
 }
 
 template <typename A, typename T, int D>
 __device__ __forceinline__ void paged_body(const att_args &a) {
-    __shared__ __attribute__((aligned(1024))) uint8_t S[max_of(max_of(tile<T, D, false>::LDS, tile<T, D, true>::LDS), WAVES * 32 * (D + 2) * 4)];
+    __shared__ __attribute__((aligned(1024))) uint8_t S[max_of(max_of(tile<T, D, false>::LDS + VOTES, tile<T, D, true>::LDS), WAVES * 32 * (D + 2) * 4)];
     const att_item it = item_of(a);
     if (it.mode == ATT_FEW) attend_item<A, T, D, 1, true, true>(a, it, S);
     else if (it.mode == ATT_SOME) attend_item<A, T, D, 2, true, true>(a, it, S);

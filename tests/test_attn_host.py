@@ -373,16 +373,15 @@ def test_how_a_step_is_laid_out(amd, L):
     alone = c.new()
     assert step([alone], [1]) == {"sllm_k_attend_f32_64": 2}         # one part: straight to the output
     got = step([a], [1])
-    assert "sllm_k_attn_join_f32_64" in got and got["sllm_k_attend_f32_64"] % 2 == 0
+    assert "sllm_k_attn_join_f32_64" in got and got["sllm_k_attend_f32_64"] > 2
     counts = []
-    for n in (8, 16):
+    for n in (8, 16, 32):
         kids = c.fork(a, 1000, n)
-        got = step(kids, [1] * n)
         # each has keys of its own from position 992 on, once for each KV head
-        counts.append(got["sllm_k_attend_f32_64"] - 2 * n)
+        counts.append(step(kids, [1] * n)["sllm_k_attend_f32_64"] - 2 * n)
         assert L.sllm_gfx950_seq_free(c.p, I(*kids), n) == 0
-    assert counts[0] == counts[1] > 0
-    assert step([alone], [40]) == {"sllm_k_attend_f32_64": 4}        # 160 rows of each KV head: two tiles
+    assert all(0 < x <= 32 for x in counts), counts
+    assert step([alone], [100]) == {"sllm_k_attend_f32_64": 8}       # 400 rows of each KV head: four tiles
     L.sllm_gfx950_free(mem)
     c.close()
 
