@@ -571,7 +571,15 @@ static int by_table(const void *a, const void *b) {
     return ia < ib ? -1 : ia > ib;
 }
 
-static uint32_t mode_of(uint32_t rows) { return rows <= ATT_FEW_ROWS ? ATT_FEW : rows <= ATT_SOME_ROWS ? ATT_SOME : ATT_MANY; }
+static const uint32_t k_rows[] = { ATT_FEW_ROWS, ATT_HALF_ROWS, ATT_MANY_ROWS };      /* by mode */
+
+/* A segment's rows: f32 takes two tiles of few before half of many (8 sequences
+ * behind 4096 shared positions, 32 rows: 19.7 us against 24.7), 16 bits one (12.0
+ * for half of many, 13.1 for two of few). */
+static uint32_t mode_of(uint32_t rows, int32_t dtype) {
+    const uint32_t few = dtype == SLLM_GFX950_F32 ? 2 * ATT_FEW_ROWS : ATT_FEW_ROWS;
+    return rows <= few ? ATT_FEW : rows <= ATT_HALF_ROWS ? ATT_HALF : ATT_MANY;
+}
 
 /*
  * A split's keys. Few rows: the work is cut so that 25/32 of the CUs have a
@@ -587,15 +595,14 @@ static uint32_t mode_of(uint32_t rows) { return rows <= ATT_FEW_ROWS ? ATT_FEW :
 #define LONG_SPLIT 512u
 
 static uint32_t seg_tiles(const segment *s, uint32_t group) {
-    const uint32_t tile = s->mode == ATT_MANY ? ATT_ROWS : ATT_SOME_ROWS;
-    return (s->n_tok * group + tile - 1) / tile;
+    return (s->n_tok * group + k_rows[s->mode] - 1) / k_rows[s->mode];
 }
 
 static uint32_t split_keys(const plan *x, uint32_t group, uint32_t n_head_kv, int many, uint32_t step) {
     uint64_t work = 0;
     for (int32_t i = 0; i < x->n_seg; ++i) {
         const segment *s = &x->seg[i];
-        if ((s->mode == ATT_MANY) == many) work += (uint64_t) seg_tiles(s, group) * (uint64_t) s->n_keys * n_head_kv;
+        if ((s->mode >= ATT_HALF) == many) work += (uint64_t) seg_tiles(s, group) * (uint64_t) s->n_keys * n_head_kv;
     }
     const uint64_t cu = (uint64_t) sllm_shim_cu();
     uint64_t keys = work / (cu * 25 / 32 + 1) + 1;
@@ -700,7 +707,7 @@ static int lay_out(sllm_gfx950_batch *b, plan *x, int32_t n, const int32_t *len0
         for (int32_t j = s->lo; j < s->hi; ++j) s->n_tok += (uint32_t) x->n_new[x->order[j]];
         s->list = ATT_TOKENS;
         if (s->hi - s->lo > 1) { s->list = (uint32_t) n_list; n_list += s->n_tok; }
-        s->mode = mode_of(s->n_tok * group);
+        s->mode = mode_of(s->n_tok * group, p->d.dtype);
     }
     /* segments of each sequence, and those with one part alone */
     uint32_t *seg_count = calloc((size_t) n + 1, sizeof *seg_count), *seg_at = calloc((size_t) n + 1, sizeof *seg_at);
@@ -711,7 +718,7 @@ static int lay_out(sllm_gfx950_batch *b, plan *x, int32_t n, const int32_t *len0
     uint64_t n_part = 0, n_segs = 0, n_pages = 0;
     for (int32_t i = 0; i < x->n_seg; ++i) {
         segment *s = &x->seg[i];
-        s->n_split = ((uint32_t) s->n_keys + split[s->mode == ATT_MANY] - 1) / split[s->mode == ATT_MANY];
+        s->n_split = ((uint32_t) s->n_keys + split[s->mode >= ATT_HALF] - 1) / split[s->mode >= ATT_HALF];
         s->split = ((uint32_t) s->n_keys + s->n_split - 1) / s->n_split;        /* evenly */
         s->split = (s->split + SPLIT_KEYS - 1) / SPLIT_KEYS * SPLIT_KEYS;
         s->n_split = ((uint32_t) s->n_keys + s->split - 1) / s->split;
@@ -738,7 +745,7 @@ static int lay_out(sllm_gfx950_batch *b, plan *x, int32_t n, const int32_t *len0
     for (int32_t i = 0; i < x->n_seg && st == SLLM_GFX950_OK; ++i) {
         const segment *s = &x->seg[i];
         const int32_t q = x->order[s->lo];
-        const uint32_t rows = s->n_tok * group, tile = s->mode == ATT_MANY ? ATT_ROWS : ATT_SOME_ROWS;
+        const uint32_t rows = s->n_tok * group, tile = k_rows[s->mode];
         const int own = s->hi - s->lo == 1;
         const int32_t vis0 = own ? len0[q] - (s->page0 << p->page_shift) + 1 : ATT_SEE_ALL;
         for (uint32_t hk = 0; hk < kv * s->n_split && st == SLLM_GFX950_OK; ++hk) {
@@ -1026,6 +1033,16 @@ int sllm_gfx950_prompt_create(const sllm_gfx950_prompt_desc *d, sllm_gfx950_prom
     p->n_head_kv = d->n_head_kv;
     p->head_dim = d->head_dim;
     const uint32_t group = (uint32_t) (d->n_head / d->n_head_kv);
+    /* Half the rows a workgroup where whole ones would not fill a round of two on
+     * each CU (f32: two rounds, since its products take so long that they cover what
+     * the smaller tile costs). us at half / whole: bf16 one prompt of 2048 rows (320
+     * whole ones) 46 / 57, of 4096 (640) 135 / 113; f32 of 4096 778 / 844, two of up
+     * to 8192 (2000) 3000 / 2789. */
+    uint64_t whole = 0;
+    for (int32_t i = 0; i < d->n_seq; ++i) {
+        if (d->q_len[i] > 0) whole += ((uint64_t) d->q_len[i] * group + ATT_MANY_ROWS - 1) / ATT_MANY_ROWS * (uint32_t) d->n_head_kv;
+    }
+    const uint32_t mode = whole < (d->dtype == SLLM_GFX950_F32 ? 4u : 2u) * (uint64_t) sllm_shim_cu() ? ATT_HALF : ATT_MANY, tile = k_rows[mode];
     for (int32_t i = 0; i < d->n_seq && st == SLLM_GFX950_OK; ++i) {
         const int32_t nq = d->q_len[i], nk = d->k_len ? d->k_len[i] : nq;
         if (nq < 0 || nk < 0 || p->n_q + (uint64_t) nq > SLLM_GFX950_ATTN_MAX_TOKENS || p->n_k + (uint64_t) nk > SLLM_GFX950_ATTN_MAX_TOKENS) {
@@ -1034,13 +1051,13 @@ int sllm_gfx950_prompt_create(const sllm_gfx950_prompt_desc *d, sllm_gfx950_prom
         }
         const uint32_t rows = (uint32_t) nq * group;
         for (int32_t h = 0; h < d->n_head_kv && st == SLLM_GFX950_OK; ++h) {
-            for (uint32_t r = 0; r < rows; r += ATT_ROWS) {
-                const uint32_t n = rows - r < ATT_ROWS ? rows - r : ATT_ROWS;
+            for (uint32_t r = 0; r < rows; r += tile) {
+                const uint32_t n = rows - r < tile ? rows - r : tile;
                 const int32_t last = (int32_t) ((r + n - 1) / group) + nk - nq + 1;    /* keys that the last row sees */
                 att_item *a = items_add(&it);
                 if (a == NULL) { st = FAIL_NOMEM("prompt_create: work items"); break; }
                 *a = (att_item) { r, n, (uint32_t) p->n_q, ATT_TOKENS, nk - nq + 1, 0, last > 0 ? (uint32_t) last : 0,
-                                  (uint32_t) p->n_k, (uint32_t) h, ATT_DIRECT, ATT_MANY, 0 };
+                                  (uint32_t) p->n_k, (uint32_t) h, ATT_DIRECT, mode, 0 };
             }
         }
         p->n_q += (uint64_t) nq;

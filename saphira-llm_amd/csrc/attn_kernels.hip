@@ -144,28 +144,28 @@ struct attention {
     uint32_t kcopy[KEYS ? QC : COPIES], vcopy[COPIES], vput[KEYS ? COPIES : 1];
 
     __device__ __forceinline__ void places() {
+        const uint32_t row = a.hd * (uint32_t) sizeof(T);
+        const uint32_t rowk = PAGED ? row : (uint32_t) a.k_tok, rowv = PAGED ? row : (uint32_t) a.v_tok;
 #pragma unroll
         for (int q = 0; q < QC; ++q) {
             if (!KEYS) koff[q] = li * L::ROWB + (((4u * q + g) ^ L::ksw(li)) * 16u);
-            else kcopy[q] = (4u * q + g) * 16u < a.hd * (uint32_t) sizeof(T) ? li * a.hd * (uint32_t) sizeof(T) + (4u * q + g) * 16u : PAST;
+            else kcopy[q] = (4u * q + g) * 16u < row ? li * rowk + (4u * q + g) * 16u : PAST;
         }
         const uint32_t r = WIDE ? 4u * g : 4u * g + (li >> 2);
         voff = L::VALUES + r * L::ROWB + (WIDE ? ((li >> 2) ^ L::vsw(r)) * 16u + (li & 3u) * 4u
                                              : (((li >> 1) & 1u) ^ L::vsw(r)) * 16u + (li & 1u) * 8u);
-        const uint32_t rowk = PAGED ? a.hd * (uint32_t) sizeof(T) : (uint32_t) a.k_tok;
-        const uint32_t rowv = PAGED ? rowk : (uint32_t) a.v_tok;
 #pragma unroll
         for (int j = 0; j < COPIES; ++j) {
             const uint32_t rg = (uint32_t) j * RPI + lane / L::CH, ch = lane % L::CH;
             if constexpr (KEYS) {                                // (16 rows further on: the same swap)
-                vcopy[j] = ch * 16u < rowv ? rg * rowv + ch * 16u : PAST;
+                vcopy[j] = ch * 16u < row ? rg * rowv + ch * 16u : PAST;
                 vput[j] = rg * L::ROWB + (ch ^ L::vsw(rg)) * 16u;
                 continue;
             }
             const uint32_t rt = wave * (uint32_t) GROUP + rg;
             const uint32_t ck = (ch ^ L::ksw(rt)) * 16u, cv = (ch ^ L::vsw(rt)) * 16u;
-            if (!KEYS) kcopy[j] = ck < a.hd * (uint32_t) sizeof(T) ? rg * rowk + ck : PAST;
-            vcopy[j] = cv < a.hd * (uint32_t) sizeof(T) ? rg * rowv + cv : PAST;
+            kcopy[j] = ck < row ? rg * rowk + ck : PAST;
+            vcopy[j] = cv < row ? rg * rowv + cv : PAST;
         }
     }
 
@@ -306,9 +306,10 @@ struct attention {
         __amdgpu_buffer_rsrc_t k[GROUPS], v[GROUPS];
 #pragma unroll
         for (int gr = 0; gr < GROUPS; ++gr) {
-            const int bytes = (int) uniform(rows_in(t * KT + (uint32_t) gr * GROUP) * (a.hd * (uint32_t) sizeof(T)));
-            k[gr] = __builtin_amdgcn_make_buffer_rsrc((void *) at.m[gr].k, (short) 0, bytes, 0x00020000);
-            v[gr] = __builtin_amdgcn_make_buffer_rsrc((void *) at.m[gr].v, (short) 0, bytes, 0x00020000);
+            const uint32_t n = rows_in(t * KT + (uint32_t) gr * GROUP), row = a.hd * (uint32_t) sizeof(T);
+            const uint32_t rowk = PAGED ? row : (uint32_t) a.k_tok, rowv = PAGED ? row : (uint32_t) a.v_tok;
+            k[gr] = __builtin_amdgcn_make_buffer_rsrc((void *) at.m[gr].k, (short) 0, (int) uniform(n ? n * rowk - (rowk - row) : 0u), 0x00020000);
+            v[gr] = __builtin_amdgcn_make_buffer_rsrc((void *) at.m[gr].v, (short) 0, (int) uniform(n ? n * rowv - (rowv - row) : 0u), 0x00020000);
         }
         // read once, and not kept (2: nontemporal): 64.9 -> 60.6 us for 8 sequences of 16384 positions, bf16
 #pragma unroll
@@ -793,6 +794,8 @@ __device__ __forceinline__ void attend_item(const att_args &a, const att_item &i
 // before it reads it anywhere.
 constexpr int VOTES = WAVES * 4;
 constexpr int max_of(int a, int b) { return a > b ? a : b; }
+template <typename T, int D> constexpr int LDS_BYTES =
+    max_of(max_of(tile<T, D, false>::LDS + VOTES, tile<T, D, true>::LDS), WAVES * ATT_FEW_ROWS * (D + 2) * 4);
 
 __device__ __forceinline__ att_item item_of(const att_args &a) {
     att_item it;
@@ -805,16 +808,18 @@ __device__ __forceinline__ att_item item_of(const att_args &a) {
 
 template <typename T, int D>
 __device__ __forceinline__ void prompt_body(const att_args &a) {
-    __shared__ __attribute__((aligned(1024))) uint8_t S[tile<T, D, false>::LDS + VOTES];
-    attend_item<T, T, D, 2, false, false>(a, item_of(a), S);
+    __shared__ __attribute__((aligned(1024))) uint8_t S[LDS_BYTES<T, D>];
+    const att_item it = item_of(a);
+    if (it.mode == ATT_HALF) attend_item<T, T, D, 1, false, false>(a, it, S);
+    else attend_item<T, T, D, 2, false, false>(a, it, S);
 }
 
 template <typename A, typename T, int D>
 __device__ __forceinline__ void paged_body(const att_args &a) {
-    __shared__ __attribute__((aligned(1024))) uint8_t S[max_of(max_of(tile<T, D, false>::LDS + VOTES, tile<T, D, true>::LDS), WAVES * 32 * (D + 2) * 4)];
+    __shared__ __attribute__((aligned(1024))) uint8_t S[LDS_BYTES<T, D>];
     const att_item it = item_of(a);
     if (it.mode == ATT_FEW) attend_item<A, T, D, 1, true, true>(a, it, S);
-    else if (it.mode == ATT_SOME) attend_item<A, T, D, 2, true, true>(a, it, S);
+    else if (it.mode == ATT_HALF) attend_item<A, T, D, 1, false, true>(a, it, S);
     else attend_item<A, T, D, 2, false, true>(a, it, S);
 }
 

@@ -7,13 +7,13 @@
 
 #include <stdint.h>
 
-/* rows (query token x head of one KV head) that a workgroup takes: with the
- * four waves on different rows, or on different keys of the same 16 or 32 */
-#define ATT_ROWS      128
+/* rows (query token x head of one KV head) that a workgroup takes: the four
+ * waves on different keys of the same 16, or with 16 or 32 rows each */
 #define ATT_FEW_ROWS  16
-#define ATT_SOME_ROWS 32
+#define ATT_HALF_ROWS 64
+#define ATT_MANY_ROWS 128
 #define ATT_THREADS   256
-enum { ATT_FEW, ATT_SOME, ATT_MANY };
+enum { ATT_FEW, ATT_HALF, ATT_MANY };
 
 #define ATT_DIRECT    0xffffffffu    /* att_item.part: rows go to the output */
 #define ATT_TOKENS    0xffffffffu    /* att_item.list: tokens in order */
@@ -33,7 +33,7 @@ typedef struct att_item {
     uint32_t kv;            /* paged: where the segment's page numbers start; packed: the first key's row */
     uint32_t head;
     uint32_t part;          /* row of the partial results that row0's go to, or ATT_DIRECT */
-    uint32_t mode;          /* ATT_FEW, ATT_SOME, ATT_MANY (prompts: unused) */
+    uint32_t mode;          /* ATT_FEW .. ATT_MANY */
     uint32_t pad;
 } att_item;
 
