@@ -13,11 +13,18 @@
  * pointers and row strides are multiples of 16 bytes. head_dim is a multiple
  * of 8, at most 128; n_head is a multiple of n_head_kv, and query head h reads
  * KV head h / (n_head / n_head_kv). Scores, softmax sums and products are held
- * in f32.
+ * in f32; the sum of weights times values that is carried along may be 256
+ * times the number of keys larger than the result, and overflows there.
  *
- * Calls may come from several threads: a cache's calls exclude each other, and
- * everything runs in call order on the one stream. Memory that another stream
- * writes or reads is the caller's to order with the library's stream.
+ * Calls may come from several threads, whichever device each has current: a
+ * cache's calls exclude each other, and everything runs in call order on the
+ * one stream. Memory that another stream writes or reads is the caller's to
+ * order with the library's stream.
+ *
+ * batch_store, batch_attend and prompt_attend are launches alone and may be
+ * captured into a graph. What takes pages or lays out work (batch_create,
+ * seq_fork, seq_copy, pages_compact, prompt_create) is refused while the stream
+ * is captured.
  */
 #ifndef SAPHIRA_AMD_SLLM_GFX950_ATTN_H
 #define SAPHIRA_AMD_SLLM_GFX950_ATTN_H
@@ -36,7 +43,7 @@ extern "C" {
 #define SLLM_GFX950_ATTN_MAX_HEAD_DIM 128
 #define SLLM_GFX950_ATTN_MAX_HEADS    1024
 #define SLLM_GFX950_ATTN_MAX_SEQS     65536       /* of one cache, batch or prompt plan */
-#define SLLM_GFX950_ATTN_MAX_TOKENS   (1 << 22)   /* new tokens of a batch, rows of a prompt plan */
+#define SLLM_GFX950_ATTN_MAX_TOKENS   (1 << 22)   /* new tokens of a batch, query or key rows of a prompt plan */
 #define SLLM_GFX950_ATTN_MAX_ROWS     (1 << 24)   /* new tokens x query heads of a batch */
 #define SLLM_GFX950_ATTN_MAX_LEN      (1 << 28)   /* positions of a sequence */
 
@@ -122,8 +129,10 @@ int     sllm_gfx950_pages_compact(sllm_gfx950_pages *p, int32_t *n_moved);
  * over an f16 cache (rounded to nearest by store; queries are not rounded).
  *
  * A batch holds its pages until it is destroyed, whatever happens to its
- * sequences meanwhile. Its launches may be captured into a graph, which is
- * valid while the batch lives.
+ * sequences meanwhile; the next batch of a sequence that was truncated may
+ * write into the last of them. Its launches may be captured into a graph, which
+ * is valid while the batch lives. They share the batch's memory for partial
+ * results: graphs of one batch are replayed one after the other.
  */
 typedef struct sllm_gfx950_batch sllm_gfx950_batch;
 
@@ -142,7 +151,7 @@ int  sllm_gfx950_batch_store(sllm_gfx950_batch *b, int32_t layer, const void *k,
  * out = softmax(scale q . k) v for q and out [rows][n_head][head_dim]: a row
  * sees its sequence's positions up to its own. Whole pages that several of the
  * batch's sequences share are read once for all of them. scale > 0; strides as
- * above (0: n_head * head_dim).
+ * above (0: n_head * head_dim). out overlaps neither q nor the cache.
  */
 int  sllm_gfx950_batch_attend(sllm_gfx950_batch *b, int32_t layer, const void *q, size_t q_stride, float scale,
                               void *out, size_t out_stride);

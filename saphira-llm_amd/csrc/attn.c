@@ -24,6 +24,32 @@
         if (!sllm_shim_is_open()) return sllm_shim_fail(SLLM_GFX950_ERR_NO_DEVICE, "library not open"); \
     } while (0)
 
+/*
+ * The library's device is the current one for the rest of the call and the
+ * caller's is afterwards: memory is taken on the current device, and a caller
+ * may have another one current, or be a thread that never set one.
+ */
+typedef struct device_scope { int was, moved; } device_scope;
+
+static int device_enter(device_scope *s) {
+    if (!sllm_shim_is_open()) return sllm_shim_fail(SLLM_GFX950_ERR_NO_DEVICE, "library not open");
+    hipError_t e = hipGetDevice(&s->was);
+    if (e != hipSuccess) return sllm_shim_hip_fail(e, "hipGetDevice");
+    if (s->was == sllm_shim_device()) return SLLM_GFX950_OK;
+    e = hipSetDevice(sllm_shim_device());
+    if (e != hipSuccess) return sllm_shim_hip_fail(e, "hipSetDevice");
+    s->moved = 1;
+    return SLLM_GFX950_OK;
+}
+static void device_leave(device_scope *s) { if (s->moved) hipSetDevice(s->was); }
+
+#define ATT_ON_DEVICE()                                                                  \
+    device_scope scope __attribute__((cleanup(device_leave))) = { 0, 0 };                \
+    do {                                                                                 \
+        const int scope_st = device_enter(&scope);                                       \
+        if (scope_st != SLLM_GFX950_OK) return scope_st;                                 \
+    } while (0)
+
 #define FAIL_ARG(...)   sllm_shim_fail(SLLM_GFX950_ERR_ARG, __VA_ARGS__)
 #define FAIL_NOMEM(...) sllm_shim_fail(SLLM_GFX950_ERR_NOMEM, __VA_ARGS__)
 
@@ -41,6 +67,15 @@ static int type_pair(int32_t act, int32_t cache) {
 static int bad_heads(int32_t n_head, int32_t n_head_kv, int32_t head_dim) {
     return n_head_kv < 1 || n_head < n_head_kv || n_head > SLLM_GFX950_ATTN_MAX_HEADS || n_head % n_head_kv != 0 ||
            head_dim < 8 || head_dim > SLLM_GFX950_ATTN_MAX_HEAD_DIM || head_dim % 8 != 0;
+}
+
+/* What changes who holds which page runs once, on the host: a graph would replay
+ * its copies into pages that are others' by then. */
+static int not_in_capture(const char *who) {
+    hipStreamCaptureStatus is = hipStreamCaptureStatusNone;
+    const hipError_t e = hipStreamIsCapturing(sllm_shim_stream(), &is);
+    if (e != hipSuccess) return sllm_shim_hip_fail(e, "hipStreamIsCapturing");
+    return is == hipStreamCaptureStatusNone ? SLLM_GFX950_OK : FAIL_ARG("%s: the stream is being captured", who);
 }
 
 static int misaligned(const void *p) { return ((uintptr_t) p & 15u) != 0; }
@@ -99,7 +134,7 @@ size_t sllm_gfx950_pages_bytes(const sllm_gfx950_pages_desc *d) {
 }
 
 int sllm_gfx950_pages_new(const sllm_gfx950_pages_desc *d, sllm_gfx950_pages **out) {
-    ATT_NEED_OPEN();
+    ATT_ON_DEVICE();
     if (out == NULL) return FAIL_ARG("pages_new: NULL out");
     *out = NULL;
     if (bad_desc(d)) return FAIL_ARG("pages_new: sizes, page length or type outside what a cache takes");
@@ -163,7 +198,14 @@ void sllm_gfx950_pages_free(sllm_gfx950_pages *p) {
 }
 
 void *sllm_gfx950_pages_mem(const sllm_gfx950_pages *p) { return p ? p->mem : NULL; }
-int32_t sllm_gfx950_pages_in_use(const sllm_gfx950_pages *p) { return p ? p->d.n_pages - p->n_free : 0; }
+int32_t sllm_gfx950_pages_in_use(const sllm_gfx950_pages *p) {
+    if (p == NULL) return 0;
+    pthread_mutex_t *mtx = (pthread_mutex_t *) &p->mtx;
+    pthread_mutex_lock(mtx);
+    const int32_t n = p->d.n_pages - p->n_free;
+    pthread_mutex_unlock(mtx);
+    return n;
+}
 
 /* (the cache's lock is held by everything below that takes or gives pages) */
 
@@ -283,13 +325,14 @@ int sllm_gfx950_seq_new(sllm_gfx950_pages *p, int32_t *seq) {
 }
 
 int sllm_gfx950_seq_fork(sllm_gfx950_pages *p, int32_t src, int32_t n_tokens, int32_t n, int32_t *seqs) {
-    ATT_NEED_OPEN();
+    ATT_ON_DEVICE();
     if (p == NULL || n < 0 || (n > 0 && seqs == NULL)) return FAIL_ARG("seq_fork: NULL or a count below 0");
     if (n > SLLM_GFX950_ATTN_MAX_SEQS) return FAIL_ARG("seq_fork: %d copies", n);
     pthread_mutex_lock(&p->mtx);
-    int st = SLLM_GFX950_OK;
+    int st = not_in_capture("seq_fork");
     const sequence *s = find(p, src);
-    if (s == NULL) st = FAIL_ARG("seq_fork: no sequence %d", src);
+    if (st != SLLM_GFX950_OK) { }
+    else if (s == NULL) st = FAIL_ARG("seq_fork: no sequence %d", src);
     else if (n_tokens < 0 || n_tokens > s->len) st = FAIL_ARG("seq_fork: %d of %d positions", n_tokens, s->len);
     const int32_t whole = n_tokens >> p->page_shift, rows = n_tokens & (p->d.page_tokens - 1);
     if (st == SLLM_GFX950_OK && rows && n > p->n_free) st = FAIL_NOMEM("seq_fork: %d pages wanted, %d free", n, p->n_free);
@@ -320,13 +363,13 @@ int sllm_gfx950_seq_fork(sllm_gfx950_pages *p, int32_t src, int32_t n_tokens, in
 }
 
 int sllm_gfx950_seq_copy(sllm_gfx950_pages *p, const int32_t *src, int32_t n, int32_t *seqs) {
-    ATT_NEED_OPEN();
+    ATT_ON_DEVICE();
     if (p == NULL || n < 0 || (n > 0 && (src == NULL || seqs == NULL))) return FAIL_ARG("seq_copy: NULL or a count below 0");
     if (n > SLLM_GFX950_ATTN_MAX_SEQS) return FAIL_ARG("seq_copy: %d copies", n);
     int32_t *ids = malloc((size_t) (n ? n : 1) * sizeof *ids);      /* (src and seqs may be one array) */
     if (ids == NULL) return FAIL_NOMEM("seq_copy: %d sequences", n);
     pthread_mutex_lock(&p->mtx);
-    int st = SLLM_GFX950_OK;
+    int st = not_in_capture("seq_copy");
     int64_t want = 0;
     for (int32_t i = 0; i < n && st == SLLM_GFX950_OK; ++i) {
         const sequence *s = find(p, src[i]);
@@ -429,15 +472,16 @@ int32_t sllm_gfx950_seq_tables(sllm_gfx950_pages *p, const int32_t *seqs, int32_
 }
 
 int sllm_gfx950_pages_compact(sllm_gfx950_pages *p, int32_t *n_moved) {
-    ATT_NEED_OPEN();
+    ATT_ON_DEVICE();
     if (n_moved) *n_moved = 0;
     if (p == NULL) return FAIL_ARG("pages_compact: NULL");
     pthread_mutex_lock(&p->mtx);
-    int st = SLLM_GFX950_OK;
+    int st = not_in_capture("pages_compact");
     const int32_t n_used = p->d.n_pages - p->n_free;
     /* where each page above n_used goes */
     int32_t *to = NULL, moved = 0;
-    if (p->open > 0) st = FAIL_ARG("pages_compact: %d batches are open", p->open);
+    if (st != SLLM_GFX950_OK) { }
+    else if (p->open > 0) st = FAIL_ARG("pages_compact: %d batches are open", p->open);
     else if ((to = malloc((size_t) p->d.n_pages * sizeof *to)) == NULL) st = FAIL_NOMEM("pages_compact: %d pages", p->d.n_pages);
     if (st == SLLM_GFX950_OK) {
         copies c;
@@ -495,7 +539,7 @@ struct sllm_gfx950_batch {
     int32_t   n_head, pair;
     uint32_t  n_tok;
     uint32_t  n_items;
-    int       join;                  /* a row has partial results */
+    uint32_t  join;                  /* the most partial results that a row has */
     buffer    buf;
     size_t    off_tables, off_list, off_toks, off_segs, off_part_o, off_part_ml;     /* (its items are at 0) */
     int32_t  *held;                  /* the pages it holds */
@@ -711,8 +755,9 @@ static int lay_out(sllm_gfx950_batch *b, plan *x, int32_t n, const int32_t *len0
     }
     /* segments of each sequence, and those with one part alone */
     uint32_t *seg_count = calloc((size_t) n + 1, sizeof *seg_count), *seg_at = calloc((size_t) n + 1, sizeof *seg_at);
+    uint32_t *parts = calloc((size_t) n + 1, sizeof *parts);
     uint8_t *alone = calloc((size_t) n + 1, 1);
-    if (seg_count == NULL || seg_at == NULL || alone == NULL) { st = FAIL_NOMEM("batch_create: tables"); goto out; }
+    if (seg_count == NULL || seg_at == NULL || parts == NULL || alone == NULL) { st = FAIL_NOMEM("batch_create: tables"); goto out; }
     const uint32_t step = p->d.dtype == SLLM_GFX950_F32 ? 16 : 32;
     const uint32_t split[2] = { split_keys(x, group, kv, 0, step), split_keys(x, group, kv, 1, step) };
     uint64_t n_part = 0, n_segs = 0, n_pages = 0;
@@ -739,7 +784,12 @@ static int lay_out(sllm_gfx950_batch *b, plan *x, int32_t n, const int32_t *len0
         seg_count[i] = 0;
         n_pages += (uint64_t) p->seq[x->seqs[i]].n_pages;
     }
-    b->join = n_part > 0;
+    for (int32_t i = 0; i < x->n_seg; ++i) {
+        const segment *s = &x->seg[i];
+        for (int32_t j = s->lo; j < s->hi; ++j) if (!alone[x->order[j]]) parts[x->order[j]] += s->n_split;
+    }
+    b->join = 0;
+    for (int32_t i = 0; i < n; ++i) if (parts[i] > b->join) b->join = parts[i];
 
     /* the work */
     for (int32_t i = 0; i < x->n_seg && st == SLLM_GFX950_OK; ++i) {
@@ -812,13 +862,14 @@ out:
     free(it.v);
     free(seg_count);
     free(seg_at);
+    free(parts);
     free(alone);
     return st;
 }
 
 int sllm_gfx950_batch_create(sllm_gfx950_pages *p, const int32_t *seqs, const int32_t *n_new, int32_t n, int32_t n_head,
                              int32_t act_dtype, sllm_gfx950_batch **out) {
-    ATT_NEED_OPEN();
+    ATT_ON_DEVICE();
     if (out == NULL) return FAIL_ARG("batch_create: NULL out");
     *out = NULL;
     if (p == NULL || n < 0 || n > SLLM_GFX950_ATTN_MAX_SEQS || (n > 0 && (seqs == NULL || n_new == NULL))) {
@@ -827,6 +878,8 @@ int sllm_gfx950_batch_create(sllm_gfx950_pages *p, const int32_t *seqs, const in
     if (bad_heads(n_head, p->d.n_head_kv, p->d.head_dim)) return FAIL_ARG("batch_create: %d query heads over %d", n_head, p->d.n_head_kv);
     const int pair = bad_type(act_dtype) ? -1 : type_pair(act_dtype, p->d.dtype);
     if (pair < 0) return FAIL_ARG("batch_create: rows of type %d over a cache of type %d", act_dtype, p->d.dtype);
+    int st = not_in_capture("batch_create");
+    if (st != SLLM_GFX950_OK) return st;
 
     const size_t n1 = (size_t) n + 1;
     sllm_gfx950_batch *b = calloc(1, sizeof *b);
@@ -834,7 +887,6 @@ int sllm_gfx950_batch_create(sllm_gfx950_pages *p, const int32_t *seqs, const in
     uint32_t *uwork = malloc(n1 * 2 * sizeof *uwork);
     segment *seg = calloc(n1 * 2, sizeof *seg);
     plan x = { .p = p, .seqs = seqs, .n_new = n_new, .seg = seg };
-    int st = SLLM_GFX950_OK;
     if (b == NULL || work == NULL || uwork == NULL || seg == NULL) {
         st = FAIL_NOMEM("batch_create: %d sequences", n);
         goto out;
@@ -948,7 +1000,7 @@ static uint64_t row_bytes(size_t stride, uint64_t width, uint32_t size) {
 }
 
 int sllm_gfx950_batch_store(sllm_gfx950_batch *b, int32_t layer, const void *k, size_t k_stride, const void *v, size_t v_stride) {
-    ATT_NEED_OPEN();
+    ATT_ON_DEVICE();
     if (b == NULL) return FAIL_ARG("batch_store: NULL");
     sllm_gfx950_pages *p = b->p;
     if (layer < 0 || layer >= p->d.n_layer) return FAIL_ARG("batch_store: layer %d of %d", layer, p->d.n_layer);
@@ -966,11 +1018,11 @@ int sllm_gfx950_batch_store(sllm_gfx950_batch *b, int32_t layer, const void *k, 
                             (uint32_t) ((threads + ATT_THREADS - 1) / ATT_THREADS), 2u * kv, ATT_THREADS, 0, args);
 }
 
-static int bad_scale(float scale) { return !(scale > 0.0f) || isinf(scale); }
+static int bad_scale(float scale) { return !(scale > 0.0f) || isinf((float) ((double) scale * LOG2E)); }
 
 int sllm_gfx950_batch_attend(sllm_gfx950_batch *b, int32_t layer, const void *q, size_t q_stride, float scale, void *out,
                              size_t out_stride) {
-    ATT_NEED_OPEN();
+    ATT_ON_DEVICE();
     if (b == NULL) return FAIL_ARG("batch_attend: NULL");
     sllm_gfx950_pages *p = b->p;
     if (layer < 0 || layer >= p->d.n_layer) return FAIL_ARG("batch_attend: layer %d of %d", layer, p->d.n_layer);
@@ -994,12 +1046,17 @@ int sllm_gfx950_batch_attend(sllm_gfx950_batch *b, int32_t layer, const void *q,
     int st = SLLM_GFX950_OK;
     void *args[] = { &a };
     st = sllm_shim_launch(sllm_shim_attn_function(SLLM_ATTN_ATTEND + b->pair * 2 + (int) wide), a.n_items, 1, ATT_THREADS, 0, args);
-    if (st == SLLM_GFX950_OK && b->join) {
+    if (st == SLLM_GFX950_OK && b->join > 0) {
         att_join_args j = { out, a.part_o, a.part_ml, (const att_tok *) (dev + b->off_toks), (const att_seg *) (dev + b->off_segs), ot,
-                            hd, group };
+                            hd, group, (uint32_t) b->n_head, 0 };
         void *jargs[] = { &j };
-        st = sllm_shim_launch(sllm_shim_attn_function(SLLM_ATTN_JOIN + (b->pair < 2 ? 0 : b->pair - 1) * 2 + (int) wide),
-                              b->n_tok, (uint32_t) b->n_head, ATT_THREADS, 0, jargs);
+        /* a workgroup a row, or where none has more than eight partial results a wave
+         * (us, a wave / a workgroup: 5120 rows of up to 4, 26.5 / 29.8; 8 sequences of
+         * over 16 parts a row 16.9 / 12.1; 5 to 16 parts alike) */
+        const int whole = b->join > 8;
+        const uint32_t heads = (uint32_t) b->n_head, gy = whole ? heads : (heads + ATT_THREADS / 64 - 1) / (ATT_THREADS / 64);
+        st = sllm_shim_launch(sllm_shim_attn_function(SLLM_ATTN_JOIN + 6 * whole + (b->pair < 2 ? 0 : b->pair - 1) * 2 + (int) wide),
+                              b->n_tok, gy, ATT_THREADS, 0, jargs);
     }
     pthread_mutex_unlock(&p->mtx);
     return st;
@@ -1017,16 +1074,17 @@ struct sllm_gfx950_prompt {
 };
 
 int sllm_gfx950_prompt_create(const sllm_gfx950_prompt_desc *d, sllm_gfx950_prompt **out) {
-    ATT_NEED_OPEN();
+    ATT_ON_DEVICE();
     if (out == NULL) return FAIL_ARG("prompt_create: NULL out");
     *out = NULL;
     if (d == NULL || bad_type(d->dtype) || bad_heads(d->n_head, d->n_head_kv, d->head_dim) || d->n_seq < 0 ||
         d->n_seq > SLLM_GFX950_ATTN_MAX_SEQS || (d->n_seq > 0 && d->q_len == NULL)) {
         return FAIL_ARG("prompt_create: type, heads, head dimension or sequences outside what a plan takes");
     }
+    int st = not_in_capture("prompt_create");
+    if (st != SLLM_GFX950_OK) return st;
     sllm_gfx950_prompt *p = calloc(1, sizeof *p);
     items it = { 0 };
-    int st = SLLM_GFX950_OK;
     if (p == NULL) return FAIL_NOMEM("prompt_create");
     p->dtype = d->dtype;
     p->n_head = d->n_head;
@@ -1049,6 +1107,7 @@ int sllm_gfx950_prompt_create(const sllm_gfx950_prompt_desc *d, sllm_gfx950_prom
             st = FAIL_ARG("prompt_create: sequence %d of %d and %d rows, or too many", i, nq, nk);
             break;
         }
+        if (whole > MAX_ITEMS) { st = FAIL_ARG("prompt_create: too many rows"); break; }
         const uint32_t rows = (uint32_t) nq * group;
         for (int32_t h = 0; h < d->n_head_kv && st == SLLM_GFX950_OK; ++h) {
             for (uint32_t r = 0; r < rows; r += tile) {
@@ -1095,9 +1154,9 @@ void sllm_gfx950_prompt_destroy(sllm_gfx950_prompt *p) {
 }
 
 /* A tensor [n][heads][hd] with strides tok and head in elements, 0 and 0: packed.
- * Bytes into *t and *h and how far it reaches into *extent; 0: not what a call takes. */
-static int strides(size_t tok, size_t head, uint64_t heads, uint64_t hd, uint64_t n, uint32_t size, uint64_t *t, uint64_t *h,
-                   uint64_t *extent) {
+ * Bytes into *t and *h; 0: not what a call takes (32 rows of a tile are apart by
+ * less than 2^32 bytes). */
+static int strides(size_t tok, size_t head, uint64_t heads, uint64_t hd, uint32_t size, uint64_t *t, uint64_t *h) {
     if (tok == 0 && head == 0) {
         tok = (size_t) (heads * hd);
         head = (size_t) hd;
@@ -1105,22 +1164,20 @@ static int strides(size_t tok, size_t head, uint64_t heads, uint64_t hd, uint64_
     if (tok > (1u << 25) || (uint64_t) head > 1ull << 40 || tok * size % 16u != 0 || head * size % 16u != 0) return 0;
     *t = (uint64_t) tok * size;
     *h = (uint64_t) head * size;
-    *extent = n == 0 ? 0 : (n - 1) * *t + (heads - 1) * *h + hd * size;
     return 1;
 }
 
 int sllm_gfx950_prompt_attend(sllm_gfx950_prompt *p, const sllm_gfx950_prompt_io *io) {
-    ATT_NEED_OPEN();
+    ATT_ON_DEVICE();
     if (p == NULL || io == NULL) return FAIL_ARG("prompt_attend: NULL");
     if (bad_scale(io->scale)) return FAIL_ARG("prompt_attend: scale %g", (double) io->scale);
     const uint32_t size = type_size(p->dtype), hd = (uint32_t) p->head_dim;
     att_args a = { .q = io->q, .out = io->out, .k = io->k, .v = io->v, .items = p->items, .hd = hd,
                    .group = (uint32_t) (p->n_head / p->n_head_kv), .n_items = p->n_items, .c = (float) ((double) io->scale * LOG2E) };
-    uint64_t qx, kx, vx, ox;
-    if (!strides(io->q_tok, io->q_head, (uint64_t) p->n_head, hd, p->n_q, size, &a.q_tok, &a.q_head, &qx) ||
-        !strides(io->k_tok, io->k_head, (uint64_t) p->n_head_kv, hd, p->n_k, size, &a.k_tok, &a.k_head, &kx) ||
-        !strides(io->v_tok, io->v_head, (uint64_t) p->n_head_kv, hd, p->n_k, size, &a.v_tok, &a.v_head, &vx) ||
-        !strides(io->out_tok, io->out_head, (uint64_t) p->n_head, hd, p->n_q, size, &a.out_tok, &a.out_head, &ox)) {
+    if (!strides(io->q_tok, io->q_head, (uint64_t) p->n_head, hd, size, &a.q_tok, &a.q_head) ||
+        !strides(io->k_tok, io->k_head, (uint64_t) p->n_head_kv, hd, size, &a.k_tok, &a.k_head) ||
+        !strides(io->v_tok, io->v_head, (uint64_t) p->n_head_kv, hd, size, &a.v_tok, &a.v_head) ||
+        !strides(io->out_tok, io->out_head, (uint64_t) p->n_head, hd, size, &a.out_tok, &a.out_head)) {
         return FAIL_ARG("prompt_attend: strides");
     }
     /* rows of out apart: heads within a token, or tokens within a head */

@@ -35,10 +35,6 @@ typedef short s16x4 __attribute__((ext_vector_type(4)));
 #define LDS_PTR(p) ((__attribute__((address_space(3))) void *) (p))
 
 constexpr int WAVES = 4;
-#ifndef ILV_A
-#define ILV_A 4
-#define ILV_B 4
-#endif
 
 // what copies to LDS read in place of keys past the end and dimensions past head_dim
 __device__ __attribute__((aligned(16))) uint32_t att_zeros[4];
@@ -117,7 +113,7 @@ struct attention {
     static constexpr int KS = KT / 16;                           // 16-key subtiles
     static constexpr int DT = D / 16;
     static constexpr int QC = D * (int) sizeof(T) / 64;          // 16-byte pieces of a row that a lane holds
-    static constexpr int GROUP = KEYS ? (KT < 16 ? KT : 16) : KT / WAVES;   // rows that one address serves: within a page
+    static constexpr int GROUP = KEYS ? 16 : KT / WAVES;   // rows that one address serves: within a page
     static constexpr int GROUPS = (KEYS ? KT : KT / WAVES) / GROUP;
     static constexpr int RPI = 1024 / L::ROWB;                   // rows of a copy instruction
     typedef typename vec8<T>::type t8;
@@ -577,21 +573,23 @@ struct attention {
     }
 
     // The order of a loop iteration's instructions: the keys' reads, then each matrix
-    // instruction with its share of the vector ones and of the values' reads.
+    // instruction with its share of the vector ones and of the values' reads. (2 to 8
+    // vector instructions each: within 2 % of each other.)
     __device__ __forceinline__ static void interleave() {
+        constexpr int VECTOR = 4;
         constexpr int PER = (WIDE ? 4 : 1) * NT * (SPLIT ? 2 : 1);
         constexpr int MS = KS * QC * PER, MP = DT * PER, DV = WIDE ? 4 * DT : 0;
         __builtin_amdgcn_sched_group_barrier(0x100, KS * QC, 0);
 #pragma unroll
         for (int i = 0; i < MS; ++i) {
             __builtin_amdgcn_sched_group_barrier(0x8, 1, 0);
-            __builtin_amdgcn_sched_group_barrier(0x2, ILV_A, 0);
+            __builtin_amdgcn_sched_group_barrier(0x2, VECTOR, 0);
             if (i < DV) __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
         }
 #pragma unroll
         for (int i = 0; i < MP; ++i) {
             __builtin_amdgcn_sched_group_barrier(0x8, 1, 0);
-            __builtin_amdgcn_sched_group_barrier(0x2, ILV_B, 0);
+            __builtin_amdgcn_sched_group_barrier(0x2, VECTOR, 0);
         }
     }
 
@@ -845,33 +843,35 @@ PROMPT(sllm_k_prompt_bf16_128, __bf16, 128)
 
 namespace {
 
-// The partial results of one row, a workgroup a row: out = sum_i f_i o_i / sum_i f_i l_i
-// with f_i = 2^(m_i - M), M the largest m_i. The waves take every fourth split of a
-// segment and are added up in order, so the same call gives the same bits. What costs
-// is the chain of loads (token, segment, parts): a part's o, m and l are asked for
-// together, and several splits at once.
-template <typename A, int D>
+// The partial results of one row: out = sum_i f_i o_i / sum_i f_i l_i with f_i =
+// 2^(m_i - M), M the largest m_i, added up in an order that the split alone gives,
+// so that the same call gives the same bits. WHOLE: a workgroup a row, its waves
+// taking every fourth split of a segment; else a wave a row. What costs is the chain
+// of loads (token, segment, parts): a part's o, m and l are asked for together, and
+// several splits at once.
+template <typename A, int D, bool WHOLE>
 __device__ __forceinline__ void join_body(const att_join_args &a) {
-    constexpr int V = D / 64;
+    constexpr int V = D / 64, UN = 4;
     typedef float vec __attribute__((ext_vector_type(V)));
-    __shared__ float so[WAVES][D], sm[WAVES][2];
     const uint32_t lane = threadIdx.x & 63u, wave = uniform(threadIdx.x >> 6);
-    const uint32_t tok = blockIdx.x, h = blockIdx.y, kvh = h / a.group, hh = h % a.group;
+    const uint32_t tok = blockIdx.x, h = WHOLE ? blockIdx.y : blockIdx.y * WAVES + wave;
+    if (h >= a.n_head) return;
+    const uint32_t kvh = h / a.group, hh = h % a.group;
     const uint32_t seg0 = C_CAST(uint32_t, &a.toks[tok].seg0)[0], n_seg = C_CAST(uint32_t, &a.toks[tok].n_seg)[0];
     const uint32_t at = C_CAST(uint32_t, &a.toks[tok].t)[0] * a.group + hh;
     if (n_seg == 0) return;                                      // written already
+    constexpr uint32_t STEP = WHOLE ? WAVES : 1;
     float top = LOWEST, sum = 0.0f, x[V] = {};
     for (uint32_t i = 0; i < n_seg; ++i) {
         const uint32_t part0 = C_CAST(uint32_t, &a.segs[seg0 + i].part0)[0], n_rows = C_CAST(uint32_t, &a.segs[seg0 + i].n_rows)[0];
         const uint32_t n_split = C_CAST(uint32_t, &a.segs[seg0 + i].n_split)[0], off = C_CAST(uint32_t, &a.segs[seg0 + i].row_off)[0];
         const uint64_t row = part0 + (uint64_t) kvh * n_split * n_rows + off + at;
-        constexpr int UN = 4;
-        for (uint32_t k = wave; k < n_split; k += WAVES * UN) {
+        for (uint32_t k = WHOLE ? wave : 0u; k < n_split; k += STEP * UN) {
             float m[UN], l[UN];
             vec o[UN];
 #pragma unroll
             for (int u = 0; u < UN; ++u) {                       // (past the end: the last split again, with no weight)
-                const uint64_t r = row + (uint64_t) min(k + (uint32_t) u * WAVES, n_split - 1u) * n_rows;
+                const uint64_t r = row + (uint64_t) min(k + (uint32_t) u * STEP, n_split - 1u) * n_rows;
                 m[u] = G_CAST(const float, a.part_ml)[2 * r];
                 l[u] = G_CAST(const float, a.part_ml)[2 * r + 1];
                 o[u] = *G_CAST(const vec, a.part_o + r * D + V * lane);
@@ -886,7 +886,7 @@ __device__ __forceinline__ void join_body(const att_join_args &a) {
             for (int v = 0; v < V; ++v) x[v] *= f;
 #pragma unroll
             for (int u = 0; u < UN; ++u) {
-                if (k + (uint32_t) u * WAVES < n_split) {
+                if (k + (uint32_t) u * STEP < n_split) {
                     const float e = __builtin_amdgcn_exp2f(m[u] - up);
                     sum = fmaf(l[u], e, sum);
 #pragma unroll
@@ -895,22 +895,31 @@ __device__ __forceinline__ void join_body(const att_join_args &a) {
             }
         }
     }
+    A *out = (A *) ((uint8_t *) a.out + tok * a.out_tok) + (uint64_t) h * a.hd;
+    if constexpr (!WHOLE) {
+        if (V * lane < a.hd) {
 #pragma unroll
-    for (int v = 0; v < V; ++v) so[wave][V * lane + v] = x[v];
-    if (lane == 0) {
-        sm[wave][0] = top;
-        sm[wave][1] = sum;
-    }
-    __syncthreads();
-    if (threadIdx.x >= a.hd) return;
-    float all = fmaxf(fmaxf(sm[0][0], sm[1][0]), fmaxf(sm[2][0], sm[3][0])), l = 0.0f, o = 0.0f;
+            for (int v = 0; v < V; ++v) G_CAST(A, out)[V * lane + v] = (A) (x[v] / sum);
+        }
+    } else {
+        __shared__ float so[WAVES][D], sm[WAVES][2];
 #pragma unroll
-    for (int w = 0; w < WAVES; ++w) {
-        const float e = __builtin_amdgcn_exp2f(sm[w][0] - all);
-        l = fmaf(sm[w][1], e, l);
-        o = fmaf(so[w][threadIdx.x], e, o);
+        for (int v = 0; v < V; ++v) so[wave][V * lane + v] = x[v];
+        if (lane == 0) {
+            sm[wave][0] = top;
+            sm[wave][1] = sum;
+        }
+        __syncthreads();
+        if (threadIdx.x >= a.hd) return;
+        float all = fmaxf(fmaxf(sm[0][0], sm[1][0]), fmaxf(sm[2][0], sm[3][0])), l = 0.0f, o = 0.0f;
+#pragma unroll
+        for (int w = 0; w < WAVES; ++w) {
+            const float e = __builtin_amdgcn_exp2f(sm[w][0] - all);
+            l = fmaf(sm[w][1], e, l);
+            o = fmaf(so[w][threadIdx.x], e, o);
+        }
+        G_CAST(A, out)[threadIdx.x] = (A) (o / l);
     }
-    *G_CAST(A, (uint8_t *) a.out + tok * a.out_tok + (uint64_t) (h * a.hd + threadIdx.x) * sizeof(A)) = (A) (o / l);
 }
 
 // A step's rows into their pages: a thread for each eight values of a row,
@@ -942,7 +951,9 @@ __device__ __forceinline__ void store_body(const att_store_args &a) {
 
 }  // namespace
 
-#define JOIN(name, A, D) extern "C" __global__ void __launch_bounds__(ATT_THREADS) name(const att_join_args a) { join_body<A, D>(a); }
+#define JOIN(name, A, D)                                                                                                                  \
+    extern "C" __global__ void __launch_bounds__(ATT_THREADS) name(const att_join_args a) { join_body<A, D, false>(a); }                  \
+    extern "C" __global__ void __launch_bounds__(ATT_THREADS) name##_whole(const att_join_args a) { join_body<A, D, true>(a); }
 #define STORE(name, A, T) extern "C" __global__ void __launch_bounds__(ATT_THREADS) name(const att_store_args a) { store_body<A, T>(a); }
 
 JOIN(sllm_k_attn_join_f32_64, float, 64)

@@ -75,7 +75,7 @@ typedef struct att_join_args {
     const att_tok  *toks;
     const att_seg  *segs;
     uint64_t        out_tok;         /* bytes */
-    uint32_t        hd, group;
+    uint32_t        hd, group, n_head, pad;
 } att_join_args;
 
 typedef struct att_store_args {

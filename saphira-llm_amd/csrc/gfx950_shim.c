@@ -295,11 +295,11 @@ static int load_attn_functions(void) {
     static const char *const rest[4] = { "store_f32", "store_f32f16", "store_16", "copy" };
     for (int i = 0; i < SLLM_ATTN_FUNCTIONS; ++i) {
         char name[64];
-        const int of = i < SLLM_ATTN_PROMPT ? i : i < SLLM_ATTN_JOIN ? i - SLLM_ATTN_PROMPT : i - SLLM_ATTN_JOIN;
+        const int of = i < SLLM_ATTN_PROMPT ? i : i < SLLM_ATTN_JOIN ? i - SLLM_ATTN_PROMPT : (i - SLLM_ATTN_JOIN) % 6;
         const int type = i < SLLM_ATTN_PROMPT ? of / 2 : of / 2 ? of / 2 + 1 : 0;        /* (rows of f32, f16, bf16) */
         if (i >= SLLM_ATTN_STORE) snprintf(name, sizeof name, "sllm_k_attn_%s", rest[i - SLLM_ATTN_STORE]);
-        else snprintf(name, sizeof name, "sllm_k_%s_%s_%d", i < SLLM_ATTN_PROMPT ? "attend" : i < SLLM_ATTN_JOIN ? "prompt" : "attn_join",
-                      types[type], of % 2 ? 128 : 64);
+        else snprintf(name, sizeof name, "sllm_k_%s_%s_%d%s", i < SLLM_ATTN_PROMPT ? "attend" : i < SLLM_ATTN_JOIN ? "prompt" : "attn_join",
+                      types[type], of % 2 ? 128 : 64, i >= SLLM_ATTN_JOIN + 6 ? "_whole" : "");
         HIP_TRY(hipModuleGetFunction(&g.k_attn[i], g.attn_mod, name));
     }
     return SLLM_GFX950_OK;
@@ -550,6 +550,7 @@ static int launch(hipFunction_t f, uint32_t grid, uint32_t block, uint32_t lds, 
 int sllm_shim_is_open(void) { return g.open; }
 hipStream_t sllm_shim_stream(void) { return g.stream; }
 int sllm_shim_cu(void) { return g.cu; }
+int sllm_shim_device(void) { return g.device; }
 
 int sllm_shim_fail(int status, const char *fmt, ...) {
     va_list ap;

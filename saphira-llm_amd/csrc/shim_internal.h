@@ -59,6 +59,7 @@ SLLM_HIDDEN int         sllm_shim_d2h_host(void *dst, const void *src, size_t by
 SLLM_HIDDEN int         sllm_shim_is_open(void);
 SLLM_HIDDEN hipStream_t sllm_shim_stream(void);
 SLLM_HIDDEN int         sllm_shim_cu(void);
+SLLM_HIDDEN int         sllm_shim_device(void);
 SLLM_HIDDEN int         sllm_shim_fail(int status, const char *fmt, ...)
     __attribute__((format(printf, 2, 3)));
 SLLM_HIDDEN int         sllm_shim_hip_fail(hipError_t e, const char *what);
@@ -72,8 +73,8 @@ SLLM_HIDDEN int         sllm_shim_decode_function(const char *name, hipFunction_
 enum {
     SLLM_ATTN_ATTEND = 0,                        /* + types * 2 + wide */
     SLLM_ATTN_PROMPT = 8,                        /* + type * 2 + wide */
-    SLLM_ATTN_JOIN = 14,                         /* + type * 2 + wide */
-    SLLM_ATTN_STORE = 20, SLLM_ATTN_COPY = 23, SLLM_ATTN_FUNCTIONS = 24
+    SLLM_ATTN_JOIN = 14,                         /* + type * 2 + wide, a wave a row; + 6: a workgroup a row */
+    SLLM_ATTN_STORE = 26, SLLM_ATTN_COPY = 29, SLLM_ATTN_FUNCTIONS = 30
 };
 SLLM_HIDDEN hipFunction_t sllm_shim_attn_function(int i);
 /* grid gx x gy of `block` threads on the library stream */

@@ -59,6 +59,32 @@ def attend(q, k, v, sees, scale, act, cache):
     return out, tol
 
 
+def attend_rows(q, k, v, sees, scale, act, cache):
+    """attend() with a head's rows at once, for many of them."""
+    rows, heads, d = q.shape
+    keys, kv = k.shape[:2]
+    half = {"float32": 2.0 ** -24, "float16": 2.0 ** -11, "bfloat16": 2.0 ** -8}
+    up = 0.0 if cache == "float32" else 2.0 ** -22 if act == "float32" else half[cache]
+    sub = 2.0 ** -25 if cache == "float16" else 0.0
+    out, tol = np.zeros((rows, heads, d)), np.zeros((rows, heads, d))
+    n = np.clip(np.asarray(sees), 0, keys)
+    some = n > 0
+    seen = np.arange(keys)[None] < n[some, None]
+    for h in range(heads if some.any() else 0):
+        kh, vh, qh = k[:, h // (heads // kv)], v[:, h // (heads // kv)], q[some, h]
+        s = scale * (qh @ kh.T)
+        p = np.where(seen, np.exp(s - np.where(seen, s, -np.inf).max(1, keepdims=True)), 0.0)
+        total = p.sum(1, keepdims=True)
+        out[some, h] = p @ vh / total
+        a = p @ np.abs(vh) / total
+        b = (scale * np.where(seen, np.abs(qh) @ np.abs(kh).T, 0.0)).max(1)
+        t = np.where(seen, np.abs(s), 0.0).max(1) * 1.4427 * 2
+        e = ((d + 4) * 2.0 ** -24 * b + 3 * 2.0 ** -24 * t + 2.0 ** -23)[:, None]
+        tol[some, h] = (a * (2 * e + (n[some, None] + 8) * 2.0 ** -24 + up) + sub * (seen.astype(float) @ np.abs(vh)) +
+                        half[act] * np.abs(out[some, h]) + 1e-37)
+    return out, tol
+
+
 def check(got, want, tol, what=""):
     got = got.double().numpy().reshape(want.shape)
     bad = ~(np.abs(got - want) <= tol)

@@ -19,6 +19,10 @@
  *   fakehip_live()               resources held: memory, modules, streams,
  *                                events, graphs
  *   fakehip_calls()              HIP calls made so far
+ *   fakehip_current(d)           device d is the calling thread's current one: it
+ *                                is not the reported one unless 0, and takes
+ *                                neither memory nor launches
+ *   fakehip_capture(on)          the streams are being captured, or not
  *   fakehip_launches()           kernels launched since the last fakehip_clear:
  *                                name:grid, a space behind each
  */
@@ -39,6 +43,8 @@ static long     g_live;
 static unsigned long g_calls;
 static char     g_launches[4096];     /* (names past its end are dropped) */
 static size_t   g_launches_len;
+static __thread int g_current;
+static int      g_capturing;
 
 FAKE_EXPORT void fakehip_fail(const char *fn, int err, unsigned skip) {
     snprintf(g_fail_fn, sizeof g_fail_fn, "%s", fn);
@@ -50,6 +56,8 @@ FAKE_EXPORT void fakehip_clear(void) { g_fail_skip = -1; g_fired = 0; g_launches
 FAKE_EXPORT const char *fakehip_launches(void) { return g_launches; }
 FAKE_EXPORT int  fakehip_fired(void) { return g_fired; }
 FAKE_EXPORT long fakehip_live(void) { return g_live; }
+FAKE_EXPORT void fakehip_current(int d) { g_current = d; }
+FAKE_EXPORT void fakehip_capture(int on) { g_capturing = on; }
 FAKE_EXPORT unsigned long fakehip_calls(void) { return g_calls; }
 
 static int inject(const char *fn) {
@@ -88,6 +96,7 @@ static hipError_t fake_release(void *p) {
 hipError_t hipMalloc(void **p, size_t bytes) {
     *p = NULL;
     INJECT();
+    if (g_current != 0) return hipErrorInvalidDevice;
     *p = fake_alloc(bytes);
     return *p ? hipSuccess : hipErrorOutOfMemory;
 }
@@ -138,7 +147,13 @@ hipError_t hipGetDeviceProperties(hipDeviceProp_t *p, int d) {
     p->totalGlobalMem = (size_t) 288 << 30;
     return hipSuccess;
 }
-hipError_t hipSetDevice(int d) { INJECT(); return d == 0 ? hipSuccess : hipErrorInvalidDevice; }
+hipError_t hipSetDevice(int d) {
+    INJECT();
+    if (d != 0 && d != 1) return hipErrorInvalidDevice;
+    g_current = d;
+    return hipSuccess;
+}
+hipError_t hipGetDevice(int *d) { INJECT(); *d = g_current; return hipSuccess; }
 const char *hipGetErrorString(hipError_t e) {
     static char buf[64];
     snprintf(buf, sizeof buf, "fake HIP error %d", (int) e);
@@ -183,6 +198,7 @@ hipError_t hipModuleLaunchKernel(hipFunction_t f, unsigned int gx, unsigned int 
                                  hipStream_t s, void **args, void **extra) {
     (void) gx; (void) gy; (void) gz; (void) bx; (void) by; (void) bz; (void) lds; (void) s; (void) extra;
     INJECT();
+    if (g_current != 0) return hipErrorInvalidHandle;
     const char *name = ((const fake_fn *) f)->name;
     if (g_launches_len + strlen(name) + 13 <= sizeof g_launches) {
         g_launches_len += (size_t) snprintf(g_launches + g_launches_len, sizeof g_launches - g_launches_len, "%s:%u ", name, gx);
@@ -224,6 +240,12 @@ hipError_t hipStreamEndCapture(hipStream_t s, hipGraph_t *g) {
     INJECT();
     *g = (hipGraph_t) malloc(1);
     ++g_live;
+    return hipSuccess;
+}
+hipError_t hipStreamIsCapturing(hipStream_t s, hipStreamCaptureStatus *is) {
+    (void) s;
+    INJECT();
+    *is = g_capturing ? hipStreamCaptureStatusActive : hipStreamCaptureStatusNone;
     return hipSuccess;
 }
 hipError_t hipGraphInstantiate(hipGraphExec_t *x, hipGraph_t g, hipGraphNode_t *node, char *log, size_t n) {

@@ -21,7 +21,7 @@ def normal(seed, *shape):
     return torch.randn(*shape, generator=g)
 
 
-def prompt(amd, dev, dtype, heads, kv, d, q_len, k_len=None, seed=0, edit=None, scale=None):
+def prompt(amd, dev, dtype, heads, kv, d, q_len, k_len=None, seed=0, edit=None, scale=None, oracle=ora.attend):
     """Run and check one prompt plan on packed tensors; returns the output."""
     k_len = q_len if k_len is None else k_len
     T = ora.TYPES[dtype]
@@ -38,8 +38,8 @@ def prompt(amd, dev, dtype, heads, kv, d, q_len, k_len=None, seed=0, edit=None, 
     got = ora.from_bits(out.download(ora.store_type(dtype), sum(q_len) * heads * d), dtype).view(-1, heads, d)
     a = b = 0
     for i, (nq, nk) in enumerate(zip(q_len, k_len)):
-        want, tol = ora.attend(q[a:a + nq].double().numpy(), k[b:b + nk].double().numpy(), v[b:b + nk].double().numpy(),
-                               np.arange(nq) + nk - nq + 1, scale, dtype, dtype)
+        want, tol = oracle(q[a:a + nq].double().numpy(), k[b:b + nk].double().numpy(), v[b:b + nk].double().numpy(),
+                           np.arange(nq) + nk - nq + 1, scale, dtype, dtype)
         ora.check(got[a:a + nq], want, tol, f"sequence {i}")
         a, b = a + nq, b + nk
     plan.close()
@@ -144,6 +144,59 @@ def test_prompt_strides(amd, dev, dtype):
     again = ora.from_bits(bo.download(ora.store_type(dtype), n * heads * d), dtype).view(heads, n, d).transpose(0, 1)
     assert torch.equal(again, rows[:, :, :d])
     for b in bufs + [bx, bo]:
+        b.free()
+
+
+# Plans of over a thousand tiles of 128 rows: those take workgroups of 128 rows, smaller plans 64.
+
+@pytest.mark.parametrize("dtype", list(ora.TYPES))
+@pytest.mark.parametrize("heads,kv,d,q_len,k_len", [(512, 512, 64, [129, 130], None), (768, 256, 64, [100, 45, 7], [100, 145, 4]),
+                                                    (256, 256, 128, [300, 129], None), (512, 256, 80, [70, 131, 1], [75, 131, 260])])
+def test_prompt_many_tiles(amd, dev, dtype, heads, kv, d, q_len, k_len):
+    assert sum(-(-n * (heads // kv) // 128) for n in q_len) * kv >= 1024
+    prompt(amd, dev, dtype, heads, kv, d, q_len, k_len, seed=17, oracle=ora.attend_rows)
+
+
+@pytest.mark.parametrize("dtype", list(ora.TYPES))
+def test_prompt_many_tiles_with_strides_and_what_is_not_finite(amd, dev, dtype):
+    """As packed, from rows with gaps and as [head][token]; then a key and values
+    that are not finite, which reach the rows that see them alone."""
+    heads, kv, d, lens = 512, 512, 64, [129, 130]
+    clean = prompt(amd, dev, dtype, heads, kv, d, lens, seed=18, oracle=ora.attend_rows)
+    T, n = ora.TYPES[dtype], sum(lens)
+    q, k, v = (normal(18 + i, n, heads, d).to(T) for i in range(3))
+    row, size = 3 * heads * d + 24, q.element_size()
+    x = torch.zeros(n, row, dtype=T)
+    for i, y in enumerate((q, k, v)):
+        x[:, i * (heads * d + 8):][:, :heads * d] = y.view(n, -1)
+    plan = amd.PromptAttention(dev, dtype, heads, kv, d, lens)
+    bo, bx = dev.alloc(clean.numel() * size), dev.put(ora.bits(x))
+
+    def out():
+        dev.sync()
+        return ora.from_bits(bo.download(ora.store_type(dtype), clean.numel()), dtype)
+
+    plan.run(bx.ptr, bx.ptr + (heads * d + 8) * size, bx.ptr + 2 * (heads * d + 8) * size, bo.ptr, d ** -0.5, (row, d), (row, d),
+             (row, d))
+    assert torch.equal(out().view_as(clean), clean)
+    bufs = [dev.put(ora.bits(y.transpose(0, 1).contiguous())) for y in (q, k, v)]
+    plan.run(*(b.ptr for b in bufs), bo.ptr, d ** -0.5, (d, n * d), (d, n * d), (d, n * d), (d, n * d))
+    assert torch.equal(out().view(heads, n, d).transpose(0, 1), clean)
+    k[129 + 60, 5, 3] = math.nan
+    v[129 + 20, 6, 5] = math.inf
+    v[129 + 129, :, 7] = -math.inf
+    more = [dev.put(ora.bits(y)) for y in (q, k, v)]
+    plan.run(*(b.ptr for b in more), bo.ptr, d ** -0.5)
+    got = out().view_as(clean)
+    seen = torch.zeros_like(clean, dtype=torch.bool)
+    seen[129 + 60:, 5] = True
+    seen[129 + 20:, 6, 5] = True
+    seen[129 + 129, :, 7] = True
+    assert torch.equal(got[~seen], clean[~seen])
+    assert not torch.isfinite(got[129 + 60:, 5].float()).any() and not torch.isfinite(got[129 + 20:, 6, 5].float()).any()
+    assert not torch.isfinite(got[129 + 129, :, 7].float()).any()
+    plan.close()
+    for b in bufs + more + [bo, bx]:
         b.free()
 
 
@@ -598,6 +651,34 @@ def test_batch_in_a_graph(amd, dev):
             y.free()
     c.close()
     bx.free()
+
+
+def test_what_takes_pages_is_refused_in_a_capture(amd, dev):
+    torch.cuda.init()
+    stream = torch.cuda.ExternalStream(amd.lib().sllm_gfx950_stream())
+    m = Model(amd, dev, "float16", "float16", 1, 2, 64, 16, 40)
+    s = m.new()
+    b, first = m.step([s], [50], 4, keep=True)
+    q = normal(m.seed, 50, 4, 64).half()
+    bq, bo = dev.put(ora.bits(q)), dev.alloc(q.numel() * 2)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g, stream=stream, capture_error_mode="thread_local"):
+        for call in (lambda: m.cache.batch([s], [1], 4, "float16"), lambda: m.cache.fork(s, 37, 1), lambda: m.cache.copy([s]),
+                     m.cache.compact, lambda: amd.PromptAttention(dev, "float16", 4, 2, 64, [9])):
+            with pytest.raises(amd.GFX950Error, match="captured"):
+                call()
+        b.attend(0, bq.ptr, bo.ptr, 0.125)
+    assert m.cache.length(s) == 50 and m.cache.in_use() == 4
+    for _ in range(3):
+        bo.upload(np.zeros(q.numel(), np.int16))
+        with torch.cuda.stream(stream):
+            g.replay()
+        dev.sync()
+        assert torch.equal(ora.from_bits(bo.download(np.int16, q.numel()), "float16").view_as(first[0]), first[0])
+        m.check_memory()
+    b.close()
+    m.close()
+    bq.free(), bo.free()
 
 
 def test_the_same_call_gives_the_same_bits(amd, dev):
