@@ -168,7 +168,7 @@ struct attention {
     // rows: lane li of row tile nt
     int lim[NT];                    // keys the row sees
     float c[NT];
-    float m[NT], l[NT];
+    float m[NT], l[NT];             // c times the running maximum, and the lane's share of the sum
     f32x4 o[DT][NT];
     // a lane's pieces of q: 8 values (SPLIT: and what rounding left of them), or 4 f32
     t8 qf[WIDE ? 1 : NT][WIDE ? 1 : QC], ql[SPLIT ? NT : 1][SPLIT ? QC : 1];
@@ -365,38 +365,43 @@ struct attention {
         f32x4 w[WIDE ? NT : 1];
     };
 
-    // s to p. The maximum moves only where a score is over it by 8 or more (as a power of
-    // two): until then p is at most 256, which costs no precision, and the sums need no
-    // scaling. Whether any did; then f is what the sums so far are to be scaled by.
-    __device__ __forceinline__ bool soften(const scores &s, probs &p, float (&f)[NT]) {
+    // The maximum moves only where a score is over it by 8 or more (as a power of two):
+    // until then p is at most 256, which costs no precision, the sums need no scaling, and
+    // the lanes that hold a row need not agree on its largest score. Whether any did; then
+    // f is what the sums of products so far are to be scaled by.
+    __device__ __forceinline__ bool adjust(const scores &s, float (&f)[NT]) {
         float top[NT];
-        bool over[NT], any = false;
+        bool over = false;
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
-            top[nt] = m[nt];
+            top[nt] = s[0][nt][0];
 #pragma unroll
             for (int ks = 0; ks < KS; ++ks) {
 #pragma unroll
                 for (int i = 0; i < 4; ++i) top[nt] = fmaxf(top[nt], s[ks][nt][i]);
             }
-            top[nt] = row_max(top[nt]);
-            over[nt] = (top[nt] - m[nt]) * c[nt] > 8.0f;             // (the row's own scores alone decide)
-            any |= over[nt];
+            over |= fmaf(top[nt], c[nt], -m[nt]) > 8.0f;
         }
-        const bool moved = __any(any);
+        if (!__any(over)) return false;
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
-            const float to = over[nt] ? top[nt] : m[nt];
-            f[nt] = __builtin_amdgcn_exp2f((m[nt] - to) * c[nt]);
+            const float t = row_max(top[nt]), to = fmaf(t, c[nt], -m[nt]) > 8.0f ? t * c[nt] : m[nt];   // (by the row's own scores alone)
+            f[nt] = __builtin_amdgcn_exp2f(m[nt] - to);
+            l[nt] *= f[nt];
             m[nt] = to;
-            // m is at least the lowest float, so a masked -inf gives 2^-inf = 0 and never inf - inf
-            const float mc = fmaxf(to * c[nt], LOWEST);
+        }
+        return true;
+    }
+    // s to p (m is at least the lowest float: a masked -inf gives 2^-inf = 0 and never inf - inf)
+    __device__ __forceinline__ void soften(const scores &s, probs &p) {
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
             float sum = 0.0f;
 #pragma unroll
             for (int ks = 0; ks < KS; ++ks) {
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                    const float x = __builtin_amdgcn_exp2f(fmaf(s[ks][nt][i], c[nt], -mc));
+                    const float x = __builtin_amdgcn_exp2f(fmaf(s[ks][nt][i], c[nt], -m[nt]));
                     sum += x;
                     if constexpr (WIDE) {
                         p.w[nt][i] = x;
@@ -406,13 +411,11 @@ struct attention {
                     }
                 }
             }
-            l[nt] = fmaf(l[nt], f[nt], sum);
+            l[nt] += sum;
         }
-        return moved;
     }
 
-    __device__ __forceinline__ void rescale(bool moved, const float (&f)[NT]) {
-        if (!moved) return;
+    __device__ __forceinline__ void rescale(const float (&f)[NT]) {
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
@@ -538,7 +541,8 @@ struct attention {
         mask(s, t * KT);
         probs p;
         float f[NT];
-        rescale(soften(s, p, f), f);
+        if (adjust(s, f)) rescale(f);
+        soften(s, p);
         __builtin_amdgcn_sched_barrier(0);
         values v;
         values_of(v, stage(0));
@@ -614,10 +618,11 @@ struct attention {
             meet<VM>();
             scores_of(next, stage(1));
             mask(s, t * KT);
-            bool moved = soften(s, p, f);
+            bool moved = adjust(s, f);
+            soften(s, p);
             uint32_t n = 1;                                      // tile t + n's scores are `next`
             for (; t + n < t1; ++n) {
-                rescale(moved, f);
+                if (moved) rescale(f);
                 meet<0>();
                 // (the transposing reads before the copy: the compiler waits for copies to LDS before one)
                 values v;
@@ -630,15 +635,16 @@ struct attention {
                     for (int nt = 0; nt < NT; ++nt) s[ks][nt] = next[ks][nt];
                 }
                 mask(s, (t + n) * KT);
+                moved = adjust(s, f);                            // (the tile before it is still on its way into o)
                 __builtin_amdgcn_sched_barrier(0);
                 probs q;
                 scores_of(next, stage((n + 1) & 3u));
                 products<false>(v, p, (t + n - 1) * KT, stage((n - 1) & 3u));
-                moved = soften(s, q, f);
+                soften(s, q);
                 p = q;
                 interleave();
             }
-            rescale(moved, f);
+            if (moved) rescale(f);
             wait_vmem<0>();                                      // nothing comes into LDS any more
             values v;
             values_of(v, stage((n - 1) & 3u));
@@ -664,7 +670,8 @@ struct attention {
                 float f[NT];
                 scores_of(s, stage(0));
                 mask(s, t * KT);
-                rescale(soften(s, p, f), f);
+                if (adjust(s, f)) rescale(f);
+                soften(s, p);
                 values_of(v, stage(0));
                 products<true>(v, p, t * KT, stage(0));
                 meet<0>();
@@ -728,19 +735,15 @@ struct attention {
             __syncthreads();
             if ((votes[0] | votes[1] | votes[2] | votes[3]) != 0) careful_pass();
         }
-        float mc[NT];
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt) {
-            l[nt] = row_sum(l[nt]);
-            mc[nt] = fmaxf(m[nt] * c[nt], LOWEST);
-        }
+        for (int nt = 0; nt < NT; ++nt) l[nt] = row_sum(l[nt]);
         if constexpr (!KEYS) {
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt) {
                 const uint32_t row = wave * (16u * NT) + 16u * nt + li;
                 if (row < it.n_rows) {
 #pragma unroll
-                    for (int dt = 0; dt < DT; ++dt) finish(row, 16u * dt + 4u * g, o[dt][nt], mc[nt], l[nt], lim[nt] > 0);
+                    for (int dt = 0; dt < DT; ++dt) finish(row, 16u * dt + 4u * g, o[dt][nt], m[nt], l[nt], lim[nt] > 0);
                 }
             }
         } else {
@@ -754,7 +757,7 @@ struct attention {
 #pragma unroll
                 for (int dt = 0; dt < DT; ++dt) *reinterpret_cast<f32x4 *>(so + row * D + 16 * dt + 4 * g) = o[dt][nt];
                 if (g == 0) {
-                    sm[2 * row] = mc[nt];
+                    sm[2 * row] = m[nt];
                     sm[2 * row + 1] = l[nt];
                 }
             }
