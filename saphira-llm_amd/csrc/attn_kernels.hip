@@ -692,29 +692,38 @@ struct attention {
         return bad;
     }
 
-    // four of a row's results, from dimension d on
-    __device__ __forceinline__ void put(uint32_t row, uint32_t d, f32x4 x) const {
-        if (d >= a.hd) return;
+    // where a row's results go, once for all its dimensions
+    __device__ __forceinline__ uint8_t *out_row(uint32_t row) const {
         const uint32_t r = it.row0 + row, t = r / a.group, h = it.head * a.group + r % a.group;
-        uint8_t *dst = (uint8_t *) a.out + token(t) * a.out_tok + h * a.out_head + d * sizeof(A);
+        return (uint8_t *) a.out + token(t) * a.out_tok + h * a.out_head;
+    }
+    // four of them, from dimension d on
+    __device__ __forceinline__ void put(uint8_t *dst, uint32_t d, f32x4 x) const {
+        if (d >= a.hd) return;
         if constexpr (sizeof(A) == 4) {
-            *G_CAST(f32x4, dst) = x;
+            *G_CAST(f32x4, dst + d * sizeof(A)) = x;
         } else {
             typename vec4<A>::type y;
 #pragma unroll
             for (int i = 0; i < 4; ++i) y[i] = (A) x[i];
-            *G_CAST(u32x2, dst) = __builtin_bit_cast(u32x2, y);
+            *G_CAST(u32x2, dst + d * sizeof(A)) = __builtin_bit_cast(u32x2, y);
         }
     }
-    __device__ __forceinline__ void finish(uint32_t row, uint32_t d, f32x4 x, float mc, float sum, bool sees) const {
+    // a row of N times four results, STEP dimensions apart from d on
+    template <int N, int STEP>
+    __device__ __forceinline__ void finish(uint32_t row, uint32_t d, const f32x4 (&x)[N], float top, float sum, bool sees) const {
         if (it.part == ATT_DIRECT) {
-            put(row, d, sees ? x / sum : (f32x4) { 0, 0, 0, 0 });
+            uint8_t *dst = out_row(row);
+            const float by = sees ? 1.0f / sum : 0.0f;
+#pragma unroll
+            for (int n = 0; n < N; ++n) put(dst, d + n * STEP, sees ? x[n] * by : (f32x4) { 0, 0, 0, 0 });
         } else {
             const uint64_t at = it.part + row;
-            *G_CAST(f32x4, a.part_o + at * D + d) = x;
+#pragma unroll
+            for (int n = 0; n < N; ++n) *G_CAST(f32x4, a.part_o + at * D + d + n * STEP) = x[n];
             if (d == 0) {
-                a.part_ml[2 * at] = mc;
-                a.part_ml[2 * at + 1] = sum;
+                G_CAST(float, a.part_ml)[2 * at] = top;
+                G_CAST(float, a.part_ml)[2 * at + 1] = sum;
             }
         }
     }
@@ -742,8 +751,10 @@ struct attention {
             for (int nt = 0; nt < NT; ++nt) {
                 const uint32_t row = wave * (16u * NT) + 16u * nt + li;
                 if (row < it.n_rows) {
+                    f32x4 x[DT];
 #pragma unroll
-                    for (int dt = 0; dt < DT; ++dt) finish(row, 16u * dt + 4u * g, o[dt][nt], m[nt], l[nt], lim[nt] > 0);
+                    for (int dt = 0; dt < DT; ++dt) x[dt] = o[dt][nt];
+                    finish<DT, 16>(row, 4u * g, x, m[nt], l[nt], lim[nt] > 0);
                 }
             }
         } else {
@@ -771,14 +782,14 @@ struct attention {
                     ml[w][1] = sm[2 * (w * 16 * NT + row) + 1];
                     top = fmaxf(top, ml[w][0]);
                 }
-                f32x4 x = { 0, 0, 0, 0 };
+                f32x4 x[1] = { { 0, 0, 0, 0 } };
 #pragma unroll
                 for (int w = 0; w < WAVES; ++w) {
                     const float f = __builtin_amdgcn_exp2f(ml[w][0] - top);
                     sum += f * ml[w][1];
-                    x += f * *reinterpret_cast<const f32x4 *>(so + (w * 16 * NT + row) * D + d);
+                    x[0] += f * *reinterpret_cast<const f32x4 *>(so + (w * 16 * NT + row) * D + d);
                 }
-                finish(row, d, x, top, sum, limit((it.row0 + row) / a.group) > 0);
+                finish<1, 0>(row, d, x, top, sum, limit((it.row0 + row) / a.group) > 0);
             }
         }
     }
