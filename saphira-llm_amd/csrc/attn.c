@@ -670,11 +670,11 @@ static int by_work(const void *a, const void *b) {
     const att_item *x = a, *y = b;
     if (x->mode != y->mode) return x->mode > y->mode ? -1 : 1;
     if (item_keys(x) != item_keys(y)) return item_keys(x) > item_keys(y) ? -1 : 1;
-    return x->pad < y->pad ? -1 : x->pad > y->pad;       /* (the order they came in) */
+    return x->order < y->order ? -1 : x->order > y->order;
 }
 
 static void order_work(items *x) {
-    for (size_t i = 0; i < x->n; ++i) x->v[i].pad = (uint32_t) i;
+    for (size_t i = 0; i < x->n; ++i) x->v[i].order = (uint32_t) i;
     if (x->n > 0) qsort(x->v, x->n, sizeof *x->v, by_work);
 }
 
@@ -807,8 +807,8 @@ static int lay_out(sllm_gfx950_batch *b, plan *x, int32_t n, const int32_t *len0
                 if (key1 > sees) key1 = (uint32_t) sees;
                 att_item *a = items_add(&it);
                 if (a == NULL) { st = FAIL_NOMEM("batch_create: work items"); break; }
-                *a = (att_item) { r, nr, own ? x->tok0[q] : 0, s->list, vis0, key0, key1, x->table[q] + (uint32_t) s->page0, h,
-                                  alone[q] ? ATT_DIRECT : s->part0 + hk * rows + r, s->mode, 0 };
+                *a = (att_item) { r / group, nr, own ? x->tok0[q] : 0, s->list, vis0, key0, key1, x->table[q] + (uint32_t) s->page0, h,
+                                  alone[q] ? ATT_DIRECT : s->part0 + hk * rows + r, (uint16_t) s->mode, (uint16_t) (r % group), 0 };
             }
         }
     }
@@ -1040,7 +1040,7 @@ int sllm_gfx950_batch_attend(sllm_gfx950_batch *b, int32_t layer, const void *q,
                    .part_o = (float *) (dev + b->off_part_o), .part_ml = (float *) (dev + b->off_part_ml),
                    .q_tok = qt, .q_head = (uint64_t) hd * size, .out_tok = ot, .out_head = (uint64_t) hd * size,
                    .page_bytes = p->page_bytes, .page_shift = p->page_shift, .hd = hd, .group = group,
-                   .c = (float) ((double) scale * LOG2E) };
+                   .per_group = 1.0f / (float) group, .c = (float) ((double) scale * LOG2E) };
     /* the partial results are one set of memory: a call's launches stay together */
     pthread_mutex_lock(&p->mtx);
     int st = SLLM_GFX950_OK;
@@ -1115,8 +1115,8 @@ int sllm_gfx950_prompt_create(const sllm_gfx950_prompt_desc *d, sllm_gfx950_prom
                 const int32_t last = (int32_t) ((r + n - 1) / group) + nk - nq + 1;    /* keys that the last row sees */
                 att_item *a = items_add(&it);
                 if (a == NULL) { st = FAIL_NOMEM("prompt_create: work items"); break; }
-                *a = (att_item) { r, n, (uint32_t) p->n_q, ATT_TOKENS, nk - nq + 1, 0, last > 0 ? (uint32_t) last : 0,
-                                  (uint32_t) p->n_k, (uint32_t) h, ATT_DIRECT, mode, 0 };
+                *a = (att_item) { r / group, n, (uint32_t) p->n_q, ATT_TOKENS, nk - nq + 1, 0, last > 0 ? (uint32_t) last : 0,
+                                  (uint32_t) p->n_k, (uint32_t) h, ATT_DIRECT, (uint16_t) mode, (uint16_t) (r % group), 0 };
             }
         }
         p->n_q += (uint64_t) nq;
@@ -1173,7 +1173,8 @@ int sllm_gfx950_prompt_attend(sllm_gfx950_prompt *p, const sllm_gfx950_prompt_io
     if (bad_scale(io->scale)) return FAIL_ARG("prompt_attend: scale %g", (double) io->scale);
     const uint32_t size = type_size(p->dtype), hd = (uint32_t) p->head_dim;
     att_args a = { .q = io->q, .out = io->out, .k = io->k, .v = io->v, .items = p->items, .hd = hd,
-                   .group = (uint32_t) (p->n_head / p->n_head_kv), .n_items = p->n_items, .c = (float) ((double) io->scale * LOG2E) };
+                   .group = (uint32_t) (p->n_head / p->n_head_kv), .per_group = 1.0f / (float) (p->n_head / p->n_head_kv),
+                   .n_items = p->n_items, .c = (float) ((double) io->scale * LOG2E) };
     if (!strides(io->q_tok, io->q_head, (uint64_t) p->n_head, hd, size, &a.q_tok, &a.q_head) ||
         !strides(io->k_tok, io->k_head, (uint64_t) p->n_head_kv, hd, size, &a.k_tok, &a.k_head) ||
         !strides(io->v_tok, io->v_head, (uint64_t) p->n_head_kv, hd, size, &a.v_tok, &a.v_head) ||

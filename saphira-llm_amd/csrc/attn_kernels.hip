@@ -178,6 +178,13 @@ struct attention {
     __device__ __forceinline__ uint32_t row_of(int nt) const {
         return min((KEYS ? 0u : wave * (16u * NT)) + 16u * (uint32_t) nt + li, it.n_rows - 1u);
     }
+    // the token and the head of one of the item's rows (h0 + row is small: the product
+    // with 1 / group, half a step up, is rounded down to the quotient without error)
+    struct place { uint32_t t, h; };
+    __device__ __forceinline__ place place_of(uint32_t row) const {
+        const uint32_t x = it.h0 + row, t = (uint32_t) (((float) x + 0.5f) * a.per_group);
+        return { it.t0 + t, it.head * a.group + x - t * a.group };
+    }
     __device__ __forceinline__ uint32_t token(uint32_t t) const {
         return it.list == ATT_TOKENS ? it.tok0 + t : *G_CAST(const uint32_t, a.list + it.list + t);
     }
@@ -187,16 +194,16 @@ struct attention {
 
     __device__ __forceinline__ void load_q() {
         const uint32_t first = KEYS ? 0u : wave * (16u * NT);
-        lim_min = limit((it.row0 + min(first, it.n_rows - 1u)) / a.group);
-        lim_max = limit((it.row0 + min(first + 16u * NT, it.n_rows) - 1u) / a.group);
+        lim_min = limit(place_of(min(first, it.n_rows - 1u)).t);
+        lim_max = limit(place_of(min(first + 16u * NT, it.n_rows) - 1u).t);
         lim_min = (int) uniform((uint32_t) lim_min);
         lim_max = (int) uniform((uint32_t) lim_max);
         if (first >= it.n_rows) lim_max = 0;                     // a wave without rows
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
-            const uint32_t r = it.row0 + row_of(nt), t = r / a.group, h = it.head * a.group + r % a.group;
-            lim[nt] = limit(t);
-            const uint8_t *src = (const uint8_t *) a.q + token(t) * a.q_tok + h * a.q_head;
+            const place at = place_of(row_of(nt));
+            lim[nt] = limit(at.t);
+            const uint8_t *src = (const uint8_t *) a.q + token(at.t) * a.q_tok + at.h * a.q_head;
             c[nt] = a.c;
             if constexpr (WIDE) {
 #pragma unroll
@@ -694,8 +701,8 @@ struct attention {
 
     // where a row's results go, once for all its dimensions
     __device__ __forceinline__ uint8_t *out_row(uint32_t row) const {
-        const uint32_t r = it.row0 + row, t = r / a.group, h = it.head * a.group + r % a.group;
-        return (uint8_t *) a.out + token(t) * a.out_tok + h * a.out_head;
+        const place at = place_of(row);
+        return (uint8_t *) a.out + token(at.t) * a.out_tok + at.h * a.out_head;
     }
     // four of them, from dimension d on
     __device__ __forceinline__ void put(uint8_t *dst, uint32_t d, f32x4 x) const {
@@ -789,7 +796,7 @@ struct attention {
                     sum += f * ml[w][1];
                     x[0] += f * *reinterpret_cast<const f32x4 *>(so + (w * 16 * NT + row) * D + d);
                 }
-                finish<1, 0>(row, d, x, top, sum, limit((it.row0 + row) / a.group) > 0);
+                finish<1, 0>(row, d, x, top, sum, limit(place_of(row).t) > 0);
             }
         }
     }

@@ -20,21 +20,21 @@ enum { ATT_FEW, ATT_HALF, ATT_MANY };
 #define ATT_SEE_ALL   (1 << 30)      /* att_item.vis0: every key of the range */
 
 /*
- * One workgroup's share: rows row0 .. row0 + n_rows of a segment (a run of
- * keys and the tokens that read it) against its keys key0 .. key1. Row r is
- * token r / group and head r % group of KV head `head`; token t is row
+ * One workgroup's share: n_rows rows of a segment (a run of keys and the tokens
+ * that read it), from row t0 * group + h0 on, against its keys key0 .. key1. Row
+ * r is token r / group and head r % group of KV head `head`; token t is row
  * tok0 + t of the query tensor, or what list[list + t] names, and sees the
  * keys below vis0 + t.
  */
 typedef struct att_item {
-    uint32_t row0, n_rows, tok0, list;
+    uint32_t t0, n_rows, tok0, list;
     int32_t  vis0;
     uint32_t key0, key1;
     uint32_t kv;            /* paged: where the segment's page numbers start; packed: the first key's row */
     uint32_t head;
-    uint32_t part;          /* row of the partial results that row0's go to, or ATT_DIRECT */
-    uint32_t mode;          /* ATT_FEW .. ATT_MANY */
-    uint32_t pad;
+    uint32_t part;          /* row of the partial results that the first row's go to, or ATT_DIRECT */
+    uint16_t mode, h0;      /* ATT_FEW .. ATT_MANY */
+    uint32_t order;         /* the order they came in */
 } att_item;
 
 typedef struct att_args {
@@ -51,7 +51,7 @@ typedef struct att_args {
     uint64_t        page_bytes;
     uint32_t        page_shift, hd, group, n_items;
     float           c;               /* scale * log2(e) */
-    uint32_t        pad;
+    float           per_group;       /* 1 / group */
 } att_args;
 
 /* the partial results of a token: those of n_split splits of a segment, whose
