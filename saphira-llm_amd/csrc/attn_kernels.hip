@@ -704,17 +704,27 @@ struct attention {
         const place at = place_of(row);
         return (uint8_t *) a.out + token(at.t) * a.out_tok + at.h * a.out_head;
     }
+    // four of them, as they are stored: 16 bits, a pair a register
+    __device__ __forceinline__ static u32x2 packed(f32x4 x) {
+        typename vec4<A>::type y;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) y[i] = (A) x[i];
+        return __builtin_bit_cast(u32x2, y);
+    }
     // four of them, from dimension d on
     __device__ __forceinline__ void put(uint8_t *dst, uint32_t d, f32x4 x) const {
         if (d >= a.hd) return;
-        if constexpr (sizeof(A) == 4) {
-            *G_CAST(f32x4, dst + d * sizeof(A)) = x;
-        } else {
-            typename vec4<A>::type y;
-#pragma unroll
-            for (int i = 0; i < 4; ++i) y[i] = (A) x[i];
-            *G_CAST(u32x2, dst + d * sizeof(A)) = __builtin_bit_cast(u32x2, y);
-        }
+        if constexpr (sizeof(A) == 4) *G_CAST(f32x4, dst + d * sizeof(A)) = x;
+        else *G_CAST(u32x2, dst + d * sizeof(A)) = packed(x);
+    }
+    // Two dimension tiles of 16 bits: the lanes of a row swap, so that each has eight
+    // values that are adjacent and a row's 64 bytes are written by one instruction.
+    __device__ __forceinline__ void put_two(uint8_t *dst, int dt, f32x4 x0, f32x4 x1) const {
+        const u32x2 p = packed(x0), q = packed(x1);
+        const u32x2 lo = __builtin_amdgcn_permlane16_swap(p[0], q[0], false, false);
+        const u32x2 hi = __builtin_amdgcn_permlane16_swap(p[1], q[1], false, false);
+        const uint32_t d = 16u * ((uint32_t) dt + (g & 1u)) + 8u * (g >> 1);
+        if (d < a.hd) *G_CAST(u32x4, dst + d * sizeof(A)) = (u32x4) { lo[0], hi[0], lo[1], hi[1] };
     }
     // a row of N times four results, STEP dimensions apart from d on
     template <int N, int STEP>
@@ -722,8 +732,16 @@ struct attention {
         if (it.part == ATT_DIRECT) {
             uint8_t *dst = out_row(row);
             const float by = sees ? 1.0f / sum : 0.0f;
+            f32x4 y[N];
 #pragma unroll
-            for (int n = 0; n < N; ++n) put(dst, d + n * STEP, sees ? x[n] * by : (f32x4) { 0, 0, 0, 0 });
+            for (int n = 0; n < N; ++n) y[n] = sees ? x[n] * by : (f32x4) { 0, 0, 0, 0 };
+            if constexpr (sizeof(A) == 2 && N > 1) {             // (the four lanes of a row are here together)
+#pragma unroll
+                for (int n = 0; n < N; n += 2) put_two(dst, n, y[n], y[n + 1]);
+            } else {
+#pragma unroll
+                for (int n = 0; n < N; ++n) put(dst, d + n * STEP, y[n]);
+            }
         } else {
             const uint64_t at = it.part + row;
 #pragma unroll
