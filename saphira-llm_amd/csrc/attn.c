@@ -1073,6 +1073,36 @@ struct sllm_gfx950_prompt {
     att_item *items;                 /* device */
 };
 
+/*
+ * The rows of a plan's workgroups. Smaller ones read the keys more often but are
+ * more, and each is done sooner: what counts is all work against the longest row
+ * tile's, in tiles of keys, of which starting a workgroup costs about eight. Many
+ * rows take 1.1 us a tile with two workgroups a CU and 0.85 alone (16 bits; f32 4.3
+ * and 2.8 for half the keys), half as many 0.73 and 0.69 (2.3 and 1.9); few rows
+ * go through their keys with four waves at once. Measured, us at few / half / many:
+ * bf16, one prompt of 128 rows 6.0 / 6.6 / 8.8, 512 16.5 / 13.8 / 18.1, 2048
+ * 104 / 44 / 55, 4096 376 / 127 / 108, four of up to 2048 123 / 45 / 55, 64 of up
+ * to 200 70 / 27 / 23; f32, 512 30 / 48 / 85, 2048 217 / 237 / 357, 4096
+ * 782 / 765 / 862, four of up to 2048 254 / 239 / 367 and, longer, 606 / 502 / 490.
+ */
+static uint32_t prompt_mode(const sllm_gfx950_prompt_desc *d, uint32_t group) {
+    const int wide = d->dtype == SLLM_GFX950_F32;
+    const int64_t tile = wide ? 16 : 32;
+    uint64_t all = 0, longest = 0;
+    for (int32_t i = 0; i < d->n_seq; ++i) {
+        const int64_t nq = d->q_len[i], nk = d->k_len ? d->k_len[i] : nq, rows = nq * group;
+        for (int64_t r = 0; r < rows; r += ATT_MANY_ROWS) {
+            const int64_t end = (r + ATT_MANY_ROWS < rows ? r + ATT_MANY_ROWS : rows) - 1, keys = end / group + nk - nq + 1;
+            const uint64_t tiles = keys > 0 ? (uint64_t) ((keys + tile - 1) / tile) : 0;
+            all += (tiles + 8) * (uint32_t) d->n_head_kv;
+            if (tiles > longest) longest = tiles;
+        }
+    }
+    const uint64_t cu = (uint64_t) sllm_shim_cu();
+    if (all * 32 < cu * (wide ? 25 : 8) * longest) return ATT_FEW;
+    return all * 8 < cu * (wide ? 11 : 9) * (longest + 8) ? ATT_HALF : ATT_MANY;
+}
+
 int sllm_gfx950_prompt_create(const sllm_gfx950_prompt_desc *d, sllm_gfx950_prompt **out) {
     ATT_ON_DEVICE();
     if (out == NULL) return FAIL_ARG("prompt_create: NULL out");
@@ -1091,16 +1121,11 @@ int sllm_gfx950_prompt_create(const sllm_gfx950_prompt_desc *d, sllm_gfx950_prom
     p->n_head_kv = d->n_head_kv;
     p->head_dim = d->head_dim;
     const uint32_t group = (uint32_t) (d->n_head / d->n_head_kv);
-    /* Half the rows a workgroup where whole ones would not fill a round of two on
-     * each CU (f32: two rounds, since its products take so long that they cover what
-     * the smaller tile costs). us at half / whole: bf16 one prompt of 2048 rows (320
-     * whole ones) 46 / 57, of 4096 (640) 135 / 113; f32 of 4096 778 / 844, two of up
-     * to 8192 (2000) 3000 / 2789. */
     uint64_t whole = 0;
     for (int32_t i = 0; i < d->n_seq; ++i) {
         if (d->q_len[i] > 0) whole += ((uint64_t) d->q_len[i] * group + ATT_MANY_ROWS - 1) / ATT_MANY_ROWS * (uint32_t) d->n_head_kv;
     }
-    const uint32_t mode = whole < (d->dtype == SLLM_GFX950_F32 ? 4u : 2u) * (uint64_t) sllm_shim_cu() ? ATT_HALF : ATT_MANY, tile = k_rows[mode];
+    const uint32_t mode = whole > MAX_ITEMS ? ATT_MANY : prompt_mode(d, group);
     for (int32_t i = 0; i < d->n_seq && st == SLLM_GFX950_OK; ++i) {
         const int32_t nq = d->q_len[i], nk = d->k_len ? d->k_len[i] : nq;
         if (nq < 0 || nk < 0 || p->n_q + (uint64_t) nq > SLLM_GFX950_ATTN_MAX_TOKENS || p->n_k + (uint64_t) nk > SLLM_GFX950_ATTN_MAX_TOKENS) {
@@ -1109,6 +1134,7 @@ int sllm_gfx950_prompt_create(const sllm_gfx950_prompt_desc *d, sllm_gfx950_prom
         }
         if (whole > MAX_ITEMS) { st = FAIL_ARG("prompt_create: too many rows"); break; }
         const uint32_t rows = (uint32_t) nq * group;
+        const uint32_t own = mode_of(rows, d->dtype) == ATT_FEW ? ATT_FEW : mode, tile = k_rows[own];
         for (int32_t h = 0; h < d->n_head_kv && st == SLLM_GFX950_OK; ++h) {
             for (uint32_t r = 0; r < rows; r += tile) {
                 const uint32_t n = rows - r < tile ? rows - r : tile;
@@ -1116,7 +1142,7 @@ int sllm_gfx950_prompt_create(const sllm_gfx950_prompt_desc *d, sllm_gfx950_prom
                 att_item *a = items_add(&it);
                 if (a == NULL) { st = FAIL_NOMEM("prompt_create: work items"); break; }
                 *a = (att_item) { r / group, n, (uint32_t) p->n_q, ATT_TOKENS, nk - nq + 1, 0, last > 0 ? (uint32_t) last : 0,
-                                  (uint32_t) p->n_k, (uint32_t) h, ATT_DIRECT, (uint16_t) mode, (uint16_t) (r % group), 0 };
+                                  (uint32_t) p->n_k, (uint32_t) h, ATT_DIRECT, (uint16_t) own, (uint16_t) (r % group), 0 };
             }
         }
         p->n_q += (uint64_t) nq;

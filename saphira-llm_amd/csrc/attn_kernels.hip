@@ -314,16 +314,18 @@ struct attention {
             k[gr] = __builtin_amdgcn_make_buffer_rsrc((void *) at.m[gr].k, (short) 0, (int) uniform(n ? n * rowk - (rowk - row) : 0u), 0x00020000);
             v[gr] = __builtin_amdgcn_make_buffer_rsrc((void *) at.m[gr].v, (short) 0, (int) uniform(n ? n * rowv - (rowv - row) : 0u), 0x00020000);
         }
-        // read once, and not kept (2: nontemporal): 64.9 -> 60.6 us for 8 sequences of 16384 positions, bf16
+        // a sequence's own keys are read once and not kept (2: nontemporal): 64.9 -> 60.6 us
+        // for 8 sequences of 16384 positions, bf16; a prompt's are read by many workgroups
+        constexpr int KEPT = PAGED ? 2 : 0;
 #pragma unroll
         for (int gr = 0; gr < GROUPS; ++gr) {
 #pragma unroll
-            for (int q = 0; q < QC; ++q) x.k[gr][q] = __builtin_amdgcn_raw_buffer_load_b128(k[gr], kcopy[q], 0, 2);
+            for (int q = 0; q < QC; ++q) x.k[gr][q] = __builtin_amdgcn_raw_buffer_load_b128(k[gr], kcopy[q], 0, KEPT);
         }
 #pragma unroll
         for (int gr = 0; gr < GROUPS; ++gr) {
 #pragma unroll
-            for (int j = 0; j < COPIES; ++j) x.v[gr][j] = __builtin_amdgcn_raw_buffer_load_b128(v[gr], vcopy[j], 0, 2);
+            for (int j = 0; j < COPIES; ++j) x.v[gr][j] = __builtin_amdgcn_raw_buffer_load_b128(v[gr], vcopy[j], 0, KEPT);
         }
     }
 
@@ -855,7 +857,8 @@ template <typename T, int D>
 __device__ __forceinline__ void prompt_body(const att_args &a) {
     __shared__ __attribute__((aligned(1024))) uint8_t S[LDS_BYTES<T, D>];
     const att_item it = item_of(a);
-    if (it.mode == ATT_HALF) attend_item<T, T, D, 1, false, false>(a, it, S);
+    if (it.mode == ATT_FEW) attend_item<T, T, D, 1, true, false>(a, it, S);
+    else if (it.mode == ATT_HALF) attend_item<T, T, D, 1, false, false>(a, it, S);
     else attend_item<T, T, D, 2, false, false>(a, it, S);
 }
 

@@ -62,6 +62,44 @@ def test_prompt_longer(amd, dev, dtype, d):
 
 
 @pytest.mark.parametrize("dtype", list(ora.TYPES))
+@pytest.mark.parametrize("heads,kv,d", [(8, 4, 64), (15, 5, 128), (12, 6, 80)])
+def test_prompt_several_of_one_length(amd, dev, dtype, heads, kv, d):
+    prompt(amd, dev, dtype, heads, kv, d, [130] * 16 + [65, 1], seed=19, oracle=ora.attend_rows)
+
+
+@pytest.mark.parametrize("dtype", list(ora.TYPES))
+def test_prompt_several_of_one_length_and_what_is_not_finite(amd, dev, dtype):
+    heads, kv, d, lens = 8, 4, 64, [130] * 16
+    clean = prompt(amd, dev, dtype, heads, kv, d, lens, seed=21, oracle=ora.attend_rows)
+    T = ora.TYPES[dtype]
+    q, k, v = (normal(21 + i, sum(lens), h, d).to(T) for i, h in enumerate((heads, kv, kv)))
+    k[130 + 60, 1, 3] = math.nan
+    v[130 + 20, 2, 5] = math.inf
+    v[130 + 129, :, 7] = -math.inf
+    bufs = [dev.put(ora.bits(x)) for x in (q, k, v)]
+    out = dev.alloc(clean.numel() * clean.element_size())
+    plan = amd.PromptAttention(dev, dtype, heads, kv, d, lens)
+    plan.run(bufs[0].ptr, bufs[1].ptr, bufs[2].ptr, out.ptr, d ** -0.5)
+    dev.sync()
+    got = ora.from_bits(out.download(ora.store_type(dtype), clean.numel()), dtype).view_as(clean)
+    seen = torch.zeros_like(clean, dtype=torch.bool)
+    seen[130 + 60:260, 2:4] = True
+    seen[130 + 20:260, 4:6, 5] = True
+    seen[130 + 129, :, 7] = True
+    assert torch.equal(got[~seen], clean[~seen])
+    assert not torch.isfinite(got[130 + 60:260, 2:4].float()).any() and not torch.isfinite(got[130 + 20:260, 4:6, 5].float()).any()
+    assert not torch.isfinite(got[130 + 129, :, 7].float()).any()
+    plan.close()
+    for x in bufs + [out]:
+        x.free()
+
+
+@pytest.mark.parametrize("dtype", list(ora.TYPES))
+def test_prompt_few_rows_over_many_keys(amd, dev, dtype):
+    prompt(amd, dev, dtype, 4, 2, 128, [1, 5, 8, 9, 1], [700, 333, 1, 90, 1500], seed=20)
+
+
+@pytest.mark.parametrize("dtype", list(ora.TYPES))
 def test_prompt_behind_earlier_keys_and_rows_that_see_none(amd, dev, dtype):
     """Keys in front of the prompt's own; more rows than keys: the first see none
     and are 0, keys or no keys at all."""
@@ -147,7 +185,8 @@ def test_prompt_strides(amd, dev, dtype):
         b.free()
 
 
-# Plans of over a thousand tiles of 128 rows: those take workgroups of 128 rows, smaller plans 64.
+# A plan's workgroups have 16, 64 or 128 rows, by how much work there is beside its longest rows: one short prompt,
+# a few of one length, many of one length.
 
 @pytest.mark.parametrize("dtype", list(ora.TYPES))
 @pytest.mark.parametrize("heads,kv,d,q_len,k_len", [(512, 512, 64, [129, 130], None), (768, 256, 64, [100, 45, 7], [100, 145, 4]),
