@@ -845,14 +845,16 @@ __device__ __forceinline__ att_item item_of(const att_args &a) {
     return it;
 }
 
-// Whole prompts. The matrix unit bounds them: 4 head_dim operations for a row and a key
-// that it sees. Two workgroups a CU, 64 KB of LDS and at most 256 registers each, so
-// that one's barrier falls into the other's products; 128 rows a workgroup read a tile
-// of keys from LDS once for two products. With 20 heads over 5 of 128: 16384 rows f16
-// 1.52 ms, 0.90 PFLOP/s (a large product here reaches 1.20; the clock goes down to
-// 1.85 GHz under both), 24 prompts of up to 2048 rows bf16 173 us, 0.61; 4 prompts f32
-// 511 us, 107 TFLOP/s of 153, the matrix unit busy 73 % of the time. 32 rows a wave and
-// not 64, one wave a SIMD: 1.52 against 1.85 ms.
+// Whole prompts. 4 head_dim operations for a row and a key that it sees: the matrix unit
+// bounds f32, the vector unit beside it 16 bits (four instructions to a matrix one, of
+// which one in seven is an exponential). Two workgroups a CU, 64 KB of LDS and at most 256
+// registers each, so that one's barrier falls into the other's products; 128 rows a
+// workgroup read a tile of keys from LDS once for two products. With 20 heads over 5 of
+// 128: 16384 rows f16 1.41 to 1.47 ms, 0.93 to 0.97 PFLOP/s (a large product here
+// reaches 1.20; the clock goes down to about 1.9 GHz under both); 24 prompts of up to 2048
+// rows bf16 155 us, 0.66, where reading q and writing the results (37 us of copying) is
+// little hidden; 4 prompts f32 495 us, 110 TFLOP/s of 153, the matrix unit busy 81 % of
+// the time. 32 rows a wave and not 64, one wave a SIMD: 1.52 against 1.85 ms.
 template <typename T, int D>
 __device__ __forceinline__ void prompt_body(const att_args &a) {
     __shared__ __attribute__((aligned(1024))) uint8_t S[LDS_BYTES<T, D>];
