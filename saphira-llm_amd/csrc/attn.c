@@ -618,8 +618,8 @@ static int by_table(const void *a, const void *b) {
 static const uint32_t k_rows[] = { ATT_FEW_ROWS, ATT_HALF_ROWS, ATT_MANY_ROWS };      /* by mode */
 
 /* A segment's rows: f32 takes two tiles of few before half of many (8 sequences
- * behind 4096 shared positions, 32 rows: 19.7 us against 24.7), 16 bits one (12.0
- * for half of many, 13.1 for two of few). */
+ * behind 4096 shared positions, 32 rows: 18.7 us against 24.8), 16 bits one (12.6
+ * for half of many, 13.0 for two of few). */
 static uint32_t mode_of(uint32_t rows, int32_t dtype) {
     const uint32_t few = dtype == SLLM_GFX950_F32 ? 2 * ATT_FEW_ROWS : ATT_FEW_ROWS;
     return rows <= few ? ATT_FEW : rows <= ATT_HALF_ROWS ? ATT_HALF : ATT_MANY;
@@ -1125,7 +1125,8 @@ int sllm_gfx950_prompt_create(const sllm_gfx950_prompt_desc *d, sllm_gfx950_prom
     for (int32_t i = 0; i < d->n_seq; ++i) {
         if (d->q_len[i] > 0) whole += ((uint64_t) d->q_len[i] * group + ATT_MANY_ROWS - 1) / ATT_MANY_ROWS * (uint32_t) d->n_head_kv;
     }
-    const uint32_t mode = whole > MAX_ITEMS ? ATT_MANY : prompt_mode(d, group);
+    /* (so many that smaller ones might not fit a launch) */
+    const uint32_t mode = whole > MAX_ITEMS / (ATT_MANY_ROWS / ATT_FEW_ROWS) ? ATT_MANY : prompt_mode(d, group);
     for (int32_t i = 0; i < d->n_seq && st == SLLM_GFX950_OK; ++i) {
         const int32_t nq = d->q_len[i], nk = d->k_len ? d->k_len[i] : nq;
         if (nq < 0 || nk < 0 || p->n_q + (uint64_t) nq > SLLM_GFX950_ATTN_MAX_TOKENS || p->n_k + (uint64_t) nk > SLLM_GFX950_ATTN_MAX_TOKENS) {

@@ -541,6 +541,16 @@ def test_prompts_of_more_rows_than_32_bits_count(amd, L):
         assert L.sllm_gfx950_prompt_create(byref(d), byref(plan)) == ARG and not plan.value
 
 
+def test_a_long_row_beside_many_short_prompts(amd, L):
+    """Small tiles for the one's sake would be more than a launch takes."""
+    n = 30000
+    q, k = I(1, *[64] * n), I(1 << 21, *[64] * n)
+    plan = c_void_p()
+    d = amd.PromptDesc(F32, 128, 16, 64, n + 1, ctypes.cast(q, c_void_p), ctypes.cast(k, c_void_p))
+    assert L.sllm_gfx950_prompt_create(byref(d), byref(plan)) == 0, L.sllm_gfx950_last_error()
+    L.sllm_gfx950_prompt_destroy(plan)
+
+
 def test_threads_on_one_cache(amd, L):
     """Calls from several threads exclude each other: no page is lost."""
     import threading
