@@ -61,6 +61,8 @@ __device__ __forceinline__ float row_sum(float x) {
 }
 
 template <typename T> struct vec8 { typedef T type __attribute__((ext_vector_type(8))); };
+template <typename T> struct is_f16 { static constexpr bool value = false; };
+template <> struct is_f16<_Float16> { static constexpr bool value = true; };
 template <typename T> struct vec4 { typedef T type __attribute__((ext_vector_type(4))); };
 
 __device__ __forceinline__ f32x4 mfma(vec8<_Float16>::type a, vec8<_Float16>::type b, f32x4 c) {
@@ -168,7 +170,7 @@ struct attention {
     // rows: lane li of row tile nt
     int lim[NT];                    // keys the row sees
     float c[NT];
-    float m[NT], l[NT];             // c times the running maximum, and the lane's share of the sum
+    float m[NT], l[NT];             // c times the running maximum (- UP), and the lane's share of the sum
     f32x4 o[DT][NT];
     // a lane's pieces of q: 8 values (SPLIT: and what rounding left of them), or 4 f32
     t8 qf[WIDE ? 1 : NT][WIDE ? 1 : QC], ql[SPLIT ? NT : 1][SPLIT ? QC : 1];
@@ -376,8 +378,13 @@ struct attention {
 
     // The maximum moves only where a score is over it by 8 or more (as a power of two):
     // until then p is at most 256, which costs no precision, the sums need no scaling, and
-    // the lanes that hold a row need not agree on its largest score. Whether any did; then
-    // f is what the sums of products so far are to be scaled by.
+    // the lanes that hold a row need not agree on its largest score. f16 weights are 2^7
+    // larger: at most 2^15, which f16 holds, so that its smallest, 2^-24, is 2^-31 or less of
+    // a row's largest weight and not 2^-24 (the share of 4000
+    // keys with weights about 2^-25 of one's was 0.8 % off). The sums and the parts of a split
+    // carry the factor alike. Whether any did; then f is what the sums of products so far are
+    // to be scaled by.
+    static constexpr float UP = is_f16<T>::value ? 7.0f : 0.0f;
     __device__ __forceinline__ bool adjust(const scores &s, float (&f)[NT]) {
         float top[NT];
         bool over = false;
@@ -389,12 +396,12 @@ struct attention {
 #pragma unroll
                 for (int i = 0; i < 4; ++i) top[nt] = fmaxf(top[nt], s[ks][nt][i]);
             }
-            over |= fmaf(top[nt], c[nt], -m[nt]) > 8.0f;
+            over |= fmaf(top[nt], c[nt], -m[nt]) > 8.0f + UP;
         }
         if (!__any(over)) return false;
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
-            const float t = row_max(top[nt]), to = fmaf(t, c[nt], -m[nt]) > 8.0f ? t * c[nt] : m[nt];   // (by the row's own scores alone)
+            const float t = row_max(top[nt]), to = fmaf(t, c[nt], -m[nt]) > 8.0f + UP ? fmaf(t, c[nt], -UP) : m[nt];   // (by the row's own scores alone)
             f[nt] = __builtin_amdgcn_exp2f(m[nt] - to);
             l[nt] *= f[nt];
             m[nt] = to;

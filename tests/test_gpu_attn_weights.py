@@ -1,0 +1,63 @@
+"""The softmax weights of attention on the GPU, as the products with the values
+take them (sllm_gfx950_attn.h): those far below a row's largest keep their share.
+Tolerances: attn_bounds.py."""
+import numpy as np
+import pytest
+import torch
+
+import attn_bounds as bounds
+import attn_oracle as ora
+
+pytestmark = pytest.mark.gpu
+
+PAIRS = [("float32", "float32"), ("float32", "float16"), ("float16", "float16"), ("bfloat16", "bfloat16")]
+# new positions of two rows each: 16, 64 and 128 rows a workgroup
+N_NEW = [1, 25, 70]
+
+
+def sinks(n, at, d, T, seed):
+    """Keys whose scores, by the first dimension, are 15 to 19 below those at `at`,
+    whose values are 0, so that only the others' share is in the result."""
+    r = np.random.RandomState(seed)
+    k, v = np.zeros((n, 1, d)), r.uniform(32, 96, (n, 1, d))
+    k[:, 0, 0] = -r.uniform(15.0, 19.0, n)
+    k[at, 0, 0], v[at] = 0.0, 0.0
+    return torch.tensor(k).to(T), torch.tensor(v).to(T)
+
+
+def sink_queries(n, heads, d, T):
+    q = torch.zeros(n, heads, d)
+    q[:, :, 0] = 4.0
+    return q.to(T)
+
+
+@pytest.mark.parametrize("act,dtype", PAIRS)
+@pytest.mark.parametrize("n_new", N_NEW)
+@pytest.mark.parametrize("where", ["first", "last"])
+def test_many_keys_far_below_a_few(amd, dev, act, dtype, n_new, where):
+    """Enough sequences and heads that a wave has hundreds of keys in a row; each finds
+    one of the large ones, in its first tiles or in its last."""
+    n, d, kv, T = 2000, 64, 32, ora.TYPES[act]
+    at = [i for i in range(0, n, 32) if (i % 512 < 128) == (where == "first")]
+    k, v = sinks(n, at, d, T, 5)
+    seq = tuple(x.expand(n, kv, d).contiguous() for x in (k, v))
+    q = sink_queries(8 * n_new, 2 * kv, d, T)
+    got = bounds.step(amd, dev, act, dtype, 2 * kv, [seq] * 8, q, [n_new] * 8, 0.25, page=64).view(8, n_new, 2 * kv, d)
+    assert torch.equal(got, got[:1, :, :1].expand_as(got))
+    some = sorted({0, n_new // 2, n_new - 1})
+    cached = (x.to(ora.TYPES[dtype]).double().numpy() for x in (k, v))
+    want, tol = bounds.attend(q[some][:, :1].double().numpy(), *cached, np.array(some) + n - n_new + 1, 0.25, act, dtype)
+    ora.check(got[0, some][:, :1], want, tol)
+
+
+@pytest.mark.parametrize("dtype", list(ora.TYPES))
+@pytest.mark.parametrize("n_q", [1, 40, 300])
+def test_many_keys_of_a_prompt_far_below_one(amd, dev, dtype, n_q):
+    n, d, T = 4000, 128, ora.TYPES[dtype]
+    k, v = sinks(n, [0], d, T, 6)
+    q = sink_queries(n_q, 2, d, T)
+    got = bounds.prompt(amd, dev, dtype, q, k, v, [n_q], [n], 0.25)
+    some = sorted({0, n_q // 2, n_q - 1})
+    want, tol = bounds.attend(q[some].double().numpy(), k.double().numpy(), v.double().numpy(), np.array(some) + n - n_q + 1, 0.25,
+                              dtype, dtype)
+    ora.check(got[some], want, tol)
