@@ -12,10 +12,13 @@
  * Rows are [token][head][head_dim]; a row's head_dim values are adjacent, and
  * pointers and row strides are multiples of 16 bytes. head_dim is a multiple
  * of 8, at most 128; n_head is a multiple of n_head_kv, and query head h reads
- * KV head h / (n_head / n_head_kv). Scores, softmax sums and products are held
- * in f32; the sum of weights times values that is carried along may be 256 times
- * (f16 caches: 2^15 times) the number of keys larger than the result, and over
- * f32 and bf16 caches, whose values may be that large, overflows there.
+ * KV head h / (n_head / n_head_kv). Scores, softmax sums and sums of products
+ * are held in f32. The weights that multiply the values are rounded to the
+ * cache's type, so a 16-bit result's error is about sqrt(2) times what rounding
+ * it alone leaves; f32 rows over an f16 cache keep 22 bits of weights. The sum
+ * of weights times values that is carried along may be 256 times (f16 caches:
+ * 2^15 times) the number of keys larger than the result, and over f32 and bf16
+ * caches, whose values may be that large, overflows there.
  *
  * Calls may come from several threads, whichever device each has current: a
  * cache's calls exclude each other, and everything runs in call order on the

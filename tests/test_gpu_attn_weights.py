@@ -1,6 +1,6 @@
 """The softmax weights of attention on the GPU, as the products with the values
-take them (sllm_gfx950_attn.h): those far below a row's largest keep their share.
-Tolerances: attn_bounds.py."""
+take them (sllm_gfx950_attn.h): those far below a row's largest keep their share,
+and what they are divided by is the sum of just these. Tolerances: attn_bounds.py."""
 import numpy as np
 import pytest
 import torch
@@ -61,3 +61,51 @@ def test_many_keys_of_a_prompt_far_below_one(amd, dev, dtype, n_q):
     want, tol = bounds.attend(q[some].double().numpy(), k.double().numpy(), v.double().numpy(), np.array(some) + n - n_q + 1, 0.25,
                               dtype, dtype)
     ora.check(got[some], want, tol)
+
+
+def uneven(n, d, dtype):
+    """(keys, scale): with queries of 1 in the first dimension, one key in 16 has the
+    largest score, and the others' weights are 0.9 half steps of the type over a half,
+    so that all round down."""
+    k = torch.zeros(n, 1, d)
+    k[:, 0, 0] = -1.0
+    k[::16] = 0.0
+    return k.to(ora.TYPES[dtype]), float(np.log(2.0) - np.log1p(0.9 * bounds.HALF[dtype]))
+
+
+def alike(n, d, T):
+    v = torch.ones(n, 1, d)
+    v[..., 1::2] = -2.0 ** 6
+    v[..., 2::3] = 2.0 ** -6
+    return v.to(T)
+
+
+@pytest.mark.parametrize("act,dtype", PAIRS)
+@pytest.mark.parametrize("n_new", N_NEW)
+def test_values_that_are_all_alike(amd, dev, act, dtype, n_new):
+    """They come back as they are. Sums of weights and of weights times a power of two
+    differ by the roundings of sums alone, (n + 8) 2^-24 each and a division, which
+    rounding to 16 bits does not see."""
+    n, d, heads, T = 1000, 64, 2, ora.TYPES[act]
+    k, scale = uneven(n, d, dtype if dtype != "float32" else "bfloat16")
+    v = alike(n, d, T)
+    q = torch.zeros(n_new, heads, d)
+    q[:, :, 0] = 1.0
+    got = bounds.step(amd, dev, act, dtype, heads, [(k.to(T), v)], q.to(T), [n_new], scale, page=64)
+    want = v[:1].expand(n_new, heads, d)
+    if act == "float32":
+        assert ((got - want).abs() <= (2 * (n + 8) + 3) * 2.0 ** -24 * want.abs()).all()
+    else:
+        assert (2 * (n + 8) + 3) * 2.0 ** -24 < bounds.HALF[act] / 2
+        assert torch.equal(got, want)
+
+
+@pytest.mark.parametrize("dtype", ["float16", "bfloat16"])
+@pytest.mark.parametrize("n_q", [1, 40, 300])
+def test_values_of_a_prompt_that_are_all_alike(amd, dev, dtype, n_q):
+    n, d, T = 1000, 128, ora.TYPES[dtype]
+    k, scale = uneven(n, d, dtype)
+    v = alike(n, d, T)
+    q = torch.zeros(n_q, 2, d, dtype=T)
+    q[:, :, 0] = 1.0
+    assert torch.equal(bounds.prompt(amd, dev, dtype, q, k, v, [n_q], [n], scale), v[:1].expand(n_q, 2, d))
