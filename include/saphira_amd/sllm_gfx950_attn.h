@@ -15,8 +15,9 @@
  * KV head h / (n_head / n_head_kv). Scores, softmax sums and sums of products
  * are held in f32. The weights that multiply the values are rounded to the
  * cache's type, so a 16-bit result's error is about sqrt(2) times what rounding
- * it alone leaves; f32 rows over an f16 cache keep 22 bits of weights. The sum
- * of weights times values that is carried along may be 256 times (f16 caches:
+ * it alone leaves; f32 rows over an f16 cache keep 22 bits of weights and of
+ * queries (of elements below 2^-17 of a row's largest, all but 2^-39 of that). The
+ * sum of weights times values that is carried along may be 256 times (f16 caches:
  * 2^15 times) the number of keys larger than the result, and over f32 and bf16
  * caches, whose values may be that large, overflows there.
  *

@@ -231,9 +231,11 @@ struct attention {
                     qf[nt][s] = __builtin_bit_cast(t8, v);
                 }
             } else {
-                // f32 queries as the sum of two f16 values: 22 bits of each. The row is
-                // first scaled by a power of two to a largest magnitude of 1..2, so that
-                // neither part leaves f16's range; c takes the power back.
+                // f32 queries as the sum of two f16 values. The row is first scaled by a
+                // power of two to a largest magnitude of 2^14..2^15, the upper end of f16's
+                // range; c takes the power back. So an element keeps 22 bits down to 2^-17 of
+                // the largest, and below that is off by at most 2^-39 of it (at 1..2 it was
+                // 2^-25, which a key's large element makes a score's largest error).
                 f32x4 x[QC][2];
                 float top = 0.0f;
 #pragma unroll
@@ -247,14 +249,13 @@ struct attention {
                     }
                 }
                 top = row_max(top);
-                const int e2 = min(max((int) (__float_as_uint(top) >> 23) - 127, -100), 100);
-                const float down = __uint_as_float((uint32_t) (127 - e2) << 23);
-                c[nt] = a.c * __uint_as_float((uint32_t) (127 + e2) << 23);
+                const int up = 15 - __builtin_amdgcn_frexp_expf(top);        // (the exponent of 0 is 0)
+                c[nt] = __builtin_amdgcn_ldexpf(a.c, -up);
 #pragma unroll
                 for (int s = 0; s < QC; ++s) {
 #pragma unroll
                     for (int e = 0; e < 8; ++e) {
-                        const float f = x[s][e >> 2][e & 3] * down;
+                        const float f = __builtin_amdgcn_ldexpf(x[s][e >> 2][e & 3], up);
                         const T hi = (T) f;
                         qf[nt][s][e] = hi;
                         ql[nt][s][e] = (T) (f - (float) hi);

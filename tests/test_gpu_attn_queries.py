@@ -1,0 +1,49 @@
+"""Queries of any size and shape over a paged cache (sllm_gfx950_attn.h) on the GPU,
+f32 rows over an f16 cache above all: a row whose elements are many powers of two
+apart, rows at the ends of f32's range.
+Tolerances: attn_bounds.py."""
+import numpy as np
+import pytest
+import torch
+
+import attn_bounds as bounds
+import attn_oracle as ora
+
+pytestmark = pytest.mark.gpu
+
+PAIRS = [("float32", "float32"), ("float32", "float16"), ("float16", "float16"), ("bfloat16", "bfloat16")]
+# new positions of two rows each: 16, 64 and 128 rows a workgroup
+N_NEW = [1, 25, 70]
+
+
+def normal(seed, *shape):
+    g = torch.Generator()
+    g.manual_seed(seed)
+    return torch.randn(*shape, generator=g)
+
+
+@pytest.mark.parametrize("act,dtype", PAIRS)
+@pytest.mark.parametrize("n_new", N_NEW)
+@pytest.mark.parametrize("d,outlier", [(8, 3e4), (64, 300.0)])
+def test_small_elements_beside_a_large_one_meet_a_large_key(amd, dev, act, dtype, n_new, d, outlier):
+    """One element of the query is 3, the others are small, and so is the product of
+    one of them with a key's outlier: what it adds to a score is all there is between
+    the keys."""
+    n, T = 300, ora.TYPES[act]
+    q = normal(1, n_new, 2, d) * (3.0 / outlier)
+    q[:, :, 0] = 3.0
+    k, v = normal(2, n, 1, d) * 1e-3, normal(3, n, 1, d)
+    k[:, :, 5] = outlier * normal(4, n, 1).sign()
+    bounds.check_step(amd, dev, act, dtype, 2, [(k.to(T), v.to(T))], q.to(T), [n_new], 1.0, page=32)
+
+
+@pytest.mark.parametrize("exponent", [-149, -140, -126, -113, -101, -100, -60, 60, 99, 100, 112, 113, 116, 127])
+def test_f32_rows_at_the_ends_of_the_range(amd, dev, exponent):
+    """Rows of up to 2^exponent, with the scale that makes their scores ordinary (as far as
+    there is one: less than 2^-126 or over 2^126 it is not)."""
+    n, n_new, d = 90, 3, 64
+    q = torch.from_numpy(np.ldexp(np.random.RandomState(7).uniform(-1, 1, (n_new, 4, d)), exponent).astype(np.float32))
+    scale = 2.0 ** max(min(-exponent - 1, 126), -126)
+    seqs = [(normal(8, n, 2, d), normal(9, n, 2, d))]
+    got = bounds.check_step(amd, dev, "float32", "float16", 4, seqs, q, [n_new], scale)
+    assert torch.isfinite(got).all()
