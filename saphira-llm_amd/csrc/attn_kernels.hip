@@ -250,7 +250,9 @@ struct attention {
                 }
                 top = row_max(top);
                 const int up = 15 - __builtin_amdgcn_frexp_expf(top);        // (the exponent of 0 is 0)
-                c[nt] = __builtin_amdgcn_ldexpf(a.c, -up);
+                // not 0, which times a masked -inf is NaN, nor infinite: scores this small or
+                // large make the weights 1, or 0 and 1, whatever c is exactly
+                c[nt] = fminf(fmaxf(__builtin_amdgcn_ldexpf(a.c, -up), 0x1p-126f), -LOWEST);
 #pragma unroll
                 for (int s = 0; s < QC; ++s) {
 #pragma unroll

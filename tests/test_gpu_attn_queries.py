@@ -1,6 +1,6 @@
 """Queries of any size and shape over a paged cache (sllm_gfx950_attn.h) on the GPU,
 f32 rows over an f16 cache above all: a row whose elements are many powers of two
-apart, rows at the ends of f32's range.
+apart, rows at the ends of f32's range, rows of zeros.
 Tolerances: attn_bounds.py."""
 import numpy as np
 import pytest
@@ -46,4 +46,18 @@ def test_f32_rows_at_the_ends_of_the_range(amd, dev, exponent):
     scale = 2.0 ** max(min(-exponent - 1, 126), -126)
     seqs = [(normal(8, n, 2, d), normal(9, n, 2, d))]
     got = bounds.check_step(amd, dev, "float32", "float16", 4, seqs, q, [n_new], scale)
+    assert torch.isfinite(got).all()
+
+
+@pytest.mark.parametrize("act,dtype", PAIRS)
+@pytest.mark.parametrize("n_new", N_NEW)
+@pytest.mark.parametrize("scale", [1.0, 1e-20, 1e-37, 1e-44])
+def test_rows_of_zeros(amd, dev, act, dtype, n_new, scale):
+    """Every key a row sees weighs the same, and none that it does not see, whatever the
+    scale; rows beside them that are not zero stay right."""
+    n, d, T = 100, 64, ora.TYPES[act]
+    q = normal(11, n_new, 2, d)
+    q[:, 0] = 0.0
+    seqs = [(normal(12, n, 1, d).to(T), normal(13, n, 1, d).to(T))]
+    got = bounds.check_step(amd, dev, act, dtype, 2, seqs, q.to(T), [n_new], scale)
     assert torch.isfinite(got).all()
