@@ -237,7 +237,7 @@ struct attention {
                 // the largest, and below that is off by at most 2^-39 of it (at 1..2 it was
                 // 2^-25, which a key's large element makes a score's largest error).
                 f32x4 x[QC][2];
-                float top = 0.0f;
+                float top = 0.0f, least = -LOWEST;
 #pragma unroll
                 for (int s = 0; s < QC; ++s) {
                     const uint32_t d = 8u * (4u * s + g);
@@ -245,7 +245,10 @@ struct attention {
                     for (int i = 0; i < 2; ++i) {
                         x[s][i] = d < a.hd ? *G_CAST(const f32x4, src + d * 4u + 16u * i) : (f32x4) { 0, 0, 0, 0 };
 #pragma unroll
-                        for (int e = 0; e < 4; ++e) top = fmaxf(top, fabsf(x[s][i][e]));
+                        for (int e = 0; e < 4; ++e) {
+                            top = fmaxf(top, fabsf(x[s][i][e]));
+                            least = fminf(least, d < a.hd ? fabsf(x[s][i][e]) : -LOWEST);
+                        }
                     }
                 }
                 top = row_max(top);
@@ -261,6 +264,21 @@ struct attention {
                         const T hi = (T) f;
                         qf[nt][s][e] = hi;
                         ql[nt][s][e] = (T) (f - (float) hi);
+                    }
+                }
+                // An element too small for f16 keeps its sign, as f16's smallest, for infinite
+                // elements of keys; what is left of it is the difference. (Such rows alone: for
+                // every row it is 0.6 us of a step of 64 sequences behind 4096 positions.)
+                if (__any(__builtin_amdgcn_ldexpf(least, up) < 0x1p-24f)) {
+#pragma unroll
+                    for (int s = 0; s < QC; ++s) {
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) {
+                            const float f = __builtin_amdgcn_ldexpf(x[s][e >> 2][e & 3], up);
+                            if (f == 0.0f || qf[nt][s][e] != (T) 0.0f) continue;
+                            qf[nt][s][e] = (T) copysignf(0x1p-24f, f);
+                            ql[nt][s][e] = (T) (f - copysignf(0x1p-24f, f));
+                        }
                     }
                 }
             }
@@ -349,6 +367,10 @@ struct attention {
 
     typedef f32x4 scores[KS][NT];
 
+    // CAREFUL, SPLIT: what rounding left of a query may be 0 or of the other sign, and times
+    // an infinite element of a key would be NaN where the product is infinite: the rest is
+    // multiplied by 0 there.
+    template <bool CAREFUL>
     __device__ __forceinline__ void score(f32x4 (&s)[NT], const u32x4 &piece, int q) const {
         if constexpr (WIDE) {
             const f32x4 kf = __builtin_bit_cast(f32x4, piece);
@@ -362,8 +384,13 @@ struct attention {
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt) s[nt] = mfma(kf, qf[nt][q], s[nt]);
             if constexpr (SPLIT) {
+                t8 kr = kf;
+                if constexpr (CAREFUL) {
 #pragma unroll
-                for (int nt = 0; nt < NT; ++nt) s[nt] = mfma(kf, ql[nt][q], s[nt]);
+                    for (int e = 0; e < 8; ++e) kr[e] = odd((float) kr[e]) ? (T) 0.0f : kr[e];
+                }
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt) s[nt] = mfma(kr, ql[nt][q], s[nt]);
             }
         }
     }
@@ -568,7 +595,7 @@ struct attention {
 #pragma unroll
         for (int ks = 0; ks < KS; ++ks) {
 #pragma unroll
-            for (int q = 0; q < QC; ++q) score(s[ks], x.k[ks][q], q);
+            for (int q = 0; q < QC; ++q) score<CAREFUL>(s[ks], x.k[ks][q], q);
         }
 #pragma unroll
         for (int gr = 0; gr < GROUPS; ++gr) {
@@ -588,12 +615,13 @@ struct attention {
         products<CAREFUL>(v, p, t * KT, stage(0));
     }
 
+    template <bool CAREFUL>
     __device__ __forceinline__ void scores_of(scores &s, uint32_t at) const {
         clear(s);
 #pragma unroll
         for (int ks = 0; ks < KS; ++ks) {
 #pragma unroll
-            for (int q = 0; q < QC; ++q) score(s[ks], *reinterpret_cast<const u32x4 *>(S + at + koff[q] + 16u * ks * L::ROWB), q);
+            for (int q = 0; q < QC; ++q) score<CAREFUL>(s[ks], *reinterpret_cast<const u32x4 *>(S + at + koff[q] + 16u * ks * L::ROWB), q);
         }
     }
     // not KEYS: all but the last N of the wave's loads have arrived, and the other
@@ -653,9 +681,9 @@ struct attention {
             float f[NT];
             meet<VM>();
             issue(t + 2, stage(2));
-            scores_of(s, stage(0));
+            scores_of<false>(s, stage(0));
             meet<VM>();
-            scores_of(next, stage(1));
+            scores_of<false>(next, stage(1));
             mask(s, t * KT);
             bool moved = adjust(s, f);
             soften(s, p);
@@ -677,7 +705,7 @@ struct attention {
                 moved = adjust(s, f);                            // (the tile before it is still on its way into o)
                 __builtin_amdgcn_sched_barrier(0);
                 probs q;
-                scores_of(next, stage((n + 1) & 3u));
+                scores_of<false>(next, stage((n + 1) & 3u));
                 products<false>(v, p, (t + n - 1) * KT, stage((n - 1) & 3u));
                 soften(s, q);
                 p = q;
@@ -707,7 +735,7 @@ struct attention {
                 probs p;
                 values v;
                 float f[NT];
-                scores_of(s, stage(0));
+                scores_of<true>(s, stage(0));
                 mask(s, t * KT);
                 if (adjust(s, f)) rescale(f);
                 soften(s, p);

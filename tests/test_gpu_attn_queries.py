@@ -1,7 +1,9 @@
 """Queries of any size and shape over a paged cache (sllm_gfx950_attn.h) on the GPU,
 f32 rows over an f16 cache above all: a row whose elements are many powers of two
-apart, rows at the ends of f32's range, rows of zeros.
+apart, rows at the ends of f32's range, rows of zeros, keys with infinite elements.
 Tolerances: attn_bounds.py."""
+import math
+
 import numpy as np
 import pytest
 import torch
@@ -61,3 +63,36 @@ def test_rows_of_zeros(amd, dev, act, dtype, n_new, scale):
     seqs = [(normal(12, n, 1, d).to(T), normal(13, n, 1, d).to(T))]
     got = bounds.check_step(amd, dev, act, dtype, 2, seqs, q.to(T), [n_new], scale)
     assert torch.isfinite(got).all()
+
+
+@pytest.mark.parametrize("act,dtype", PAIRS)
+@pytest.mark.parametrize("n_new", N_NEW)
+def test_keys_at_minus_infinity_weigh_nothing(amd, dev, act, dtype, n_new):
+    """An infinite element of a key that takes a row's score to -inf: the row is that of
+    the other keys. Queries of few bits, whose rest is 0; one of any; a tiny element
+    beside a large one. The other KV head's rows, which see none, are untouched."""
+    n, d, T = 200, 64, ora.TYPES[act]
+    q = normal(21, n_new, 4, d)
+    q[:, 0] = q[:, 0].half().float().mul(4).round().div(4)
+    q[:, :2, 5] = q[:, :2, 5].abs() + 0.25
+    q[:, :2, 9] = -q[:, :2, 9].abs() - 0.25
+    if act != "float16":                                   # (it would be 0 there, which times infinity is NaN)
+        q[0, 0, 9] = -2.0 ** -60                           # beside elements of about 1
+    q = q.to(T)
+    k, v = normal(22, n, 2, d).to(T), normal(23, n, 2, d).to(T)
+    bad = [0, 40, n - n_new]
+    k[bad, 0, 5] = -math.inf
+    k[[77], 0, 9] = math.inf
+    got = bounds.step(amd, dev, act, dtype, 4, [(k, v)], q, [n_new], 0.125)
+    left = [i for i in range(n) if i not in bad + [77]]
+    kc, vc = (x.to(ora.TYPES[dtype]).double().numpy() for x in (k, v))
+    sees = n - n_new + 1 + np.arange(n_new)
+    want, tol = bounds.attend(q[:, :2].double().numpy(), kc[left][:, :1], vc[left][:, :1], [sum(x < s for x in left) for s in sees],
+                              0.125, act, dtype)
+    ora.check(got[:, :2], want, tol)
+    want, tol = bounds.attend(q[:, 2:].double().numpy(), kc[:, 1:], vc[:, 1:], sees, 0.125, act, dtype)
+    ora.check(got[:, 2:], want, tol)
+    # at +inf the row is not finite, from the key's position on
+    k[bad, 0, 5] = math.inf
+    got = bounds.step(amd, dev, act, dtype, 4, [(k, v)], q, [n_new], 0.125)
+    assert not torch.isfinite(got[:, :2].float()).any() and torch.isfinite(got[:, 2:].float()).all()
