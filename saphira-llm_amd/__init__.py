@@ -692,6 +692,7 @@ class PagedCache:
         self.dev, self.p = dev, None
         self.desc = PagesDesc(n_layer, n_head_kv, head_dim, page_tokens, n_pages, DTYPES[dtype], mem)
         self.dtype = dtype
+        self.room = 256                                  # page numbers that _page_numbers has room for at first
         p = c_void_p()
         check(lib().sllm_gfx950_pages_new(ctypes.byref(self.desc), ctypes.byref(p)), "pages_new")
         self.p = p
@@ -737,24 +738,26 @@ class PagedCache:
         check(min(n, 0), "seq_len")
         return n
 
+    def _page_numbers(self, seqs):
+        """Of n sequences, one behind another, as they all are at one time: from the call
+        that had room for them (other threads may give them pages between two calls)."""
+        n = len(seqs)
+        ids = (c_int32 * max(n, 1))(*seqs)
+        while True:
+            out = np.empty(self.room, np.int32)
+            total = lib().sllm_gfx950_seq_tables(self.p, ids, n, ptr(out), out.size)
+            check(min(total, 0), "seq_tables")
+            if total <= out.size:
+                return out[:total].copy()
+            self.room = max(self.room, total + total // 4)
+
     def table(self, seq):
         """A sequence's page numbers (int32)."""
-        one = (c_int32 * 1)(seq)
-        n = lib().sllm_gfx950_seq_tables(self.p, one, 1, None, 0)
-        check(min(n, 0), "seq_tables")
-        out = np.empty(n, np.int32)
-        check(min(lib().sllm_gfx950_seq_tables(self.p, one, 1, ptr(out) if n else None, n), 0), "seq_tables")
-        return out
+        return self._page_numbers([seq])
 
     def tables(self, seqs):
         """The page numbers of sequences that have equally many (int32[n][pages])."""
-        n = len(seqs)
-        ids = (c_int32 * max(n, 1))(*seqs)
-        total = lib().sllm_gfx950_seq_tables(self.p, ids, n, None, 0)
-        check(min(total, 0), "seq_tables")
-        out = np.empty(total, np.int32)
-        check(min(lib().sllm_gfx950_seq_tables(self.p, ids, n, ptr(out) if total else None, total), 0), "seq_tables")
-        return out.reshape(n, -1) if n else out.reshape(0, 0)
+        return self._page_numbers(seqs).reshape((len(seqs), -1) if len(seqs) else (0, 0))
 
     def compact(self):
         """Move the pages in use to the front; how many were moved."""
