@@ -73,7 +73,7 @@ def test_tables_beside_a_thread(amd, cache):
     def change():
         r = np.random.RandomState(1)
         while not stop.is_set():
-            grow(cache, s, int(r.randint(0, 900)))
+            grow(cache, s, int(r.randint(50, 900)))
             cache.truncate(s, int(r.randint(0, 50)))
 
     t = threading.Thread(target=change)
