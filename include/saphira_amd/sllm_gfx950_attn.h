@@ -29,7 +29,8 @@
  * batch_store, batch_attend and prompt_attend are launches alone and may be
  * captured into a graph. What takes pages or lays out work (batch_create,
  * seq_fork, seq_copy, pages_compact, prompt_create) is refused while the stream
- * is captured.
+ * is captured. What is freed or destroyed during a capture keeps its memory until
+ * a later call can wait for the stream; the capture goes on.
  */
 #ifndef SAPHIRA_AMD_SLLM_GFX950_ATTN_H
 #define SAPHIRA_AMD_SLLM_GFX950_ATTN_H

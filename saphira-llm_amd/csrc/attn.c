@@ -69,13 +69,72 @@ static int bad_heads(int32_t n_head, int32_t n_head_kv, int32_t head_dim) {
            head_dim < 8 || head_dim > SLLM_GFX950_ATTN_MAX_HEAD_DIM || head_dim % 8 != 0;
 }
 
+/* device memory, and the pinned memory that what is in it is sent from (`sent`: the
+ * copy out of `pin` is done) */
+typedef struct buffer {
+    uint8_t   *dev, *pin;
+    size_t     dev_bytes, pin_bytes;
+    hipEvent_t sent;
+} buffer;
+
+static void buffer_drop(buffer *b) {
+    if (b->dev) hipFree(b->dev);
+    if (b->pin) hipHostFree(b->pin);
+    if (b->sent) hipEventDestroy(b->sent);
+    memset(b, 0, sizeof *b);
+}
+
+/* What was released while the stream was captured: waiting for the stream would end the
+ * capture. The next call that may wait frees it, or close. */
+static struct { pthread_mutex_t mtx; buffer *v; size_t n, cap; } g_later = { PTHREAD_MUTEX_INITIALIZER, NULL, 0, 0 };
+
+static void release_later(void) {
+    pthread_mutex_lock(&g_later.mtx);
+    if (g_later.n > 0) {
+        if (sllm_shim_is_open()) hipStreamSynchronize(sllm_shim_stream());
+        for (size_t i = 0; i < g_later.n; ++i) buffer_drop(&g_later.v[i]);
+        free(g_later.v);
+        g_later.v = NULL;
+        g_later.n = g_later.cap = 0;
+    }
+    pthread_mutex_unlock(&g_later.mtx);
+}
+
+void sllm_shim_attn_close(void) { release_later(); }
+
+/* Frees n buffers once what is on the stream is done with them. */
+static void release(buffer *b, int n) {
+    hipStreamCaptureStatus is = hipStreamCaptureStatusNone;
+    if (sllm_shim_is_open() && hipStreamIsCapturing(sllm_shim_stream(), &is) == hipSuccess && is != hipStreamCaptureStatusNone) {
+        pthread_mutex_lock(&g_later.mtx);
+        for (int i = 0; i < n; ++i) {
+            if (g_later.n == g_later.cap) {
+                const size_t cap = g_later.cap ? g_later.cap * 2 : 16;
+                buffer *v = realloc(g_later.v, cap * sizeof *v);
+                if (v == NULL) break;                    /* (it stays until the process ends) */
+                g_later.v = v;
+                g_later.cap = cap;
+            }
+            g_later.v[g_later.n++] = b[i];
+        }
+        pthread_mutex_unlock(&g_later.mtx);
+        memset(b, 0, (size_t) n * sizeof *b);
+        return;
+    }
+    release_later();
+    if (sllm_shim_is_open()) hipStreamSynchronize(sllm_shim_stream());
+    for (int i = 0; i < n; ++i) buffer_drop(&b[i]);
+}
+
 /* What changes who holds which page runs once, on the host: a graph would replay
  * its copies into pages that are others' by then. */
 static int not_in_capture(const char *who) {
     hipStreamCaptureStatus is = hipStreamCaptureStatusNone;
     const hipError_t e = hipStreamIsCapturing(sllm_shim_stream(), &is);
     if (e != hipSuccess) return sllm_shim_hip_fail(e, "hipStreamIsCapturing");
-    return is == hipStreamCaptureStatusNone ? SLLM_GFX950_OK : FAIL_ARG("%s: the stream is being captured", who);
+    if (is != hipStreamCaptureStatusNone) return FAIL_ARG("%s: the stream is being captured", who);
+    release_later();
+    return SLLM_GFX950_OK;
 }
 
 static int misaligned(const void *p) { return ((uintptr_t) p & 15u) != 0; }
@@ -91,14 +150,7 @@ typedef struct sequence {
     uint32_t mark;                   /* the call that named it last (pool's stamp) */
 } sequence;
 
-/* a batch's device memory and the pinned memory its tables are sent from; kept
- * by the cache for the next batch (`sent`: the copy out of `pin` is done) */
-typedef struct buffer {
-    uint8_t   *dev, *pin;
-    size_t     dev_bytes, pin_bytes;
-    hipEvent_t sent;
-} buffer;
-
+/* a batch's buffer is kept by the cache for the next batch */
 #define KEPT_BUFFERS 4
 
 struct sllm_gfx950_pages {
@@ -170,17 +222,10 @@ int sllm_gfx950_pages_new(const sllm_gfx950_pages_desc *d, sllm_gfx950_pages **o
     return SLLM_GFX950_OK;
 }
 
-static void buffer_drop(buffer *b) {
-    if (b->dev) hipFree(b->dev);
-    if (b->pin) hipHostFree(b->pin);
-    if (b->sent) hipEventDestroy(b->sent);
-    memset(b, 0, sizeof *b);
-}
-
 static void pages_drop(sllm_gfx950_pages *p) {
-    if (sllm_shim_is_open()) hipStreamSynchronize(sllm_shim_stream());
-    for (int i = 0; i < p->n_kept; ++i) buffer_drop(&p->kept[i]);
-    if (p->own_mem) hipFree(p->mem);
+    buffer own = { .dev = p->own_mem ? p->mem : NULL };
+    release(p->kept, p->n_kept);
+    release(&own, 1);
     for (int32_t i = 0; i < p->n_seq; ++i) free(p->seq[i].page);
     free(p->seq);
     free(p->refs);
@@ -716,8 +761,7 @@ static void buffer_put(sllm_gfx950_pages *p, buffer *b) {
             p->kept[least] = *b;
             *b = t;
         }
-        if (sllm_shim_is_open()) hipStreamSynchronize(sllm_shim_stream());
-        buffer_drop(b);
+        release(b, 1);
         return;
     }
     p->kept[p->n_kept++] = *b;
@@ -1173,10 +1217,8 @@ int sllm_gfx950_prompt_create(const sllm_gfx950_prompt_desc *d, sllm_gfx950_prom
 
 void sllm_gfx950_prompt_destroy(sllm_gfx950_prompt *p) {
     if (p == NULL) return;
-    if (p->items) {
-        if (sllm_shim_is_open()) hipStreamSynchronize(sllm_shim_stream());
-        hipFree(p->items);
-    }
+    buffer own = { .dev = (uint8_t *) p->items };
+    release(&own, 1);
     free(p);
 }
 

@@ -404,6 +404,7 @@ void sllm_gfx950_close(void) {
     pthread_mutex_lock(&g_mtx);
     if (g.open) {
         hipStreamSynchronize(g.stream);
+        sllm_shim_attn_close();
         d2h_free();
         for (size_t i = 0; i < g.n_regs; ++i) hipFree(g.regs[i].dev);
         free(g.regs);

@@ -77,6 +77,8 @@ enum {
     SLLM_ATTN_STORE = 26, SLLM_ATTN_COPY = 29, SLLM_ATTN_FUNCTIONS = 30
 };
 SLLM_HIDDEN hipFunction_t sllm_shim_attn_function(int i);
+/* attn.c's part of close: what could not be freed during a capture */
+SLLM_HIDDEN void        sllm_shim_attn_close(void);
 /* grid gx x gy of `block` threads on the library stream */
 SLLM_HIDDEN int         sllm_shim_launch(hipFunction_t f, uint32_t gx, uint32_t gy, uint32_t block,
                                          uint32_t lds, void **args);

@@ -23,6 +23,8 @@
  *                                is not the reported one unless 0, and takes
  *                                neither memory nor launches
  *   fakehip_capture(on)          the streams are being captured, or not
+ *   fakehip_broken()             calls made meanwhile that a capture does not allow:
+ *                                they wait, or free memory
  *   fakehip_launches()           kernels launched since the last fakehip_clear:
  *                                name:grid, a space behind each
  */
@@ -45,6 +47,7 @@ static char     g_launches[4096];     /* (names past its end are dropped) */
 static size_t   g_launches_len;
 static __thread int g_current;
 static int      g_capturing;
+static int      g_broken;
 
 FAKE_EXPORT void fakehip_fail(const char *fn, int err, unsigned skip) {
     snprintf(g_fail_fn, sizeof g_fail_fn, "%s", fn);
@@ -58,6 +61,7 @@ FAKE_EXPORT int  fakehip_fired(void) { return g_fired; }
 FAKE_EXPORT long fakehip_live(void) { return g_live; }
 FAKE_EXPORT void fakehip_current(int d) { g_current = d; }
 FAKE_EXPORT void fakehip_capture(int on) { g_capturing = on; }
+FAKE_EXPORT int  fakehip_broken(void) { return g_broken; }
 FAKE_EXPORT unsigned long fakehip_calls(void) { return g_calls; }
 
 static int inject(const char *fn) {
@@ -100,7 +104,7 @@ hipError_t hipMalloc(void **p, size_t bytes) {
     *p = fake_alloc(bytes);
     return *p ? hipSuccess : hipErrorOutOfMemory;
 }
-hipError_t hipFree(void *p) { ++g_calls; return fake_release(p); }
+hipError_t hipFree(void *p) { ++g_calls; g_broken += g_capturing; return fake_release(p); }
 /* pinned memory, for hipPointerGetAttributes (past the table: not known) */
 static struct { const uint8_t *p; size_t bytes; } g_pinned[64];
 hipError_t hipHostMalloc(void **p, size_t bytes, unsigned int flags) {
@@ -115,6 +119,7 @@ hipError_t hipHostMalloc(void **p, size_t bytes, unsigned int flags) {
 }
 hipError_t hipHostFree(void *p) {
     ++g_calls;
+    g_broken += g_capturing;
     for (size_t i = 0; i < sizeof g_pinned / sizeof *g_pinned; ++i) if (g_pinned[i].p == p) g_pinned[i].p = NULL;
     return fake_release(p);
 }
@@ -221,12 +226,12 @@ hipError_t hipStreamCreateWithFlags(hipStream_t *s, unsigned int flags) {
     return hipSuccess;
 }
 hipError_t hipStreamDestroy(hipStream_t s) { ++g_calls; free(s); --g_live; return hipSuccess; }
-hipError_t hipStreamSynchronize(hipStream_t s) { (void) s; INJECT(); return hipSuccess; }
+hipError_t hipStreamSynchronize(hipStream_t s) { (void) s; g_broken += g_capturing; INJECT(); return hipSuccess; }
 hipError_t hipEventCreate(hipEvent_t *e) { *e = NULL; INJECT(); *e = (hipEvent_t) malloc(1); ++g_live; return hipSuccess; }
 hipError_t hipEventCreateWithFlags(hipEvent_t *e, unsigned flags) { (void) flags; return hipEventCreate(e); }
 hipError_t hipEventDestroy(hipEvent_t e) { ++g_calls; free(e); --g_live; return hipSuccess; }
 hipError_t hipEventRecord(hipEvent_t e, hipStream_t s) { (void) e; (void) s; INJECT(); return hipSuccess; }
-hipError_t hipEventSynchronize(hipEvent_t e) { (void) e; INJECT(); return hipSuccess; }
+hipError_t hipEventSynchronize(hipEvent_t e) { (void) e; g_broken += g_capturing; INJECT(); return hipSuccess; }
 hipError_t hipEventElapsedTime(float *ms, hipEvent_t a, hipEvent_t b) {
     (void) a; (void) b;
     INJECT();
