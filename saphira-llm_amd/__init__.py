@@ -745,7 +745,8 @@ class PagedCache:
         ids = (c_int32 * max(n, 1))(*seqs)
         while True:
             out = np.empty(self.room, np.int32)
-            total = lib().sllm_gfx950_seq_tables(self.p, ids, n, ptr(out), out.size)
+            # (the address as a number: ptr() took 0.8 us of 3 here)
+            total = lib().sllm_gfx950_seq_tables(self.p, ids, n, out.__array_interface__["data"][0], out.size)
             check(min(total, 0), "seq_tables")
             if total <= out.size:
                 return out[:total].copy()
