@@ -185,7 +185,7 @@ struct attention {
     // a lane's pieces of q: 8 values (SPLIT: and what rounding left of them), or 4 f32
     t8 qf[WIDE ? 1 : NT][WIDE ? 1 : QC], ql[SPLIT ? NT : 1][SPLIT ? QC : 1];
     f32x4 qw[WIDE ? NT : 1][WIDE ? QC : 1];
-    int lim_min, lim_max;           // of the wave's rows
+    int lim_min;                    // of the wave's rows
 
     __device__ __forceinline__ uint32_t row_of(int nt) const {
         return min((KEYS ? 0u : wave * (16u * NT)) + 16u * (uint32_t) nt + li, it.n_rows - 1u);
@@ -207,10 +207,7 @@ struct attention {
     __device__ __forceinline__ void load_q() {
         const uint32_t first = KEYS ? 0u : wave * (16u * NT);
         lim_min = limit(place_of(min(first, it.n_rows - 1u)).t);
-        lim_max = limit(place_of(min(first + 16u * NT, it.n_rows) - 1u).t);
         lim_min = (int) uniform((uint32_t) lim_min);
-        lim_max = (int) uniform((uint32_t) lim_max);
-        if (first >= it.n_rows) lim_max = 0;                     // a wave without rows
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
             const place at = place_of(row_of(nt));
