@@ -109,3 +109,17 @@ def test_values_of_a_prompt_that_are_all_alike(amd, dev, dtype, n_q):
     q = torch.zeros(n_q, 2, d, dtype=T)
     q[:, :, 0] = 1.0
     assert torch.equal(bounds.prompt(amd, dev, dtype, q, k, v, [n_q], [n], scale), v[:1].expand(n_q, 2, d))
+
+
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("n_q", [20, 300, 2000])
+def test_f32_results_are_divided_with_one_rounding_each(amd, dev, d, n_q):
+    """Scores of 0 and values of 1: the sums are whole numbers n, and a prompt's result is n
+    times the reciprocal of n, both correctly rounded; a step's, joined from parts or
+    not, is n / n."""
+    q, k, v = torch.ones(n_q, 2, d), torch.zeros(n_q, 1, d), torch.ones(n_q, 1, d)
+    n = np.arange(1, n_q + 1, dtype=np.float32)
+    want = torch.from_numpy(n * (np.float32(1) / n))[:, None, None].expand(n_q, 2, d)
+    assert torch.equal(bounds.prompt(amd, dev, "float32", q, k, v, [n_q], [n_q], 1.0), want)
+    got = bounds.step(amd, dev, "float32", "float32", 2, [(k, v)], q[:1], [1], 1.0, page=64)
+    assert ((got == 1) | (got == want[-1:])).all()
