@@ -739,26 +739,33 @@ class PagedCache:
         return n
 
     def _page_numbers(self, seqs):
-        """Of n sequences, one behind another, as they all are at one time: from the call
-        that had room for them (other threads may give them pages between two calls)."""
+        """Of n sequences, one behind another, as they all are at one time: (ints, how many of
+        them), from the call that had room for them, since other threads may give them pages
+        between two calls. (A ctypes array, and what it holds as an array of numpy in one
+        call: an address through numpy costs as much as the rest of a small fork's host part.)"""
         n = len(seqs)
         ids = (c_int32 * max(n, 1))(*seqs)
         while True:
-            out = np.empty(self.room, np.int32)
-            # (the address as a number: ptr() took 0.8 us of 3 here)
-            total = lib().sllm_gfx950_seq_tables(self.p, ids, n, out.__array_interface__["data"][0], out.size)
+            room = self.room
+            out = (c_int32 * room)()
+            total = lib().sllm_gfx950_seq_tables(self.p, ids, n, out, room)
             check(min(total, 0), "seq_tables")
-            if total <= out.size:
-                return out[:total].copy()
-            self.room = max(self.room, total + total // 4)
+            if total <= room:
+                return out, total
+            self.room = 1 << total.bit_length()
 
     def table(self, seq):
         """A sequence's page numbers (int32)."""
-        return self._page_numbers([seq])
+        out, total = self._page_numbers((seq,))
+        return np.ndarray(total, np.int32, out)
 
     def tables(self, seqs):
         """The page numbers of sequences that have equally many (int32[n][pages])."""
-        return self._page_numbers(seqs).reshape((len(seqs), -1) if len(seqs) else (0, 0))
+        out, total = self._page_numbers(seqs)
+        n = len(seqs)
+        if n and total % n:
+            raise ValueError("tables: sequences of different numbers of pages")
+        return np.ndarray((n, total // n if n else 0), np.int32, out)
 
     def compact(self):
         """Move the pages in use to the front; how many were moved."""

@@ -95,3 +95,8 @@ def test_tables_of_several(amd, cache):
     assert cache.tables([]).shape == (0, 0) and cache.tables([c, c]).shape == (2, 0) and cache.table(c).size == 0
     with pytest.raises(amd.GFX950Error):
         cache.table(77)
+    with pytest.raises(ValueError):                     # 3 and 0 pages
+        cache.tables([a, c])
+    got = cache.table(a)
+    got[0] = 9                                          # (the caller's own)
+    assert cache.table(a).tolist() == [0, 1, 2] and got.dtype == np.int32
