@@ -1,11 +1,14 @@
 """Caches, batches and prompt plans that end while the stream is captured, against
 the HIP stand-in of tests/fakehip: nothing is waited for or freed until it is not."""
 import ctypes
+import os
+import subprocess
+import sys
 from ctypes import byref, c_int, c_void_p
 
 import pytest
 
-from test_attn_host import F32, I, Cache, L  # noqa: F401  (the fixture)
+from test_attn_host import F32, I, ROOT, Cache, L  # noqa: F401  (the fixture)
 
 
 @pytest.fixture
@@ -69,8 +72,25 @@ def test_a_cache_that_goes_with_its_last_batch(amd, L):  # noqa: F811
 
 
 def test_or_by_close(amd, L, ends):  # noqa: F811
-    """(the last of this file: the library is closed and opened again)"""
+    """(the library is closed and opened again)"""
     in_capture(L, ends)
     L.sllm_gfx950_close()
     assert L.fakehip_live() == 0
     assert L.sllm_gfx950_open(0) == 0
+
+
+def test_under_asan_and_ubsan():
+    """This file's other tests, and those of the tables, against the sanitizer build."""
+    if os.environ.get("SLLM_FAKEHIP_SAN"):
+        pytest.skip("this is that run")
+    asan = subprocess.run(["gcc", "-print-file-name=libasan.so"], capture_output=True, text=True).stdout.strip()
+    if not os.path.isabs(asan) or not os.path.exists(asan):
+        pytest.skip("gcc's AddressSanitizer runtime is not installed")
+    env = dict(os.environ, SLLM_FAKEHIP_SAN="1", UBSAN_OPTIONS="print_stacktrace=1:halt_on_error=1",
+               ASAN_OPTIONS="detect_leaks=0:abort_on_error=1",
+               LD_PRELOAD=asan + (":" + os.environ["LD_PRELOAD"] if os.environ.get("LD_PRELOAD") else ""))
+    here = os.path.dirname(os.path.abspath(__file__))
+    r = subprocess.run([sys.executable, "-m", "pytest", "-x", "-q", "-p", "no:cacheprovider", os.path.abspath(__file__),
+                        os.path.join(here, "test_attn_tables_host.py")], cwd=ROOT, env=env, capture_output=True, text=True, timeout=600)
+    out = r.stdout + r.stderr
+    assert r.returncode == 0 and "AddressSanitizer" not in out and "runtime error:" not in out, out[-5000:]
