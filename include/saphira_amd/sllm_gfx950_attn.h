@@ -64,7 +64,7 @@ extern "C" {
  *   [page][layer][K, V][KV head][position in the page][head_dim]
  *
  * mem: that much device memory of the caller's, 16-byte aligned, kept until
- * the cache is freed; NULL: the cache allocates it. Its contents are not
+ * the cache is freed and its batches are destroyed; NULL: the cache allocates it. Its contents are not
  * cleared; what no store has written is never part of a result.
  *
  * A sequence is a number of positions and the pages that hold them, in order.
@@ -170,7 +170,8 @@ int  sllm_gfx950_batch_attend(sllm_gfx950_batch *b, int32_t layer, const void *q
  * Causal attention over n_seq packed sequences: sequence i has q_len[i] query
  * rows and k_len[i] key rows (k_len NULL: as many), one sequence behind the
  * other, and its query row j sees key rows 0 .. j + k_len[i] - q_len[i]. A row
- * that sees none is 0. Every length may be 0.
+ * that sees none is 0. Every length may be 0. A plan serves any number of calls,
+ * one after the other or captured into graphs, which are valid while it lives.
  */
 typedef struct sllm_gfx950_prompt_desc {
     int32_t dtype, n_head, n_head_kv, head_dim, n_seq;

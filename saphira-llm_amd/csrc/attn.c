@@ -616,7 +616,9 @@ typedef struct plan {
 
 /* The runs of order[lo .. hi), which share their pages below `from`. At most two
  * per sequence: one of its own, and one at each place where it parts from its
- * neighbour. */
+ * neighbour. A range is gone through once for each depth in pages at which some of
+ * it part, so a sequence no more often than it has shared pages: less work than
+ * copying its page numbers is, also for a chain of forks. */
 static void find_segments(plan *x, int32_t lo, int32_t hi, int32_t from) {
     while (hi - lo > 1) {
         int32_t common = INT32_MAX;

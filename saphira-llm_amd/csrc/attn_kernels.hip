@@ -901,15 +901,17 @@ __device__ __forceinline__ att_item item_of(const att_args &a) {
 }
 
 // Whole prompts. 4 head_dim operations for a row and a key that it sees: the matrix unit
-// bounds f32, the vector unit beside it 16 bits (four instructions to a matrix one, of
+// bounds f32, the vector unit beside it 16 bits (3.8 instructions to a matrix one, of
 // which one in seven is an exponential). Two workgroups a CU, 64 KB of LDS and at most 256
 // registers each, so that one's barrier falls into the other's products; 128 rows a
 // workgroup read a tile of keys from LDS once for two products. With 20 heads over 5 of
-// 128: 16384 rows f16 1.41 to 1.47 ms, 0.93 to 0.97 PFLOP/s (a large product here
+// 128: 16384 rows f16 1.40 to 1.50 ms by machine, 0.92 to 0.98 PFLOP/s (a large product
 // reaches 1.20; the clock goes down to about 1.9 GHz under both); 24 prompts of up to 2048
-// rows bf16 155 us, 0.66, where reading q and writing the results (37 us of copying) is
-// little hidden; 4 prompts f32 495 us, 110 TFLOP/s of 153, the matrix unit busy 81 % of
-// the time. 32 rows a wave and not 64, one wave a SIMD: 1.52 against 1.85 ms.
+// rows bf16 149 to 155 us, 0.66 to 0.69, where reading q and writing the results (37 us of
+// copying) is little hidden; 4 prompts f32 497 us, 110 TFLOP/s of 153, the matrix unit busy
+// 81 % of the time. 32 rows a wave and not 64, one wave a SIMD: 1.52 against 1.85 ms. A
+// head_dim is padded to 64 or 128: 4096 rows bf16 take 85 us at 64, 117 at 80, 118 at 96
+// (no tile's rows are whole there, so each copy asks) and 112 at 128.
 template <typename T, int D>
 __device__ __forceinline__ void prompt_body(const att_args &a) {
     __shared__ __attribute__((aligned(1024))) uint8_t S[LDS_BYTES<T, D>];
@@ -922,10 +924,11 @@ __device__ __forceinline__ void prompt_body(const att_args &a) {
 // A step over the cache. Few rows (one sequence's own keys) are bound by memory: each
 // key is read once, straight into registers, by one wave, and a split's four waves are
 // joined in LDS. 8 sequences of up to 65536 positions, bf16, 20 heads over 5 of 128: 374
-// MB in 62.8 us with the join, 5.9 TB/s. Many rows (keys that sequences share, prompts
+// MB in 63.0 us with the join, 5.9 TB/s. Many rows (keys that sequences share, prompts
 // behind a prefix) go as prompts do: 64 sequences behind 4096 shared positions and up to
-// 1024 of their own, f32 rows over f16, 30.3 us. All kinds in one launch, which is no
-// longer than its longest workgroup: at these sizes that, and the join's launch, bound it.
+// 1024 of their own, f32 rows over f16, 30.1 us. All kinds in one launch, so
+// that few and many rows run side by side: at these sizes a workgroup's start, the
+// uneven shares and the join's launch bound it.
 template <typename A, typename T, int D>
 __device__ __forceinline__ void paged_body(const att_args &a) {
     __shared__ __attribute__((aligned(1024))) uint8_t S[LDS_BYTES<T, D>];
