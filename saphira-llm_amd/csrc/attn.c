@@ -223,9 +223,9 @@ int sllm_gfx950_pages_new(const sllm_gfx950_pages_desc *d, sllm_gfx950_pages **o
 }
 
 static void pages_drop(sllm_gfx950_pages *p) {
-    buffer own = { .dev = p->own_mem ? p->mem : NULL };
+    buffer own = { .dev = p->mem };
     release(p->kept, p->n_kept);
-    release(&own, 1);
+    if (p->own_mem) release(&own, 1);
     for (int32_t i = 0; i < p->n_seq; ++i) free(p->seq[i].page);
     free(p->seq);
     free(p->refs);
@@ -1220,7 +1220,7 @@ int sllm_gfx950_prompt_create(const sllm_gfx950_prompt_desc *d, sllm_gfx950_prom
 void sllm_gfx950_prompt_destroy(sllm_gfx950_prompt *p) {
     if (p == NULL) return;
     buffer own = { .dev = (uint8_t *) p->items };
-    release(&own, 1);
+    if (p->items) release(&own, 1);
     free(p);
 }
 
