@@ -17,9 +17,8 @@
  * cache's type, so a 16-bit result's error is about sqrt(2) times what rounding
  * it alone leaves; f32 rows over an f16 cache keep 22 bits of weights and of
  * queries (of elements below 2^-17 of a row's largest, all but 2^-39 of that). The
- * sum of weights times values that is carried along may be 256 times (f16 caches:
- * 2^15 times) the number of keys larger than the result, and over f32 and bf16
- * caches, whose values may be that large, overflows there.
+ * sum of weights times values overflows where that with weights of at most 1 does:
+ * values times their number beyond f32's range; values below 2^-118 may lose bits.
  *
  * Calls may come from several threads, whichever device each has current: a
  * cache's calls exclude each other, and everything runs in call order on the

@@ -417,14 +417,18 @@ struct attention {
     };
 
     // The maximum moves only where a score is over it by 8 or more (as a power of two):
-    // until then p is at most 256, which costs no precision, the sums need no scaling, and
-    // the lanes that hold a row need not agree on its largest score. f16 weights are 2^7
-    // larger: at most 2^15, which f16 holds, so that its smallest, 2^-24, is 2^-31 or less of
-    // a row's largest weight and not 2^-24 (the share of 4000
-    // keys with weights about 2^-25 of one's was 0.8 % off). The sums and the parts of a split
-    // carry the factor alike. Whether any did; then f is what the sums of products so far are
-    // to be scaled by.
-    static constexpr float UP = is_f16<T>::value ? 7.0f : 0.0f;
+    // until then weights are at most 256 times what they were when it moved, which costs no
+    // precision, the sums need no scaling, and the lanes that hold a row need not agree on its
+    // largest score. m is UP below the maximum, so weights are 2^UP where it moved and up to
+    // 2^(UP + 8) after. f32 and bf16, whose values may be as large as f32 holds: at most 1, so
+    // that sums overflow no sooner than with the true maximum (at 256 they did; values under
+    // 2^-118 lose bits to it instead). f16: at
+    // most 2^15, which it holds, so that its smallest, 2^-24, is 2^-31 or less of a row's
+    // largest weight and not 2^-24 (the share of 4000 keys with weights about 2^-25 of one's
+    // was 0.8 % off); its values times that are far from f32's end. The sums and the parts of
+    // a split carry the factor alike. Whether any did; then f is what the sums of products
+    // so far are to be scaled by.
+    static constexpr float UP = is_f16<T>::value ? 7.0f : -8.0f;
     __device__ __forceinline__ bool adjust(const scores &s, float (&f)[NT]) {
         float top[NT];
         bool over = false;
@@ -441,7 +445,7 @@ struct attention {
         if (!__any(over)) return false;
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
-            const float t = row_max(top[nt]), to = fmaf(t, c[nt], -m[nt]) > 8.0f + UP ? fmaf(t, c[nt], -UP) : m[nt];   // (by the row's own scores alone)
+            const float t = row_max(top[nt]), to = fmaf(t, c[nt], -m[nt]) > 8.0f + UP ? t * c[nt] - UP : m[nt];   // (by the row's own scores alone)
             f[nt] = __builtin_amdgcn_exp2f(m[nt] - to);
             l[nt] *= f[nt];
             m[nt] = to;

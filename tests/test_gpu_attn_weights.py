@@ -123,3 +123,37 @@ def test_f32_results_are_divided_with_one_rounding_each(amd, dev, d, n_q):
     assert torch.equal(bounds.prompt(amd, dev, "float32", q, k, v, [n_q], [n_q], 1.0), want)
     got = bounds.step(amd, dev, "float32", "float32", 2, [(k, v)], q[:1], [1], 1.0, page=64)
     assert ((got == 1) | (got == want[-1:])).all()
+
+
+def ramp(n, d, T, value):
+    """Keys whose scores rise by 2^5 (as weights) over every 500, with large values: the
+    running maximum need not move, and a sum of 2^5 times the values would overflow."""
+    k = torch.zeros(n, 1, d)
+    k[:, 0, 0] = torch.arange(n) % 500 * (5 * np.log(2.0) / 500)
+    return k.to(T), torch.full((n, 1, d), value).to(T)
+
+
+@pytest.mark.parametrize("act,dtype", PAIRS)
+@pytest.mark.parametrize("n_new", N_NEW)
+def test_sums_of_large_values(amd, dev, act, dtype, n_new):
+    """2000 values of 2^117 (f16: 2^15) and weights that sum up to 560 of the largest: within
+    f32's range where no weight is over 1, and not where they may be 2^5."""
+    n, d, kv, T = 2000, 64, 32, ora.TYPES[act]
+    value = 2.0 ** (15 if dtype == "float16" else 117)
+    k, v = ramp(n, d, T, value)
+    seq = tuple(x.expand(n, kv, d).contiguous() for x in (k, v))
+    q = sink_queries(8 * n_new, 2 * kv, d, T)
+    got = bounds.step(amd, dev, act, dtype, 2 * kv, [seq] * 8, q, [n_new] * 8, 0.25, page=64)
+    want = torch.full_like(got, value)
+    assert ((got.double() - value).abs() <= (2 * (n + 8) + 3) * 2.0 ** -24 * value).all() if act == "float32" else torch.equal(got, want)
+
+
+@pytest.mark.parametrize("dtype", list(ora.TYPES))
+@pytest.mark.parametrize("n_q", [1, 40, 300])
+def test_sums_of_large_values_of_a_prompt(amd, dev, dtype, n_q):
+    n, d, T = 2000, 128, ora.TYPES[dtype]
+    value = 2.0 ** (15 if dtype == "float16" else 117)
+    k, v = ramp(n, d, T, value)
+    got = bounds.prompt(amd, dev, dtype, sink_queries(n_q, 2, d, T), k, v, [n_q], [n], 0.25)
+    want = torch.full_like(got, value)
+    assert ((got.double() - value).abs() <= (2 * (n + 8) + 3) * 2.0 ** -24 * value).all() if dtype == "float32" else torch.equal(got, want)
