@@ -12,6 +12,7 @@ The directory name carries a hyphen, so load it by path::
 """
 from __future__ import annotations
 
+import array
 import ctypes
 import os
 from ctypes import POINTER, c_char_p, c_float, c_int, c_int32, c_size_t, c_uint, c_uint64, c_void_p
@@ -721,17 +722,18 @@ class PagedCache:
 
     def copy(self, seqs):
         """A sequence with pages of its own for each of seqs."""
-        n = len(seqs)
+        ids = array.array("i", seqs)
+        n = len(ids)
         out = (c_int32 * max(n, 1))()
-        check(lib().sllm_gfx950_seq_copy(self.p, (c_int32 * max(n, 1))(*seqs), n, out), "seq_copy")
+        check(lib().sllm_gfx950_seq_copy(self.p, ids.buffer_info()[0], n, out), "seq_copy")
         return out[:n]
 
     def truncate(self, seq, n_tokens):
         check(lib().sllm_gfx950_seq_truncate(self.p, seq, n_tokens), "seq_truncate")
 
     def free(self, seqs):
-        n = len(seqs)
-        check(lib().sllm_gfx950_seq_free(self.p, (c_int32 * max(n, 1))(*seqs), n), "seq_free")
+        ids = array.array("i", seqs)
+        check(lib().sllm_gfx950_seq_free(self.p, *ids.buffer_info()), "seq_free")
 
     def length(self, seq):
         n = lib().sllm_gfx950_seq_len(self.p, seq)
@@ -743,12 +745,11 @@ class PagedCache:
         them), from the call that had room for them, since other threads may give them pages
         between two calls. (A ctypes array, and what it holds as an array of numpy in one
         call: an address through numpy costs as much as the rest of a small fork's host part.)"""
-        n = len(seqs)
-        ids = (c_int32 * max(n, 1))(*seqs)
+        ids = array.array("i", seqs)
         while True:
             room = self.room
             out = (c_int32 * room)()
-            total = lib().sllm_gfx950_seq_tables(self.p, ids, n, out, room)
+            total = lib().sllm_gfx950_seq_tables(self.p, *ids.buffer_info(), out, room)
             check(min(total, 0), "seq_tables")
             if total <= room:
                 return out, total

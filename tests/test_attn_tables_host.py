@@ -100,3 +100,21 @@ def test_tables_of_several(amd, cache):
     got = cache.table(a)
     got[0] = 9                                          # (the caller's own)
     assert cache.table(a).tolist() == [0, 1, 2] and got.dtype == np.int32
+
+
+def test_sequence_numbers_of_any_kind(amd, cache):
+    """Lists, tuples, ranges and arrays of numpy; none; what is no sequence number."""
+    s = [cache.new() for _ in range(4)]
+    grow(cache, s[1], 20)
+    for kind in (list, tuple, np.array, lambda x: np.array(x, np.int64), iter):
+        out = cache.copy(kind(s[:2]))
+        assert len(out) == 2 and cache.length(out[1]) == 20
+        cache.free(kind(out))
+    assert cache.copy([]) == [] and cache.free([]) is None
+    with pytest.raises(OverflowError):
+        cache.free([1 << 32])                           # (not sequence 0)
+    with pytest.raises(TypeError):
+        cache.free([1.5])
+    with pytest.raises(amd.GFX950Error):
+        cache.free([s[0], 9])
+    assert cache.length(s[0]) == 0
