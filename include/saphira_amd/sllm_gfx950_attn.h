@@ -14,8 +14,8 @@
  * of 8, at most 128; n_head is a multiple of n_head_kv, and query head h reads
  * KV head h / (n_head / n_head_kv). Scores, softmax sums and sums of products
  * are held in f32. The weights that multiply the values are rounded to the
- * cache's type, so a 16-bit result's error is about sqrt(2) times what rounding
- * it alone leaves; f32 rows over an f16 cache keep 22 bits of weights and of
+ * cache's type, so a 16-bit result's error is up to 1.4 times what rounding it
+ * alone leaves; f32 rows over an f16 cache keep 22 bits of weights and of
  * queries (of elements below 2^-17 of a row's largest, all but 2^-39 of that). The
  * sum of weights times values overflows where that with weights of at most 1 does:
  * values times their number beyond f32's range; values below 2^-118 may lose bits.

@@ -407,9 +407,9 @@ struct attention {
     }
 
     // p of a tile as the products take it: the cache's type (SPLIT: and what rounding to
-    // it left), or f32. Rounding p to 16 bits makes a result's error sqrt(2) times what
-    // rounding the result alone leaves, and halves the products and their operands; the sum
-    // is of p as it was rounded, so that weights still add up to 1: values that are all alike
+    // it left), or f32. Rounding p to 16 bits halves the products and their operands, and
+    // makes a result's error up to 1.4 times what rounding the result alone leaves. The sum is
+    // of p as it was rounded, so that weights still add up to 1: values that are all alike
     // come back as they are (they were 0.4 % off where bf16 rounded all weights one way).
     struct probs {
         t8 p[WIDE ? 1 : NT], rest[SPLIT ? NT : 1];
@@ -422,12 +422,11 @@ struct attention {
     // largest score. m is UP below the maximum, so weights are 2^UP where it moved and up to
     // 2^(UP + 8) after. f32 and bf16, whose values may be as large as f32 holds: at most 1, so
     // that sums overflow no sooner than with the true maximum (at 256 they did; values under
-    // 2^-118 lose bits to it instead). f16: at
-    // most 2^15, which it holds, so that its smallest, 2^-24, is 2^-31 or less of a row's
-    // largest weight and not 2^-24 (the share of 4000 keys with weights about 2^-25 of one's
-    // was 0.8 % off); its values times that are far from f32's end. The sums and the parts of
-    // a split carry the factor alike. Whether any did; then f is what the sums of products
-    // so far are to be scaled by.
+    // 2^-118 lose bits to it instead). f16: at most 2^15, which it holds, so that its
+    // smallest, 2^-24, is 2^-31 or less of a row's largest weight and not 2^-24 (the share of
+    // 4000 keys with weights about 2^-25 of one's was 0.8 % off); its values times that are
+    // far from f32's end. The sums and the parts of a split carry the factor alike. Whether
+    // any moved; then f is what the sums of products so far are to be scaled by.
     static constexpr float UP = is_f16<T>::value ? 7.0f : -8.0f;
     __device__ __forceinline__ bool adjust(const scores &s, float (&f)[NT]) {
         float top[NT];

@@ -1,6 +1,7 @@
 """Keys and values that are not finite among many new positions over a paged cache
 (sllm_gfx950_attn.h) on the GPU: workgroups of 16, 64 and 128 rows, their keys in
-parts, with and without a shared prefix. Rows that do not see them keep every bit."""
+parts, with and without a shared prefix. Rows that do not see them keep every bit.
+And such steps without them, against 64 bits (attn_bounds.py)."""
 import math
 
 import pytest
@@ -50,6 +51,19 @@ def test_what_a_row_does_not_see(amd, dev, act, dtype, d, n_new, prefix, bad):
     assert not torch.isfinite(got[1, at - 1:, 2:, 5].float()).any() and not torch.isfinite(got[1, n_new - 1, :, 7].float()).any()
     if math.isnan(bad):
         assert torch.isnan(got[1, at:, :2].float()).all()
+
+
+@pytest.mark.parametrize("act,dtype", PAIRS)
+@pytest.mark.parametrize("heads,kv,d", [(4, 2, 128), (6, 2, 72), (5, 5, 96), (8, 1, 64)])
+@pytest.mark.parametrize("n_new,prefix", [([3, 25, 70], 0), ([90, 1, 200], 400), ([1, 1, 150], 0)])
+def test_many_new_positions(amd, dev, act, dtype, heads, kv, d, n_new, prefix):
+    """Chunks of prompts and single positions in one step, against 64 bits."""
+    T = ora.TYPES[act]
+    shared = [normal(1 + i, prefix, kv, d).to(T) for i in range(2)]
+    seqs = [tuple(torch.cat([s, normal(10 * j + i + 3, 300 + 77 * j + n, kv, d).to(T)]) for i, s in enumerate(shared))
+            for j, n in enumerate(n_new)]
+    q = normal(50, sum(n_new), heads, d).to(T)
+    bounds.check_step(amd, dev, act, dtype, heads, seqs, q, n_new, d ** -0.5, page=32, prefix=prefix)
 
 
 @pytest.mark.parametrize("act,dtype", PAIRS)
