@@ -44,6 +44,9 @@ extern "C" {
 #define SLLM_GFX950_F32  0
 #define SLLM_GFX950_F16  1
 #define SLLM_GFX950_BF16 2
+/* of a cache alone: 8 bits and a scale for each row (a position's keys or values of a head) */
+#define SLLM_GFX950_I8   4           /* -127 .. 127 */
+#define SLLM_GFX950_E4M3 5           /* floating-point: 4 bits of exponent, 3 of mantissa, up to 448 */
 
 #define SLLM_GFX950_ATTN_MAX_HEAD_DIM 128
 #define SLLM_GFX950_ATTN_MAX_HEADS    1024
@@ -65,6 +68,14 @@ extern "C" {
  * mem: that much device memory of the caller's, 16-byte aligned, kept until
  * the cache is freed and its batches are destroyed; NULL: the cache allocates it. Its contents are not
  * cleared; what no store has written is never part of a result.
+ *
+ * I8 and E4M3 (head_dim a multiple of 16): a KV head's keys or values of a page are its
+ * positions' codes, then a scale byte for each. A code stands for code * 2^(byte - 127): the
+ * smallest such power of two, 2^-126 or more (E4M3: 2^-117), that 127 (448) times it is at
+ * least the row's largest magnitude; codes are rounded to nearest, ties to even. So a row
+ * depends on its own values alone, whatever comes before or after it or with it, and what it
+ * stands for is exact in f32 and bf16. A row of which something is not finite, or over
+ * 127 * 2^120, stands for NaN throughout (its byte is 255).
  *
  * A sequence is a number of positions and the pages that hold them, in order.
  * Pages are handed out lowest free number first. Pages that several sequences
@@ -104,6 +115,14 @@ int     sllm_gfx950_seq_fork(sllm_gfx950_pages *p, int32_t src, int32_t n_tokens
 int     sllm_gfx950_seq_copy(sllm_gfx950_pages *p, const int32_t *src, int32_t n, int32_t *seqs);
 /* drop the positions from n_tokens on; pages that nobody holds any more are free again */
 int     sllm_gfx950_seq_truncate(sllm_gfx950_pages *p, int32_t seq, int32_t n_tokens);
+/*
+ * Beams that go on from other beams: seqs[i], each named once, becomes what
+ * seqs[parent[i]] was (0 <= parent[i] < n), all at one time. Whole pages are shared; the
+ * page that a sequence ends in is kept by itself, or else by the first that goes on from
+ * it, and copied for each other, in pages that are free then. SLLM_GFX950_ERR_NOMEM where
+ * these are too few, and nothing is changed.
+ */
+int     sllm_gfx950_seq_reorder(sllm_gfx950_pages *p, const int32_t *seqs, const int32_t *parent, int32_t n);
 /* end n sequences: all of them, or none where one is unknown or named twice */
 int     sllm_gfx950_seq_free(sllm_gfx950_pages *p, const int32_t *seqs, int32_t n);
 /* positions of a sequence, or a negative status */
@@ -131,7 +150,9 @@ int     sllm_gfx950_pages_compact(sllm_gfx950_pages *p, int32_t *n_moved);
  * for each layer, store writes the rows' keys and values and attend reads them.
  *
  * act_dtype is the type of every row given or returned: the cache's, or f32
- * over an f16 cache (rounded to nearest by store; queries are not rounded).
+ * over an f16 cache (rounded to nearest by store; queries are not rounded), or
+ * any of the three over 8 bits. Over 8 bits keys and values are what their codes
+ * stand for, and queries and weights keep all their bits (f32), 16 (f16) or the 8 of bf16.
  *
  * A batch holds its pages until it is destroyed, whatever happens to its
  * sequences meanwhile; the next batch of a sequence that was truncated may
@@ -153,6 +174,14 @@ int32_t sllm_gfx950_batch_rows(const sllm_gfx950_batch *b);
 int  sllm_gfx950_batch_store(sllm_gfx950_batch *b, int32_t layer, const void *k, size_t k_stride, const void *v,
                              size_t v_stride);
 /*
+ * The keys and values of a layer read back as rows of act_dtype, every position of
+ * the batch's sequences, old and new, sequence by sequence: k, v [batch_positions][n_head_kv]
+ * [head_dim], strides as above. Rounded to nearest where act_dtype holds less (f16 of 8 bits).
+ * k and v overlap neither each other nor the cache. At most SLLM_GFX950_ATTN_MAX_LEN positions.
+ */
+int64_t sllm_gfx950_batch_positions(const sllm_gfx950_batch *b);
+int  sllm_gfx950_batch_read(sllm_gfx950_batch *b, int32_t layer, void *k, size_t k_stride, void *v, size_t v_stride);
+/*
  * out = softmax(scale q . k) v for q and out [rows][n_head][head_dim]: a row
  * sees its sequence's positions up to its own. Whole pages that several of the
  * batch's sequences share are read once for all of them. scale > 0; strides as
@@ -160,6 +189,67 @@ int  sllm_gfx950_batch_store(sllm_gfx950_batch *b, int32_t layer, const void *k,
  */
 int  sllm_gfx950_batch_attend(sllm_gfx950_batch *b, int32_t layer, const void *q, size_t q_stride, float scale,
                               void *out, size_t out_stride);
+
+/* ------------------------------------------------------------------ */
+/* rotary positions                                                    */
+/* ------------------------------------------------------------------ */
+
+/*
+ * The first n_rot of a head's dimensions, a multiple of 8, are pairs that turn by
+ * position times a frequency: (a, b) becomes magnitude (a cos - b sin, b cos + a sin).
+ * Pair i is dimensions i and i + n_rot / 2 (HALVES) or 2 i and 2 i + 1 (PAIRS), and turns by
+ * freq[i], or base^(-2 i / n_rot), radians a position. For long contexts:
+ *
+ *   LINEAR  the frequency divided by factor
+ *   NTK     base times factor^(n_rot / (n_rot - 2))
+ *   PARTS   with turns = original * frequency / (2 pi): as it is from `fast` turns on,
+ *           divided by factor below `slow`, and between them in proportion
+ *
+ * Angles are exact to 2^-30 of a turn at any position of 32 bits; rows are computed in f32
+ * and rounded once.
+ */
+enum { SLLM_GFX950_ROPE_HALVES, SLLM_GFX950_ROPE_PAIRS };
+enum { SLLM_GFX950_ROPE_PLAIN, SLLM_GFX950_ROPE_LINEAR, SLLM_GFX950_ROPE_NTK, SLLM_GFX950_ROPE_PARTS };
+
+typedef struct sllm_gfx950_rope_desc {
+    int32_t head_dim, n_rot, layout, scaling;
+    double  base, factor;            /* factor > 0 where there is scaling */
+    double  original, fast, slow;    /* PARTS: slow < fast */
+    double  magnitude;               /* 0: 1 */
+    const double *freq;              /* n_rot / 2, or NULL; not with NTK */
+} sllm_gfx950_rope_desc;
+
+typedef struct sllm_gfx950_rope sllm_gfx950_rope;
+
+/* rope_new is refused while the stream is captured */
+int  sllm_gfx950_rope_new(const sllm_gfx950_rope_desc *d, sllm_gfx950_rope **out);
+/* (graphs that turn rows by it are valid while it lives) */
+void sllm_gfx950_rope_free(sllm_gfx950_rope *r);
+
+/*
+ * Rows of q [n_rows][n_head][head_dim] and, or NULL, k [n_rows][n_head_kv][head_dim], row i
+ * at position pos[i] (device memory; below 0 too), into q_out and k_out: where they come from
+ * (same pointer and stride), or memory that overlaps nothing the call reads. Strides in
+ * elements, multiples of 16 bytes, 0: packed. back: turned the other way, which is the
+ * gradient of what the call did.
+ */
+typedef struct sllm_gfx950_rope_io {
+    int32_t dtype, n_rows, n_head, n_head_kv, back;
+    const int32_t *pos;
+    const void *q, *k;
+    void       *q_out, *k_out;
+    size_t      q_stride, q_out_stride, k_stride, k_out_stride;
+} sllm_gfx950_rope_io;
+int  sllm_gfx950_rope_rows(sllm_gfx950_rope *r, const sllm_gfx950_rope_io *io);
+
+/*
+ * A batch's rows at their own positions in one launch: queries turned into q_out (q
+ * itself, or apart from q, k and v), keys turned and stored, values stored, as
+ * rope_rows and batch_store would (but that turned keys are not rounded to act_dtype before they
+ * are to the cache's type).
+ */
+int  sllm_gfx950_batch_rope_store(sllm_gfx950_batch *b, int32_t layer, sllm_gfx950_rope *r, const void *q, size_t q_stride, void *q_out,
+                                  size_t q_out_stride, const void *k, size_t k_stride, const void *v, size_t v_stride);
 
 /* ------------------------------------------------------------------ */
 /* whole prompts                                                       */

@@ -15,7 +15,7 @@ from __future__ import annotations
 import array
 import ctypes
 import os
-from ctypes import POINTER, c_char_p, c_float, c_int, c_int32, c_size_t, c_uint, c_uint64, c_void_p
+from ctypes import POINTER, c_char_p, c_double, c_float, c_int, c_int32, c_int64, c_size_t, c_uint, c_uint64, c_void_p
 
 import numpy as np
 
@@ -96,8 +96,23 @@ class PromptIO(ctypes.Structure):
                [(n, c_size_t) for n in ("q_tok", "q_head", "k_tok", "k_head", "v_tok", "v_head", "out_tok", "out_head")]
 
 
-# element types of a cache and of attention's rows (sllm_gfx950_attn.h)
-DTYPES = {"float32": 0, "float16": 1, "bfloat16": 2}
+class RopeDesc(ctypes.Structure):
+    """sllm_gfx950_rope_desc."""
+    _fields_ = [("head_dim", c_int32), ("n_rot", c_int32), ("layout", c_int32), ("scaling", c_int32)] + \
+               [(n, c_double) for n in ("base", "factor", "original", "fast", "slow", "magnitude")] + [("freq", c_void_p)]
+
+
+class RopeIO(ctypes.Structure):
+    """sllm_gfx950_rope_io."""
+    _fields_ = [(n, c_int32) for n in ("dtype", "n_rows", "n_head", "n_head_kv", "back")] + \
+               [(n, c_void_p) for n in ("pos", "q", "k", "q_out", "k_out")] + \
+               [(n, c_size_t) for n in ("q_stride", "q_out_stride", "k_stride", "k_out_stride")]
+
+
+# element types of a cache and of attention's rows (sllm_gfx950_attn.h); the last two of a cache alone
+DTYPES = {"float32": 0, "float16": 1, "bfloat16": 2, "int8": 4, "float8_e4m3": 5}
+ROPE_LAYOUTS = {"half": 0, "pairs": 1}
+ROPE_SCALINGS = {"none": 0, "linear": 1, "ntk": 2, "parts": 3}
 
 # Every function the C ABI exports: name -> (restype, argtypes).
 PROTOTYPES = {
@@ -191,12 +206,20 @@ PROTOTYPES = {
     "sllm_gfx950_seq_free": (c_int, [c_void_p, c_void_p, c_int32]),
     "sllm_gfx950_seq_len": (c_int32, [c_void_p, c_int32]),
     "sllm_gfx950_seq_tables": (c_int32, [c_void_p, c_void_p, c_int32, c_void_p, c_int32]),
+    "sllm_gfx950_seq_reorder": (c_int, [c_void_p, c_void_p, c_void_p, c_int32]),
     "sllm_gfx950_pages_compact": (c_int, [c_void_p, POINTER(c_int32)]),
     "sllm_gfx950_batch_create": (c_int, [c_void_p, c_void_p, c_void_p, c_int32, c_int32, c_int32, POINTER(c_void_p)]),
     "sllm_gfx950_batch_destroy": (None, [c_void_p]),
     "sllm_gfx950_batch_rows": (c_int32, [c_void_p]),
     "sllm_gfx950_batch_store": (c_int, [c_void_p, c_int32, c_void_p, c_size_t, c_void_p, c_size_t]),
     "sllm_gfx950_batch_attend": (c_int, [c_void_p, c_int32, c_void_p, c_size_t, c_float, c_void_p, c_size_t]),
+    "sllm_gfx950_batch_positions": (c_int64, [c_void_p]),
+    "sllm_gfx950_batch_read": (c_int, [c_void_p, c_int32, c_void_p, c_size_t, c_void_p, c_size_t]),
+    "sllm_gfx950_rope_new": (c_int, [POINTER(RopeDesc), POINTER(c_void_p)]),
+    "sllm_gfx950_rope_free": (None, [c_void_p]),
+    "sllm_gfx950_rope_rows": (c_int, [c_void_p, POINTER(RopeIO)]),
+    "sllm_gfx950_batch_rope_store": (c_int, [c_void_p, c_int32, c_void_p, c_void_p, c_size_t, c_void_p, c_size_t, c_void_p, c_size_t,
+                                             c_void_p, c_size_t]),
     "sllm_gfx950_prompt_create": (c_int, [POINTER(PromptDesc), POINTER(c_void_p)]),
     "sllm_gfx950_prompt_attend": (c_int, [c_void_p, POINTER(PromptIO)]),
     "sllm_gfx950_prompt_destroy": (None, [c_void_p]),
@@ -728,6 +751,13 @@ class PagedCache:
         check(lib().sllm_gfx950_seq_copy(self.p, ids.buffer_info()[0], n, out), "seq_copy")
         return out[:n]
 
+    def reorder(self, seqs, parents):
+        """seqs[i] becomes what seqs[parents[i]] was, for all i at one time."""
+        ids, to = array.array("i", seqs), array.array("i", parents)
+        if len(ids) != len(to):
+            raise ValueError("reorder: one parent for each sequence")
+        check(lib().sllm_gfx950_seq_reorder(self.p, ids.buffer_info()[0], *to.buffer_info()), "seq_reorder")
+
     def truncate(self, seq, n_tokens):
         check(lib().sllm_gfx950_seq_truncate(self.p, seq, n_tokens), "seq_truncate")
 
@@ -809,6 +839,19 @@ class Batch:
     def store(self, layer, k, v, k_stride=0, v_stride=0):
         check(lib().sllm_gfx950_batch_store(self.b, layer, k, k_stride, v, v_stride), "batch_store")
 
+    def rope_store(self, layer, rope, q, q_out, k, v, q_stride=0, q_out_stride=0, k_stride=0, v_stride=0):
+        """Queries turned into q_out (q itself: in place), turned keys and values stored."""
+        check(lib().sllm_gfx950_batch_rope_store(self.b, layer, rope.r, q, q_stride, q_out, q_out_stride, k, k_stride, v, v_stride),
+              "batch_rope_store")
+
+    @property
+    def positions(self):
+        return lib().sllm_gfx950_batch_positions(self.b)
+
+    def read(self, layer, k, v, k_stride=0, v_stride=0):
+        """Every position's keys and values as rows of the batch's type."""
+        check(lib().sllm_gfx950_batch_read(self.b, layer, k, k_stride, v, v_stride), "batch_read")
+
     def attend(self, layer, q, out, scale, q_stride=0, out_stride=0):
         check(lib().sllm_gfx950_batch_attend(self.b, layer, q, q_stride, scale, out, out_stride), "batch_attend")
 
@@ -819,6 +862,37 @@ class Batch:
 
     def __del__(self):
         if getattr(self, "b", None) and _lib is not None:
+            self.close()
+
+
+class Rope:
+    """sllm_gfx950_rope: rotary positions of the first n_rot dimensions of heads of head_dim."""
+
+    def __init__(self, dev, head_dim, n_rot=None, base=10000.0, layout="half", scaling="none", factor=1.0, original=0.0, fast=0.0,
+                 slow=0.0, magnitude=1.0, freq=None):
+        self.dev, self.r = dev, None
+        n_rot = head_dim if n_rot is None else n_rot
+        f = None if freq is None else np.ascontiguousarray(freq, np.float64)
+        if f is not None and f.shape != (n_rot // 2,):
+            raise ValueError("rope: n_rot / 2 frequencies")
+        d = RopeDesc(head_dim, n_rot, ROPE_LAYOUTS[layout], ROPE_SCALINGS[scaling], base, factor, original, fast, slow, magnitude,
+                     None if f is None else ptr(f))
+        r = c_void_p()
+        check(lib().sllm_gfx950_rope_new(ctypes.byref(d), ctypes.byref(r)), "rope_new")
+        self.r = r
+
+    def rows(self, dtype, pos, n_rows, q, n_head, q_out, k=None, n_head_kv=0, k_out=None, strides=(0, 0, 0, 0), back=False):
+        """Device addresses; strides of q, q_out, k and k_out in elements, 0: packed."""
+        io = RopeIO(DTYPES[dtype], n_rows, n_head, n_head_kv, 1 if back else 0, pos, q, k, q_out, k_out, *strides)
+        check(lib().sllm_gfx950_rope_rows(self.r, ctypes.byref(io)), "rope_rows")
+
+    def close(self):
+        if self.r:
+            lib().sllm_gfx950_rope_free(self.r)
+            self.r = None
+
+    def __del__(self):
+        if getattr(self, "r", None) and _lib is not None:
             self.close()
 
 

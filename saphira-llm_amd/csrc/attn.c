@@ -55,11 +55,13 @@ static void device_leave(device_scope *s) { if (s->moved) hipSetDevice(s->was); 
 
 #define LOG2E 1.44269504088896340736
 
-static uint32_t type_size(int32_t dtype) { return dtype == SLLM_GFX950_F32 ? 4u : 2u; }
+static int held8(int32_t dtype) { return dtype == SLLM_GFX950_I8 || dtype == SLLM_GFX950_E4M3; }
+static uint32_t type_size(int32_t dtype) { return dtype == SLLM_GFX950_F32 ? 4u : held8(dtype) ? 1u : 2u; }
 static int bad_type(int32_t dtype) { return dtype != SLLM_GFX950_F32 && dtype != SLLM_GFX950_F16 && dtype != SLLM_GFX950_BF16; }
 
 /* the kernels' instances for rows and a cache of these types (shim_internal.h), or -1 */
 static int type_pair(int32_t act, int32_t cache) {
+    if (held8(cache)) return SLLM_ATTN_HELD8 + 3 * (cache == SLLM_GFX950_E4M3) + act;
     if (act == cache) return act == SLLM_GFX950_F32 ? 0 : act == SLLM_GFX950_F16 ? 2 : 3;
     return act == SLLM_GFX950_F32 && cache == SLLM_GFX950_F16 ? 1 : -1;
 }
@@ -137,6 +139,12 @@ static int not_in_capture(const char *who) {
     return SLLM_GFX950_OK;
 }
 
+/* what the kernels of rows call a cache's type */
+static uint32_t held_as(int32_t dtype) {
+    return dtype == SLLM_GFX950_F32 ? ATT_HELD_F32 : dtype == SLLM_GFX950_F16 ? ATT_HELD_F16 : dtype == SLLM_GFX950_BF16 ? ATT_HELD_BF16 :
+           dtype == SLLM_GFX950_I8 ? ATT_HELD_I8 : ATT_HELD_E4M3;
+}
+
 static int misaligned(const void *p) { return ((uintptr_t) p & 15u) != 0; }
 
 /* ------------------------------------------------------------------ */
@@ -172,11 +180,13 @@ struct sllm_gfx950_pages {
 };
 
 static uint64_t desc_page_bytes(const sllm_gfx950_pages_desc *d) {
-    return (uint64_t) d->n_layer * 2u * (uint64_t) d->n_head_kv * (uint64_t) d->page_tokens * (uint64_t) d->head_dim * type_size(d->dtype);
+    /* (8 bits: a scale byte for each row) */
+    const uint64_t row = (uint64_t) d->head_dim * type_size(d->dtype) + (uint64_t) held8(d->dtype);
+    return (uint64_t) d->n_layer * 2u * (uint64_t) d->n_head_kv * (uint64_t) d->page_tokens * row;
 }
 
 static int bad_desc(const sllm_gfx950_pages_desc *d) {
-    return d == NULL || bad_type(d->dtype) || bad_heads(d->n_head_kv, d->n_head_kv, d->head_dim) || d->n_layer < 1 ||
+    return d == NULL || (bad_type(d->dtype) && !held8(d->dtype)) || (held8(d->dtype) && d->head_dim % 16 != 0) || bad_heads(d->n_head_kv, d->n_head_kv, d->head_dim) || d->n_layer < 1 ||
            d->n_layer > 65536 || d->page_tokens < 16 || d->page_tokens > 1024 || (d->page_tokens & (d->page_tokens - 1)) != 0 ||
            d->n_pages < 1 || d->n_pages > (1 << 28) || desc_page_bytes(d) > 1ull << 32;
 }
@@ -205,7 +215,7 @@ int sllm_gfx950_pages_new(const sllm_gfx950_pages_desc *d, sllm_gfx950_pages **o
     p->page_bytes = desc_page_bytes(d);
     p->layer_bytes = p->page_bytes / (uint64_t) d->n_layer;
     p->row_bytes = (uint32_t) d->head_dim * type_size(d->dtype);
-    p->block_bytes = (uint32_t) d->page_tokens * p->row_bytes;
+    p->block_bytes = (uint32_t) d->page_tokens * (p->row_bytes + (uint32_t) held8(d->dtype));
     while ((1 << p->page_shift) < d->page_tokens) ++p->page_shift;
     p->mem = d->mem;
     if (p->mem == NULL) {
@@ -339,15 +349,16 @@ static void copies_start(copies *c, const sllm_gfx950_pages *p) {
     c->a.block_bytes = p->block_bytes;
     c->a.row_bytes = p->row_bytes;
     c->a.n_blocks = (uint32_t) (p->page_bytes / p->block_bytes);
+    c->a.scales = held8(p->d.dtype) ? (uint32_t) p->d.page_tokens * p->row_bytes : 0;
     c->a.n_pairs = c->most = 0;
     c->st = SLLM_GFX950_OK;
 }
 
 static int copies_flush(copies *c) {
     if (c->st == SLLM_GFX950_OK && c->a.n_pairs > 0) {
-        const uint64_t chunks = (uint64_t) c->most * c->a.row_bytes / 16u * c->a.n_blocks;
+        const uint64_t chunks = ((uint64_t) c->most * c->a.row_bytes / 16u + (c->a.scales ? (c->most + 15u) / 16u : 0u)) * c->a.n_blocks;
         void *args[] = { &c->a };
-        c->st = sllm_shim_launch(sllm_shim_attn_function(SLLM_ATTN_COPY),
+        c->st = sllm_shim_launch(sllm_shim_attn_function(c->a.scales ? SLLM_ATTN_COPY8 : SLLM_ATTN_COPY),
                                  (uint32_t) ((chunks + ATT_COPY_CHUNKS - 1) / ATT_COPY_CHUNKS), c->a.n_pairs, ATT_THREADS, 0, args);
     }
     c->a.n_pairs = c->most = 0;
@@ -475,6 +486,103 @@ static int check_names(sllm_gfx950_pages *p, const int32_t *seqs, int32_t n, con
     return SLLM_GFX950_OK;
 }
 
+static void hold_page(sllm_gfx950_pages *p, int32_t page) {      /* (one that may be free) */
+    if (p->refs[page]++ == 0 && p->holds[page] == 0) --p->n_free;
+}
+
+/* The new pages of seqs[i]: its parent's, `was` their old tables (at[i] .. at[i + 1]); the page
+ * that the parent ends in goes to keeper[parent] alone. hold: they are taken up, else given back. */
+static void reorder_pages(sllm_gfx950_pages *p, const int32_t *parent, const int32_t *keeper, const int32_t *was, const int32_t *at,
+                          const int32_t *len, int32_t i, int hold) {
+    const int32_t q = parent[i], whole = len[q] >> p->page_shift, n = keeper[q] == i ? at[q + 1] - at[q] : whole;
+    for (int32_t j = 0; j < n; ++j) {
+        if (hold) hold_page(p, was[at[q] + j]);
+        else give_page(p, was[at[q] + j]);
+    }
+}
+
+int sllm_gfx950_seq_reorder(sllm_gfx950_pages *p, const int32_t *seqs, const int32_t *parent, int32_t n) {
+    ATT_ON_DEVICE();
+    if (p == NULL || n < 0 || (n > 0 && (seqs == NULL || parent == NULL))) return FAIL_ARG("seq_reorder: NULL or a count below 0");
+    if (n > SLLM_GFX950_ATTN_MAX_SEQS) return FAIL_ARG("seq_reorder: %d sequences", n);
+    for (int32_t i = 0; i < n; ++i) {
+        if (parent[i] < 0 || parent[i] >= n) return FAIL_ARG("seq_reorder: sequence %d of %d goes on from %d", i, n, parent[i]);
+    }
+    int32_t *work = malloc(((size_t) n * 3 + 1) * sizeof *work), *was = NULL;
+    if (work == NULL) return FAIL_NOMEM("seq_reorder: %d sequences", n);
+    int32_t *keeper = work, *len = work + n, *at = work + 2 * (size_t) n;
+    pthread_mutex_lock(&p->mtx);
+    int st = not_in_capture("seq_reorder");
+    if (st == SLLM_GFX950_OK) st = check_names(p, seqs, n, "seq_reorder");
+    int64_t total = 0, need = 0;
+    if (st == SLLM_GFX950_OK) {
+        for (int32_t i = 0; i < n; ++i) {
+            keeper[i] = -1;
+            len[i] = p->seq[seqs[i]].len;
+            total += p->seq[seqs[i]].n_pages;
+        }
+        for (int32_t i = n - 1; i >= 0; --i) if (keeper[parent[i]] != parent[i]) keeper[parent[i]] = i;     /* itself, or the first */
+        for (int32_t i = 0; i < n; ++i) need += keeper[parent[i]] != i && (len[parent[i]] & (p->d.page_tokens - 1)) != 0;
+        if (total > INT32_MAX) st = FAIL_ARG("seq_reorder: too many pages");
+        else if ((was = malloc((size_t) (total ? total : 1) * sizeof *was)) == NULL) st = FAIL_NOMEM("seq_reorder: %lld pages", (long long) total);
+    }
+    if (st == SLLM_GFX950_OK) {
+        at[0] = 0;
+        for (int32_t i = 0; i < n; ++i) {
+            const sequence *s = &p->seq[seqs[i]];
+            if (s->n_pages > 0) memcpy(was + at[i], s->page, (size_t) s->n_pages * sizeof *was);
+            at[i + 1] = at[i] + s->n_pages;
+        }
+        for (int32_t i = 0; i < n && st == SLLM_GFX950_OK; ++i) {
+            if (!reserve(&p->seq[seqs[i]], at[parent[i] + 1] - at[parent[i]])) st = FAIL_NOMEM("seq_reorder: page table");
+        }
+    }
+    if (st == SLLM_GFX950_OK) {
+        /* what is held on, then what nobody holds any more: that may be enough for the copies.
+         * (What a copy reads is held, so no copy writes it.) */
+        for (int32_t i = 0; i < n; ++i) if (parent[i] != i) reorder_pages(p, parent, keeper, was, at, len, i, 1);
+        for (int32_t i = 0; i < n; ++i) if (parent[i] != i) for (int32_t j = at[i]; j < at[i + 1]; ++j) give_page(p, was[j]);
+        int32_t got = 0;
+        if (need > p->n_free) st = FAIL_NOMEM("seq_reorder: %lld pages wanted, %d free", (long long) need, p->n_free);
+        else {
+            copies c;
+            copies_start(&c, p);
+            for (; got < n; ++got) {
+                const int32_t q = parent[got], whole = len[q] >> p->page_shift, rows = len[q] & (p->d.page_tokens - 1);
+                sequence *s = &p->seq[seqs[got]];
+                if (q == got) continue;
+                s->n_pages = at[q + 1] - at[q];
+                s->len = len[q];
+                if (s->n_pages > 0) memcpy(s->page, was + at[q], (size_t) s->n_pages * sizeof *was);
+                if (rows && keeper[q] != got) {
+                    s->page[whole] = take_page(p);
+                    copies_add(&c, was[at[q] + whole], s->page[whole], rows);
+                }
+            }
+            st = copies_flush(&c);
+        }
+        if (st != SLLM_GFX950_OK) {                      /* as it was */
+            for (int32_t i = 0; i < got; ++i) {
+                const int32_t q = parent[i], whole = len[q] >> p->page_shift;
+                if (q != i && keeper[q] != i && (len[q] & (p->d.page_tokens - 1)) != 0) give_page(p, p->seq[seqs[i]].page[whole]);
+            }
+            for (int32_t i = 0; i < n; ++i) if (parent[i] != i) for (int32_t j = at[i]; j < at[i + 1]; ++j) hold_page(p, was[j]);
+            for (int32_t i = 0; i < n; ++i) if (parent[i] != i) reorder_pages(p, parent, keeper, was, at, len, i, 0);
+            for (int32_t i = 0; i < got; ++i) {
+                sequence *s = &p->seq[seqs[i]];
+                if (parent[i] == i) continue;
+                s->n_pages = at[i + 1] - at[i];
+                s->len = len[i];
+                if (s->n_pages > 0) memcpy(s->page, was + at[i], (size_t) s->n_pages * sizeof *was);
+            }
+        }
+    }
+    pthread_mutex_unlock(&p->mtx);
+    free(work);
+    free(was);
+    return st;
+}
+
 int sllm_gfx950_seq_free(sllm_gfx950_pages *p, const int32_t *seqs, int32_t n) {
     ATT_NEED_OPEN();
     if (p == NULL || n < 0 || (n > 0 && seqs == NULL)) return FAIL_ARG("seq_free: NULL or a count below 0");
@@ -581,12 +689,14 @@ static att_item *items_add(items *x) {
 
 struct sllm_gfx950_batch {
     sllm_gfx950_pages *p;
-    int32_t   n_head, pair;
-    uint32_t  n_tok;
+    int32_t   n_head, act, pair;
+    int32_t   n_seq;
+    int64_t   n_pos;                 /* positions of its sequences, old and new */
+    uint32_t  n_tok, n_pages;
     uint32_t  n_items;
     uint32_t  join;                  /* the most partial results that a row has */
     buffer    buf;
-    size_t    off_tables, off_list, off_toks, off_segs, off_part_o, off_part_ml;     /* (its items are at 0) */
+    size_t    off_tables, off_list, off_toks, off_segs, off_seqs, off_part_o, off_part_ml;     /* (its items are at 0) */
     int32_t  *held;                  /* the pages it holds */
     int32_t   n_held;
 };
@@ -667,7 +777,8 @@ static const uint32_t k_rows[] = { ATT_FEW_ROWS, ATT_HALF_ROWS, ATT_MANY_ROWS };
 /* A segment's rows: f32 takes two tiles of few before half of many (8 sequences
  * behind 4096 shared positions, 32 rows: 18.7 us against 24.8), 16 bits one (12.6
  * for half of many, 13.0 for two of few). */
-static uint32_t mode_of(uint32_t rows, int32_t dtype) {
+static uint32_t mode_of(uint32_t rows, int32_t dtype, int32_t act) {
+    if (held8(dtype) && act == SLLM_GFX950_F32) return rows <= ATT_FEW_ROWS ? ATT_FEW : ATT_HALF;    /* (held8_body) */
     const uint32_t few = dtype == SLLM_GFX950_F32 ? 2 * ATT_FEW_ROWS : ATT_FEW_ROWS;
     return rows <= few ? ATT_FEW : rows <= ATT_HALF_ROWS ? ATT_HALF : ATT_MANY;
 }
@@ -797,7 +908,7 @@ static int lay_out(sllm_gfx950_batch *b, plan *x, int32_t n, const int32_t *len0
         for (int32_t j = s->lo; j < s->hi; ++j) s->n_tok += (uint32_t) x->n_new[x->order[j]];
         s->list = ATT_TOKENS;
         if (s->hi - s->lo > 1) { s->list = (uint32_t) n_list; n_list += s->n_tok; }
-        s->mode = mode_of(s->n_tok * group, p->d.dtype);
+        s->mode = mode_of(s->n_tok * group, p->d.dtype, b->act);
     }
     /* segments of each sequence, and those with one part alone */
     uint32_t *seg_count = calloc((size_t) n + 1, sizeof *seg_count), *seg_at = calloc((size_t) n + 1, sizeof *seg_at);
@@ -868,6 +979,7 @@ static int lay_out(sllm_gfx950_batch *b, plan *x, int32_t n, const int32_t *len0
     b->off_list = at;    at = align256(at + n_list * 4);
     b->off_toks = at;    at = align256(at + (size_t) b->n_tok * sizeof(att_tok));
     b->off_segs = at;    at = align256(at + n_segs * sizeof(att_seg));
+    b->off_seqs = at;    at = align256(at + ((size_t) n + 1) * sizeof(att_seq));
     const size_t sent = at;
     b->off_part_ml = at; at = align256(at + n_part * 8);
     b->off_part_o = at;  at = align256(at + n_part * hd_pad * 4);
@@ -888,6 +1000,16 @@ static int lay_out(sllm_gfx950_batch *b, plan *x, int32_t n, const int32_t *len0
             t += (uint32_t) x->n_new[q];
         }
     }
+    att_seq *seqs = (att_seq *) (to + b->off_seqs);
+    uint64_t row0 = 0;
+    for (int32_t i = 0; i < n; ++i) {
+        seqs[i] = (att_seq) { x->table[i], (uint32_t) row0 };        /* (past 32 bits: batch_read refuses) */
+        row0 += (uint64_t) p->seq[x->seqs[i]].len;
+    }
+    seqs[n] = (att_seq) { (uint32_t) n_pages, (uint32_t) row0 };
+    b->n_seq = n;
+    b->n_pos = (int64_t) row0;
+    b->n_pages = (uint32_t) n_pages;
     for (int32_t i = 0; i < n; ++i) {
         const sequence *s = &p->seq[x->seqs[i]];
         if (s->n_pages > 0) memcpy(tables + x->table[i], s->page, (size_t) s->n_pages * 4);
@@ -944,6 +1066,7 @@ int sllm_gfx950_batch_create(sllm_gfx950_pages *p, const int32_t *seqs, const in
     x.table = uwork + n1;
     b->p = p;
     b->n_head = n_head;
+    b->act = act_dtype;
     b->pair = pair;
 
     pthread_mutex_lock(&p->mtx);
@@ -1038,6 +1161,36 @@ void sllm_gfx950_batch_destroy(sllm_gfx950_batch *b) {
 
 int32_t sllm_gfx950_batch_rows(const sllm_gfx950_batch *b) { return b ? (int32_t) b->n_tok : 0; }
 
+/* n rows of `row` bytes, `tok` bytes apart */
+typedef struct rows_at { const void *p; uint64_t tok, row; int64_t n; } rows_at;
+
+/* whether any of their bytes are the same, as far as can be told from their ends and, where
+ * they are equally far apart, from their places between */
+static int overlap(const rows_at *a, const rows_at *b) {
+    if (a->p == NULL || b->p == NULL || a->n == 0 || b->n == 0) return 0;
+    const uint64_t x = (uint64_t) (uintptr_t) a->p, y = (uint64_t) (uintptr_t) b->p;
+    if (x + (uint64_t) (a->n - 1) * a->tok + a->row <= y || y + (uint64_t) (b->n - 1) * b->tok + b->row <= x) return 0;
+    if (a->tok != b->tok) return 1;
+    const uint64_t off = x < y ? (y - x) % a->tok : (a->tok - (x - y) % a->tok) % a->tok;      /* of b behind a row of a */
+    return off < a->row || off + b->row > a->tok;
+}
+
+/* waves of a CU that rows are spread over before a wave takes more of a token's */
+#define ROWS_WAVES 16u
+
+/* Rows on their way (att_rows_args): a token's heads are gone through by one wave, or where
+ * there are few tokens by several. */
+static int rows_go(att_rows_args *a, int32_t dtype) {
+    const uint32_t at_once = a->hd > 64 ? 4 : 8, rows = (a->q ? a->n_head : 0) + (a->k ? a->n_head_kv : 0) + (a->v ? a->n_head_kv : 0);
+    const uint32_t most = (rows + at_once - 1) / at_once, places = (uint32_t) sllm_shim_cu() * ROWS_WAVES;
+    a->waves = (places + a->n_tok - 1) / a->n_tok;
+    if (a->waves > most) a->waves = most;
+    void *args[] = { a };
+    const uint64_t waves = (uint64_t) a->n_tok * a->waves;
+    return sllm_shim_launch(sllm_shim_attn_function(SLLM_ATTN_ROWS + dtype), (uint32_t) ((waves + ATT_THREADS / 64 - 1) / (ATT_THREADS / 64)), 1,
+                            ATT_THREADS, 0, args);
+}
+
 /* bytes between a tensor's rows of `width` elements; 0: not what a call takes */
 static uint64_t row_bytes(size_t stride, uint64_t width, uint32_t size) {
     if (stride == 0) stride = (size_t) width;
@@ -1045,16 +1198,39 @@ static uint64_t row_bytes(size_t stride, uint64_t width, uint32_t size) {
     return (uint64_t) stride * size;
 }
 
+/* A batch's rows into the cache, turned or not (a->k, v, q as given), or its rows of q alone. */
+static int launch_rows(sllm_gfx950_batch *b, int32_t layer, att_rows_args *a) {
+    const sllm_gfx950_pages *p = b->p;
+    uint8_t *layer_mem = p->mem + (uint64_t) layer * p->layer_bytes;
+    a->ck = layer_mem;
+    a->cv = layer_mem + (uint64_t) p->d.n_head_kv * p->block_bytes;
+    a->tables = (const uint32_t *) (b->buf.dev + b->off_tables);
+    a->toks = (const att_tok *) (b->buf.dev + b->off_toks);
+    a->page_bytes = p->page_bytes;
+    a->page_shift = p->page_shift;
+    a->block_bytes = p->block_bytes;
+    a->n_tok = b->n_tok;
+    a->n_head = (uint32_t) b->n_head;
+    a->n_head_kv = (uint32_t) p->d.n_head_kv;
+    a->hd = (uint32_t) p->d.head_dim;
+    a->held = held_as(p->d.dtype);
+    return rows_go(a, b->act);
+}
+
 int sllm_gfx950_batch_store(sllm_gfx950_batch *b, int32_t layer, const void *k, size_t k_stride, const void *v, size_t v_stride) {
     ATT_ON_DEVICE();
     if (b == NULL) return FAIL_ARG("batch_store: NULL");
     sllm_gfx950_pages *p = b->p;
     if (layer < 0 || layer >= p->d.n_layer) return FAIL_ARG("batch_store: layer %d of %d", layer, p->d.n_layer);
-    const uint32_t kv = (uint32_t) p->d.n_head_kv, hd = (uint32_t) p->d.head_dim, size = b->pair <= 1 ? 4u : 2u;
+    const uint32_t kv = (uint32_t) p->d.n_head_kv, hd = (uint32_t) p->d.head_dim, size = type_size(b->act);
     const uint64_t kt = row_bytes(k_stride, (uint64_t) kv * hd, size), vt = row_bytes(v_stride, (uint64_t) kv * hd, size);
     if (kt == 0 || vt == 0) return FAIL_ARG("batch_store: stride");
     if (b->n_tok == 0) return SLLM_GFX950_OK;
     if (k == NULL || v == NULL || misaligned(k) || misaligned(v)) return FAIL_ARG("batch_store: NULL or misaligned rows");
+    if (held8(p->d.dtype)) {
+        att_rows_args r = { .k = k, .v = v, .k_tok = kt, .v_tok = vt };
+        return launch_rows(b, layer, &r);
+    }
     uint8_t *layer_mem = p->mem + (uint64_t) layer * p->layer_bytes;
     att_store_args a = { k, v, layer_mem, layer_mem + (uint64_t) kv * p->block_bytes,
                          (const uint32_t *) (b->buf.dev + b->off_tables), (const att_tok *) (b->buf.dev + b->off_toks), kt, vt, p->page_bytes, p->page_shift, hd, kv, b->n_tok };
@@ -1062,6 +1238,31 @@ int sllm_gfx950_batch_store(sllm_gfx950_batch *b, int32_t layer, const void *k, 
     const uint64_t threads = (uint64_t) b->n_tok * (hd / 8u);
     return sllm_shim_launch(sllm_shim_attn_function(SLLM_ATTN_STORE + (b->pair < 2 ? b->pair : 2)),
                             (uint32_t) ((threads + ATT_THREADS - 1) / ATT_THREADS), 2u * kv, ATT_THREADS, 0, args);
+}
+
+int64_t sllm_gfx950_batch_positions(const sllm_gfx950_batch *b) { return b ? b->n_pos : 0; }
+
+int sllm_gfx950_batch_read(sllm_gfx950_batch *b, int32_t layer, void *k, size_t k_stride, void *v, size_t v_stride) {
+    ATT_ON_DEVICE();
+    if (b == NULL) return FAIL_ARG("batch_read: NULL");
+    const sllm_gfx950_pages *p = b->p;
+    if (layer < 0 || layer >= p->d.n_layer) return FAIL_ARG("batch_read: layer %d of %d", layer, p->d.n_layer);
+    const uint32_t kv = (uint32_t) p->d.n_head_kv, hd = (uint32_t) p->d.head_dim, size = type_size(b->act);
+    const uint64_t width = (uint64_t) kv * hd, kt = row_bytes(k_stride, width, size), vt = row_bytes(v_stride, width, size);
+    if (kt == 0 || vt == 0) return FAIL_ARG("batch_read: stride");
+    if (b->n_pos > SLLM_GFX950_ATTN_MAX_LEN || b->n_pages > MAX_ITEMS) return FAIL_ARG("batch_read: %lld positions", (long long) b->n_pos);
+    if (b->n_pos == 0) return SLLM_GFX950_OK;
+    if (k == NULL || v == NULL || misaligned(k) || misaligned(v)) return FAIL_ARG("batch_read: NULL or misaligned rows");
+    const rows_at ko = { k, kt, width * size, b->n_pos }, vo = { v, vt, width * size, b->n_pos };
+    if (overlap(&ko, &vo)) return FAIL_ARG("batch_read: rows of k and v overlap");
+    const uint8_t *layer_mem = p->mem + (uint64_t) layer * p->layer_bytes;
+    att_read_args a = { k, v, layer_mem, layer_mem + (uint64_t) kv * p->block_bytes, (const uint32_t *) (b->buf.dev + b->off_tables),
+                        (const att_seq *) (b->buf.dev + b->off_seqs), kt, vt, p->page_bytes, (uint32_t) b->n_seq, hd, kv, held_as(p->d.dtype),
+                        p->page_shift, p->block_bytes };
+    void *args[] = { &a };
+    const uint64_t units = (uint64_t) p->d.page_tokens * (hd / 8u) * 2u * kv;
+    const uint32_t per = ATT_THREADS * ATT_READ_UNITS;
+    return sllm_shim_launch(sllm_shim_attn_function(SLLM_ATTN_READ + b->act), b->n_pages, (uint32_t) ((units + per - 1) / per), ATT_THREADS, 0, args);
 }
 
 static int bad_scale(float scale) { return !(scale > 0.0f) || isinf((float) ((double) scale * LOG2E)); }
@@ -1072,7 +1273,7 @@ int sllm_gfx950_batch_attend(sllm_gfx950_batch *b, int32_t layer, const void *q,
     if (b == NULL) return FAIL_ARG("batch_attend: NULL");
     sllm_gfx950_pages *p = b->p;
     if (layer < 0 || layer >= p->d.n_layer) return FAIL_ARG("batch_attend: layer %d of %d", layer, p->d.n_layer);
-    const uint32_t kv = (uint32_t) p->d.n_head_kv, hd = (uint32_t) p->d.head_dim, size = b->pair <= 1 ? 4u : 2u;
+    const uint32_t kv = (uint32_t) p->d.n_head_kv, hd = (uint32_t) p->d.head_dim, size = type_size(b->act);
     const uint64_t qt = row_bytes(q_stride, (uint64_t) b->n_head * hd, size), ot = row_bytes(out_stride, (uint64_t) b->n_head * hd, size);
     if (qt == 0 || ot == 0) return FAIL_ARG("batch_attend: stride");
     if (bad_scale(scale)) return FAIL_ARG("batch_attend: scale %g", (double) scale);
@@ -1086,12 +1287,13 @@ int sllm_gfx950_batch_attend(sllm_gfx950_batch *b, int32_t layer, const void *q,
                    .part_o = (float *) (dev + b->off_part_o), .part_ml = (float *) (dev + b->off_part_ml),
                    .q_tok = qt, .q_head = (uint64_t) hd * size, .out_tok = ot, .out_head = (uint64_t) hd * size,
                    .page_bytes = p->page_bytes, .page_shift = p->page_shift, .hd = hd, .group = group,
-                   .per_group = 1.0f / (float) group, .c = (float) ((double) scale * LOG2E) };
+                   .per_group = 1.0f / (float) group, .c = (float) ((double) scale * LOG2E), .block_bytes = p->block_bytes };
     /* the partial results are one set of memory: a call's launches stay together */
     pthread_mutex_lock(&p->mtx);
     int st = SLLM_GFX950_OK;
     void *args[] = { &a };
-    st = sllm_shim_launch(sllm_shim_attn_function(SLLM_ATTN_ATTEND + b->pair * 2 + (int) wide), a.n_items, 1, ATT_THREADS, 0, args);
+    st = sllm_shim_launch(sllm_shim_attn_function(b->pair >= SLLM_ATTN_HELD8 ? SLLM_ATTN_ATTEND8 + (b->pair - SLLM_ATTN_HELD8) * 2 + (int) wide :
+                                                  SLLM_ATTN_ATTEND + b->pair * 2 + (int) wide), a.n_items, 1, ATT_THREADS, 0, args);
     if (st == SLLM_GFX950_OK && b->join > 0) {
         att_join_args j = { out, a.part_o, a.part_ml, (const att_tok *) (dev + b->off_toks), (const att_seg *) (dev + b->off_segs), ot,
                             hd, group, (uint32_t) b->n_head, 0 };
@@ -1101,7 +1303,7 @@ int sllm_gfx950_batch_attend(sllm_gfx950_batch *b, int32_t layer, const void *q,
          * over 16 parts a row 16.9 / 12.1; 5 to 16 parts alike) */
         const int whole = b->join > 8;
         const uint32_t heads = (uint32_t) b->n_head, gy = whole ? heads : (heads + ATT_THREADS / 64 - 1) / (ATT_THREADS / 64);
-        st = sllm_shim_launch(sllm_shim_attn_function(SLLM_ATTN_JOIN + 6 * whole + (b->pair < 2 ? 0 : b->pair - 1) * 2 + (int) wide),
+        st = sllm_shim_launch(sllm_shim_attn_function(SLLM_ATTN_JOIN + 6 * whole + b->act * 2 + (int) wide),
                               b->n_tok, gy, ATT_THREADS, 0, jargs);
     }
     pthread_mutex_unlock(&p->mtx);
@@ -1181,7 +1383,7 @@ int sllm_gfx950_prompt_create(const sllm_gfx950_prompt_desc *d, sllm_gfx950_prom
         }
         if (whole > MAX_ITEMS) { st = FAIL_ARG("prompt_create: too many rows"); break; }
         const uint32_t rows = (uint32_t) nq * group;
-        const uint32_t own = mode_of(rows, d->dtype) == ATT_FEW ? ATT_FEW : mode, tile = k_rows[own];
+        const uint32_t own = mode_of(rows, d->dtype, d->dtype) == ATT_FEW ? ATT_FEW : mode, tile = k_rows[own];
         for (int32_t h = 0; h < d->n_head_kv && st == SLLM_GFX950_OK; ++h) {
             for (uint32_t r = 0; r < rows; r += tile) {
                 const uint32_t n = rows - r < tile ? rows - r : tile;
@@ -1265,4 +1467,147 @@ int sllm_gfx950_prompt_attend(sllm_gfx950_prompt *p, const sllm_gfx950_prompt_io
     const int type = p->dtype == SLLM_GFX950_F32 ? 0 : p->dtype == SLLM_GFX950_F16 ? 1 : 2;
     void *args[] = { &a };
     return sllm_shim_launch(sllm_shim_attn_function(SLLM_ATTN_PROMPT + type * 2 + (hd > 64)), p->n_items, 1, ATT_THREADS, 0, args);
+}
+
+/* ------------------------------------------------------------------ */
+/* rotary positions                                                    */
+/* ------------------------------------------------------------------ */
+
+struct sllm_gfx950_rope {
+    int32_t   head_dim, n_rot, pairs;
+    float     magnitude;
+    uint64_t *freq;                  /* device */
+};
+
+/* The turns a position of pair i, modulo 1, times 2^64: a position times that, modulo 2^64, is its
+ * angle to 2^-64 of a turn a position, however far it is. */
+static int rope_turns(const sllm_gfx950_rope_desc *d, uint64_t *to) {
+    const long double two_pi = 6.283185307179586476925286766559L;
+    const long double base = d->scaling == SLLM_GFX950_ROPE_NTK ? d->base * powl(d->factor, (long double) d->n_rot / (d->n_rot - 2)) : d->base;
+    for (int32_t i = 0; i < d->n_rot / 2; ++i) {
+        long double f = d->freq ? d->freq[i] : powl(base, -2.0L * i / d->n_rot);
+        if (d->scaling == SLLM_GFX950_ROPE_LINEAR) f /= d->factor;
+        if (d->scaling == SLLM_GFX950_ROPE_PARTS) {
+            long double keep = (d->original * f / two_pi - d->slow) / ((long double) d->fast - d->slow);
+            keep = keep < 0 ? 0 : keep > 1 ? 1 : keep;
+            f = f * keep + f / d->factor * (1 - keep);
+        }
+        if (!isfinite(f)) return 0;
+        long double t = f / two_pi;
+        t -= floorl(t);
+        t = ldexpl(t, 64);
+        to[i] = t >= 18446744073709551615.0L ? UINT64_MAX : (uint64_t) t;
+    }
+    return 1;
+}
+
+int sllm_gfx950_rope_new(const sllm_gfx950_rope_desc *d, sllm_gfx950_rope **out) {
+    ATT_ON_DEVICE();
+    if (out == NULL) return FAIL_ARG("rope_new: NULL out");
+    *out = NULL;
+    if (d == NULL || bad_heads(1, 1, d->head_dim) || d->n_rot < 8 || d->n_rot > d->head_dim || d->n_rot % 8 != 0 ||
+        (d->layout != SLLM_GFX950_ROPE_HALVES && d->layout != SLLM_GFX950_ROPE_PAIRS)) {
+        return FAIL_ARG("rope_new: head dimension, dimensions that turn, or their layout");
+    }
+    if (d->scaling < SLLM_GFX950_ROPE_PLAIN || d->scaling > SLLM_GFX950_ROPE_PARTS || !isfinite(d->magnitude) ||
+        (d->freq == NULL && !(d->base > 0 && isfinite(d->base))) ||
+        (d->scaling != SLLM_GFX950_ROPE_PLAIN && !(d->factor > 0 && isfinite(d->factor))) || (d->scaling == SLLM_GFX950_ROPE_NTK && d->freq != NULL) ||
+        (d->scaling == SLLM_GFX950_ROPE_PARTS && !(d->original > 0 && isfinite(d->original) && isfinite(d->slow) && d->fast > d->slow && isfinite(d->fast)))) {
+        return FAIL_ARG("rope_new: base, frequencies or scaling");
+    }
+    int st = not_in_capture("rope_new");
+    if (st != SLLM_GFX950_OK) return st;
+    uint64_t turns[SLLM_GFX950_ATTN_MAX_HEAD_DIM / 2];
+    if (!rope_turns(d, turns)) return FAIL_ARG("rope_new: a frequency that is not finite");
+    sllm_gfx950_rope *r = calloc(1, sizeof *r);
+    if (r == NULL) return FAIL_NOMEM("rope_new");
+    r->head_dim = d->head_dim;
+    r->n_rot = d->n_rot;
+    r->pairs = d->layout == SLLM_GFX950_ROPE_PAIRS;
+    r->magnitude = d->magnitude == 0 ? 1.0f : (float) d->magnitude;
+    const size_t bytes = (size_t) (d->n_rot / 2) * sizeof *turns;
+    hipError_t e = hipMalloc((void **) &r->freq, bytes);
+    const char *what = "hipMalloc(rope)";
+    if (e != hipSuccess) r->freq = NULL;
+    else {
+        what = "rope_new";
+        e = hipMemcpyAsync(r->freq, turns, bytes, hipMemcpyHostToDevice, sllm_shim_stream());
+        if (e == hipSuccess) e = hipStreamSynchronize(sllm_shim_stream());
+    }
+    if (e != hipSuccess) {
+        if (r->freq) hipFree(r->freq);
+        free(r);
+        return sllm_shim_hip_fail(e, what);
+    }
+    *out = r;
+    return SLLM_GFX950_OK;
+}
+
+void sllm_gfx950_rope_free(sllm_gfx950_rope *r) {
+    if (r == NULL) return;
+    buffer own = { .dev = (uint8_t *) r->freq };
+    release(&own, 1);
+    free(r);
+}
+
+static void rope_args(const sllm_gfx950_rope *r, att_rows_args *a) {
+    a->freq = r->freq;
+    a->half = (uint32_t) r->n_rot / 2;
+    a->pairs = (uint32_t) r->pairs;
+    a->magnitude = r->magnitude;
+}
+
+/* where rows may go: to where they come from, or apart from all that is read */
+static int bad_target(const rows_at *out, const rows_at *own, const rows_at *other, const rows_at *third) {
+    if ((out->p != own->p || out->tok != own->tok) && overlap(out, own)) return 1;
+    return overlap(out, other) || overlap(out, third);
+}
+
+int sllm_gfx950_rope_rows(sllm_gfx950_rope *r, const sllm_gfx950_rope_io *io) {
+    ATT_ON_DEVICE();
+    if (r == NULL || io == NULL) return FAIL_ARG("rope_rows: NULL");
+    if (bad_type(io->dtype) || io->n_rows < 0 || io->n_rows > SLLM_GFX950_ATTN_MAX_TOKENS || io->n_head < 1 || io->n_head > SLLM_GFX950_ATTN_MAX_HEADS ||
+        (io->k != NULL && (io->n_head_kv < 1 || io->n_head_kv > SLLM_GFX950_ATTN_MAX_HEADS))) {
+        return FAIL_ARG("rope_rows: type, rows or heads");
+    }
+    const uint32_t size = type_size(io->dtype), hd = (uint32_t) r->head_dim;
+    const uint64_t qw = (uint64_t) io->n_head * hd, kw = io->k ? (uint64_t) io->n_head_kv * hd : hd;
+    const uint64_t qt = row_bytes(io->q_stride, qw, size), qo = row_bytes(io->q_out_stride, qw, size);
+    const uint64_t kt = io->k ? row_bytes(io->k_stride, kw, size) : 1, ko = io->k ? row_bytes(io->k_out_stride, kw, size) : 1;
+    if (qt == 0 || qo == 0 || kt == 0 || ko == 0) return FAIL_ARG("rope_rows: stride");
+    if (io->n_rows == 0) return SLLM_GFX950_OK;
+    if (io->q == NULL || io->q_out == NULL || io->pos == NULL || (io->k != NULL) != (io->k_out != NULL) || misaligned(io->q) || misaligned(io->q_out) ||
+        misaligned(io->k) || misaligned(io->k_out) || ((uintptr_t) io->pos & 3u) != 0) {
+        return FAIL_ARG("rope_rows: NULL or misaligned rows or positions");
+    }
+    const rows_at q = { io->q, qt, qw * size, io->n_rows }, k = { io->k, kt, kw * size, io->n_rows }, pos = { io->pos, 4, 4, io->n_rows };
+    const rows_at qo_at = { io->q_out, qo, qw * size, io->n_rows }, ko_at = { io->k_out, ko, kw * size, io->n_rows };
+    if (bad_target(&qo_at, &q, &k, &pos) || bad_target(&ko_at, &k, &q, &pos) || overlap(&qo_at, &ko_at)) return FAIL_ARG("rope_rows: rows overlap");
+    att_rows_args a = { .q = io->q, .k = io->k, .q_out = io->q_out, .k_out = io->k_out, .pos = io->pos, .q_tok = qt, .k_tok = kt, .qo_tok = qo, .ko_tok = ko,
+                        .n_tok = (uint32_t) io->n_rows, .n_head = (uint32_t) io->n_head, .n_head_kv = (uint32_t) io->n_head_kv, .hd = hd,
+                        .back = io->back != 0 };
+    rope_args(r, &a);
+    return rows_go(&a, io->dtype);
+}
+
+int sllm_gfx950_batch_rope_store(sllm_gfx950_batch *b, int32_t layer, sllm_gfx950_rope *r, const void *q, size_t q_stride, void *q_out, size_t q_out_stride,
+                                 const void *k, size_t k_stride, const void *v, size_t v_stride) {
+    ATT_ON_DEVICE();
+    if (b == NULL || r == NULL) return FAIL_ARG("batch_rope_store: NULL");
+    const sllm_gfx950_pages *p = b->p;
+    if (layer < 0 || layer >= p->d.n_layer) return FAIL_ARG("batch_rope_store: layer %d of %d", layer, p->d.n_layer);
+    if (r->head_dim != p->d.head_dim) return FAIL_ARG("batch_rope_store: heads of %d and %d", r->head_dim, p->d.head_dim);
+    const uint32_t kv = (uint32_t) p->d.n_head_kv, hd = (uint32_t) p->d.head_dim, size = type_size(b->act);
+    const uint64_t qw = (uint64_t) b->n_head * hd, kw = (uint64_t) kv * hd;
+    const uint64_t qt = row_bytes(q_stride, qw, size), qo = row_bytes(q_out_stride, qw, size), kt = row_bytes(k_stride, kw, size), vt = row_bytes(v_stride, kw, size);
+    if (qt == 0 || qo == 0 || kt == 0 || vt == 0) return FAIL_ARG("batch_rope_store: stride");
+    if (b->n_tok == 0) return SLLM_GFX950_OK;
+    if (q == NULL || q_out == NULL || k == NULL || v == NULL || misaligned(q) || misaligned(q_out) || misaligned(k) || misaligned(v)) {
+        return FAIL_ARG("batch_rope_store: NULL or misaligned rows");
+    }
+    const rows_at out = { q_out, qo, qw * size, b->n_tok }, qr = { q, qt, qw * size, b->n_tok }, kr = { k, kt, kw * size, b->n_tok }, vr = { v, vt, kw * size, b->n_tok };
+    if (bad_target(&out, &qr, &kr, &vr)) return FAIL_ARG("batch_rope_store: rows overlap");
+    att_rows_args a = { .q = q, .k = k, .v = v, .q_out = q_out, .q_tok = qt, .k_tok = kt, .v_tok = vt, .qo_tok = qo };
+    rope_args(r, &a);
+    return launch_rows(b, layer, &a);
 }

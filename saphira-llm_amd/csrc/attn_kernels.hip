@@ -63,6 +63,8 @@ __device__ __forceinline__ float row_sum(float x) {
 template <typename T> struct vec8 { typedef T type __attribute__((ext_vector_type(8))); };
 template <typename T> struct is_f16 { static constexpr bool value = false; };
 template <> struct is_f16<_Float16> { static constexpr bool value = true; };
+template <typename X, typename Y> struct is_same { static constexpr bool value = false; };
+template <typename X> struct is_same<X, X> { static constexpr bool value = true; };
 template <typename T> struct vec4 { typedef T type __attribute__((ext_vector_type(4))); };
 
 __device__ __forceinline__ f32x4 mfma(vec8<_Float16>::type a, vec8<_Float16>::type b, f32x4 c) {
@@ -86,6 +88,28 @@ __device__ __forceinline__ float add_two(__bf16 a, __bf16 b, float c) {
 }
 
 constexpr float LOWEST = -3.402823466e38f;
+
+// what a cache of 8 bits holds
+struct int8_codes {};
+struct e4m3_codes {};
+
+// Codes and their scale as bf16, which holds each of their products exactly (S is 0 where
+// the byte is, of rows that are not there, whose codes are 0).
+__device__ __forceinline__ float scale_value(uint32_t byte) { return __uint_as_float(byte << 23); }
+template <typename S> __device__ __forceinline__ u32x2 values_of_codes(uint32_t v, float by) {
+    typedef __bf16 two __attribute__((ext_vector_type(2)));
+    two a, b;
+    if constexpr (is_same<S, int8_codes>::value) {
+        const uint32_t u = v ^ 0x80808080u;                      // code + 128
+        const float off = -128.0f * by;
+        a = (two) { (__bf16) fmaf((float) (u & 255u), by, off), (__bf16) fmaf((float) (u >> 8 & 255u), by, off) };
+        b = (two) { (__bf16) fmaf((float) (u >> 16 & 255u), by, off), (__bf16) fmaf((float) (u >> 24), by, off) };
+    } else {
+        a = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(v, by, false);
+        b = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(v, by, true);
+    }
+    return (u32x2) { __builtin_bit_cast(uint32_t, a), __builtin_bit_cast(uint32_t, b) };
+}
 
 // ---------------------------------------------------------------------------
 // attention
@@ -115,12 +139,18 @@ template <typename T, int D, bool KEYS> struct tile {
 // A: the type of q and out. T: of the keys and values. D: head_dim, padded. A
 // wave has NT tiles of 16 rows. KEYS: the waves take the item's tiles in turn,
 // all for the same rows, and their results are joined in LDS; else each wave
-// has rows of its own and all share a tile. PAGED: keys are found by page.
-template <typename A, typename T, int D, int NT, bool KEYS, bool PAGED>
+// has rows of its own and all share a tile. PAGED: keys are found by page. C: what a
+// cache of 8 bits holds, T what its values are turned into on their way to LDS or to the
+// products: bf16, which holds a code times its scale exactly. Queries and weights are then
+// sums of bf16 values, one for rows of bf16, two for f16 (16 bits), three for f32 (24).
+template <typename A, typename T, int D, int NT, bool KEYS, bool PAGED, typename C = T>
 struct attention {
     typedef tile<T, D, KEYS> L;
     static constexpr bool WIDE = L::WIDE;
-    static constexpr bool SPLIT = !WIDE && sizeof(A) == 4;       // f32 rows against f16 keys
+    static constexpr bool HELD8 = !is_same<C, T>::value;
+    static constexpr bool SPLIT = !HELD8 && !WIDE && sizeof(A) == 4;       // f32 rows against f16 keys
+    static constexpr int PIECES = !HELD8 ? 1 : sizeof(A) == 4 ? 3 : is_f16<A>::value ? 2 : 1;
+    static constexpr int MORE = PIECES - 1 + SPLIT;              // values beside the first that a query or weight is the sum of
     static constexpr int KT = L::KT;
     static constexpr int KS = KT / 16;                           // 16-key subtiles
     static constexpr int DT = D / 16;
@@ -134,6 +164,9 @@ struct attention {
     static constexpr uint32_t PAST = 0xfffffff0u;                // a place past any end
     static constexpr int DA = WIDE ? 4 : 2;                      // 16-byte pieces of 16 dimensions
     static constexpr int VM = 2 * COPIES;                        // a wave's copies for a tile (not KEYS)
+    // 8 bits: 16-byte pieces of codes. A lane's of a row of keys (KEYS), lanes a row of
+    // values (not KEYS: of either), and instructions of a group's
+    static constexpr int KL = D / 64, LPR = D / 16, CL = GROUP * LPR > 64 ? GROUP * LPR / 64 : 1;
 
     const att_args &a;
     const att_item it;
@@ -150,20 +183,50 @@ struct attention {
     // KEYS: keys are read as the products take them, and values are swapped when they
     // are written to LDS, at vput.
     uint32_t kcopy[KEYS ? QC : COPIES], vcopy[COPIES], vput[KEYS ? COPIES : 1];
+    // 8 bits: kcopy and vcopy are places of codes, krow and vrow of their scales; where a
+    // row's two pieces of T go in LDS
+    uint32_t krow, vrow[HELD8 ? CL : 1], kput2[2], vput2[HELD8 ? CL : 1][2];
+
+    // the first of the eight dimensions that a lane's step q of the products takes (any
+    // order does if queries and keys have the same)
+    __device__ __forceinline__ uint32_t dim(int q) const {
+        return HELD8 && KEYS ? 64u * (q >> 1) + 16u * g + 8u * (q & 1) : 8u * (4u * q + g);
+    }
+
+    __device__ __forceinline__ void places8() {
+        const uint32_t ch = lane % LPR;
+        krow = KEYS ? li : lane / LPR < (uint32_t) GROUP ? lane / LPR : PAST;
+#pragma unroll
+        for (int j = 0; j < KL && KEYS; ++j) kcopy[j] = (4u * j + g) * 16u < a.hd ? li * a.hd + (4u * j + g) * 16u : PAST;
+        if (!KEYS) kcopy[0] = ch * 16u < a.hd && krow != PAST ? krow * a.hd + ch * 16u : PAST;
+#pragma unroll
+        for (int j = 0; j < CL; ++j) {
+            const uint32_t rg = (uint32_t) j * (64 / LPR) + lane / LPR;
+            vrow[j] = rg < (uint32_t) GROUP ? rg : PAST;
+            vcopy[j] = ch * 16u < a.hd && vrow[j] != PAST ? rg * a.hd + ch * 16u : PAST;
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                const uint32_t rt = KEYS ? rg : wave * (uint32_t) GROUP + rg;
+                vput2[j][e] = L::VALUES + rt * L::ROWB + ((2u * ch + e) ^ L::vsw(rt)) * 16u;
+                if (!KEYS) kput2[e] = rt * L::ROWB + ((2u * ch + e) ^ L::ksw(rt)) * 16u;
+            }
+        }
+    }
 
     __device__ __forceinline__ void places() {
+        if constexpr (HELD8) places8();
         const uint32_t row = a.hd * (uint32_t) sizeof(T);
         const uint32_t rowk = PAGED ? row : (uint32_t) a.k_tok, rowv = PAGED ? row : (uint32_t) a.v_tok;
 #pragma unroll
         for (int q = 0; q < QC; ++q) {
             if (!KEYS) koff[q] = li * L::ROWB + (((4u * q + g) ^ L::ksw(li)) * 16u);
-            else kcopy[q] = (4u * q + g) * 16u < row ? li * rowk + (4u * q + g) * 16u : PAST;
+            else if (!HELD8) kcopy[q] = (4u * q + g) * 16u < row ? li * rowk + (4u * q + g) * 16u : PAST;
         }
         const uint32_t r = WIDE ? 4u * g : 4u * g + (li >> 2);
         voff = L::VALUES + r * L::ROWB + (WIDE ? ((li >> 2) ^ L::vsw(r)) * 16u + (li & 3u) * 4u
                                              : (((li >> 1) & 1u) ^ L::vsw(r)) * 16u + (li & 1u) * 8u);
 #pragma unroll
-        for (int j = 0; j < COPIES; ++j) {
+        for (int j = 0; j < COPIES && !HELD8; ++j) {
             const uint32_t rg = (uint32_t) j * RPI + lane / L::CH, ch = lane % L::CH;
             if constexpr (KEYS) {                                // (16 rows further on: the same swap)
                 vcopy[j] = ch * 16u < row ? rg * rowv + ch * 16u : PAST;
@@ -183,7 +246,7 @@ struct attention {
     float m[NT], l[NT];             // c times the running maximum (- UP), and the lane's share of the sum
     f32x4 o[DT][NT];
     // a lane's pieces of q: 8 values (SPLIT: and what rounding left of them), or 4 f32
-    t8 qf[WIDE ? 1 : NT][WIDE ? 1 : QC], ql[SPLIT ? NT : 1][SPLIT ? QC : 1];
+    t8 qf[WIDE ? 1 : NT][WIDE ? 1 : QC], ql[MORE ? NT : 1][MORE ? QC : 1], qm[MORE > 1 ? NT : 1][MORE > 1 ? QC : 1];
     f32x4 qw[WIDE ? NT : 1][WIDE ? QC : 1];
     int lim_min;                    // of the wave's rows
 
@@ -204,6 +267,21 @@ struct attention {
         return min((int) it.key1, it.vis0 + (int) t);
     }
 
+    // x as a sum of PIECES bf16 values: cut off, so that none is over x where x is near f32's
+    // end, and what is left rounded to the last
+    __device__ __forceinline__ static void pieces(float x, T (&p)[3]) {
+        const float hi = __uint_as_float(__float_as_uint(x) & 0xffff0000u);
+        p[0] = (T) hi;
+        x -= hi;
+        if constexpr (PIECES > 2) {
+            const float mid = __uint_as_float(__float_as_uint(x) & 0xffff0000u);
+            p[1] = (T) mid;
+            p[2] = (T) (x - mid);
+        } else {
+            p[1] = (T) x;
+        }
+    }
+
     __device__ __forceinline__ void load_q() {
         const uint32_t first = KEYS ? 0u : wave * (16u * NT);
         lim_min = limit(place_of(min(first, it.n_rows - 1u)).t);
@@ -220,10 +298,37 @@ struct attention {
                     const uint32_t d = 4u * (4u * s + g);
                     qw[nt][s] = d < a.hd ? *G_CAST(const f32x4, src + d * 4u) : (f32x4) { 0, 0, 0, 0 };
                 }
+            } else if constexpr (PIECES > 1) {
+#pragma unroll
+                for (int s = 0; s < QC; ++s) {
+                    const uint32_t d = dim(s);
+                    float x[8];
+                    if constexpr (sizeof(A) == 4) {
+#pragma unroll
+                        for (int i = 0; i < 2; ++i) {
+                            const f32x4 v = d < a.hd ? *G_CAST(const f32x4, src + d * 4u + 16u * i) : (f32x4) { 0, 0, 0, 0 };
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) x[4 * i + e] = v[e];
+                        }
+                    } else {
+                        const u32x4 v = d < a.hd ? *G_CAST(const u32x4, src + d * 2u) : (u32x4) { 0, 0, 0, 0 };
+                        const typename vec8<A>::type y = __builtin_bit_cast(typename vec8<A>::type, v);
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) x[e] = (float) y[e];
+                    }
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) {
+                        T p[3];
+                        pieces(x[e], p);
+                        qf[nt][s][e] = p[0];
+                        ql[nt][s][e] = p[1];
+                        if constexpr (PIECES > 2) qm[nt][s][e] = p[2];
+                    }
+                }
             } else if constexpr (!SPLIT) {
 #pragma unroll
                 for (int s = 0; s < QC; ++s) {
-                    const uint32_t d = 8u * (4u * s + g);
+                    const uint32_t d = dim(s);
                     const u32x4 v = d < a.hd ? *G_CAST(const u32x4, src + d * 2u) : (u32x4) { 0, 0, 0, 0 };
                     qf[nt][s] = __builtin_bit_cast(t8, v);
                 }
@@ -284,15 +389,21 @@ struct attention {
 
     // Where GROUP rows of keys and of values are, from `key` on (of which the rows below
     // the range's end are read).
-    struct span { const uint8_t *k, *v; };
+    // (8 bits: off is where a block's codes and scales are, and `slot` the first row.)
+    struct span { const uint8_t *k, *v; uint32_t slot; };
     __device__ __forceinline__ span rows_at(uint32_t key) const {
-        if constexpr (PAGED) {
+        if constexpr (HELD8) {
+            const uint32_t at = min(key, it.key1 - 1u);
+            const uint32_t page = *C_CAST(uint32_t, a.tables + it.kv + (at >> a.page_shift));
+            const uint64_t off = page * a.page_bytes + (uint64_t) it.head * a.block_bytes;
+            return { a.k + off, a.v + off, at & ((1u << a.page_shift) - 1u) & ~(uint32_t) (GROUP - 1) };
+        } else if constexpr (PAGED) {
             const uint32_t at = min(key, it.key1 - 1u);
             const uint32_t page = *C_CAST(uint32_t, a.tables + it.kv + (at >> a.page_shift));
             const uint64_t off = page * a.page_bytes + ((uint64_t) (it.head << a.page_shift) + (at & ((1u << a.page_shift) - 1u) & ~(uint32_t) (GROUP - 1))) * (a.hd * (uint32_t) sizeof(T));
-            return { a.k + off, a.v + off };
+            return { a.k + off, a.v + off, 0 };
         } else {
-            return { a.k + (uint64_t) (it.kv + key) * a.k_tok + it.head * a.k_head, a.v + (uint64_t) (it.kv + key) * a.v_tok + it.head * a.v_head };
+            return { a.k + (uint64_t) (it.kv + key) * a.k_tok + it.head * a.k_head, a.v + (uint64_t) (it.kv + key) * a.v_tok + it.head * a.v_head, 0 };
         }
     }
 
@@ -313,6 +424,67 @@ struct attention {
     // rows of a group of tile row r0 that are below the range's end, and whether a tile's all are
     __device__ __forceinline__ uint32_t rows_in(uint32_t key) const { return key < it.key1 ? min(it.key1 - key, (uint32_t) GROUP) : 0u; }
     __device__ __forceinline__ bool is_whole(uint32_t t) const { return (t + 1u) * KT <= it.key1 && a.hd == D; }
+
+    // 8 bits: a group's codes and scales on their way in registers (by a buffer's bounds, what
+    // is past the end or past head_dim is zero)
+    struct codes {
+        u32x4 k[KEYS ? KL : 1], v[CL];
+        uint32_t ks, vs[CL];
+    };
+    // a sequence's own keys are read once and not kept (2: nontemporal): 64.9 -> 60.6 us
+    // for 8 sequences of 16384 positions, bf16; a prompt's are read by many workgroups
+    static constexpr int KEPT = PAGED ? 2 : 0;
+    __device__ __forceinline__ void fetch8(codes &x, const span &m, uint32_t key) const {
+        const uint32_t n = rows_in(key);
+        const uint8_t *k = m.k + m.slot * a.hd, *v = m.v + m.slot * a.hd;
+        const uint32_t scales = (a.hd << a.page_shift) + m.slot;
+        const __amdgpu_buffer_rsrc_t rk = __builtin_amdgcn_make_buffer_rsrc((void *) k, (short) 0, (int) uniform(n * a.hd), 0x00020000);
+        const __amdgpu_buffer_rsrc_t rv = __builtin_amdgcn_make_buffer_rsrc((void *) v, (short) 0, (int) uniform(n * a.hd), 0x00020000);
+        const __amdgpu_buffer_rsrc_t sk = __builtin_amdgcn_make_buffer_rsrc((void *) (m.k + scales), (short) 0, (int) uniform(n), 0x00020000);
+        const __amdgpu_buffer_rsrc_t sv = __builtin_amdgcn_make_buffer_rsrc((void *) (m.v + scales), (short) 0, (int) uniform(n), 0x00020000);
+        constexpr int KEEP = KEYS ? KEPT : 0;
+#pragma unroll
+        for (int j = 0; j < (KEYS ? KL : 1); ++j) x.k[j] = __builtin_amdgcn_raw_buffer_load_b128(rk, kcopy[j], 0, KEEP);
+        x.ks = __builtin_amdgcn_raw_buffer_load_b8(sk, krow, 0, KEEP);
+#pragma unroll
+        for (int j = 0; j < CL; ++j) {
+            x.v[j] = __builtin_amdgcn_raw_buffer_load_b128(rv, vcopy[j], 0, KEEP);
+            x.vs[j] = __builtin_amdgcn_raw_buffer_load_b8(sv, vrow[j], 0, KEEP);
+        }
+    }
+    // sixteen codes as two pieces of T
+    struct two { u32x4 p[2]; };
+    __device__ __forceinline__ static two widen(const u32x4 &v, uint32_t scale) {
+        const float by = scale_value(scale);
+        two y;
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+            const u32x2 lo = values_of_codes<C>(v[2 * e], by), hi = values_of_codes<C>(v[2 * e + 1], by);
+            y.p[e] = (u32x4) { lo[0], lo[1], hi[0], hi[1] };
+        }
+        return y;
+    }
+    // a group's values (KEYS) or keys and values into LDS, at `to` more than their places
+    __device__ __forceinline__ void land(const codes &x, uint32_t to) const {
+        if (!KEYS && krow != PAST) {
+            const two y = widen(x.k[0], x.ks);
+#pragma unroll
+            for (int e = 0; e < 2; ++e) *reinterpret_cast<u32x4 *>(S + to + kput2[e]) = y.p[e];
+        }
+#pragma unroll
+        for (int j = 0; j < CL; ++j) {
+            if (vrow[j] == PAST) continue;
+            const two y = widen(x.v[j], x.vs[j]);
+#pragma unroll
+            for (int e = 0; e < 2; ++e) *reinterpret_cast<u32x4 *>(S + to + vput2[j][e]) = y.p[e];
+        }
+    }
+    codes c8[HELD8 && KEYS ? GROUPS : 1];
+    // not KEYS, 8 bits: this wave's rows of a tile set off
+    __device__ __forceinline__ void issue8(uint32_t t) {
+        const uint32_t key = t * KT + wave * (uint32_t) GROUP;
+        fetch8(c8[0], rows_at(key), key);
+    }
 
     // not KEYS: this wave's rows of a tile into the stage at `to`
     __device__ __forceinline__ void issue(uint32_t t, uint32_t to) const {
@@ -344,9 +516,6 @@ struct attention {
             k[gr] = __builtin_amdgcn_make_buffer_rsrc((void *) at.m[gr].k, (short) 0, (int) uniform(n ? n * rowk - (rowk - row) : 0u), 0x00020000);
             v[gr] = __builtin_amdgcn_make_buffer_rsrc((void *) at.m[gr].v, (short) 0, (int) uniform(n ? n * rowv - (rowv - row) : 0u), 0x00020000);
         }
-        // a sequence's own keys are read once and not kept (2: nontemporal): 64.9 -> 60.6 us
-        // for 8 sequences of 16384 positions, bf16; a prompt's are read by many workgroups
-        constexpr int KEPT = PAGED ? 2 : 0;
 #pragma unroll
         for (int gr = 0; gr < GROUPS; ++gr) {
 #pragma unroll
@@ -380,6 +549,14 @@ struct attention {
             const t8 kf = __builtin_bit_cast(t8, piece);
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt) s[nt] = mfma(kf, qf[nt][q], s[nt]);
+            if constexpr (PIECES > 1) {
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt) s[nt] = mfma(kf, ql[nt][q], s[nt]);
+            }
+            if constexpr (PIECES > 2) {
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt) s[nt] = mfma(kf, qm[nt][q], s[nt]);
+            }
             if constexpr (SPLIT) {
                 t8 kr = kf;
                 if constexpr (CAREFUL) {
@@ -412,7 +589,7 @@ struct attention {
     // of p as it was rounded, so that weights still add up to 1: values that are all alike
     // come back as they are (they were 0.4 % off where bf16 rounded all weights one way).
     struct probs {
-        t8 p[WIDE ? 1 : NT], rest[SPLIT ? NT : 1];
+        t8 p[WIDE ? 1 : NT], rest[MORE ? NT : 1], last[MORE > 1 ? NT : 1];
         f32x4 w[WIDE ? NT : 1];
     };
 
@@ -461,16 +638,22 @@ struct attention {
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
                     const float x = __builtin_amdgcn_exp2f(fmaf(s[ks][nt][i], c[nt], -m[nt]));
-                    if constexpr (WIDE) sum += x;
+                    if constexpr (WIDE || PIECES > 1) sum += x;
                     if constexpr (WIDE) {
                         p.w[nt][i] = x;
+                    } else if constexpr (PIECES > 1) {           // (16 or more bits of x: as good as x in the sum)
+                        T y[3];
+                        pieces(x, y);
+                        p.p[nt][4 * ks + i] = y[0];
+                        p.rest[nt][4 * ks + i] = y[1];
+                        if constexpr (PIECES > 2) p.last[nt][4 * ks + i] = y[2];
                     } else {
                         p.p[nt][4 * ks + i] = (T) x;
                         if constexpr (SPLIT) p.rest[nt][4 * ks + i] = (T) (x - (float) p.p[nt][4 * ks + i]);
                     }
                 }
             }
-            if constexpr (!WIDE) {
+            if constexpr (!WIDE && PIECES == 1) {
 #pragma unroll
                 for (int e = 0; e < 8; e += 2) {
                     sum = add_two(p.p[nt][e], p.p[nt][e + 1], sum);
@@ -535,7 +718,8 @@ struct attention {
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt) {
                     o[dt][nt] = mfma(vf, p.p[nt], o[dt][nt]);
-                    if constexpr (SPLIT) o[dt][nt] = mfma(vf, p.rest[nt], o[dt][nt]);
+                    if constexpr (MORE > 0) o[dt][nt] = mfma(vf, p.rest[nt], o[dt][nt]);
+                    if constexpr (MORE > 1) o[dt][nt] = mfma(vf, p.last[nt], o[dt][nt]);
                 }
             }
         }
@@ -576,11 +760,22 @@ struct attention {
     __device__ __forceinline__ void start() {
         if (it.key0 >= it.key1) return;
         const uint32_t t = first_tile();
-        if constexpr (KEYS) {
+        if constexpr (HELD8) {
+            set_off(t);
+        } else if constexpr (KEYS) {
             fetch(x, spans(t), t);
         } else {
             issue(t, stage(0));
             issue(t + 1, stage(1));
+        }
+    }
+    // 8 bits: tile t's codes, into registers
+    __device__ __forceinline__ void set_off(uint32_t t) {
+        if constexpr (KEYS) {
+#pragma unroll
+            for (int gr = 0; gr < GROUPS; ++gr) fetch8(c8[gr], rows_at(t * KT + (uint32_t) gr * GROUP), t * KT + (uint32_t) gr * GROUP);
+        } else {
+            issue8(t);
         }
     }
 
@@ -589,9 +784,30 @@ struct attention {
     template <bool CAREFUL>
     __device__ __forceinline__ void turn(uint32_t t) {
         const uint32_t then = t + STEP;
-        const span_of_tile m = spans(then);                      // (past the end: the last page again)
         scores s;
         clear(s);
+        if constexpr (HELD8) {
+            span m[GROUPS];
+#pragma unroll
+            for (int gr = 0; gr < GROUPS; ++gr) m[gr] = rows_at(then * KT + (uint32_t) gr * GROUP);
+#pragma unroll
+            for (int ks = 0; ks < KS; ++ks) {
+#pragma unroll
+                for (int j = 0; j < KL; ++j) {
+                    const two k = widen(c8[ks].k[j], c8[ks].ks);
+                    score<CAREFUL>(s[ks], k.p[0], 2 * j);
+                    score<CAREFUL>(s[ks], k.p[1], 2 * j + 1);
+                }
+            }
+#pragma unroll
+            for (int gr = 0; gr < GROUPS; ++gr) land(c8[gr], stage(0) + gr * GROUP * L::ROWB);
+            __builtin_amdgcn_sched_barrier(0);
+            if (then * KT < it.key1) {
+#pragma unroll
+                for (int gr = 0; gr < GROUPS; ++gr) fetch8(c8[gr], m[gr], then * KT + (uint32_t) gr * GROUP);
+            }
+        } else {
+        const span_of_tile m = spans(then);                      // (past the end: the last page again)
 #pragma unroll
         for (int ks = 0; ks < KS; ++ks) {
 #pragma unroll
@@ -604,6 +820,7 @@ struct attention {
         }
         __builtin_amdgcn_sched_barrier(0);
         if (then * KT < it.key1) fetch(x, m, then);
+        }
         mask(s, t * KT);
         probs p;
         float f[NT];
@@ -675,6 +892,8 @@ struct attention {
         uint32_t t = first_tile();
         if constexpr (KEYS) {
             for (; t < t1; t += STEP) turn<false>(t);
+        } else if constexpr (HELD8) {
+            pass8(t, t1);
         } else {
             scores s, next;
             probs p;
@@ -719,6 +938,56 @@ struct attention {
         }
     }
 
+    // 8 bits: the same steps, but a tile comes into registers and is put into LDS an
+    // iteration later, as T.
+    __device__ __forceinline__ void meet8() const {
+        __builtin_amdgcn_s_waitcnt(0xC07F);
+        __builtin_amdgcn_s_barrier();
+        __builtin_amdgcn_sched_barrier(0);
+    }
+    __device__ __forceinline__ void pass8(const uint32_t t, const uint32_t t1) {
+        scores s, next;
+        probs p;
+        float f[NT];
+#pragma unroll
+        for (uint32_t i = 0; i < 3; ++i) {                       // (a tile past the end is zeros)
+            land(c8[0], stage(i));
+            issue8(t + i + 1);
+        }
+        meet8();
+        scores_of<false>(s, stage(0));
+        scores_of<false>(next, stage(1));
+        mask(s, t * KT);
+        bool moved = adjust(s, f);
+        soften(s, p);
+        uint32_t n = 1;                                          // tile t + n's scores are `next`
+        for (; t + n < t1; ++n) {
+            if (moved) rescale(f);
+            meet8();
+            values v;
+            values_of(v, stage((n - 1) & 3u));
+            land(c8[0], stage((n + 2) & 3u));
+            issue8(t + n + 3);
+#pragma unroll
+            for (int ks = 0; ks < KS; ++ks) {
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt) s[ks][nt] = next[ks][nt];
+            }
+            mask(s, (t + n) * KT);
+            moved = adjust(s, f);
+            __builtin_amdgcn_sched_barrier(0);
+            probs q;
+            scores_of<false>(next, stage((n + 1) & 3u));
+            products<false>(v, p, (t + n - 1) * KT, stage((n - 1) & 3u));
+            soften(s, q);
+            p = q;
+        }
+        if (moved) rescale(f);
+        values v;
+        values_of(v, stage((n - 1) & 3u));
+        products<false>(v, p, (t + n - 1) * KT, stage((n - 1) & 3u));
+    }
+
     // The same with care, a tile after the other.
     __device__ __forceinline__ void careful_pass() {
         begin();
@@ -726,10 +995,16 @@ struct attention {
         const uint32_t t1 = (it.key1 + KT - 1u) / KT;
         for (uint32_t t = first_tile(); t < t1; t += STEP) {
             if constexpr (KEYS) {
-                fetch(x, spans(t), t);
+                if constexpr (HELD8) set_off(t);
+                else fetch(x, spans(t), t);
                 turn<true>(t);
             } else {
-                issue(t, stage(0));
+                if constexpr (HELD8) {
+                    set_off(t);
+                    land(c8[0], stage(0));
+                } else {
+                    issue(t, stage(0));
+                }
                 meet<0>();
                 scores s;
                 probs p;
@@ -880,10 +1155,10 @@ struct attention {
     }
 };
 
-template <typename A, typename T, int D, int NT, bool KEYS, bool PAGED>
+template <typename A, typename T, int D, int NT, bool KEYS, bool PAGED, typename C = T>
 __device__ __forceinline__ void attend_item(const att_args &a, const att_item &it, uint8_t *S) {
     const uint32_t lane = threadIdx.x & 63u;
-    attention<A, T, D, NT, KEYS, PAGED> x = { a, it, S, lane, uniform(threadIdx.x >> 6), lane >> 4, lane & 15u };
+    attention<A, T, D, NT, KEYS, PAGED, C> x = { a, it, S, lane, uniform(threadIdx.x >> 6), lane >> 4, lane & 15u };
     x.run();
 }
 
@@ -941,11 +1216,31 @@ __device__ __forceinline__ void paged_body(const att_args &a) {
     else attend_item<A, T, D, 2, false, true>(a, it, S);
 }
 
+// The same over 8 bits. (Queries of f32 take three times the registers: no 32 rows a wave.)
+template <typename A, typename C, int D>
+__device__ __forceinline__ void held8_body(const att_args &a) {
+    __shared__ __attribute__((aligned(1024))) uint8_t S[LDS_BYTES<__bf16, D>];
+    const att_item it = item_of(a);
+    if (it.mode == ATT_FEW) attend_item<A, __bf16, D, 1, true, true, C>(a, it, S);
+    else if (sizeof(A) == 4 || it.mode == ATT_HALF) attend_item<A, __bf16, D, 1, false, true, C>(a, it, S);
+    else if constexpr (sizeof(A) == 2) attend_item<A, __bf16, D, 2, false, true, C>(a, it, S);
+}
+
 }  // namespace
 
 #define PROMPT(name, T, D) extern "C" __global__ void __launch_bounds__(ATT_THREADS, 2) name(const att_args a) { prompt_body<T, D>(a); }
 #define PAGED(name, A, T, D) extern "C" __global__ void __launch_bounds__(ATT_THREADS, 2) name(const att_args a) { paged_body<A, T, D>(a); }
 
+#define HELD8(name, A, C)                                                                                                                                   \
+    extern "C" __global__ void __launch_bounds__(ATT_THREADS, 2) sllm_k_attend_##name##_64(const att_args a) { held8_body<A, C, 64>(a); }        \
+    extern "C" __global__ void __launch_bounds__(ATT_THREADS, 2) sllm_k_attend_##name##_128(const att_args a) { held8_body<A, C, 128>(a); }
+
+HELD8(f32i8, float, int8_codes)
+HELD8(f16i8, _Float16, int8_codes)
+HELD8(bf16i8, __bf16, int8_codes)
+HELD8(f32e4m3, float, e4m3_codes)
+HELD8(f16e4m3, _Float16, e4m3_codes)
+HELD8(bf16e4m3, __bf16, e4m3_codes)
 PAGED(sllm_k_attend_f32_64, float, float, 64)
 PAGED(sllm_k_attend_f32_128, float, float, 128)
 PAGED(sllm_k_attend_f32f16_64, float, _Float16, 64)
@@ -1089,13 +1384,16 @@ STORE(sllm_k_attn_store_f32, float, float)
 STORE(sllm_k_attn_store_f32f16, float, _Float16)
 STORE(sllm_k_attn_store_16, _Float16, _Float16)
 
+namespace {
+
 // Pages to pages: blockIdx.y a pair of them, ATT_COPY_CHUNKS 16-byte pieces of
 // what it holds a workgroup, all four of a thread's in flight together. Bound by
 // memory: 396 pages of 655 KB moved or copied in two launches 92 us, 5.5 TB/s; 16 copies
 // of 41 positions of 30 layers, a source that the caches hold, 15.2 us, 3.5 TB/s.
-extern "C" __global__ void __launch_bounds__(ATT_THREADS) sllm_k_attn_copy(const att_copy_args a) {
+// SCALES: of each block also the scale bytes of those rows, the last of them one by one.
+template <bool SCALES> __device__ __forceinline__ void copy_body(const att_copy_args &a) {
     const att_pair p = a.pair[blockIdx.y];
-    const uint32_t per = p.rows * a.row_bytes / 16u, n = per * a.n_blocks;
+    const uint32_t codes = p.rows * a.row_bytes / 16u, per = codes + (SCALES ? (p.rows + 15u) / 16u : 0u), n = per * a.n_blocks;
     const uint8_t *src = a.mem + p.src * a.page_bytes;
     uint8_t *dst = a.mem + p.dst * a.page_bytes;
     constexpr int UN = ATT_COPY_CHUNKS / ATT_THREADS;
@@ -1104,12 +1402,315 @@ extern "C" __global__ void __launch_bounds__(ATT_THREADS) sllm_k_attn_copy(const
 #pragma unroll
     for (int i = 0; i < UN; ++i) {
         const uint32_t x = blockIdx.x * ATT_COPY_CHUNKS + (uint32_t) i * ATT_THREADS + threadIdx.x;
-        at[i] = (uint64_t) (x / per) * a.block_bytes + (x % per) * 16u;
+        const uint32_t y = x % per;
+        at[i] = (uint64_t) (x / per) * a.block_bytes + (!SCALES || y < codes ? y * 16u : a.scales + (y - codes) * 16u);
         if (x < n) v[i] = *G_CAST(const u32x4, src + at[i]);
     }
 #pragma unroll
     for (int i = 0; i < UN; ++i) {
         const uint32_t x = blockIdx.x * ATT_COPY_CHUNKS + (uint32_t) i * ATT_THREADS + threadIdx.x;
-        if (x < n) *G_CAST(u32x4, dst + at[i]) = v[i];
+        if (x >= n) return;
+        if constexpr (SCALES) {
+            const uint32_t y = x % per, left = y < codes ? 16u : p.rows - (y - codes) * 16u;
+            if (left < 16u) {
+#pragma unroll
+                for (uint32_t j = 0; j < 15u; ++j) if (j < left) G_CAST(uint8_t, dst + at[i])[j] = (uint8_t) (v[i][j >> 2] >> (8u * (j & 3u)));
+                continue;
+            }
+        }
+        *G_CAST(u32x4, dst + at[i]) = v[i];
     }
 }
+
+}  // namespace
+
+extern "C" __global__ void __launch_bounds__(ATT_THREADS) sllm_k_attn_copy(const att_copy_args a) { copy_body<false>(a); }
+extern "C" __global__ void __launch_bounds__(ATT_THREADS) sllm_k_attn_copy8(const att_copy_args a) { copy_body<true>(a); }
+
+// ---------------------------------------------------------------------------
+// rows on their way: rotary positions, a cache of 8 bits
+// ---------------------------------------------------------------------------
+
+namespace {
+
+// cos and sin of p / 2^32 turns: the quarter turn that p is nearest to, and the two series
+// on what is left, |x| <= pi / 4 (the first terms left out are x^13 / 13! and x^12 / 12!,
+// under 2^-32). p is exact to 2 of 2^-32 turns however far the position.
+__device__ __forceinline__ void cos_sin(uint32_t p, float &c, float &s) {
+    const uint32_t quarter = (p + 0x20000000u) >> 30;
+    const float x = (float) (int32_t) (p - (quarter << 30)) * 1.46291807926715968e-9f, x2 = x * x;      // 2 pi / 2^32
+    float a = fmaf(x2, -2.50521083854417188e-8f, 2.75573192239858907e-6f);
+    a = fmaf(x2, a, -1.98412698412698413e-4f);
+    a = fmaf(x2, a, 8.33333333333333333e-3f);
+    a = fmaf(x2, a, -1.66666666666666667e-1f);
+    a = fmaf(x2 * x, a, x);
+    float b = fmaf(x2, -2.75573192239858907e-7f, 2.48015873015873016e-5f);
+    b = fmaf(x2, b, -1.38888888888888889e-3f);
+    b = fmaf(x2, b, 4.16666666666666667e-2f);
+    b = fmaf(x2, b, -0.5f);
+    b = fmaf(x2, b, 1.0f);
+    c = quarter & 1u ? a : b;
+    s = quarter & 1u ? b : a;
+    c = quarter == 1u || quarter == 2u ? -c : c;
+    s = quarter >= 2u ? -s : s;
+}
+
+// eight values in two halves of four, at d0 and d1
+template <typename A> struct eight {
+    f32x4 x[2];
+    __device__ __forceinline__ static f32x4 wide(u32x2 v) {
+        const typename vec4<A>::type y = __builtin_bit_cast(typename vec4<A>::type, v);
+        return (f32x4) { (float) y[0], (float) y[1], (float) y[2], (float) y[3] };
+    }
+    __device__ __forceinline__ void load(const uint8_t *row, uint32_t d0, uint32_t d1, bool whole) {
+        if constexpr (sizeof(A) == 4) {
+            x[0] = *G_CAST(const f32x4, row + d0 * 4u);
+            x[1] = *G_CAST(const f32x4, row + d1 * 4u);
+        } else if (whole) {
+            const u32x4 v = *G_CAST(const u32x4, row + d0 * 2u);
+            x[0] = wide((u32x2) { v[0], v[1] });
+            x[1] = wide((u32x2) { v[2], v[3] });
+        } else {
+            x[0] = wide(*G_CAST(const u32x2, row + d0 * 2u));
+            x[1] = wide(*G_CAST(const u32x2, row + d1 * 2u));
+        }
+    }
+    __device__ __forceinline__ void store(uint8_t *row, uint32_t d0, uint32_t d1, bool whole) const {
+        if constexpr (sizeof(A) == 4) {
+            *G_CAST(f32x4, row + d0 * 4u) = x[0];
+            *G_CAST(f32x4, row + d1 * 4u) = x[1];
+        } else {
+            u32x2 y[2];
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                typename vec4<A>::type h;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) h[e] = (A) x[i][e];
+                y[i] = __builtin_bit_cast(u32x2, h);
+            }
+            if (whole) {
+                *G_CAST(u32x4, row + d0 * 2u) = (u32x4) { y[0][0], y[0][1], y[1][0], y[1][1] };
+            } else {
+                *G_CAST(u32x2, row + d0 * 2u) = y[0];
+                *G_CAST(u32x2, row + d1 * 2u) = y[1];
+            }
+        }
+    }
+};
+
+template <int CTRL> __device__ __forceinline__ uint32_t dpp(uint32_t x) {
+    return (uint32_t) __builtin_amdgcn_update_dpp(0, (int) x, CTRL, 0xf, 0xf, true);
+}
+
+// A row's largest magnitude, as bits, over the 8 or 16 lanes that hold it (infinities and
+// NaN are larger than all others).
+__device__ __forceinline__ uint32_t top_of(const f32x4 (&x)[2], bool in, bool wide) {
+    uint32_t m = 0;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) m = max(m, __float_as_uint(x[i][e]) & 0x7fffffffu);
+    }
+    m = in ? m : 0u;
+    m = max(m, dpp<0xb1>(m));                                    // lane ^ 1
+    m = max(m, dpp<0x4e>(m));                                    // lane ^ 2
+    m = max(m, dpp<0x141>(m));                                   // 7 - lane, of eight
+    return wide ? max(m, dpp<0x128>(m)) : m;                     // 8 further, of sixteen
+}
+
+// The scale byte of a row of that largest magnitude: the smallest 2^e, e >= -126 (e4m3:
+// -117), with top <= 127 2^e (448 2^e), whose values are all normal f32 and bf16. Up to 127 2^120.
+__device__ __forceinline__ uint32_t scale_of(uint32_t top, bool i8) {
+    if (top > 0x7efe0000u) return ATT_NAN_ROW;
+    const int e = (int) (top >> 23), m = (int) (top & 0x7fffffu);
+    return (uint32_t) (i8 ? max(e - 6 + (m > 0x7e0000), 1) : max(e - 8 + (m > 0x600000), 10));
+}
+// four of a row's codes, each rounded once to the nearest, ties to even (a product with a
+// power of two is exact, or so small that its code is 0)
+__device__ __forceinline__ uint32_t codes_of(f32x4 x, uint32_t scale, bool i8) {
+    if (scale == ATT_NAN_ROW) return i8 ? 0u : 0x7f7f7f7fu;
+    const float by = __uint_as_float((254u - scale) << 23);
+    if (i8) {
+        uint32_t y = 0;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) y |= ((uint32_t) (int) __builtin_rintf(x[e] * by) & 255u) << (8 * e);
+        return y;
+    }
+    int y = __builtin_amdgcn_cvt_pk_fp8_f32(x[0] * by, x[1] * by, 0, false);
+    return (uint32_t) __builtin_amdgcn_cvt_pk_fp8_f32(x[2] * by, x[3] * by, y, true);
+}
+
+// A wave takes the heads of one token, four rows of up to 128 values at a time (eight of up
+// to 64), eight values a lane; cos and sin of a lane's four pairs are formed once for all of
+// them. So a token's rows are read and written once, and nothing crosses lanes but a row's
+// largest magnitude.
+template <typename A>
+__device__ __forceinline__ void rows_body(const att_rows_args &a) {
+    const uint32_t lane = threadIdx.x & 63u, w = blockIdx.x * (ATT_THREADS / 64) + uniform(threadIdx.x >> 6);
+    const uint32_t tok = w / a.waves, part = w % a.waves;
+    if (tok >= a.n_tok) return;
+    const bool wide = a.hd > 64;
+    const uint32_t per = wide ? 16u : 8u, at_once = 64u / per, unit = lane & (per - 1u);
+    const bool in = unit < a.hd / 8u, turned = unit < a.half / 4u, whole = a.pairs != 0 || a.half == 0;
+    // the dimensions of the lane's values, of rows that turn
+    const uint32_t d0 = turned && !whole ? 4u * unit : 8u * unit, d1 = turned && !whole ? a.half + 4u * unit : 8u * unit + 4u;
+    const int32_t pos = a.toks ? (int32_t) a.toks[tok].pos : a.pos ? a.pos[tok] : 0;
+    float c[4] = { 1.0f, 1.0f, 1.0f, 1.0f }, s[4] = {};
+    if (turned && in) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const uint64_t f = G_CAST(const uint64_t, a.freq)[4u * unit + j];
+            cos_sin((uint32_t) ((f * (uint64_t) (int64_t) pos) >> 32), c[j], s[j]);
+            c[j] *= a.magnitude;
+            s[j] *= a.back ? -a.magnitude : a.magnitude;
+        }
+    }
+    uint64_t place = 0;                                          // the token's row of KV head 0 in the cache
+    uint32_t slot = 0;
+    if (a.ck) {
+        slot = (uint32_t) pos & ((1u << a.page_shift) - 1u);
+        place = a.tables[a.toks[tok].table + ((uint32_t) pos >> a.page_shift)] * a.page_bytes;
+    }
+    const bool held8 = a.held >= ATT_HELD_I8;
+    // (copies: a choice between two of the arguments would put them all into scratch memory)
+    const uint8_t *q = (const uint8_t *) a.q + tok * a.q_tok, *k = (const uint8_t *) a.k + tok * a.k_tok, *v = (const uint8_t *) a.v + tok * a.v_tok;
+    uint8_t *qo = (uint8_t *) a.q_out + tok * a.qo_tok, *ko = (uint8_t *) a.k_out + tok * a.ko_tok, *ck = a.ck + place, *cv = a.cv + place;
+    const uint32_t nq = a.q ? a.n_head : 0u, nk = a.k ? a.n_head_kv : 0u, nv = a.v ? a.n_head_kv : 0u, rows = nq + nk + nv;
+    for (uint32_t r = part * at_once; r < rows; r += a.waves * at_once) {
+        uint32_t h = r + lane / per;
+        const bool here = h < rows && in;
+        const bool is_q = h < nq, is_v = h >= nq + nk;
+        const uint8_t *src = is_q ? q : is_v ? v : k;
+        h -= is_q ? 0u : is_v ? nq + nk : nq;
+        // (values have the same places as keys where rows turn by halves: what is written is the row)
+        const uint32_t e0 = is_v ? 8u * unit : d0, e1 = is_v ? 8u * unit + 4u : d1;
+        eight<A> x;
+        x.x[0] = x.x[1] = (f32x4) { 0, 0, 0, 0 };
+        if (here) x.load(src + (uint64_t) h * a.hd * sizeof(A), e0, e1, whole);
+        if (turned && !is_v) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const f32x4 lo = x.x[0], hi = x.x[1], near = j < 2 ? lo : hi;
+                const float n0 = near[2 * (j & 1)], n1 = near[2 * (j & 1) + 1], f0 = lo[j], f1 = hi[j];
+                const float u = whole ? n0 : f0, v = whole ? n1 : f1;
+                const float p = fmaf(u, c[j], -(v * s[j])), q = fmaf(v, c[j], u * s[j]);
+                if (whole) {
+                    x.x[j >> 1][2 * (j & 1)] = p;
+                    x.x[j >> 1][2 * (j & 1) + 1] = q;
+                } else {
+                    x.x[0][j] = p;
+                    x.x[1][j] = q;
+                }
+            }
+        }
+        if (is_q || (!is_v && a.k_out)) {
+            uint8_t *dst = is_q ? qo : ko;
+            if (here) x.store(dst + (uint64_t) h * a.hd * sizeof(A), e0, e1, whole);
+        }
+        if (a.ck == nullptr) continue;
+        uint8_t *block = is_v ? cv : ck;
+        if (held8) {
+            const bool i8 = a.held == ATT_HELD_I8;
+            const uint32_t scale = scale_of(top_of(x.x, here, wide), i8);      // (every lane is here)
+            if (!here || is_q) continue;
+            block += (uint64_t) h * a.block_bytes;
+            uint8_t *dst = block + slot * a.hd;
+            const uint32_t y0 = codes_of(x.x[0], scale, i8), y1 = codes_of(x.x[1], scale, i8);
+            if (whole) {
+                *G_CAST(u32x2, dst + e0) = (u32x2) { y0, y1 };
+            } else {
+                *G_CAST(uint32_t, dst + e0) = y0;
+                *G_CAST(uint32_t, dst + e1) = y1;
+            }
+            if (unit == 0) *G_CAST(uint8_t, block + (a.hd << a.page_shift) + slot) = (uint8_t) scale;
+        } else if (here && !is_q) {
+            const uint64_t at = ((uint64_t) (h << a.page_shift) + slot) * a.hd;
+            if constexpr (sizeof(A) == 4) {
+                if (a.held == ATT_HELD_F16) {
+                    eight<_Float16> y;
+                    y.x[0] = x.x[0];
+                    y.x[1] = x.x[1];
+                    y.store(block + at * 2u, e0, e1, whole);
+                    continue;
+                }
+            }
+            x.store(block + at * sizeof(A), e0, e1, whole);
+        }
+    }
+}
+
+}  // namespace
+
+namespace {
+
+// A batch's positions out of their pages. A workgroup's pieces of eight values are of one page;
+// whose page it is, is searched for 64 sequences at a time.
+template <typename A>
+__device__ __forceinline__ void read_body(const att_read_args &a) {
+    const uint32_t lane = threadIdx.x & 63u, entry = blockIdx.x;
+    uint32_t lo = 0, n = a.n_seq;                                // the last of n sequences from lo on whose pages start at or before it
+    while (n > 1) {
+        const uint32_t step = (n + 63u) / 64u, at = lo + lane * step;
+        const bool before = lane * step < n && G_CAST(const att_seq, a.seqs)[at].table <= entry;
+        const uint32_t last = (uint32_t) __popcll(__ballot(before)) - 1u;
+        lo += last * step;
+        n = min(step, n - last * step);
+    }
+    lo = uniform(lo);
+    const uint32_t first = C_CAST(uint32_t, &a.seqs[lo].table)[0], row0 = C_CAST(uint32_t, &a.seqs[lo].row0)[0];
+    const uint32_t end = C_CAST(uint32_t, &a.seqs[lo + 1].row0)[0], start = row0 + ((entry - first) << a.page_shift);
+    const uint32_t page_rows = 1u << a.page_shift, n_rows = min(end - start, page_rows);
+    const uint64_t page = (uint64_t) C_CAST(uint32_t, a.tables)[entry] * a.page_bytes;
+    const uint32_t per = a.hd / 8u, per_block = n_rows * per, all = per_block * 2u * a.n_head_kv;
+    const uint32_t base = blockIdx.y * (ATT_THREADS * ATT_READ_UNITS) + threadIdx.x;
+#pragma unroll
+    for (uint32_t i = 0; i < ATT_READ_UNITS; ++i) {
+        const uint32_t x = base + i * ATT_THREADS;
+        if (x >= all) return;
+        const uint32_t b = x / per_block, y = x % per_block, row = y / per, d = 8u * (y % per);
+        const bool v = b >= a.n_head_kv;
+        const uint32_t h = v ? b - a.n_head_kv : b;
+        const uint8_t *src = (v ? a.cv : a.ck) + page;
+        uint8_t *dst = (uint8_t *) (v ? a.v : a.k) + (uint64_t) (start + row) * (v ? a.v_tok : a.k_tok) + (uint64_t) (h * a.hd + d) * sizeof(A);
+        if (a.held >= ATT_HELD_I8) {
+            src += (uint64_t) h * a.block_bytes;
+            const u32x2 codes = *G_CAST(const u32x2, src + row * a.hd + d);
+            const float by = scale_value(*G_CAST(const uint8_t, src + (a.hd << a.page_shift) + row));
+            eight<A> z;
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                const u32x2 w = a.held == ATT_HELD_I8 ? values_of_codes<int8_codes>(codes[e], by) : values_of_codes<e4m3_codes>(codes[e], by);
+                z.x[e] = (f32x4) { __uint_as_float(w[0] << 16), __uint_as_float(w[0] & 0xffff0000u), __uint_as_float(w[1] << 16), __uint_as_float(w[1] & 0xffff0000u) };
+            }
+            z.store(dst, 0, 4, true);
+        } else {
+            const uint64_t at = ((uint64_t) (h << a.page_shift) + row) * a.hd + d;
+            if constexpr (sizeof(A) == 4) {
+                if (a.held == ATT_HELD_F16) {
+                    eight<_Float16> z;
+                    z.load(src + at * 2u, 0, 4, true);
+                    eight<float> f;
+                    f.x[0] = z.x[0];
+                    f.x[1] = z.x[1];
+                    f.store(dst, 0, 4, true);
+                    continue;
+                }
+            }
+            eight<A> z;
+            z.load(src + at * sizeof(A), 0, 4, true);
+            z.store(dst, 0, 4, true);
+        }
+    }
+}
+
+}  // namespace
+
+#define ROWS(name, A) extern "C" __global__ void __launch_bounds__(ATT_THREADS) name(const att_rows_args a) { rows_body<A>(a); }
+#define READ(name, A) extern "C" __global__ void __launch_bounds__(ATT_THREADS) name(const att_read_args a) { read_body<A>(a); }
+
+ROWS(sllm_k_attn_rows_f32, float)
+ROWS(sllm_k_attn_rows_f16, _Float16)
+ROWS(sllm_k_attn_rows_bf16, __bf16)
+READ(sllm_k_attn_read_f32, float)
+READ(sllm_k_attn_read_f16, _Float16)
+READ(sllm_k_attn_read_bf16, __bf16)

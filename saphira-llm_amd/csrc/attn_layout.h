@@ -52,6 +52,7 @@ typedef struct att_args {
     uint32_t        page_shift, hd, group, n_items;
     float           c;               /* scale * log2(e) */
     float           per_group;       /* 1 / group */
+    uint32_t        block_bytes, pad;    /* 8 bits: a KV head's keys or values in a page */
 } att_args;
 
 /* the partial results of a token: those of n_split splits of a segment, whose
@@ -88,6 +89,45 @@ typedef struct att_store_args {
     uint32_t        page_shift, hd, n_head_kv, n_tok;
 } att_store_args;
 
+/* what rows are held as (att_rows_args.held, att_read_args.held) */
+enum { ATT_HELD_F32, ATT_HELD_F16, ATT_HELD_BF16, ATT_HELD_I8, ATT_HELD_E4M3 };
+/* the scale byte of a row of 8 bits: 2^(byte - 127); ATT_NAN_ROW: something in it is not finite */
+#define ATT_NAN_ROW   255u
+
+/*
+ * Rows of one type on their way: queries and keys turned by their position (or,
+ * half 0, as they are) into q_out and k_out, or keys and values into the cache.
+ * A row is n_head, n_head_kv heads of hd values; NULL: there are none of these.
+ */
+typedef struct att_rows_args {
+    const void     *q, *k, *v;
+    void           *q_out, *k_out;   /* k_out NULL: to the cache */
+    uint8_t        *ck, *cv;         /* the layer's keys and values in page 0 */
+    const uint32_t *tables;
+    const att_tok  *toks;            /* positions, or NULL: */
+    const int32_t  *pos;
+    const uint64_t *freq;            /* [half] turns a position, modulo 1, times 2^64 */
+    uint64_t        q_tok, k_tok, v_tok, qo_tok, ko_tok;     /* bytes */
+    uint64_t        page_bytes;
+    uint32_t        n_tok, n_head, n_head_kv, hd, half, pairs, back;     /* pairs: 2i, 2i + 1; else i, i + half */
+    uint32_t        held, page_shift, block_bytes, waves;    /* waves a row */
+    float           magnitude;
+} att_rows_args;
+
+/* a batch's sequences: where the page numbers of each start, and its first position's row in what is read back */
+typedef struct att_seq { uint32_t table, row0; } att_seq;
+
+typedef struct att_read_args {
+    void           *k, *v;
+    const uint8_t  *ck, *cv;
+    const uint32_t *tables;
+    const att_seq  *seqs;            /* n_seq of them, then one past the last */
+    uint64_t        k_tok, v_tok;    /* bytes */
+    uint64_t        page_bytes;
+    uint32_t        n_seq, hd, n_head_kv, held, page_shift, block_bytes;
+} att_read_args;
+#define ATT_READ_UNITS 4u            /* pieces of 8 values that a thread reads back */
+
 typedef struct att_pair { uint32_t src, dst, rows; } att_pair;
 #define ATT_PAIRS 320
 
@@ -98,14 +138,15 @@ typedef struct att_copy_args {
     uint64_t  page_bytes;
     uint32_t  block_bytes, row_bytes, n_blocks, n_pairs;
     att_pair  pair[ATT_PAIRS];
+    uint32_t  scales;                /* 8 bits: where a block's scale bytes start, of which rows are copied too */
 } att_copy_args;
 
 #define ATT_COPY_CHUNKS 1024u        /* 16-byte pieces a workgroup */
 
 #if defined(__cplusplus)
-static_assert(sizeof(att_item) == 48 && sizeof(att_args) == 168 && sizeof(att_copy_args) <= 4096, "attn_layout.h");
+static_assert(sizeof(att_item) == 48 && sizeof(att_args) == 176 && sizeof(att_copy_args) <= 4096, "attn_layout.h");
 #else
-_Static_assert(sizeof(att_item) == 48 && sizeof(att_args) == 168 && sizeof(att_copy_args) <= 4096, "attn_layout.h");
+_Static_assert(sizeof(att_item) == 48 && sizeof(att_args) == 176 && sizeof(att_copy_args) <= 4096, "attn_layout.h");
 #endif
 
 #endif /* SLLM_ATTN_LAYOUT_H */

@@ -292,8 +292,8 @@ static int load_functions(void) {
 
 static int load_attn_functions(void) {
     static const char *const types[4] = { "f32", "f32f16", "f16", "bf16" };
-    static const char *const rest[4] = { "store_f32", "store_f32f16", "store_16", "copy" };
-    for (int i = 0; i < SLLM_ATTN_FUNCTIONS; ++i) {
+    static const char *const rest[5] = { "store_f32", "store_f32f16", "store_16", "copy", "copy8" };
+    for (int i = 0; i < SLLM_ATTN_ROWS; ++i) {
         char name[64];
         const int of = i < SLLM_ATTN_PROMPT ? i : i < SLLM_ATTN_JOIN ? i - SLLM_ATTN_PROMPT : (i - SLLM_ATTN_JOIN) % 6;
         const int type = i < SLLM_ATTN_PROMPT ? of / 2 : of / 2 ? of / 2 + 1 : 0;        /* (rows of f32, f16, bf16) */
@@ -301,6 +301,16 @@ static int load_attn_functions(void) {
         else snprintf(name, sizeof name, "sllm_k_%s_%s_%d%s", i < SLLM_ATTN_PROMPT ? "attend" : i < SLLM_ATTN_JOIN ? "prompt" : "attn_join",
                       types[type], of % 2 ? 128 : 64, i >= SLLM_ATTN_JOIN + 6 ? "_whole" : "");
         HIP_TRY(hipModuleGetFunction(&g.k_attn[i], g.attn_mod, name));
+    }
+    static const char *const rows[3] = { "f32", "f16", "bf16" }, *const held[2] = { "i8", "e4m3" };
+    for (int i = 0; i < 6; ++i) {
+        char name[64];
+        snprintf(name, sizeof name, "sllm_k_attn_%s_%s", i < 3 ? "rows" : "read", rows[i % 3]);
+        HIP_TRY(hipModuleGetFunction(&g.k_attn[SLLM_ATTN_ROWS + i], g.attn_mod, name));
+        for (int w = 0; w < 2; ++w) {
+            snprintf(name, sizeof name, "sllm_k_attend_%s%s_%d", rows[i % 3], held[i / 3], w ? 128 : 64);
+            HIP_TRY(hipModuleGetFunction(&g.k_attn[SLLM_ATTN_ATTEND8 + 2 * i + w], g.attn_mod, name));
+        }
     }
     return SLLM_GFX950_OK;
 }
