@@ -284,6 +284,44 @@ int  sllm_gfx950_prompt_create(const sllm_gfx950_prompt_desc *d, sllm_gfx950_pro
 int  sllm_gfx950_prompt_attend(sllm_gfx950_prompt *p, const sllm_gfx950_prompt_io *io);
 void sllm_gfx950_prompt_destroy(sllm_gfx950_prompt *p);
 
+/* ------------------------------------------------------------------ */
+/* beams                                                               */
+/* ------------------------------------------------------------------ */
+
+/*
+ * For each of n_group requests with n_beam beams: the n_pick best of their continuations
+ * scores[b] + logits[b][t] - log(sum over t of exp(logits[b][t])), best first. Within a beam
+ * they are ordered by logit, between beams by that sum in 64 bits; what is alike by the lower beam
+ * and the lower token. A NaN logit counts as -infinity. A beam whose score is not finite, or of
+ * which a logit is +infinity or all are -infinity, has nothing but -infinity.
+ *
+ * At most 64 beams and 64 picks, n_beam * n_pick at most 2048 and n_pick at most n_beam * n_vocab;
+ * n_vocab at most 2^24, n_group * n_beam at most 2^20. dtype is the logits' type.
+ *
+ * A plan serves any number of calls, one after the other or captured into graphs, which are
+ * valid while it lives and share its memory: graphs of one plan are replayed one after the other.
+ */
+#define SLLM_GFX950_BEAM_MAX 64
+
+typedef struct sllm_gfx950_beam_desc {
+    int32_t n_group, n_beam, n_vocab, n_pick, dtype;
+} sllm_gfx950_beam_desc;
+
+typedef struct sllm_gfx950_beam sllm_gfx950_beam;
+
+/* refused while the stream is captured */
+int  sllm_gfx950_beam_new(const sllm_gfx950_beam_desc *d, sllm_gfx950_beam **out);
+void sllm_gfx950_beam_free(sllm_gfx950_beam *p);
+/*
+ * Device memory: logits [n_group * n_beam][n_vocab], 16-byte aligned, rows `stride` elements
+ * apart (0: n_vocab); scores [n_group][n_beam]; ended [n_group][n_beam] or NULL: below 0, or
+ * the token that a beam ended with, which is then its one continuation, at its own
+ * score (its logits are not read). Out: score, beam (0 .. n_beam - 1: seq_reorder's parent) and token of
+ * each pick, [n_group][n_pick], which overlap nothing that is read, nor each other.
+ */
+int  sllm_gfx950_beam_select(sllm_gfx950_beam *p, const void *logits, size_t stride, const float *scores, const int32_t *ended,
+                             float *out_scores, int32_t *out_beam, int32_t *out_token);
+
 #ifdef __cplusplus
 }
 #endif

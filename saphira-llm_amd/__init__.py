@@ -102,6 +102,11 @@ class RopeDesc(ctypes.Structure):
                [(n, c_double) for n in ("base", "factor", "original", "fast", "slow", "magnitude")] + [("freq", c_void_p)]
 
 
+class BeamDesc(ctypes.Structure):
+    """sllm_gfx950_beam_desc."""
+    _fields_ = [(n, c_int32) for n in ("n_group", "n_beam", "n_vocab", "n_pick", "dtype")]
+
+
 class RopeIO(ctypes.Structure):
     """sllm_gfx950_rope_io."""
     _fields_ = [(n, c_int32) for n in ("dtype", "n_rows", "n_head", "n_head_kv", "back")] + \
@@ -220,6 +225,9 @@ PROTOTYPES = {
     "sllm_gfx950_rope_rows": (c_int, [c_void_p, POINTER(RopeIO)]),
     "sllm_gfx950_batch_rope_store": (c_int, [c_void_p, c_int32, c_void_p, c_void_p, c_size_t, c_void_p, c_size_t, c_void_p, c_size_t,
                                              c_void_p, c_size_t]),
+    "sllm_gfx950_beam_new": (c_int, [POINTER(BeamDesc), POINTER(c_void_p)]),
+    "sllm_gfx950_beam_free": (None, [c_void_p]),
+    "sllm_gfx950_beam_select": (c_int, [c_void_p, c_void_p, c_size_t, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p]),
     "sllm_gfx950_prompt_create": (c_int, [POINTER(PromptDesc), POINTER(c_void_p)]),
     "sllm_gfx950_prompt_attend": (c_int, [c_void_p, POINTER(PromptIO)]),
     "sllm_gfx950_prompt_destroy": (None, [c_void_p]),
@@ -893,6 +901,30 @@ class Rope:
 
     def __del__(self):
         if getattr(self, "r", None) and _lib is not None:
+            self.close()
+
+
+class BeamSelect:
+    """sllm_gfx950_beam: the n_pick best continuations of n_beam beams for each of n_group requests."""
+
+    def __init__(self, dev, n_group, n_beam, n_vocab, n_pick, dtype="float32"):
+        self.dev, self.p = dev, None
+        d = BeamDesc(n_group, n_beam, n_vocab, n_pick, DTYPES[dtype])
+        p = c_void_p()
+        check(lib().sllm_gfx950_beam_new(ctypes.byref(d), ctypes.byref(p)), "beam_new")
+        self.p = p
+
+    def run(self, logits, scores, ended, out_scores, out_beam, out_token, stride=0):
+        """Device addresses (ended: or None); stride of logits in elements, 0: packed."""
+        check(lib().sllm_gfx950_beam_select(self.p, logits, stride, scores, ended, out_scores, out_beam, out_token), "beam_select")
+
+    def close(self):
+        if self.p:
+            lib().sllm_gfx950_beam_free(self.p)
+            self.p = None
+
+    def __del__(self):
+        if getattr(self, "p", None) and _lib is not None:
             self.close()
 
 

@@ -1170,9 +1170,9 @@ static int overlap(const rows_at *a, const rows_at *b) {
     if (a->p == NULL || b->p == NULL || a->n == 0 || b->n == 0) return 0;
     const uint64_t x = (uint64_t) (uintptr_t) a->p, y = (uint64_t) (uintptr_t) b->p;
     if (x + (uint64_t) (a->n - 1) * a->tok + a->row <= y || y + (uint64_t) (b->n - 1) * b->tok + b->row <= x) return 0;
-    if (a->tok != b->tok) return 1;
-    const uint64_t off = x < y ? (y - x) % a->tok : (a->tok - (x - y) % a->tok) % a->tok;      /* of b behind a row of a */
-    return off < a->row || off + b->row > a->tok;
+    if (a->tok != b->tok && a->n > 1 && b->n > 1) return 1;
+    const uint64_t tok = a->n > 1 ? a->tok : b->tok, off = x < y ? (y - x) % tok : (tok - (x - y) % tok) % tok;      /* of b behind a row of a */
+    return off < a->row || off + b->row > tok;
 }
 
 /* waves of a CU that rows are spread over before a wave takes more of a token's */
@@ -1610,4 +1610,93 @@ int sllm_gfx950_batch_rope_store(sllm_gfx950_batch *b, int32_t layer, sllm_gfx95
     att_rows_args a = { .q = q, .k = k, .v = v, .q_out = q_out, .q_tok = qt, .k_tok = kt, .v_tok = vt, .qo_tok = qo };
     rope_args(r, &a);
     return launch_rows(b, layer, &a);
+}
+
+/* ------------------------------------------------------------------ */
+/* beams                                                               */
+/* ------------------------------------------------------------------ */
+
+struct sllm_gfx950_beam {
+    pthread_mutex_t mtx;
+    sllm_gfx950_beam_desc d;
+    uint32_t  n_chunk, chunk;
+    uint8_t  *mem;                   /* keys, then sums */
+    size_t    off_sums;
+};
+
+/* A row's parts: as many as give every CU BEAM_GROUPS workgroups, of whole tiles, but no more than
+ * the join's LDS holds the keys of. */
+#define BEAM_GROUPS 4u
+
+static void beam_chunks(sllm_gfx950_beam *p) {
+    const uint32_t rows = (uint32_t) (p->d.n_group * p->d.n_beam), tiles = ((uint32_t) p->d.n_vocab + BEAM_TILE - 1) / BEAM_TILE;
+    uint32_t n = ((uint32_t) sllm_shim_cu() * BEAM_GROUPS + rows - 1) / rows;
+    if (n > BEAM_MAX_KEYS / (uint32_t) p->d.n_pick) n = BEAM_MAX_KEYS / (uint32_t) p->d.n_pick;
+    const uint32_t each = (tiles + n - 1) / n;
+    p->chunk = each * BEAM_TILE;
+    p->n_chunk = (tiles + each - 1) / each;
+}
+
+int sllm_gfx950_beam_new(const sllm_gfx950_beam_desc *d, sllm_gfx950_beam **out) {
+    ATT_ON_DEVICE();
+    if (out == NULL) return FAIL_ARG("beam_new: NULL out");
+    *out = NULL;
+    if (d == NULL || bad_type(d->dtype) || d->n_group < 1 || d->n_beam < 1 || d->n_beam > (int32_t) BEAM_MAX_BEAM || d->n_vocab < 1 || d->n_vocab > 1 << 24 ||
+        d->n_pick < 1 || d->n_pick > (int32_t) BEAM_MAX_PICK || d->n_beam * d->n_pick > (int32_t) BEAM_MAX_LIST ||
+        (int64_t) d->n_pick > (int64_t) d->n_beam * d->n_vocab || (int64_t) d->n_group * d->n_beam > 1 << 20) {
+        return FAIL_ARG("beam_new: type, groups, beams, vocabulary or picks outside what a plan takes");
+    }
+    int st = not_in_capture("beam_new");
+    if (st != SLLM_GFX950_OK) return st;
+    sllm_gfx950_beam *p = calloc(1, sizeof *p);
+    if (p == NULL) return FAIL_NOMEM("beam_new");
+    p->d = *d;
+    beam_chunks(p);
+    const size_t parts = (size_t) d->n_group * (size_t) d->n_beam * p->n_chunk;
+    p->off_sums = align256(parts * (size_t) d->n_pick * sizeof(uint64_t));
+    const hipError_t e = hipMalloc((void **) &p->mem, p->off_sums + parts * 2 * sizeof(double));
+    if (e != hipSuccess) {
+        free(p);
+        return sllm_shim_hip_fail(e, "hipMalloc(beams)");
+    }
+    pthread_mutex_init(&p->mtx, NULL);
+    *out = p;
+    return SLLM_GFX950_OK;
+}
+
+void sllm_gfx950_beam_free(sllm_gfx950_beam *p) {
+    if (p == NULL) return;
+    buffer own = { .dev = p->mem };
+    release(&own, 1);
+    pthread_mutex_destroy(&p->mtx);
+    free(p);
+}
+
+int sllm_gfx950_beam_select(sllm_gfx950_beam *p, const void *logits, size_t stride, const float *scores, const int32_t *ended, float *out_scores,
+                            int32_t *out_beam, int32_t *out_token) {
+    ATT_ON_DEVICE();
+    if (p == NULL || logits == NULL || scores == NULL || out_scores == NULL || out_beam == NULL || out_token == NULL) return FAIL_ARG("beam_select: NULL");
+    const uint32_t size = type_size(p->d.dtype), rows = (uint32_t) (p->d.n_group * p->d.n_beam);
+    if (stride == 0) stride = (size_t) p->d.n_vocab;
+    if (stride < (size_t) p->d.n_vocab || stride > (1u << 28)) return FAIL_ARG("beam_select: stride");
+    if (misaligned(logits) || (((uintptr_t) scores | (uintptr_t) ended | (uintptr_t) out_scores | (uintptr_t) out_beam | (uintptr_t) out_token) & 3u) != 0) {
+        return FAIL_ARG("beam_select: misaligned");
+    }
+    const uint64_t in = (uint64_t) rows * 4u, picks = (uint64_t) p->d.n_group * (uint64_t) p->d.n_pick * 4u, width = (uint64_t) p->d.n_vocab * size;
+    const rows_at outs[3] = { { out_scores, picks, picks, 1 }, { out_beam, picks, picks, 1 }, { out_token, picks, picks, 1 } };
+    const rows_at ins[3] = { { logits, (uint64_t) stride * size, width, rows }, { scores, in, in, 1 }, { ended, in, in, 1 } };
+    for (int i = 0; i < 3; ++i) {
+        for (int j = 0; j < 3; ++j) {
+            if (overlap(&outs[i], &ins[j]) || (j < i && overlap(&outs[i], &outs[j]))) return FAIL_ARG("beam_select: what is written overlaps");
+        }
+    }
+    att_beam_args a = { logits, scores, ended, out_scores, out_beam, out_token, (double *) (p->mem + p->off_sums), (uint64_t *) p->mem,
+                        (uint64_t) stride * size, (uint32_t) p->d.n_beam, (uint32_t) p->d.n_vocab, (uint32_t) p->d.n_pick, p->n_chunk, p->chunk, 0 };
+    void *args[] = { &a };
+    /* the plan's memory is one: a call's launches stay together */
+    pthread_mutex_lock(&p->mtx);
+    int st = sllm_shim_launch(sllm_shim_attn_function(SLLM_ATTN_BEAM + p->d.dtype), p->n_chunk * rows, 1, ATT_THREADS, 0, args);
+    if (st == SLLM_GFX950_OK) st = sllm_shim_launch(sllm_shim_attn_function(SLLM_ATTN_BEAM_JOIN), (uint32_t) p->d.n_group, 1, BEAM_JOIN_THREADS, 0, args);
+    pthread_mutex_unlock(&p->mtx);
+    return st;
 }

@@ -1714,3 +1714,311 @@ ROWS(sllm_k_attn_rows_bf16, __bf16)
 READ(sllm_k_attn_read_f32, float)
 READ(sllm_k_attn_read_f16, _Float16)
 READ(sllm_k_attn_read_bf16, __bf16)
+
+// ---------------------------------------------------------------------------
+// beams
+// ---------------------------------------------------------------------------
+
+namespace {
+
+// A logit and its token as a number that is larger where it comes first: by value, then the
+// lower token. 0 is none.
+__device__ __forceinline__ uint64_t key_of(float x, uint32_t token) {
+    const uint32_t u = __float_as_uint(x + 0.0f);                // (-0 is 0)
+    const uint32_t o = u & 0x80000000u ? ~u : u | 0x80000000u;
+    return (uint64_t) o << 32 | (uint32_t) ~token;
+}
+__device__ __forceinline__ float value_of(uint64_t key) {
+    const uint32_t o = (uint32_t) (key >> 32);
+    return __uint_as_float(o & 0x80000000u ? o & 0x7fffffffu : ~o);
+}
+
+// 2^t and e^d for d <= 0 to about 2 of f32's last place: the product with log2(e) to twice f32's bits
+__device__ __forceinline__ float exp_of(float d) { return __builtin_amdgcn_exp2f(fmaf(d, 1.44269502162933350f, d * 1.92596299112661746e-8f)); }
+
+// where a thread's value i is, behind its first
+template <uint32_t PER> __device__ __forceinline__ constexpr uint32_t beam_token(uint32_t i) { return i / PER * ATT_THREADS * PER + i % PER; }
+
+// The n_pick largest keys so far, in order, and what a tile adds to them.
+struct best_keys {
+    uint64_t list[2][BEAM_MAX_PICK];
+    uint64_t tops[ATT_THREADS];
+    uint64_t found[BEAM_MAX_PICK * (BEAM_VALUES + 1)];
+    uint64_t bound;
+    uint32_t n_found, n_over, now;
+};
+
+// A workgroup's values into the list. Where more threads than picks have a key above the
+// list's last, the n_pick-th largest of their largest bounds the rest from below: so no more than
+// n_pick threads have any, and no more than n_pick * BEAM_VALUES keys are looked at, in
+// whatever order the values come.
+template <uint32_t PER>
+__device__ __forceinline__ void insert(best_keys &b, const float (&x)[BEAM_VALUES], uint32_t tok, uint32_t end, uint32_t n_pick) {
+    const uint32_t tid = threadIdx.x;
+    const uint64_t least = b.list[b.now][n_pick - 1];            // 0 while it is not full
+    uint64_t top = 0;
+#pragma unroll
+    for (uint32_t i = 0; i < BEAM_VALUES; ++i) {
+        const uint32_t at = tok + beam_token<PER>(i);
+        const uint64_t k = at < end ? key_of(x[i], at) : 0;
+        top = k > top ? k : top;
+    }
+    b.tops[tid] = top;
+    if (tid == 0) {
+        b.n_over = 0;
+        b.n_found = n_pick;
+        b.bound = least + 1;
+    }
+    __syncthreads();
+    const uint64_t over = __ballot(top > least);
+    if ((tid & 63u) == 0) atomicAdd(&b.n_over, (uint32_t) __popcll(over));
+    __syncthreads();
+    if (b.n_over > n_pick) {
+        if (top > least) {
+            uint32_t rank = 0;
+#pragma unroll 8
+            for (uint32_t i = 0; i < ATT_THREADS; ++i) rank += b.tops[i] > top;
+            if (rank == n_pick - 1) b.bound = top;
+        }
+        __syncthreads();
+    }
+    const uint64_t bound = b.bound;
+    if (tid < n_pick) b.found[tid] = b.list[b.now][tid];
+    if (top >= bound) {
+#pragma unroll
+        for (uint32_t i = 0; i < BEAM_VALUES; ++i) {
+            const uint32_t at = tok + beam_token<PER>(i);
+            const uint64_t k = at < end ? key_of(x[i], at) : 0;
+            if (k >= bound) b.found[atomicAdd(&b.n_found, 1u)] = k;
+        }
+    }
+    __syncthreads();
+    const uint32_t n = b.n_found, to = b.now ^ 1u;
+    if (tid < n_pick) b.list[to][tid] = 0;
+    __syncthreads();
+    for (uint32_t e = tid; e < n; e += ATT_THREADS) {
+        const uint64_t k = b.found[e];
+        if (k == 0) continue;
+        uint32_t rank = 0;
+        for (uint32_t i = 0; i < n; ++i) rank += b.found[i] > k;
+        if (rank < n_pick) b.list[to][rank] = k;
+    }
+    __syncthreads();
+    if (tid == 0) b.now = to;
+    __syncthreads();
+}
+
+// A part of a row of logits: the largest, the sum of exponentials relative to it, the best keys.
+// Which thread takes which is counted from the row's start, so that a row's sums are the
+// same bits wherever it lies: rows of 16 bits that start within four bytes are loaded from the
+// two bytes in front of them and moved over. Loads are bounded by the last whole four bytes of the row,
+// and a last two come by themselves.
+template <typename T> struct beam_loads {
+    static constexpr uint32_t PER = 16u / sizeof(T), N = BEAM_VALUES / PER;
+    u32x4 v[N];
+    uint32_t more[N];
+    __device__ __forceinline__ void load(__amdgpu_buffer_rsrc_t r, uint32_t at, bool odd) {
+#pragma unroll
+        for (uint32_t j = 0; j < N; ++j) {
+            const uint32_t by = (at + (j * ATT_THREADS + threadIdx.x) * PER) * (uint32_t) sizeof(T);
+            v[j] = __builtin_amdgcn_raw_buffer_load_b128(r, by, 0, 0);
+            if (sizeof(T) == 2 && odd) more[j] = __builtin_amdgcn_raw_buffer_load_b32(r, by + 16u, 0, 0);
+        }
+    }
+    __device__ __forceinline__ void values(float (&x)[BEAM_VALUES], bool odd) const {
+#pragma unroll
+        for (uint32_t j = 0; j < N; ++j) {
+            u32x4 w = v[j];
+            if (sizeof(T) == 2 && odd) {
+                w = (u32x4) { w[0] >> 16 | w[1] << 16, w[1] >> 16 | w[2] << 16, w[2] >> 16 | w[3] << 16, w[3] >> 16 | more[j] << 16 };
+            }
+#pragma unroll
+            for (uint32_t e = 0; e < PER; ++e) {
+                if constexpr (sizeof(T) == 4) x[j * PER + e] = __uint_as_float(w[e]);
+                else x[j * PER + e] = (float) __builtin_bit_cast(typename vec8<T>::type, w)[e];
+            }
+        }
+    }
+};
+
+template <typename T> __device__ __forceinline__ void beam_body(const att_beam_args &a) {
+    typedef beam_loads<T> loads;
+    __shared__ best_keys b;
+    __shared__ float part_m[ATT_THREADS / 64];
+    __shared__ double part_s[ATT_THREADS / 64];
+    const uint32_t tid = threadIdx.x, row = blockIdx.x / a.n_chunk, c = blockIdx.x % a.n_chunk, end = a.n_vocab;
+    if (a.ended && G_CAST(const int32_t, a.ended)[row] >= 0) return;
+    const float score = G_CAST(const float, a.scores)[row];
+    if (!(fabsf(score) <= -LOWEST)) return;
+    const uint8_t *from = (const uint8_t *) a.logits + row * a.stride;
+    const bool odd = sizeof(T) == 2 && ((uintptr_t) from & 2u) != 0;
+    const uint32_t bytes = end * (uint32_t) sizeof(T) + (odd ? 2u : 0u);
+    const __amdgpu_buffer_rsrc_t r = __builtin_amdgcn_make_buffer_rsrc((void *) (from - (odd ? 2 : 0)), (short) 0, (int) uniform(bytes & ~3u), 0x00020000);
+    const bool loose = (bytes & 3u) != 0;
+    const float last_x = loose ? (float) G_CAST(const T, from)[end - 1] : 0.0f;
+    if (tid < a.n_pick) b.list[0][tid] = 0;
+    if (tid == 0) b.now = 0;
+    float m = LOWEST;
+    double sum = 0.0;
+    uint64_t least = 0;
+    const uint32_t first = c * a.chunk, last = min(first + a.chunk, end);
+    loads next;
+    next.load(r, first, odd);
+    __syncthreads();
+    for (uint32_t t = first; t < last; t += BEAM_TILE) {
+        const loads now = next;
+        if (t + BEAM_TILE < last) next.load(r, t + BEAM_TILE, odd);
+        float x[BEAM_VALUES], top = LOWEST;
+        now.values(x, odd);
+        // tokens: PER of a thread side by side, ATT_THREADS * PER further each load
+        const uint32_t tok = t + tid * loads::PER;
+        if (t + BEAM_TILE > end) {
+#pragma unroll
+            for (uint32_t i = 0; i < BEAM_VALUES; ++i) {
+                const uint32_t at = tok + beam_token<loads::PER>(i);
+                if (loose && at == end - 1) x[i] = last_x;
+                x[i] = at < end ? x[i] : -INFINITY;
+            }
+        }
+#pragma unroll
+        for (uint32_t i = 0; i < BEAM_VALUES; ++i) {
+            x[i] = fmaxf(x[i], -INFINITY);                       // (NaN: -infinity)
+            top = fmaxf(top, x[i]);
+        }
+        if (top > m) {
+            sum *= (double) exp_of(m - top);
+            m = top;
+        }
+        float s = 0.0f;
+#pragma unroll
+        for (uint32_t i = 0; i < BEAM_VALUES; ++i) s += exp_of(x[i] - m);
+        sum += (double) s;
+        // (tokens rise from tile to tile: of alike values the earlier stays)
+        if (__syncthreads_or(least == 0 || top > value_of(least))) {
+            insert<loads::PER>(b, x, tok, end, a.n_pick);
+            least = b.list[b.now][a.n_pick - 1];
+        }
+    }
+    float all = m;
+#pragma unroll
+    for (int d = 32; d > 0; d >>= 1) all = fmaxf(all, __shfl_xor(all, d));
+    if ((tid & 63u) == 0) part_m[tid >> 6] = all;
+    __syncthreads();
+    all = fmaxf(fmaxf(part_m[0], part_m[1]), fmaxf(part_m[2], part_m[3]));
+    sum *= (double) exp_of(m - all);
+#pragma unroll
+    for (int d = 32; d > 0; d >>= 1) sum += __shfl_xor(sum, d);
+    if ((tid & 63u) == 0) part_s[tid >> 6] = sum;
+    __syncthreads();
+    const uint64_t at = (uint64_t) row * a.n_chunk + c;
+    if (tid == 0) {
+        G_CAST(double, a.sums)[2 * at] = (double) all;
+        G_CAST(double, a.sums)[2 * at + 1] = part_s[0] + part_s[1] + part_s[2] + part_s[3];
+    }
+    if (tid < a.n_pick) G_CAST(uint64_t, a.keys)[at * a.n_pick + tid] = b.list[b.now][tid];
+}
+
+// How many of n keys in falling order are larger than k.
+__device__ __forceinline__ uint32_t larger(const uint64_t *keys, uint32_t n, uint64_t k) {
+    uint32_t lo = 0;
+    for (uint32_t hi = n; lo < hi;) {
+        const uint32_t mid = (lo + hi) / 2;
+        if (keys[mid] > k) lo = mid + 1;
+        else hi = mid;
+    }
+    return lo;
+}
+
+}  // namespace
+
+#define BEAM(name, T) extern "C" __global__ void __launch_bounds__(ATT_THREADS) name(const att_beam_args a) { beam_body<T>(a); }
+BEAM(sllm_k_beam_f32, float)
+BEAM(sllm_k_beam_f16, _Float16)
+BEAM(sllm_k_beam_bf16, __bf16)
+
+// A group: each beam's parts joined (a key's rank is its place in its own part and how many are
+// larger in each other, which are in order), then its beams in the same way by their values in 64
+// bits. A beam that ended, or has no finite sum, is its token, and tokens from 0 on at -infinity.
+extern "C" __global__ void __launch_bounds__(BEAM_JOIN_THREADS) sllm_k_beam_join(const att_beam_args a) {
+    __shared__ uint64_t keys[BEAM_MAX_KEYS];
+    __shared__ double value[BEAM_MAX_LIST];
+    __shared__ uint32_t token[BEAM_MAX_LIST];
+    __shared__ double base[BEAM_MAX_BEAM], most[BEAM_MAX_BEAM];
+    const uint32_t tid = threadIdx.x, lane = tid & 63u, wave = tid >> 6, k = a.n_pick, row0 = blockIdx.x * a.n_beam;
+    const uint32_t n_list = min(k, a.n_vocab);                   // of a beam
+    // what is added to a beam's logits less the largest: its score less the log of its sum
+    for (uint32_t b = wave; b < a.n_beam; b += BEAM_JOIN_THREADS / 64) {
+        const uint32_t row = row0 + b;
+        const float score = G_CAST(const float, a.scores)[row];
+        const bool live = !(a.ended && G_CAST(const int32_t, a.ended)[row] >= 0) && fabsf(score) <= -LOWEST;
+        double x = -INFINITY, m = (double) LOWEST;
+        if (live) {
+            GLOBAL const double *sums = G_CAST(const double, a.sums) + 2 * (uint64_t) row * a.n_chunk;
+            double s = 0.0;
+            for (uint32_t c = lane; c < a.n_chunk; c += 64) m = fmax(m, sums[2 * c]);
+#pragma unroll
+            for (int d = 32; d > 0; d >>= 1) m = fmax(m, __shfl_xor(m, d));
+            for (uint32_t c = lane; c < a.n_chunk; c += 64) s += sums[2 * c + 1] * exp(sums[2 * c] - m);
+#pragma unroll
+            for (int d = 32; d > 0; d >>= 1) s += __shfl_xor(s, d);
+            x = (double) score - log(s);
+        }
+        if (lane == 0) {
+            base[b] = x;
+            most[b] = m;
+        }
+    }
+    __syncthreads();
+    const uint32_t per = a.n_chunk * k, at_once = BEAM_MAX_KEYS / per;
+    for (uint32_t b0 = 0; b0 < a.n_beam; b0 += at_once) {
+        const uint32_t nb = min(at_once, a.n_beam - b0);
+        for (uint32_t i = tid; i < nb * per; i += BEAM_JOIN_THREADS) {
+            if (fabs(base[b0 + i / per]) < INFINITY) keys[i] = G_CAST(const uint64_t, a.keys)[(uint64_t) (row0 + b0) * per + i];
+        }
+        __syncthreads();
+        for (uint32_t i = tid; i < nb * per; i += BEAM_JOIN_THREADS) {
+            const uint32_t b = b0 + i / per, c = i % per / k, place = i % k;
+            if (!(fabs(base[b]) < INFINITY)) {
+                if (c != 0 || place >= n_list) continue;
+                const int32_t end = a.ended ? G_CAST(const int32_t, a.ended)[row0 + b] : -1;
+                const float score = G_CAST(const float, a.scores)[row0 + b];
+                const bool first = end >= 0 && fabsf(score) <= -LOWEST;          // its own token comes first
+                uint32_t t = place;
+                if (first) t = place == 0 ? (uint32_t) end : place - 1 < (uint32_t) end ? place - 1 : place;
+                value[b * k + place] = first && place == 0 ? (double) score : -INFINITY;
+                token[b * k + place] = t;
+                continue;
+            }
+            const uint64_t key = keys[i];
+            if (key == 0) continue;
+            uint32_t rank = place;
+            for (uint32_t o = 0; o < a.n_chunk && rank < k; ++o) if (o != c) rank += larger(keys + i / per * per + o * k, k, key);
+            if (rank >= k) continue;
+            value[b * k + rank] = base[b] + ((double) value_of(key) - most[b]);
+            token[b * k + rank] = ~(uint32_t) key;
+        }
+        __syncthreads();
+    }
+    for (uint32_t i = tid; i < a.n_beam * k; i += BEAM_JOIN_THREADS) {
+        const uint32_t b = i / k, place = i % k;
+        if (place >= n_list) continue;
+        const double x = value[i];
+        uint32_t rank = place;
+        for (uint32_t o = 0; o < a.n_beam && rank < k; ++o) {
+            if (o == b) continue;
+            uint32_t lo = 0;                                     // of a lower beam what is alike comes first too
+            for (uint32_t hi = n_list; lo < hi;) {
+                const uint32_t mid = (lo + hi) / 2;
+                const double y = value[o * k + mid];
+                if (y > x || (y == x && o < b)) lo = mid + 1;
+                else hi = mid;
+            }
+            rank += lo;
+        }
+        if (rank >= k) continue;
+        const uint64_t at = (uint64_t) blockIdx.x * k + rank;
+        G_CAST(float, a.out)[at] = (float) x;
+        G_CAST(int32_t, a.beam)[at] = (int32_t) b;
+        G_CAST(int32_t, a.token)[at] = (int32_t) token[i];
+    }
+}

@@ -128,6 +128,30 @@ typedef struct att_read_args {
 } att_read_args;
 #define ATT_READ_UNITS 4u            /* pieces of 8 values that a thread reads back */
 
+/*
+ * The best continuations of beams: each workgroup of the first launch takes a part of a row of
+ * logits, `chunk` of them, and leaves its sum of exponentials and its best n_pick keys in order; the
+ * second launch joins them, a group a workgroup.
+ */
+#define BEAM_MAX_PICK  64u
+#define BEAM_MAX_BEAM  64u
+#define BEAM_MAX_LIST  2048u         /* n_beam * n_pick */
+#define BEAM_MAX_KEYS  3072u         /* n_chunk * n_pick: a beam's keys in LDS */
+#define BEAM_JOIN_THREADS 512u
+#define BEAM_VALUES    16u           /* of a thread at a time */
+#define BEAM_TILE      (ATT_THREADS * BEAM_VALUES)
+typedef struct att_beam_args {
+    const void    *logits;
+    const float   *scores;
+    const int32_t *ended;            /* or NULL */
+    float         *out;
+    int32_t       *beam, *token;
+    double        *sums;             /* [row][chunk][2]: the largest logit, the sum of exponentials */
+    uint64_t      *keys;             /* [row][chunk][n_pick] */
+    uint64_t       stride;           /* bytes */
+    uint32_t       n_beam, n_vocab, n_pick, n_chunk, chunk, pad;
+} att_beam_args;
+
 typedef struct att_pair { uint32_t src, dst, rows; } att_pair;
 #define ATT_PAIRS 320
 

@@ -303,8 +303,13 @@ static int load_attn_functions(void) {
         HIP_TRY(hipModuleGetFunction(&g.k_attn[i], g.attn_mod, name));
     }
     static const char *const rows[3] = { "f32", "f16", "bf16" }, *const held[2] = { "i8", "e4m3" };
+    HIP_TRY(hipModuleGetFunction(&g.k_attn[SLLM_ATTN_BEAM_JOIN], g.attn_mod, "sllm_k_beam_join"));
     for (int i = 0; i < 6; ++i) {
         char name[64];
+        if (i < 3) {
+            snprintf(name, sizeof name, "sllm_k_beam_%s", rows[i]);
+            HIP_TRY(hipModuleGetFunction(&g.k_attn[SLLM_ATTN_BEAM + i], g.attn_mod, name));
+        }
         snprintf(name, sizeof name, "sllm_k_attn_%s_%s", i < 3 ? "rows" : "read", rows[i % 3]);
         HIP_TRY(hipModuleGetFunction(&g.k_attn[SLLM_ATTN_ROWS + i], g.attn_mod, name));
         for (int w = 0; w < 2; ++w) {

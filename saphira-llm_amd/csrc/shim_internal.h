@@ -71,7 +71,8 @@ SLLM_HIDDEN int         sllm_shim_decode_function(const char *name, hipFunction_
  * f16/f16, bf16/bf16; prompts, and the join of partial results, for rows of
  * f32, f16, bf16; the store for f32, f32 to f16, 16 bits; page copies, plain and
  * with scales; rows that turn or go to 8 bits, and a cache's read back, for f32, f16,
- * bf16; attention over 8 bits for f32, f16, bf16 over int8 and then over e4m3 */
+ * bf16; attention over 8 bits for f32, f16, bf16 over int8 and then over e4m3; the
+ * parts of rows of logits of f32, f16, bf16, and their join */
 enum {
     SLLM_ATTN_ATTEND = 0,                        /* + types * 2 + wide */
     SLLM_ATTN_PROMPT = 8,                        /* + type * 2 + wide */
@@ -80,7 +81,8 @@ enum {
     SLLM_ATTN_ROWS = 31,                         /* + type */
     SLLM_ATTN_READ = 34,                         /* + type */
     SLLM_ATTN_ATTEND8 = 37,                      /* + types * 2 + wide */
-    SLLM_ATTN_FUNCTIONS = 49,
+    SLLM_ATTN_BEAM = 49, SLLM_ATTN_BEAM_JOIN = 52,      /* + type */
+    SLLM_ATTN_FUNCTIONS = 53,
     SLLM_ATTN_HELD8 = 4                          /* the first of the pairs of types over a cache of 8 bits */
 };
 SLLM_HIDDEN hipFunction_t sllm_shim_attn_function(int i);
