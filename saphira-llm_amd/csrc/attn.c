@@ -1625,13 +1625,13 @@ struct sllm_gfx950_beam {
 };
 
 /* A row's parts: as many as give every CU BEAM_GROUPS workgroups, of whole tiles, but no more than
- * the join's LDS holds the keys of. */
+ * the join has lanes. */
 #define BEAM_GROUPS 4u
 
 static void beam_chunks(sllm_gfx950_beam *p) {
     const uint32_t rows = (uint32_t) (p->d.n_group * p->d.n_beam), tiles = ((uint32_t) p->d.n_vocab + BEAM_TILE - 1) / BEAM_TILE;
     uint32_t n = ((uint32_t) sllm_shim_cu() * BEAM_GROUPS + rows - 1) / rows;
-    if (n > BEAM_MAX_KEYS / (uint32_t) p->d.n_pick) n = BEAM_MAX_KEYS / (uint32_t) p->d.n_pick;
+    if (n > BEAM_MAX_PARTS) n = BEAM_MAX_PARTS;
     const uint32_t each = (tiles + n - 1) / n;
     p->chunk = each * BEAM_TILE;
     p->n_chunk = (tiles + each - 1) / each;

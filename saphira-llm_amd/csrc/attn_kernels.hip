@@ -1724,7 +1724,8 @@ namespace {
 // A logit and its token as a number that is larger where it comes first: by value, then the
 // lower token. 0 is none.
 __device__ __forceinline__ uint64_t key_of(float x, uint32_t token) {
-    const uint32_t u = __float_as_uint(x + 0.0f);                // (-0 is 0)
+    uint32_t u = __float_as_uint(x);
+    u = u == 0x80000000u ? 0u : u;                               // (-0 is 0)
     const uint32_t o = u & 0x80000000u ? ~u : u | 0x80000000u;
     return (uint64_t) o << 32 | (uint32_t) ~token;
 }
@@ -1733,94 +1734,79 @@ __device__ __forceinline__ float value_of(uint64_t key) {
     return __uint_as_float(o & 0x80000000u ? o & 0x7fffffffu : ~o);
 }
 
-// 2^t and e^d for d <= 0 to about 2 of f32's last place: the product with log2(e) to twice f32's bits
-__device__ __forceinline__ float exp_of(float d) { return __builtin_amdgcn_exp2f(fmaf(d, 1.44269502162933350f, d * 1.92596299112661746e-8f)); }
+// e^d, d <= 0: off by a step of d's product with log2(e), which weighs little where d is far from 0
+__device__ __forceinline__ float exp_of(float d) { return __builtin_amdgcn_exp2f(d * 1.44269504088896341f); }
 
-// where a thread's value i is, behind its first
-template <uint32_t PER> __device__ __forceinline__ constexpr uint32_t beam_token(uint32_t i) { return i / PER * ATT_THREADS * PER + i % PER; }
-
-// The n_pick largest keys so far, in order, and what a tile adds to them.
-struct best_keys {
-    uint64_t list[2][BEAM_MAX_PICK];
-    uint64_t tops[ATT_THREADS];
-    uint64_t found[BEAM_MAX_PICK * (BEAM_VALUES + 1)];
-    uint64_t bound;
-    uint32_t n_found, n_over, now;
-};
-
-// A workgroup's values into the list. Where more threads than picks have a key above the
-// list's last, the n_pick-th largest of their largest bounds the rest from below: so no more than
-// n_pick threads have any, and no more than n_pick * BEAM_VALUES keys are looked at, in
-// whatever order the values come.
-template <uint32_t PER>
-__device__ __forceinline__ void insert(best_keys &b, const float (&x)[BEAM_VALUES], uint32_t tok, uint32_t end, uint32_t n_pick) {
-    const uint32_t tid = threadIdx.x;
-    const uint64_t least = b.list[b.now][n_pick - 1];            // 0 while it is not full
-    uint64_t top = 0;
+// A lower bound of the wave's n-th largest key, at least n of which are not 0: bit by bit,
+// counting the lanes that are not below. Sixteen bits do where no more than n more lanes are not
+// below it, else all 64.
+__device__ __forceinline__ uint64_t nth_largest(uint64_t key, uint32_t n) {
+    const uint32_t hi = (uint32_t) (key >> 32), lo = (uint32_t) key;
+    uint32_t t = 0, u = 0;
 #pragma unroll
-    for (uint32_t i = 0; i < BEAM_VALUES; ++i) {
-        const uint32_t at = tok + beam_token<PER>(i);
-        const uint64_t k = at < end ? key_of(x[i], at) : 0;
-        top = k > top ? k : top;
-    }
-    b.tops[tid] = top;
-    if (tid == 0) {
-        b.n_over = 0;
-        b.n_found = n_pick;
-        b.bound = least + 1;
-    }
-    __syncthreads();
-    const uint64_t over = __ballot(top > least);
-    if ((tid & 63u) == 0) atomicAdd(&b.n_over, (uint32_t) __popcll(over));
-    __syncthreads();
-    if (b.n_over > n_pick) {
-        if (top > least) {
-            uint32_t rank = 0;
-#pragma unroll 8
-            for (uint32_t i = 0; i < ATT_THREADS; ++i) rank += b.tops[i] > top;
-            if (rank == n_pick - 1) b.bound = top;
-        }
-        __syncthreads();
-    }
-    const uint64_t bound = b.bound;
-    if (tid < n_pick) b.found[tid] = b.list[b.now][tid];
-    if (top >= bound) {
-#pragma unroll
-        for (uint32_t i = 0; i < BEAM_VALUES; ++i) {
-            const uint32_t at = tok + beam_token<PER>(i);
-            const uint64_t k = at < end ? key_of(x[i], at) : 0;
-            if (k >= bound) b.found[atomicAdd(&b.n_found, 1u)] = k;
-        }
-    }
-    __syncthreads();
-    const uint32_t n = b.n_found, to = b.now ^ 1u;
-    if (tid < n_pick) b.list[to][tid] = 0;
-    __syncthreads();
-    for (uint32_t e = tid; e < n; e += ATT_THREADS) {
-        const uint64_t k = b.found[e];
-        if (k == 0) continue;
-        uint32_t rank = 0;
-        for (uint32_t i = 0; i < n; ++i) rank += b.found[i] > k;
-        if (rank < n_pick) b.list[to][rank] = k;
-    }
-    __syncthreads();
-    if (tid == 0) b.now = to;
-    __syncthreads();
+    for (uint32_t bit = 1u << 31; bit >= 1u << 16; bit >>= 1) if ((uint32_t) __popcll(__ballot(hi >= (t | bit))) >= n) t |= bit;
+    if ((uint32_t) __popcll(__ballot(hi >= t)) <= 2u * n) return (uint64_t) t << 32;
+    for (uint32_t bit = 1u << 15; bit > 0; bit >>= 1) if ((uint32_t) __popcll(__ballot(hi >= (t | bit))) >= n) t |= bit;
+    const uint32_t above = (uint32_t) __popcll(__ballot(hi > t));
+    for (uint32_t bit = 1u << 31; bit > 0; bit >>= 1) if (above + (uint32_t) __popcll(__ballot(hi == t && lo >= (u | bit))) >= n) u |= bit;
+    return (uint64_t) t << 32 | u;
 }
 
-// A part of a row of logits: the largest, the sum of exponentials relative to it, the best keys.
-// Which thread takes which is counted from the row's start, so that a row's sums are the
-// same bits wherever it lies: rows of 16 bits that start within four bytes are loaded from the
-// two bytes in front of them and moved over. Loads are bounded by the last whole four bytes of the row,
-// and a last two come by themselves.
+// A wave's largest keys so far, a lane each, in falling order (0: none), of which the first n_pick
+// count. A key is put in its place by one comparison in all lanes and a move of those behind it
+// to the next lane.
+struct wave_best {
+    uint32_t hi, lo;                 // the lane's
+    uint64_t least;                  // the n_pick-th
+    uint32_t n_pick;
+
+    __device__ __forceinline__ wave_best(uint32_t k) : hi(0), lo(0), least(0), n_pick(k) { }
+    __device__ __forceinline__ uint64_t mine() const { return (uint64_t) hi << 32 | lo; }
+    // the i-th, from 0 on
+    __device__ __forceinline__ uint64_t place(uint32_t i) const {
+        return (uint64_t) (uint32_t) __builtin_amdgcn_readlane((int) hi, (int) i) << 32 | (uint32_t) __builtin_amdgcn_readlane((int) lo, (int) i);
+    }
+    __device__ __forceinline__ void put_one(uint32_t h, uint32_t l) {        // (a key that is the same in all lanes)
+        const uint64_t key = (uint64_t) h << 32 | l;
+        // the lane in front's (wave_shr:1), the first lane's larger than all
+        const uint32_t h1 = (uint32_t) __builtin_amdgcn_update_dpp(-1, (int) hi, 0x138, 0xf, 0xf, false);
+        const uint32_t l1 = (uint32_t) __builtin_amdgcn_update_dpp(-1, (int) lo, 0x138, 0xf, 0xf, false);
+        const bool stays = mine() > key, next = ((uint64_t) h1 << 32 | l1) > key;
+        hi = stays ? hi : next ? h : h1;
+        lo = stays ? lo : next ? l : l1;
+    }
+    // the keys of the lanes that take part
+    __device__ __forceinline__ void put(bool take, uint64_t key) {
+        for (uint64_t who = __ballot(take); who != 0; who &= who - 1) {
+            const int at = __builtin_ctzll(who);
+            put_one((uint32_t) __builtin_amdgcn_readlane((int) (uint32_t) (key >> 32), at), (uint32_t) __builtin_amdgcn_readlane((int) (uint32_t) key, at));
+        }
+    }
+    __device__ __forceinline__ void settle() {
+        least = place(n_pick - 1);
+    }
+    // What the keys of lanes with these largest ones have to reach to be among the first. Where
+    // more lanes than picks have one above the list's last, the n_pick-th largest of them bounds the rest
+    // from below, so that few are put in, in whatever order the values come.
+    __device__ __forceinline__ uint64_t bound(uint64_t top) const {
+        return (uint32_t) __popcll(__ballot(top > least)) > n_pick ? nth_largest(top, n_pick) : least + 1;
+    }
+};
+
+// Rows of logits as a wave takes them: which lane takes which is counted from the row's start,
+// so that a row's sums are the same bits wherever it lies. Rows of 16 bits that start within
+// four bytes are loaded from the two bytes in front of them and moved over. Loads are bounded by
+// the last whole four bytes of the row; a last two come by themselves.
 template <typename T> struct beam_loads {
     static constexpr uint32_t PER = 16u / sizeof(T), N = BEAM_VALUES / PER;
     u32x4 v[N];
     uint32_t more[N];
+    // where value i of a lane is, behind its first
+    static __device__ __forceinline__ constexpr uint32_t token(uint32_t i) { return i / PER * 64u * PER + i % PER; }
     __device__ __forceinline__ void load(__amdgpu_buffer_rsrc_t r, uint32_t at, bool odd) {
 #pragma unroll
         for (uint32_t j = 0; j < N; ++j) {
-            const uint32_t by = (at + (j * ATT_THREADS + threadIdx.x) * PER) * (uint32_t) sizeof(T);
+            const uint32_t by = (at + (j * 64u + (threadIdx.x & 63u)) * PER) * (uint32_t) sizeof(T);
             v[j] = __builtin_amdgcn_raw_buffer_load_b128(r, by, 0, 0);
             if (sizeof(T) == 2 && odd) more[j] = __builtin_amdgcn_raw_buffer_load_b32(r, by + 16u, 0, 0);
         }
@@ -1841,92 +1827,179 @@ template <typename T> struct beam_loads {
     }
 };
 
+// A part of a row of logits: the largest, the sum of exponentials relative to it, the best
+// keys. Its waves take turns at 64 * BEAM_VALUES logits. Of their first ones they tell each other
+// what n_pick keys of the part are no smaller than, and from then on put down what is not below that
+// (128256 logits in four parts, 16 picks: about 100 of 32768), which is put in order at the end.
 template <typename T> __device__ __forceinline__ void beam_body(const att_beam_args &a) {
     typedef beam_loads<T> loads;
-    __shared__ best_keys b;
-    __shared__ float part_m[ATT_THREADS / 64];
-    __shared__ double part_s[ATT_THREADS / 64];
-    const uint32_t tid = threadIdx.x, row = blockIdx.x / a.n_chunk, c = blockIdx.x % a.n_chunk, end = a.n_vocab;
-    if (a.ended && G_CAST(const int32_t, a.ended)[row] >= 0) return;
-    const float score = G_CAST(const float, a.scores)[row];
+    // tiles of a wave that are on their way, 4 KB, and then gone through together
+    constexpr uint32_t TILE = 64u * BEAM_VALUES, STEP = WAVES * TILE, AHEAD = sizeof(T) == 4 ? 2 : 4;
+    typedef typename vec8<T>::type values;
+    __shared__ values kept[WAVES][64u * (AHEAD + 1u)];
+    __shared__ uint32_t kept_at[WAVES][64u * (AHEAD + 1u)];
+    __shared__ uint64_t found[WAVES][128 + 8];
+    __shared__ uint32_t n_found[WAVES];
+    __shared__ float told[WAVES], part_m[WAVES];
+    __shared__ double part_s[WAVES];
+    const uint32_t tid = threadIdx.x, lane = tid & 63u, wave = uniform(tid >> 6), row = blockIdx.x / a.n_chunk, c = blockIdx.x % a.n_chunk, end = a.n_vocab;
+    if (a.ended && C_CAST(int32_t, a.ended)[row] >= 0) return;
+    const float score = C_CAST(float, a.scores)[row];
     if (!(fabsf(score) <= -LOWEST)) return;
     const uint8_t *from = (const uint8_t *) a.logits + row * a.stride;
     const bool odd = sizeof(T) == 2 && ((uintptr_t) from & 2u) != 0;
     const uint32_t bytes = end * (uint32_t) sizeof(T) + (odd ? 2u : 0u);
     const __amdgpu_buffer_rsrc_t r = __builtin_amdgcn_make_buffer_rsrc((void *) (from - (odd ? 2 : 0)), (short) 0, (int) uniform(bytes & ~3u), 0x00020000);
     const bool loose = (bytes & 3u) != 0;
+    const uint32_t first = c * a.chunk + wave * TILE, last = min(c * a.chunk + a.chunk, end);
+    loads ring[AHEAD];
+#pragma unroll
+    for (uint32_t u = 0; u < AHEAD; ++u) ring[u].load(r, first + u * STEP, odd);
     const float last_x = loose ? (float) G_CAST(const T, from)[end - 1] : 0.0f;
-    if (tid < a.n_pick) b.list[0][tid] = 0;
-    if (tid == 0) b.now = 0;
-    float m = LOWEST;
+    wave_best best(a.n_pick);
+    uint32_t n = 0, n_kept = 0;                                  // keys in `found`, lanes whose values are in `kept`
+    float m = LOWEST, least = -INFINITY;                         // what is put down is not below `least`
     double sum = 0.0;
-    uint64_t least = 0;
-    const uint32_t first = c * a.chunk, last = min(first + a.chunk, end);
-    loads next;
-    next.load(r, first, odd);
-    __syncthreads();
-    for (uint32_t t = first; t < last; t += BEAM_TILE) {
-        const loads now = next;
-        if (t + BEAM_TILE < last) next.load(r, t + BEAM_TILE, odd);
-        float x[BEAM_VALUES], top = LOWEST;
-        now.values(x, odd);
-        // tokens: PER of a thread side by side, ATT_THREADS * PER further each load
-        const uint32_t tok = t + tid * loads::PER;
-        if (t + BEAM_TILE > end) {
+    // the waves with tiles, and which of a wave's largest it tells, from 0 on
+    const uint32_t n_waves = min((uint32_t) WAVES, (last - c * a.chunk + TILE - 1u) / TILE), q = (a.n_pick - 1u) / n_waves;
+    // what was found is put in order and given up, and what is alike the last of n_pick or below is not found again
+    auto order = [&]() {
+#pragma unroll 1
+        for (uint32_t i = 0; i < n; i += 64u) {
+            const uint64_t key = i + lane < n ? found[wave][i + lane] : 0;
+            best.put(key >= best.bound(key), key);
+            best.settle();
+        }
+        __builtin_amdgcn_wave_barrier();
+        n = 0;
+        if (best.least != 0) least = fmaxf(least, value_of(((best.least >> 32) + 1u) << 32));
+    };
+    // what was kept and is not below `least`, as keys: eight lanes' values at a time
+    auto sift = [&]() {
+#pragma unroll 1
+        for (uint32_t i = 0; i < n_kept; i += 8u) {
+            const uint32_t e = min(i + lane / BEAM_VALUES, n_kept - 1u), v = lane % BEAM_VALUES;
+            const float x = (float) reinterpret_cast<const T *>(&kept[wave][e])[v];
+            const uint32_t at = kept_at[wave][e] + loads::token(v);
+            const bool take = i + lane / BEAM_VALUES < n_kept && x >= least && at < end;
+            const uint64_t who = __ballot(take);
+            if (take) found[wave][n + __builtin_amdgcn_mbcnt_hi((uint32_t) (who >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t) who, 0))] = key_of(x, at);
+            n += (uint32_t) __popcll(who);
+            __builtin_amdgcn_wave_barrier();
+            if (n > 64u) order();
+        }
+        n_kept = 0;
+    };
+    for (uint32_t t = first; t < last; t += AHEAD * STEP) {
+        float x[AHEAD][BEAM_VALUES], top[AHEAD];
 #pragma unroll
-            for (uint32_t i = 0; i < BEAM_VALUES; ++i) {
-                const uint32_t at = tok + beam_token<loads::PER>(i);
-                if (loose && at == end - 1) x[i] = last_x;
-                x[i] = at < end ? x[i] : -INFINITY;
+        for (uint32_t u = 0; u < AHEAD; ++u) {
+            const uint32_t tu = t + u * STEP, tok = tu + lane * loads::PER;
+            top[u] = -INFINITY;
+            if (tu >= last) continue;
+            ring[u].values(x[u], odd);
+            if (tu + AHEAD * STEP < last) ring[u].load(r, tu + AHEAD * STEP, odd);
+            if (tu + TILE > end) {
+#pragma unroll
+                for (uint32_t i = 0; i < BEAM_VALUES; ++i) {
+                    const uint32_t at = tok + loads::token(i);
+                    if (loose && at == end - 1) x[u][i] = last_x;
+                    x[u][i] = at < end ? x[u][i] : -INFINITY;
+                }
             }
+#pragma unroll
+            for (uint32_t i = 0; i < BEAM_VALUES; ++i) top[u] = fmaxf(top[u], x[u][i]);  // (of NaN and a number, the number)
+            if (top[u] > m) {
+                sum *= (double) exp_of(m - top[u]);
+                m = top[u];
+            }
+            float s = 0.0f;
+#pragma unroll
+            for (uint32_t i = 0; i < BEAM_VALUES; ++i) s += exp_of(x[u][i] - m);
+            if (__any(s != s)) {                                 // NaN is -infinity
+                s = 0.0f;
+#pragma unroll
+                for (uint32_t i = 0; i < BEAM_VALUES; ++i) {
+                    x[u][i] = fmaxf(x[u][i], -INFINITY);
+                    s += exp_of(x[u][i] - m);
+                }
+            }
+            sum += (double) s;
+        }
+        if (t == first) {                                        // (all waves with tiles are here)
+            float most = top[0];
+#pragma unroll
+            for (uint32_t u = 1; u < AHEAD; ++u) most = fmaxf(most, top[u]);
+            const uint64_t nth = (uint32_t) __popcll(__ballot(most > -INFINITY)) > q ? nth_largest(most > -INFINITY ? key_of(most, 0) : 0, q + 1u) : 0;
+            if (lane == 0) told[wave] = nth == 0 ? -INFINITY : value_of(nth);
+            __syncthreads();
+            least = fminf(fminf(told[0], told[1]), fminf(told[2], told[3]));
         }
 #pragma unroll
-        for (uint32_t i = 0; i < BEAM_VALUES; ++i) {
-            x[i] = fmaxf(x[i], -INFINITY);                       // (NaN: -infinity)
-            top = fmaxf(top, x[i]);
-        }
-        if (top > m) {
-            sum *= (double) exp_of(m - top);
-            m = top;
-        }
-        float s = 0.0f;
+        for (uint32_t u = 0; u < AHEAD; ++u) {
+            const uint32_t tu = t + u * STEP, tok = tu + lane * loads::PER;
+            const bool keep = top[u] >= least;
+            const uint64_t who = __ballot(keep);
+            if (tu >= last || who == 0) continue;
+            if (keep) {                                          // (all its eight values: seldom more than one of them counts)
+                const uint32_t e = n_kept + __builtin_amdgcn_mbcnt_hi((uint32_t) (who >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t) who, 0));
+                values y;                                        // (as they came)
 #pragma unroll
-        for (uint32_t i = 0; i < BEAM_VALUES; ++i) s += exp_of(x[i] - m);
-        sum += (double) s;
-        // (tokens rise from tile to tile: of alike values the earlier stays)
-        if (__syncthreads_or(least == 0 || top > value_of(least))) {
-            insert<loads::PER>(b, x, tok, end, a.n_pick);
-            least = b.list[b.now][a.n_pick - 1];
+                for (uint32_t i = 0; i < BEAM_VALUES; ++i) y[i] = (T) x[u][i];
+                kept[wave][e] = y;
+                kept_at[wave][e] = tok;
+            }
+            n_kept += (uint32_t) __popcll(who);
+            __builtin_amdgcn_wave_barrier();
         }
+        if (n_kept > 64u) sift();
     }
+    if (first >= last) {                                         // (a wave without a tile)
+        if (lane == 0) told[wave] = INFINITY;
+        __syncthreads();
+    }
+    sift();
+    if (__any(best.hi != 0)) {
+        order();
+        if (lane < a.n_pick) found[wave][lane] = best.mine();
+        n = (uint32_t) __popcll(__ballot(lane < a.n_pick && best.hi != 0));
+    }
+    __builtin_amdgcn_wave_barrier();
+    const uint64_t mine = lane < n ? found[wave][lane] : 0;
+    if (lane < 8u) found[wave][n + lane] = 0;                    // (up to a multiple of eight)
+    if (lane == 0) n_found[wave] = n;
     float all = m;
 #pragma unroll
     for (int d = 32; d > 0; d >>= 1) all = fmaxf(all, __shfl_xor(all, d));
-    if ((tid & 63u) == 0) part_m[tid >> 6] = all;
+    if (lane == 0) part_m[wave] = all;
     __syncthreads();
     all = fmaxf(fmaxf(part_m[0], part_m[1]), fmaxf(part_m[2], part_m[3]));
     sum *= (double) exp_of(m - all);
 #pragma unroll
     for (int d = 32; d > 0; d >>= 1) sum += __shfl_xor(sum, d);
-    if ((tid & 63u) == 0) part_s[tid >> 6] = sum;
-    __syncthreads();
+    if (lane == 0) part_s[wave] = sum;
+    // what the waves found, in order: a key's rank is how many are larger
     const uint64_t at = (uint64_t) row * a.n_chunk + c;
+    uint32_t rank = 0, total = 0;
+#pragma unroll 1
+    for (uint32_t w = 0; w < WAVES; ++w) {
+        const uint32_t nw = n_found[w];
+        total += nw;
+        for (uint32_t i = 0; i < nw; i += 8) {                   // (in eights: the reads do not wait for each other)
+            uint64_t v[8];
+#pragma unroll
+            for (uint32_t e = 0; e < 8; ++e) v[e] = found[w][i + e];
+#pragma unroll
+            for (uint32_t e = 0; e < 8; ++e) rank += v[e] > mine;
+        }
+    }
+    if (mine != 0 && rank < a.n_pick) G_CAST(uint64_t, a.keys)[at * a.n_pick + rank] = mine;
+    if (tid >= total && tid < a.n_pick) G_CAST(uint64_t, a.keys)[at * a.n_pick + tid] = 0;
+    __syncthreads();
     if (tid == 0) {
         G_CAST(double, a.sums)[2 * at] = (double) all;
         G_CAST(double, a.sums)[2 * at + 1] = part_s[0] + part_s[1] + part_s[2] + part_s[3];
     }
-    if (tid < a.n_pick) G_CAST(uint64_t, a.keys)[at * a.n_pick + tid] = b.list[b.now][tid];
-}
-
-// How many of n keys in falling order are larger than k.
-__device__ __forceinline__ uint32_t larger(const uint64_t *keys, uint32_t n, uint64_t k) {
-    uint32_t lo = 0;
-    for (uint32_t hi = n; lo < hi;) {
-        const uint32_t mid = (lo + hi) / 2;
-        if (keys[mid] > k) lo = mid + 1;
-        else hi = mid;
-    }
-    return lo;
 }
 
 }  // namespace
@@ -1936,75 +2009,94 @@ BEAM(sllm_k_beam_f32, float)
 BEAM(sllm_k_beam_f16, _Float16)
 BEAM(sllm_k_beam_bf16, __bf16)
 
-// A group: each beam's parts joined (a key's rank is its place in its own part and how many are
-// larger in each other, which are in order), then its beams in the same way by their values in 64
-// bits. A beam that ended, or has no finite sum, is its token, and tokens from 0 on at -infinity.
+// A group: a wave joins a beam's parts (a lane a part, whose keys are in order: the largest of each, then
+// the second, until none can be among the first), then its beams' lists are joined by their
+// values in 64 bits. A beam that ended, or has no finite sum, is its token, and tokens from 0 on
+// at -infinity.
 extern "C" __global__ void __launch_bounds__(BEAM_JOIN_THREADS) sllm_k_beam_join(const att_beam_args a) {
-    __shared__ uint64_t keys[BEAM_MAX_KEYS];
+    constexpr uint32_t AHEAD = 4;
     __shared__ double value[BEAM_MAX_LIST];
     __shared__ uint32_t token[BEAM_MAX_LIST];
-    __shared__ double base[BEAM_MAX_BEAM], most[BEAM_MAX_BEAM];
-    const uint32_t tid = threadIdx.x, lane = tid & 63u, wave = tid >> 6, k = a.n_pick, row0 = blockIdx.x * a.n_beam;
+    const uint32_t tid = threadIdx.x, lane = tid & 63u, wave = uniform(tid >> 6), k = a.n_pick, row0 = blockIdx.x * a.n_beam;
     const uint32_t n_list = min(k, a.n_vocab);                   // of a beam
-    // what is added to a beam's logits less the largest: its score less the log of its sum
     for (uint32_t b = wave; b < a.n_beam; b += BEAM_JOIN_THREADS / 64) {
         const uint32_t row = row0 + b;
-        const float score = G_CAST(const float, a.scores)[row];
-        const bool live = !(a.ended && G_CAST(const int32_t, a.ended)[row] >= 0) && fabsf(score) <= -LOWEST;
-        double x = -INFINITY, m = (double) LOWEST;
-        if (live) {
-            GLOBAL const double *sums = G_CAST(const double, a.sums) + 2 * (uint64_t) row * a.n_chunk;
-            double s = 0.0;
-            for (uint32_t c = lane; c < a.n_chunk; c += 64) m = fmax(m, sums[2 * c]);
+        const float score = C_CAST(float, a.scores)[row];
+        const int32_t end = a.ended ? C_CAST(int32_t, a.ended)[row] : -1;
+        const bool fine = fabsf(score) <= -LOWEST, in = lane < a.n_chunk;
+        double m = (double) LOWEST, base = -INFINITY;
+        if (fine && end < 0) {
+            GLOBAL const double *sums = G_CAST(const double, a.sums) + 2 * ((uint64_t) row * a.n_chunk + lane);
+            GLOBAL const uint64_t *keys = G_CAST(const uint64_t, a.keys) + ((uint64_t) row * a.n_chunk + lane) * k;
+            // few keys: a lane each or two; else each part's first ones
+            const bool few = a.n_chunk * k <= 128u;
+            GLOBAL const uint64_t *all = G_CAST(const uint64_t, a.keys) + (uint64_t) row * a.n_chunk * k;
+            uint64_t ahead[AHEAD];
+            if (few) {
+#pragma unroll
+                for (uint32_t j = 0; j < 2; ++j) ahead[j] = lane + 64u * j < a.n_chunk * k ? all[lane + 64u * j] : 0;
+            } else {
+#pragma unroll
+                for (uint32_t j = 0; j < AHEAD; ++j) ahead[j] = in && j < k ? keys[j] : 0;
+            }
+            const double mine = in ? sums[0] : (double) LOWEST;
+            double s = in ? sums[1] : 0.0;
+            m = mine;
 #pragma unroll
             for (int d = 32; d > 0; d >>= 1) m = fmax(m, __shfl_xor(m, d));
-            for (uint32_t c = lane; c < a.n_chunk; c += 64) s += sums[2 * c + 1] * exp(sums[2 * c] - m);
+            s *= exp(mine - m);
 #pragma unroll
             for (int d = 32; d > 0; d >>= 1) s += __shfl_xor(s, d);
-            x = (double) score - log(s);
+            base = (double) score - log(s);
+            if (fabs(base) < INFINITY) {
+                wave_best best(k);
+                if (few) {
+                    const uint64_t bound = best.bound(ahead[0] > ahead[1] ? ahead[0] : ahead[1]);
+                    best.put(ahead[0] >= bound, ahead[0]);
+                    best.put(ahead[1] >= bound, ahead[1]);
+                    best.settle();
+                }
+                for (uint32_t j = 0; j < k && !few; j += AHEAD) {
+                    bool some = false;
+#pragma unroll 1
+                    for (uint32_t e = 0; e < AHEAD; ++e) {
+                        const uint64_t one = e == 0 ? ahead[0] : e == 1 ? ahead[1] : e == 2 ? ahead[2] : ahead[3];
+                        some = __any(one > best.least);
+                        if (!some) break;
+                        best.put(one >= best.bound(one), one);
+                        best.settle();
+                    }
+                    if (!some) break;
+#pragma unroll
+                    for (uint32_t e = 0; e < AHEAD; ++e) ahead[e] = in && j + AHEAD + e < k ? keys[j + AHEAD + e] : 0;
+                }
+                if (lane < n_list) {
+                    value[b * k + lane] = base + ((double) value_of(best.mine()) - m);
+                    token[b * k + lane] = ~best.lo;
+                }
+                continue;
+            }
         }
-        if (lane == 0) {
-            base[b] = x;
-            most[b] = m;
+        if (lane < n_list) {
+            const bool first = end >= 0 && fine;                 // its own token comes first
+            uint32_t t = lane;
+            if (first) t = lane == 0 ? (uint32_t) end : lane - 1 < (uint32_t) end ? lane - 1 : lane;
+            value[b * k + lane] = first && lane == 0 ? (double) score : -INFINITY;
+            token[b * k + lane] = t;
         }
     }
     __syncthreads();
-    const uint32_t per = a.n_chunk * k, at_once = BEAM_MAX_KEYS / per;
-    for (uint32_t b0 = 0; b0 < a.n_beam; b0 += at_once) {
-        const uint32_t nb = min(at_once, a.n_beam - b0);
-        for (uint32_t i = tid; i < nb * per; i += BEAM_JOIN_THREADS) {
-            if (fabs(base[b0 + i / per]) < INFINITY) keys[i] = G_CAST(const uint64_t, a.keys)[(uint64_t) (row0 + b0) * per + i];
-        }
-        __syncthreads();
-        for (uint32_t i = tid; i < nb * per; i += BEAM_JOIN_THREADS) {
-            const uint32_t b = b0 + i / per, c = i % per / k, place = i % k;
-            if (!(fabs(base[b]) < INFINITY)) {
-                if (c != 0 || place >= n_list) continue;
-                const int32_t end = a.ended ? G_CAST(const int32_t, a.ended)[row0 + b] : -1;
-                const float score = G_CAST(const float, a.scores)[row0 + b];
-                const bool first = end >= 0 && fabsf(score) <= -LOWEST;          // its own token comes first
-                uint32_t t = place;
-                if (first) t = place == 0 ? (uint32_t) end : place - 1 < (uint32_t) end ? place - 1 : place;
-                value[b * k + place] = first && place == 0 ? (double) score : -INFINITY;
-                token[b * k + place] = t;
-                continue;
-            }
-            const uint64_t key = keys[i];
-            if (key == 0) continue;
-            uint32_t rank = place;
-            for (uint32_t o = 0; o < a.n_chunk && rank < k; ++o) if (o != c) rank += larger(keys + i / per * per + o * k, k, key);
-            if (rank >= k) continue;
-            value[b * k + rank] = base[b] + ((double) value_of(key) - most[b]);
-            token[b * k + rank] = ~(uint32_t) key;
-        }
-        __syncthreads();
-    }
-    for (uint32_t i = tid; i < a.n_beam * k; i += BEAM_JOIN_THREADS) {
+    // a value's rank is its place and how many of each other beam's come first: of few values, the
+    // beams are shared out among `per` threads of each
+    const uint32_t n = a.n_beam * k;
+    uint32_t per = 1;
+    while (per < 64u && per < a.n_beam && 2u * per * n <= BEAM_JOIN_THREADS) per *= 2u;
+    for (uint32_t i = tid / per; i < n; i += BEAM_JOIN_THREADS / per) {
         const uint32_t b = i / k, place = i % k;
         if (place >= n_list) continue;
         const double x = value[i];
-        uint32_t rank = place;
-        for (uint32_t o = 0; o < a.n_beam && rank < k; ++o) {
+        uint32_t rank = 0;
+        for (uint32_t o = tid & (per - 1u); o < a.n_beam; o += per) {
             if (o == b) continue;
             uint32_t lo = 0;                                     // of a lower beam what is alike comes first too
             for (uint32_t hi = n_list; lo < hi;) {
@@ -2015,6 +2107,9 @@ extern "C" __global__ void __launch_bounds__(BEAM_JOIN_THREADS) sllm_k_beam_join
             }
             rank += lo;
         }
+        for (uint32_t d = 1; d < per; d *= 2u) rank += __shfl_xor(rank, (int) d);
+        rank += place;
+        if ((tid & (per - 1u)) != 0) continue;
         if (rank >= k) continue;
         const uint64_t at = (uint64_t) blockIdx.x * k + rank;
         G_CAST(float, a.out)[at] = (float) x;

@@ -136,9 +136,9 @@ typedef struct att_read_args {
 #define BEAM_MAX_PICK  64u
 #define BEAM_MAX_BEAM  64u
 #define BEAM_MAX_LIST  2048u         /* n_beam * n_pick */
-#define BEAM_MAX_KEYS  3072u         /* n_chunk * n_pick: a beam's keys in LDS */
+#define BEAM_MAX_PARTS 64u           /* of a row: a lane each in the join */
 #define BEAM_JOIN_THREADS 512u
-#define BEAM_VALUES    16u           /* of a thread at a time */
+#define BEAM_VALUES    8u            /* of a thread at a time */
 #define BEAM_TILE      (ATT_THREADS * BEAM_VALUES)
 typedef struct att_beam_args {
     const void    *logits;
