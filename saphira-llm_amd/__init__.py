@@ -15,6 +15,7 @@ from __future__ import annotations
 import array
 import ctypes
 import os
+import struct
 from ctypes import POINTER, c_char_p, c_double, c_float, c_int, c_int32, c_int64, c_size_t, c_uint, c_uint64, c_void_p
 
 import numpy as np
@@ -112,6 +113,10 @@ class RopeIO(ctypes.Structure):
     _fields_ = [(n, c_int32) for n in ("dtype", "n_rows", "n_head", "n_head_kv", "back")] + \
                [(n, c_void_p) for n in ("pos", "q", "k", "q_out", "k_out")] + \
                [(n, c_size_t) for n in ("q_stride", "q_out_stride", "k_stride", "k_out_stride")]
+
+
+# the same as bytes: a ctypes structure of so many fields takes longer to fill than the call
+_ROPE_IO = struct.Struct("@5i5P4N")
 
 
 # element types of a cache and of attention's rows (sllm_gfx950_attn.h); the last two of a cache alone
@@ -222,7 +227,7 @@ PROTOTYPES = {
     "sllm_gfx950_batch_read": (c_int, [c_void_p, c_int32, c_void_p, c_size_t, c_void_p, c_size_t]),
     "sllm_gfx950_rope_new": (c_int, [POINTER(RopeDesc), POINTER(c_void_p)]),
     "sllm_gfx950_rope_free": (None, [c_void_p]),
-    "sllm_gfx950_rope_rows": (c_int, [c_void_p, POINTER(RopeIO)]),
+    "sllm_gfx950_rope_rows": (c_int, [c_void_p, c_void_p]),
     "sllm_gfx950_batch_rope_store": (c_int, [c_void_p, c_int32, c_void_p, c_void_p, c_size_t, c_void_p, c_size_t, c_void_p, c_size_t,
                                              c_void_p, c_size_t]),
     "sllm_gfx950_beam_new": (c_int, [POINTER(BeamDesc), POINTER(c_void_p)]),
@@ -891,8 +896,8 @@ class Rope:
 
     def rows(self, dtype, pos, n_rows, q, n_head, q_out, k=None, n_head_kv=0, k_out=None, strides=(0, 0, 0, 0), back=False):
         """Device addresses; strides of q, q_out, k and k_out in elements, 0: packed."""
-        io = RopeIO(DTYPES[dtype], n_rows, n_head, n_head_kv, 1 if back else 0, pos, q, k, q_out, k_out, *strides)
-        check(lib().sllm_gfx950_rope_rows(self.r, ctypes.byref(io)), "rope_rows")
+        io = _ROPE_IO.pack(DTYPES[dtype], n_rows, n_head, n_head_kv, 1 if back else 0, pos or 0, q or 0, k or 0, q_out or 0, k_out or 0, *strides)
+        check(lib().sllm_gfx950_rope_rows(self.r, io), "rope_rows")
 
     def close(self):
         if self.r:
