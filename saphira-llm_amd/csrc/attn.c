@@ -800,6 +800,16 @@ static uint32_t seg_tiles(const segment *s, uint32_t group) {
     return (s->n_tok * group + k_rows[s->mode] - 1) / k_rows[s->mode];
 }
 
+/*
+ * 8 bits: where tiles of 128 rows have fewer keys than this a CU, they are made two of 64:
+ * twice the workgroups, but each key is turned into bf16 twice as often. us, 128 rows / 64, bf16
+ * rows over int8, 20 heads over 5 of 128: 64 sequences behind 4096 shared positions (160 keys a CU) 25.1 /
+ * 24.5, 6000 (234) 29.4 / 28.4, 8000 (312) 32.5 / 32.7, 11000 (430) 35.0 / 40.1, 16000 43.4 / 50.7; 128
+ * new positions behind 900 (70) 20.5 / 17.3, 4 times 512 behind 4000 88 / 112; drafts of 5 behind 1000, 32
+ * heads over 8 (150) 30.2 / 26.6.
+ */
+#define HELD8_HALF_KEYS 300u
+
 static uint32_t split_keys(const plan *x, uint32_t group, uint32_t n_head_kv, int many, uint32_t step) {
     uint64_t work = 0;
     for (int32_t i = 0; i < x->n_seg; ++i) {
@@ -902,13 +912,17 @@ static int lay_out(sllm_gfx950_batch *b, plan *x, int32_t n, const int32_t *len0
         x->common[i] = c;
     }
     if (x->n_order > 0) find_segments(x, 0, x->n_order, 0);
-    uint64_t n_list = 0;
+    uint64_t n_list = 0, many = 0;
     for (int32_t i = 0; i < x->n_seg; ++i) {
         segment *s = &x->seg[i];
         for (int32_t j = s->lo; j < s->hi; ++j) s->n_tok += (uint32_t) x->n_new[x->order[j]];
         s->list = ATT_TOKENS;
         if (s->hi - s->lo > 1) { s->list = (uint32_t) n_list; n_list += s->n_tok; }
         s->mode = mode_of(s->n_tok * group, p->d.dtype, b->act);
+        if (s->mode == ATT_MANY) many += (uint64_t) seg_tiles(s, group) * (uint64_t) s->n_keys * kv;
+    }
+    if (held8(p->d.dtype) && many < (uint64_t) sllm_shim_cu() * HELD8_HALF_KEYS) {
+        for (int32_t i = 0; i < x->n_seg; ++i) if (x->seg[i].mode == ATT_MANY) x->seg[i].mode = ATT_HALF;
     }
     /* segments of each sequence, and those with one part alone */
     uint32_t *seg_count = calloc((size_t) n + 1, sizeof *seg_count), *seg_at = calloc((size_t) n + 1, sizeof *seg_at);

@@ -1540,6 +1540,18 @@ __device__ __forceinline__ uint32_t codes_of(f32x4 x, uint32_t scale, bool i8) {
     return (uint32_t) __builtin_amdgcn_cvt_pk_fp8_f32(x[2] * by, x[3] * by, y, true);
 }
 
+// A lane's values of row h of a token's: queries, keys, values.
+template <typename A>
+__device__ __forceinline__ eight<A> row_of_token(const uint8_t *q, const uint8_t *k, const uint8_t *v, uint32_t h, uint32_t nq, uint32_t nk, uint32_t rows,
+                                                 uint32_t hd, uint32_t unit, uint32_t d0, uint32_t d1, bool in, bool whole) {
+    const bool is_q = h < nq, is_v = h >= nq + nk;
+    const uint8_t *src = is_q ? q : is_v ? v : k;
+    eight<A> x;
+    x.x[0] = x.x[1] = (f32x4) { 0, 0, 0, 0 };
+    if (h < rows && in) x.load(src + (uint64_t) (h - (is_q ? 0u : is_v ? nq + nk : nq)) * hd * sizeof(A), is_v ? 8u * unit : d0, is_v ? 8u * unit + 4u : d1, whole);
+    return x;
+}
+
 // A wave takes the heads of one token, four rows of up to 128 values at a time (eight of up
 // to 64), eight values a lane; cos and sin of a lane's four pairs are formed once for all of
 // them. So a token's rows are read and written once, and nothing crosses lanes but a row's
@@ -1554,7 +1566,20 @@ __device__ __forceinline__ void rows_body(const att_rows_args &a) {
     const bool in = unit < a.hd / 8u, turned = unit < a.half / 4u, whole = a.pairs != 0 || a.half == 0;
     // the dimensions of the lane's values, of rows that turn
     const uint32_t d0 = turned && !whole ? 4u * unit : 8u * unit, d1 = turned && !whole ? a.half + 4u * unit : 8u * unit + 4u;
-    const int32_t pos = a.toks ? (int32_t) a.toks[tok].pos : a.pos ? a.pos[tok] : 0;
+    const int32_t pos = a.toks ? C_CAST(int32_t, &a.toks[tok].pos)[0] : a.pos ? C_CAST(int32_t, a.pos)[tok] : 0;
+    uint64_t place = 0;                                          // the token's row of KV head 0 in the cache
+    uint32_t slot = 0;
+    if (a.ck) {
+        slot = (uint32_t) pos & ((1u << a.page_shift) - 1u);
+        place = C_CAST(uint32_t, a.tables)[C_CAST(uint32_t, &a.toks[tok].table)[0] + ((uint32_t) pos >> a.page_shift)] * a.page_bytes;
+    }
+    const bool held8 = a.held >= ATT_HELD_I8;
+    // (copies: a choice between two of the arguments would put them all into scratch memory)
+    const uint8_t *q = (const uint8_t *) a.q + tok * a.q_tok, *k = (const uint8_t *) a.k + tok * a.k_tok, *v = (const uint8_t *) a.v + tok * a.v_tok;
+    uint8_t *qo = (uint8_t *) a.q_out + tok * a.qo_tok, *ko = (uint8_t *) a.k_out + tok * a.ko_tok, *ck = a.ck + place, *cv = a.cv + place;
+    const uint32_t nq = a.q ? a.n_head : 0u, nk = a.k ? a.n_head_kv : 0u, nv = a.v ? a.n_head_kv : 0u, rows = nq + nk + nv;
+    // (the next rows are on their way while some are worked on, the first while the angles are)
+    eight<A> next = row_of_token<A>(q, k, v, part * at_once + lane / per, nq, nk, rows, a.hd, unit, d0, d1, in, whole);
     float c[4] = { 1.0f, 1.0f, 1.0f, 1.0f }, s[4] = {};
     if (turned && in) {
 #pragma unroll
@@ -1565,28 +1590,15 @@ __device__ __forceinline__ void rows_body(const att_rows_args &a) {
             s[j] *= a.back ? -a.magnitude : a.magnitude;
         }
     }
-    uint64_t place = 0;                                          // the token's row of KV head 0 in the cache
-    uint32_t slot = 0;
-    if (a.ck) {
-        slot = (uint32_t) pos & ((1u << a.page_shift) - 1u);
-        place = a.tables[a.toks[tok].table + ((uint32_t) pos >> a.page_shift)] * a.page_bytes;
-    }
-    const bool held8 = a.held >= ATT_HELD_I8;
-    // (copies: a choice between two of the arguments would put them all into scratch memory)
-    const uint8_t *q = (const uint8_t *) a.q + tok * a.q_tok, *k = (const uint8_t *) a.k + tok * a.k_tok, *v = (const uint8_t *) a.v + tok * a.v_tok;
-    uint8_t *qo = (uint8_t *) a.q_out + tok * a.qo_tok, *ko = (uint8_t *) a.k_out + tok * a.ko_tok, *ck = a.ck + place, *cv = a.cv + place;
-    const uint32_t nq = a.q ? a.n_head : 0u, nk = a.k ? a.n_head_kv : 0u, nv = a.v ? a.n_head_kv : 0u, rows = nq + nk + nv;
     for (uint32_t r = part * at_once; r < rows; r += a.waves * at_once) {
         uint32_t h = r + lane / per;
         const bool here = h < rows && in;
         const bool is_q = h < nq, is_v = h >= nq + nk;
-        const uint8_t *src = is_q ? q : is_v ? v : k;
         h -= is_q ? 0u : is_v ? nq + nk : nq;
-        // (values have the same places as keys where rows turn by halves: what is written is the row)
+        // (values are not turned: a lane's are side by side)
         const uint32_t e0 = is_v ? 8u * unit : d0, e1 = is_v ? 8u * unit + 4u : d1;
-        eight<A> x;
-        x.x[0] = x.x[1] = (f32x4) { 0, 0, 0, 0 };
-        if (here) x.load(src + (uint64_t) h * a.hd * sizeof(A), e0, e1, whole);
+        eight<A> x = next;
+        next = row_of_token<A>(q, k, v, r + a.waves * at_once + lane / per, nq, nk, rows, a.hd, unit, d0, d1, in, whole);
         if (turned && !is_v) {
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
@@ -1648,6 +1660,7 @@ namespace {
 template <typename A>
 __device__ __forceinline__ void read_body(const att_read_args &a) {
     const uint32_t lane = threadIdx.x & 63u, entry = blockIdx.x;
+    const uint64_t page = (uint64_t) C_CAST(uint32_t, a.tables)[entry] * a.page_bytes;
     uint32_t lo = 0, n = a.n_seq;                                // the last of n sequences from lo on whose pages start at or before it
     while (n > 1) {
         const uint32_t step = (n + 63u) / 64u, at = lo + lane * step;
@@ -1660,7 +1673,6 @@ __device__ __forceinline__ void read_body(const att_read_args &a) {
     const uint32_t first = C_CAST(uint32_t, &a.seqs[lo].table)[0], row0 = C_CAST(uint32_t, &a.seqs[lo].row0)[0];
     const uint32_t end = C_CAST(uint32_t, &a.seqs[lo + 1].row0)[0], start = row0 + ((entry - first) << a.page_shift);
     const uint32_t page_rows = 1u << a.page_shift, n_rows = min(end - start, page_rows);
-    const uint64_t page = (uint64_t) C_CAST(uint32_t, a.tables)[entry] * a.page_bytes;
     const uint32_t per = a.hd / 8u, per_block = n_rows * per, all = per_block * 2u * a.n_head_kv;
     const uint32_t base = blockIdx.y * (ATT_THREADS * ATT_READ_UNITS) + threadIdx.x;
 #pragma unroll
