@@ -1190,7 +1190,7 @@ static int overlap(const rows_at *a, const rows_at *b) {
 }
 
 /* waves of a CU that rows are spread over before a wave takes more of a token's */
-#define ROWS_WAVES 16u
+#define ROWS_WAVES 32u
 
 /* Rows on their way (att_rows_args): a token's heads are gone through by one wave, or where
  * there are few tokens by several. */

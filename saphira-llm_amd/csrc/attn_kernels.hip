@@ -442,14 +442,14 @@ struct attention {
         const __amdgpu_buffer_rsrc_t rv = __builtin_amdgcn_make_buffer_rsrc((void *) v, (short) 0, (int) uniform(n * a.hd), 0x00020000);
         const __amdgpu_buffer_rsrc_t sk = __builtin_amdgcn_make_buffer_rsrc((void *) (m.k + scales), (short) 0, (int) uniform(n), 0x00020000);
         const __amdgpu_buffer_rsrc_t sv = __builtin_amdgcn_make_buffer_rsrc((void *) (m.v + scales), (short) 0, (int) uniform(n), 0x00020000);
-        constexpr int KEEP = KEYS ? KEPT : 0;
+        constexpr int KEEP = KEYS ? KEPT : 0;                    // (of scales a line is of several tiles: kept, 59.4 -> 58.0 us)
 #pragma unroll
         for (int j = 0; j < (KEYS ? KL : 1); ++j) x.k[j] = __builtin_amdgcn_raw_buffer_load_b128(rk, kcopy[j], 0, KEEP);
-        x.ks = __builtin_amdgcn_raw_buffer_load_b8(sk, krow, 0, KEEP);
+        x.ks = __builtin_amdgcn_raw_buffer_load_b8(sk, krow, 0, 0);
 #pragma unroll
         for (int j = 0; j < CL; ++j) {
             x.v[j] = __builtin_amdgcn_raw_buffer_load_b128(rv, vcopy[j], 0, KEEP);
-            x.vs[j] = __builtin_amdgcn_raw_buffer_load_b8(sv, vrow[j], 0, KEEP);
+            x.vs[j] = __builtin_amdgcn_raw_buffer_load_b8(sv, vrow[j], 0, 0);
         }
     }
     // sixteen codes as two pieces of T
