@@ -479,11 +479,15 @@ struct attention {
             for (int e = 0; e < 2; ++e) *reinterpret_cast<u32x4 *>(S + to + vput2[j][e]) = y.p[e];
         }
     }
-    codes c8[HELD8 && KEYS ? GROUPS : 1];
+    // Tiles whose rows are in registers (not KEYS): two where 128 rows of bf16 leave room for
+    // them: 64 sequences behind 16000 shared positions 43.2 -> 41.7 us, 4 times 512 new positions behind 4000
+    // 88.4 -> 85.5; with 64 rows, and with f16's or f32's more registers, one was 1 to 3 % faster.
+    static constexpr int SETS = NT == 2 && PIECES == 1 ? 2 : 1;
+    codes c8[HELD8 ? (KEYS ? GROUPS : SETS) : 1];
     // not KEYS, 8 bits: this wave's rows of a tile set off
-    __device__ __forceinline__ void issue8(uint32_t t) {
+    template <int B> __device__ __forceinline__ void issue8(uint32_t t) {
         const uint32_t key = t * KT + wave * (uint32_t) GROUP;
-        fetch8(c8[0], rows_at(key), key);
+        fetch8(c8[B], rows_at(key), key);
     }
 
     // not KEYS: this wave's rows of a tile into the stage at `to`
@@ -762,6 +766,7 @@ struct attention {
         const uint32_t t = first_tile();
         if constexpr (HELD8) {
             set_off(t);
+            if constexpr (!KEYS && SETS == 2) issue8<SETS - 1>(t + 1);
         } else if constexpr (KEYS) {
             fetch(x, spans(t), t);
         } else {
@@ -775,7 +780,7 @@ struct attention {
 #pragma unroll
             for (int gr = 0; gr < GROUPS; ++gr) fetch8(c8[gr], rows_at(t * KT + (uint32_t) gr * GROUP), t * KT + (uint32_t) gr * GROUP);
         } else {
-            issue8(t);
+            issue8<0>(t);
         }
     }
 
@@ -945,15 +950,40 @@ struct attention {
         __builtin_amdgcn_s_barrier();
         __builtin_amdgcn_sched_barrier(0);
     }
+    // Tile t + n: the one two further comes out of registers into LDS, and the next into them.
+    template <int B>
+    __device__ __forceinline__ void step8(scores &s, scores &next, probs &p, float (&f)[NT], bool &moved, uint32_t t, uint32_t n) {
+        if (moved) rescale(f);
+        meet8();
+        values v;
+        values_of(v, stage((n - 1) & 3u));
+        land(c8[B], stage((n + 2) & 3u));
+        issue8<B>(t + n + 2 + SETS);
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks) {
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) s[ks][nt] = next[ks][nt];
+        }
+        mask(s, (t + n) * KT);
+        moved = adjust(s, f);
+        __builtin_amdgcn_sched_barrier(0);
+        probs q;
+        scores_of<false>(next, stage((n + 1) & 3u));
+        products<false>(v, p, (t + n - 1) * KT, stage((n - 1) & 3u));
+        soften(s, q);
+        p = q;
+    }
     __device__ __forceinline__ void pass8(const uint32_t t, const uint32_t t1) {
         scores s, next;
         probs p;
         float f[NT];
-#pragma unroll
-        for (uint32_t i = 0; i < 3; ++i) {                       // (a tile past the end is zeros)
-            land(c8[0], stage(i));
-            issue8(t + i + 1);
-        }
+        constexpr int ODD = SETS - 1;                            // the registers of odd tiles
+        land(c8[0], stage(0));                                   // (a tile past the end is zeros)
+        issue8<0>(t + SETS);
+        land(c8[ODD], stage(1));
+        issue8<ODD>(t + 1 + SETS);
+        land(c8[0], stage(2));
+        issue8<0>(t + 2 + SETS);
         meet8();
         scores_of<false>(s, stage(0));
         scores_of<false>(next, stage(1));
@@ -961,27 +991,13 @@ struct attention {
         bool moved = adjust(s, f);
         soften(s, p);
         uint32_t n = 1;                                          // tile t + n's scores are `next`
-        for (; t + n < t1; ++n) {
-            if (moved) rescale(f);
-            meet8();
-            values v;
-            values_of(v, stage((n - 1) & 3u));
-            land(c8[0], stage((n + 2) & 3u));
-            issue8(t + n + 3);
-#pragma unroll
-            for (int ks = 0; ks < KS; ++ks) {
-#pragma unroll
-                for (int nt = 0; nt < NT; ++nt) s[ks][nt] = next[ks][nt];
+        if constexpr (SETS == 2) {
+            for (; t + n + 1 < t1; n += 2) {
+                step8<ODD>(s, next, p, f, moved, t, n);
+                step8<0>(s, next, p, f, moved, t, n + 1);
             }
-            mask(s, (t + n) * KT);
-            moved = adjust(s, f);
-            __builtin_amdgcn_sched_barrier(0);
-            probs q;
-            scores_of<false>(next, stage((n + 1) & 3u));
-            products<false>(v, p, (t + n - 1) * KT, stage((n - 1) & 3u));
-            soften(s, q);
-            p = q;
         }
+        for (; t + n < t1; ++n) step8<ODD>(s, next, p, f, moved, t, n);
         if (moved) rescale(f);
         values v;
         values_of(v, stage((n - 1) & 3u));
