@@ -1890,7 +1890,8 @@ template <typename T> __device__ __forceinline__ void beam_body(const att_beam_a
     double sum = 0.0;
     // the waves with tiles, and which of a wave's largest it tells, from 0 on
     const uint32_t n_waves = min((uint32_t) WAVES, (last - c * a.chunk + TILE - 1u) / TILE), q = (a.n_pick - 1u) / n_waves;
-    // what was found is put in order and given up, and what is alike the last of n_pick or below is not found again
+    // what was found is put in order and given up, and what is below the last of n_pick is not found
+    // again (what is alike may yet have a lower token: a lane's are not side by side)
     auto order = [&]() {
 #pragma unroll 1
         for (uint32_t i = 0; i < n; i += 64u) {
@@ -1900,7 +1901,7 @@ template <typename T> __device__ __forceinline__ void beam_body(const att_beam_a
         }
         __builtin_amdgcn_wave_barrier();
         n = 0;
-        if (best.least != 0) least = fmaxf(least, value_of(((best.least >> 32) + 1u) << 32));
+        if (best.least != 0) least = fmaxf(least, value_of(best.least));
     };
     // what was kept and is not below `least`, as keys: eight lanes' values at a time
     auto sift = [&]() {
@@ -1980,7 +1981,11 @@ template <typename T> __device__ __forceinline__ void beam_body(const att_beam_a
             n_kept += (uint32_t) __popcll(who);
             __builtin_amdgcn_wave_barrier();
         }
-        if (n_kept > 64u) sift();
+        if (n_kept > 64u) {
+            sift();
+            // tokens rise from here on: what is alike the last comes behind it
+            if (best.least != 0) least = fmaxf(least, value_of(((best.least >> 32) + 1u) << 32));
+        }
     }
     if (first >= last) {                                         // (a wave without a tile)
         if (lane == 0) told[wave] = INFINITY;

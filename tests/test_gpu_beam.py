@@ -131,6 +131,26 @@ def test_orders_that_keep_the_list_moving(amd, dev, dtype, order, vocab):
 
 
 @pytest.mark.parametrize("dtype", list(ora.TYPES))
+@pytest.mark.parametrize("picks", [1, 7, 33, 64])
+@pytest.mark.parametrize("seed", range(6))
+def test_few_values_many_ties(amd, dev, dtype, picks, seed):
+    """Values from a handful, in runs of every length: which of those that are alike are
+    among the picks is the token's alone, however a wave comes by them."""
+    r = np.random.default_rng(seed)
+    x = torch.zeros(2, 2, 6000)
+    for g in range(2):
+        for b in range(2):
+            at = 0
+            while at < 6000:
+                n = int(r.choice([1, 4, 8, 31, 64, 128, 300]))
+                x[g, b, at:at + n] = float(r.choice([0.0, 0.0, 1.0, 1.0, 2.0] if seed % 2 else [0.0, 0.0, 0.0, 0.0, 3.0]))
+                at += n
+    x[0, 0, :] = 0
+    x[0, 0, 256:320], x[0, 0, 64:128] = 5.0, 5.0
+    check(amd, dev, x, [[-1.0, -30.0], [-1.0, -1.5]], picks, dtype)
+
+
+@pytest.mark.parametrize("dtype", list(ora.TYPES))
 @pytest.mark.parametrize("vocab", [1001, 9000])
 def test_beams_that_are_alike(amd, dev, dtype, vocab):
     """The same logits and scores: the lower beam first, wherever its row lies in memory."""
