@@ -177,7 +177,8 @@ int  sllm_gfx950_batch_store(sllm_gfx950_batch *b, int32_t layer, const void *k,
  * The keys and values of a layer read back as rows of act_dtype, every position of
  * the batch's sequences, old and new, sequence by sequence: k, v [batch_positions][n_head_kv]
  * [head_dim], strides as above. Rounded to nearest where act_dtype holds less (f16 of 8 bits).
- * k and v overlap neither each other nor the cache. At most SLLM_GFX950_ATTN_MAX_LEN positions.
+ * k and v overlap neither each other nor the cache. At most SLLM_GFX950_ATTN_MAX_LEN positions
+ * and 2^23 pages, a shared page once for each sequence.
  */
 int64_t sllm_gfx950_batch_positions(const sllm_gfx950_batch *b);
 int  sllm_gfx950_batch_read(sllm_gfx950_batch *b, int32_t layer, void *k, size_t k_stride, void *v, size_t v_stride);
@@ -205,8 +206,9 @@ int  sllm_gfx950_batch_attend(sllm_gfx950_batch *b, int32_t layer, const void *q
  *   PARTS   with turns = original * frequency / (2 pi): as it is from `fast` turns on,
  *           divided by factor below `slow`, and between them in proportion
  *
- * Angles are exact to 2^-30 of a turn at any position of 32 bits; rows are computed in f32
- * and rounded once.
+ * Angles are exact to 2^-30 of a turn at any position of 32 bits (of frequencies over a turn a
+ * position to as many times that; over 2^20 radians they are refused); rows are computed in f32 and
+ * rounded once.
  */
 enum { SLLM_GFX950_ROPE_HALVES, SLLM_GFX950_ROPE_PAIRS };
 enum { SLLM_GFX950_ROPE_PLAIN, SLLM_GFX950_ROPE_LINEAR, SLLM_GFX950_ROPE_NTK, SLLM_GFX950_ROPE_PARTS };

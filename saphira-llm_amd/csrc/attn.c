@@ -1506,7 +1506,7 @@ static int rope_turns(const sllm_gfx950_rope_desc *d, uint64_t *to) {
             keep = keep < 0 ? 0 : keep > 1 ? 1 : keep;
             f = f * keep + f / d->factor * (1 - keep);
         }
-        if (!isfinite(f)) return 0;
+        if (!(fabsl(f) <= 1048576.0L)) return 0;
         long double t = f / two_pi;
         t -= floorl(t);
         t = ldexpl(t, 64);
@@ -1523,7 +1523,7 @@ int sllm_gfx950_rope_new(const sllm_gfx950_rope_desc *d, sllm_gfx950_rope **out)
         (d->layout != SLLM_GFX950_ROPE_HALVES && d->layout != SLLM_GFX950_ROPE_PAIRS)) {
         return FAIL_ARG("rope_new: head dimension, dimensions that turn, or their layout");
     }
-    if (d->scaling < SLLM_GFX950_ROPE_PLAIN || d->scaling > SLLM_GFX950_ROPE_PARTS || !isfinite(d->magnitude) ||
+    if (d->scaling < SLLM_GFX950_ROPE_PLAIN || d->scaling > SLLM_GFX950_ROPE_PARTS || !isfinite((float) d->magnitude) ||
         (d->freq == NULL && !(d->base > 0 && isfinite(d->base))) ||
         (d->scaling != SLLM_GFX950_ROPE_PLAIN && !(d->factor > 0 && isfinite(d->factor))) || (d->scaling == SLLM_GFX950_ROPE_NTK && d->freq != NULL) ||
         (d->scaling == SLLM_GFX950_ROPE_PARTS && !(d->original > 0 && isfinite(d->original) && isfinite(d->slow) && d->fast > d->slow && isfinite(d->fast)))) {
@@ -1532,7 +1532,7 @@ int sllm_gfx950_rope_new(const sllm_gfx950_rope_desc *d, sllm_gfx950_rope **out)
     int st = not_in_capture("rope_new");
     if (st != SLLM_GFX950_OK) return st;
     uint64_t turns[SLLM_GFX950_ATTN_MAX_HEAD_DIM / 2];
-    if (!rope_turns(d, turns)) return FAIL_ARG("rope_new: a frequency that is not finite");
+    if (!rope_turns(d, turns)) return FAIL_ARG("rope_new: a frequency over 2^20 or not finite");
     sllm_gfx950_rope *r = calloc(1, sizeof *r);
     if (r == NULL) return FAIL_NOMEM("rope_new");
     r->head_dim = d->head_dim;

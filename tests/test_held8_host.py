@@ -115,7 +115,7 @@ def new_rope(amd, L, **how):
                                  dict(base=float("nan")), dict(base=float("inf")), dict(scaling=1), dict(scaling=1, factor=-2.0),
                                  dict(scaling=2, factor=float("inf")), dict(scaling=3, factor=2.0), dict(scaling=3, factor=2.0, original=8.0, fast=1.0, slow=1.0),
                                  dict(scaling=3, factor=2.0, original=float("nan"), fast=2.0, slow=1.0), dict(magnitude=float("inf")),
-                                 dict(magnitude=float("nan"))])
+                                 dict(magnitude=float("nan")), dict(magnitude=1e39), dict(scaling=1, factor=1e-7)])
 def test_ropes_that_are_refused(amd, L, how):
     r, live = c_void_p(1), L.fakehip_live()
     d = rope_desc(amd, **how)
@@ -133,8 +133,9 @@ def test_more_ropes_that_are_refused(amd, L):
     L.sllm_gfx950_rope_free(r)
     ntk = rope_desc(amd, freq=f.ctypes.data, scaling=2, factor=2.0)
     assert L.sllm_gfx950_rope_new(byref(ntk), byref(r)) == ARG
-    f[7] = np.inf
-    assert L.sllm_gfx950_rope_new(byref(ok), byref(r)) == ARG
+    for bad in (np.inf, -np.inf, np.nan, 2.0 ** 20 * 1.0001, -1e300):
+        f[7] = bad
+        assert L.sllm_gfx950_rope_new(byref(ok), byref(r)) == ARG
     L.fakehip_capture(1)
     assert L.sllm_gfx950_rope_new(byref(d), byref(r)) == ARG
     L.fakehip_capture(0)
@@ -281,6 +282,51 @@ def test_reordered_pages_against_a_model(amd, L, seed):
                 tables[i].append(room.pop(0))
         assert c.state(ids) == (len({x for t in tables for x in t}), list(zip(lens, tables)))
     c.close()
+
+
+def test_another_device_is_current(amd, L):
+    """Memory is taken and kernels run on the library's device, and the caller's is current again."""
+    mem = (ctypes.c_uint8 * (1 << 17))()
+    at = ctypes.addressof(mem) + (-ctypes.addressof(mem)) % 16
+    L.fakehip_current(1)
+    c = Cache(amd, L, dtype=I8)
+    ids = [c.new(), c.new()]
+    c.grow(ids, [20, 5])
+    b = c.batch(ids, [1, 1])
+    r = new_rope(amd, L)
+    io = amd.RopeIO(F32, 4, 4, 2, 0, at, at + 4096, None, at + 16384, None, 0, 0, 0, 0)
+    p = c_void_p()
+    d = amd.BeamDesc(1, 2, 100, 4, F32)
+    L.fakehip_clear()
+    assert L.sllm_gfx950_rope_rows(r, byref(io)) == 0
+    assert L.sllm_gfx950_batch_rope_store(b, 0, r, at, 0, at, 0, at + 16384, 0, at + 32768, 0) == 0
+    assert L.sllm_gfx950_batch_store(b, 0, at, 0, at, 0) == 0 and L.sllm_gfx950_batch_read(b, 0, at, 0, at + 65536, 0) == 0
+    assert L.sllm_gfx950_seq_reorder(c.p, I(*ids), I(0, 0), 2) == 0
+    assert L.sllm_gfx950_beam_new(byref(d), byref(p)) == 0
+    assert L.sllm_gfx950_beam_select(p, at, 0, at + 8192, None, at + 9216, at + 10240, at + 11264) == 0
+    assert len(L.fakehip_launches().split()) == 7
+    L.sllm_gfx950_beam_free(p)
+    L.sllm_gfx950_rope_free(r)
+    L.sllm_gfx950_batch_destroy(b)
+    c.close()
+    L.fakehip_current(0)
+
+
+def test_what_ends_in_a_capture(amd, L):
+    """Ropes and beams' plans that end while the stream is captured keep their memory until a call
+    that may wait; the capture is not broken."""
+    L.fakehip_broken.restype = ctypes.c_int
+    r, p = new_rope(amd, L), c_void_p()
+    d = amd.BeamDesc(1, 2, 100, 4, F32)
+    assert L.sllm_gfx950_beam_new(byref(d), byref(p)) == 0
+    live, broken = L.fakehip_live(), L.fakehip_broken()
+    L.fakehip_capture(1)
+    L.sllm_gfx950_rope_free(r)
+    L.sllm_gfx950_beam_free(p)
+    assert L.fakehip_live() == live and L.fakehip_broken() == broken
+    L.fakehip_capture(0)
+    L.sllm_gfx950_rope_free(new_rope(amd, L))
+    assert L.fakehip_live() == live - 2
 
 
 def test_every_hip_call_fails_once(amd, L):
