@@ -1813,6 +1813,19 @@ struct wave_best {
     __device__ __forceinline__ void settle() {
         least = place(n_pick - 1);
     }
+    // A first key of each lane (0: none), in order: a key's lane is how many are larger.
+    __device__ __forceinline__ void start(uint64_t key) {
+        const uint32_t h = (uint32_t) (key >> 32), l = (uint32_t) key;
+        uint32_t rank = 0;
+#pragma unroll
+        for (int i = 0; i < 64; ++i) {
+            rank += ((uint64_t) (uint32_t) __builtin_amdgcn_readlane((int) h, i) << 32 | (uint32_t) __builtin_amdgcn_readlane((int) l, i)) > key;
+        }
+        // (those that are none all go behind the others; no lane's is none too)
+        hi = (uint32_t) __builtin_amdgcn_ds_permute((int) (rank * 4u), (int) h);
+        lo = (uint32_t) __builtin_amdgcn_ds_permute((int) (rank * 4u), (int) l);
+        settle();
+    }
     // What the keys of lanes with these largest ones have to reach to be among the first. Where
     // more lanes than picks have one above the list's last, the n_pick-th largest of them bounds the rest
     // from below, so that few are put in, in whatever order the values come.
@@ -2054,26 +2067,22 @@ extern "C" __global__ void __launch_bounds__(BEAM_JOIN_THREADS) sllm_k_beam_join
     const uint32_t n_list = min(k, a.n_vocab);                   // of a beam
     for (uint32_t b = wave; b < a.n_beam; b += BEAM_JOIN_THREADS / 64) {
         const uint32_t row = row0 + b;
+        // no more keys than lanes: one each; else each part's first ones. (Asked for before it is
+        // known whether the beam has any.)
+        const bool few = a.n_chunk * k <= 64u, in = lane < a.n_chunk;
+        GLOBAL const double *sums = G_CAST(const double, a.sums) + 2 * ((uint64_t) row * a.n_chunk + lane);
+        GLOBAL const uint64_t *keys = G_CAST(const uint64_t, a.keys) + ((uint64_t) row * a.n_chunk + lane) * k;
+        uint64_t ahead[AHEAD];
+#pragma unroll
+        for (uint32_t j = 0; j < AHEAD; ++j) ahead[j] = in && j < k && !few ? keys[j] : 0;
+        if (few && lane < a.n_chunk * k) ahead[0] = G_CAST(const uint64_t, a.keys)[(uint64_t) row * a.n_chunk * k + lane];
+        const double mine = in ? sums[0] : (double) LOWEST;
+        double s = in ? sums[1] : 0.0;
         const float score = C_CAST(float, a.scores)[row];
         const int32_t end = a.ended ? C_CAST(int32_t, a.ended)[row] : -1;
-        const bool fine = fabsf(score) <= -LOWEST, in = lane < a.n_chunk;
+        const bool fine = fabsf(score) <= -LOWEST;
         double m = (double) LOWEST, base = -INFINITY;
         if (fine && end < 0) {
-            GLOBAL const double *sums = G_CAST(const double, a.sums) + 2 * ((uint64_t) row * a.n_chunk + lane);
-            GLOBAL const uint64_t *keys = G_CAST(const uint64_t, a.keys) + ((uint64_t) row * a.n_chunk + lane) * k;
-            // few keys: a lane each or two; else each part's first ones
-            const bool few = a.n_chunk * k <= 128u;
-            GLOBAL const uint64_t *all = G_CAST(const uint64_t, a.keys) + (uint64_t) row * a.n_chunk * k;
-            uint64_t ahead[AHEAD];
-            if (few) {
-#pragma unroll
-                for (uint32_t j = 0; j < 2; ++j) ahead[j] = lane + 64u * j < a.n_chunk * k ? all[lane + 64u * j] : 0;
-            } else {
-#pragma unroll
-                for (uint32_t j = 0; j < AHEAD; ++j) ahead[j] = in && j < k ? keys[j] : 0;
-            }
-            const double mine = in ? sums[0] : (double) LOWEST;
-            double s = in ? sums[1] : 0.0;
             m = mine;
 #pragma unroll
             for (int d = 32; d > 0; d >>= 1) m = fmax(m, __shfl_xor(m, d));
@@ -2083,16 +2092,11 @@ extern "C" __global__ void __launch_bounds__(BEAM_JOIN_THREADS) sllm_k_beam_join
             base = (double) score - log(s);
             if (fabs(base) < INFINITY) {
                 wave_best best(k);
-                if (few) {
-                    const uint64_t bound = best.bound(ahead[0] > ahead[1] ? ahead[0] : ahead[1]);
-                    best.put(ahead[0] >= bound, ahead[0]);
-                    best.put(ahead[1] >= bound, ahead[1]);
-                    best.settle();
-                }
+                best.start(ahead[0]);
                 for (uint32_t j = 0; j < k && !few; j += AHEAD) {
                     bool some = false;
 #pragma unroll 1
-                    for (uint32_t e = 0; e < AHEAD; ++e) {
+                    for (uint32_t e = j == 0 ? 1u : 0u; e < AHEAD; ++e) {
                         const uint64_t one = e == 0 ? ahead[0] : e == 1 ? ahead[1] : e == 2 ? ahead[2] : ahead[3];
                         some = __any(one > best.least);
                         if (!some) break;
