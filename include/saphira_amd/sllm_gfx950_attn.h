@@ -1,6 +1,7 @@
 /*
- * sllm_gfx950_attn.h -- attention for many sequences on MI355X: a paged cache,
- * a step's attention over it, and causal attention over packed prompts.
+ * sllm_gfx950_attn.h -- attention for many sequences on MI355X: a paged cache, plain
+ * or in 8 bits, a step's attention over it, rotary positions, causal attention over packed
+ * prompts, and the selection of beams.
  *
  * Device operators beside the projections of sllm_gfx950.h: they take device
  * pointers, enqueue on the library's stream (sllm_gfx950_stream) and return a
@@ -25,10 +26,10 @@
  * one stream. Memory that another stream writes or reads is the caller's to
  * order with the library's stream.
  *
- * batch_store, batch_attend and prompt_attend are launches alone and may be
- * captured into a graph. What takes pages or lays out work (batch_create,
- * seq_fork, seq_copy, pages_compact, prompt_create) is refused while the stream
- * is captured. What is freed or destroyed during a capture keeps its memory until
+ * batch_store, batch_rope_store, batch_read, batch_attend, rope_rows, prompt_attend
+ * and beam_select are launches alone and may be captured into a graph. What takes pages
+ * or lays out work (batch_create, seq_fork, seq_copy, seq_reorder, pages_compact, rope_new,
+ * prompt_create, beam_new) is refused while the stream is captured. What is freed or destroyed during a capture keeps its memory until
  * a later call can wait for the stream; the capture goes on.
  */
 #ifndef SAPHIRA_AMD_SLLM_GFX950_ATTN_H

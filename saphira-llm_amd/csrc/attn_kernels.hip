@@ -1,5 +1,6 @@
-// attn_kernels.hip -- attention over a paged cache and over packed prompts, and
-// the cache's copies (sllm_gfx950_attn.h), for gfx950.
+// attn_kernels.hip -- attention over a paged cache and over packed prompts, the
+// cache's copies, rows on their way into and out of it, and the selection of beams
+// (sllm_gfx950_attn.h), for gfx950.
 //
 // Attention of a row: out = sum_j p_j v_j / sum_j p_j, p_j = 2^(c (s_j - m)),
 // s_j = q . k_j, c = scale log2(e), m a running maximum of s. One pass over the
@@ -1232,7 +1233,15 @@ __device__ __forceinline__ void paged_body(const att_args &a) {
     else attend_item<A, T, D, 2, false, true>(a, it, S);
 }
 
-// The same over 8 bits. (Queries of f32 take three times the registers: no 32 rows a wave.)
+// The same over 8 bits: codes come into registers, half the bytes of bf16, and are turned into bf16
+// there: for few rows right before the products, else once for a workgroup on the way to LDS. A
+// scale is a power of two, so nothing is rounded and no score or weight is multiplied by it. What
+// that costs the vector unit, 2.75 instructions a value of int8 and half of one of e4m3, memory hides
+// for few rows: 8 sequences of up to 65536 positions, e4m3 under bf16, 317 MB in 58.2 us with the join,
+// 5.4 TB/s (without the loads of scales it would be 56.4). Many rows are bound as over bf16: 64
+// sequences behind 4096 shared positions, int8, 23.5 us; one of 1101 positions, f32 rows, 9.2 us, two
+// launches. Two tiles of few rows on their way at a time: 57.9 us for 58.6, but 26.8 for 26.0 behind a shared
+// prefix. (Queries of f32 take three times the registers: no 32 rows a wave.)
 template <typename A, typename C, int D>
 __device__ __forceinline__ void held8_body(const att_args &a) {
     __shared__ __attribute__((aligned(1024))) uint8_t S[LDS_BYTES<__bf16, D>];
@@ -1571,7 +1580,9 @@ __device__ __forceinline__ eight<A> row_of_token(const uint8_t *q, const uint8_t
 // A wave takes the heads of one token, four rows of up to 128 values at a time (eight of up
 // to 64), eight values a lane; cos and sin of a lane's four pairs are formed once for all of
 // them. So a token's rows are read and written once, and nothing crosses lanes but a row's
-// largest magnitude.
+// largest magnitude. Bound by memory: 18355 tokens of 20 + 5 heads of 128, bf16, turned, 235 MB in
+// 48.5 us, 4.85 TB/s; their f32 keys and values to int8 24 us, 5.0 TB/s; 4099 tokens of 40 heads of
+// 96, f16, 14.4 us. One token is its launch, 2.6 us (3.2 with the loads behind the angles).
 template <typename A>
 __device__ __forceinline__ void rows_body(const att_rows_args &a) {
     const uint32_t lane = threadIdx.x & 63u, w = blockIdx.x * (ATT_THREADS / 64) + uniform(threadIdx.x >> 6);
@@ -1672,7 +1683,9 @@ __device__ __forceinline__ void rows_body(const att_rows_args &a) {
 namespace {
 
 // A batch's positions out of their pages. A workgroup's pieces of eight values are of one page;
-// whose page it is, is searched for 64 sequences at a time.
+// whose page it is, is searched for 64 sequences at a time. Bound by memory: 19000 positions of
+// int8 to f32, 5 KV heads of 128, 25.5 us, 4.8 TB/s; 200 positions 3.9 us, which is the chain of loads from
+// the sequence to the codes.
 template <typename A>
 __device__ __forceinline__ void read_body(const att_read_args &a) {
     const uint32_t lane = threadIdx.x & 63u, entry = blockIdx.x;
@@ -1872,6 +1885,12 @@ template <typename T> struct beam_loads {
 // keys. Its waves take turns at 64 * BEAM_VALUES logits. Of their first ones they tell each other
 // what n_pick keys of the part are no smaller than, and from then on put down what is not below that
 // (128256 logits in four parts, 16 picks: about 100 of 32768), which is put in order at the end.
+//
+// 192 rows of 128256 bf16 logits, 49 MB, in 20.1 us, 2.5 TB/s; 15 without what is put down. Four rows of
+// f32 5.7 us, of which a launch and a load from memory are most. Slower on the way here, us for the
+// 192 rows: a list that all waves keep with barriers 64; a list a wave, ranked again for each tile 45;
+// kept in order a key at a time 33, by bounds told after each tile 30; single values put down
+// instead of a lane's eight 27; 8 or 16 parts a row in place of 4, 21.7 and 20.3 with a longer join.
 template <typename T> __device__ __forceinline__ void beam_body(const att_beam_args &a) {
     typedef beam_loads<T> loads;
     // tiles of a wave that are on their way, 4 KB, and then gone through together
@@ -2055,6 +2074,9 @@ BEAM(sllm_k_beam_f32, float)
 BEAM(sllm_k_beam_f16, _Float16)
 BEAM(sllm_k_beam_bf16, __bf16)
 
+// (4 beams of 63 parts 4.2 us, 32 groups of 8 beams of 4 parts 5.7: a launch, two loads that wait for each
+// other, a logarithm in 64 bits.)
+//
 // A group: a wave joins a beam's parts (a lane a part, whose keys are in order: the largest of each, then
 // the second, until none can be among the first), then its beams' lists are joined by their
 // values in 64 bits. A beam that ended, or has no finite sum, is its token, and tokens from 0 on
