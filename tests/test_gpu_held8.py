@@ -465,3 +465,84 @@ def test_offsets_past_32_bits(amd, dev):
     c.close()
     for x in [bq, bk, bv, bo] + bb:
         x.free()
+
+
+@pytest.mark.parametrize("dtype", h8.HELD + ["float16"])
+def test_a_cache_s_life(amd, dev, dtype):
+    """Random steps, forks, copies, reorders, truncations and moves: what every sequence then
+    reads back, against the rows that it was given."""
+    r = np.random.default_rng(77)
+    kv, d, page, pages, layers = 2, 48, 16, 90, 2
+    c = amd.PagedCache(dev, layers, kv, d, page, pages, dtype)
+    hold = (lambda x: x.half().float()) if dtype == "float16" else (lambda x: torch.from_numpy(h8.held(x.double().numpy(), dtype)).float())
+    rows = {c.new(): [torch.zeros(0, kv, d) for _ in range(2 * layers)] for _ in range(4)}
+
+    def check():
+        ids = list(rows)
+        b = c.batch(ids, [0] * len(ids), kv, "float32")
+        n = b.positions
+        assert n == sum(len(x[0]) for x in rows.values())
+        out = [dev.alloc(max(n, 1) * kv * d * 4) for _ in range(2)]
+        for layer in range(layers):
+            b.read(layer, out[0].ptr, out[1].ptr)
+            dev.sync()
+            for i in range(2):
+                want = torch.cat([rows[s][2 * layer + i] for s in ids])
+                got = torch.from_numpy(out[i].download(np.float32, n * kv * d)).view(n, kv, d)
+                assert torch.equal(got, want), (layer, i)
+        b.close()
+        for x in out:
+            x.free()
+
+    for step in range(120):
+        ids, op = list(rows), r.integers(0, 8)
+        room = pages - c.in_use()
+        if op <= 2:                                                          # a step
+            pick = [s for s in ids if r.random() < 0.7]
+            new = [int(r.integers(0, 20)) for _ in pick]
+            if sum(n // page + 2 for n in new) > room:
+                continue
+            b = c.batch(pick, new, kv, "float32")
+            for layer in range(layers):
+                x = [spread(1000 * step + 10 * layer + i, max(sum(new), 1), kv, d) / 64 for i in range(2)]
+                bufs = [dev.put(y.numpy()) for y in x]
+                b.store(layer, bufs[0].ptr, bufs[1].ptr)
+                dev.sync()
+                at = 0
+                for s, n in zip(pick, new):
+                    for i in range(2):
+                        rows[s][2 * layer + i] = torch.cat([rows[s][2 * layer + i], hold(x[i][at:at + n])])
+                    at += n
+                for y in bufs:
+                    y.free()
+            b.close()
+        elif op <= 4 and len(ids) > 1:                                       # beams
+            some = [ids[i] for i in r.permutation(len(ids))[:r.integers(1, len(ids) + 1)]]
+            if len(some) > room:
+                continue
+            parents = [int(r.integers(0, len(some))) for _ in some]
+            old = [rows[s] for s in some]
+            c.reorder(some, parents)
+            for s, p in zip(some, parents):
+                rows[s] = list(old[p])
+        elif op == 5 and len(ids) < 9:
+            s = ids[r.integers(0, len(ids))]
+            n = int(r.integers(0, len(rows[s][0]) + 1))
+            if room > 3:
+                for f in c.fork(s, n, 2):
+                    rows[f] = [x[:n] for x in rows[s]]
+        elif op == 6:
+            s = ids[r.integers(0, len(ids))]
+            n = int(r.integers(0, len(rows[s][0]) + 1))
+            c.truncate(s, n)
+            rows[s] = [x[:n] for x in rows[s]]
+            if len(ids) > 3:
+                c.free([ids[0]])
+                del rows[ids[0]]
+        else:
+            c.compact()
+            assert all((c.table(s) < c.in_use()).all() for s in rows)
+        if step % 6 == 5:
+            check()
+    check()
+    c.close()
