@@ -1987,14 +1987,18 @@ template <typename T> __device__ __forceinline__ void beam_body(const att_beam_a
             }
             sum += (double) s;
         }
-        if (t == first) {                                        // (all waves with tiles are here)
-            float most = top[0];
+        float most = top[0];
 #pragma unroll
-            for (uint32_t u = 1; u < AHEAD; ++u) most = fmaxf(most, top[u]);
+        for (uint32_t u = 1; u < AHEAD; ++u) most = fmaxf(most, top[u]);
+        if (t == first) {                                        // (all waves with tiles are here)
             const uint64_t nth = (uint32_t) __popcll(__ballot(most > -INFINITY)) > q ? nth_largest(most > -INFINITY ? key_of(most, 0) : 0, q + 1u) : 0;
             if (lane == 0) told[wave] = nth == 0 ? -INFINITY : value_of(nth);
             __syncthreads();
             least = fminf(fminf(told[0], told[1]), fminf(told[2], told[3]));
+        }
+        // where more lanes than picks have something, as when logits rise with the token, these bound the rest
+        if ((uint32_t) __popcll(__ballot(most >= least && most > -INFINITY)) > a.n_pick) {
+            least = fmaxf(least, value_of(nth_largest(most > -INFINITY ? key_of(most, 0) : 0, a.n_pick)));
         }
 #pragma unroll
         for (uint32_t u = 0; u < AHEAD; ++u) {
