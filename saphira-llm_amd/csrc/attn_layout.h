@@ -110,7 +110,7 @@ typedef struct att_rows_args {
     uint64_t        q_tok, k_tok, v_tok, qo_tok, ko_tok;     /* bytes */
     uint64_t        page_bytes;
     uint32_t        n_tok, n_head, n_head_kv, hd, half, pairs, back;     /* pairs: 2i, 2i + 1; else i, i + half */
-    uint32_t        held, page_shift, block_bytes, waves;    /* waves a row */
+    uint32_t        held, page_shift, block_bytes, waves;    /* waves a token */
     float           magnitude;
 } att_rows_args;
 
