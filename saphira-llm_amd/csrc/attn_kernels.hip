@@ -1916,7 +1916,7 @@ template <typename T> __device__ __forceinline__ void beam_body(const att_beam_a
     const uint32_t first = c * a.chunk + wave * TILE, last = min(c * a.chunk + a.chunk, end);
     loads ring[AHEAD];
 #pragma unroll
-    for (uint32_t u = 0; u < AHEAD; ++u) ring[u].load(r, first + u * STEP, odd);
+    for (uint32_t u = 0; u < AHEAD; ++u) if (first + u * STEP < last) ring[u].load(r, first + u * STEP, odd);
     const float last_x = loose ? (float) G_CAST(const T, from)[end - 1] : 0.0f;
     wave_best best(a.n_pick);
     uint32_t n = 0, n_kept = 0;                                  // keys in `found`, lanes whose values are in `kept`
