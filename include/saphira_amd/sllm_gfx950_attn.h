@@ -304,7 +304,7 @@ void sllm_gfx950_prompt_destroy(sllm_gfx950_prompt *p);
  * A plan serves any number of calls, one after the other or captured into graphs, which are
  * valid while it lives and share its memory: graphs of one plan are replayed one after the other.
  */
-#define SLLM_GFX950_BEAM_MAX 64
+#define SLLM_GFX950_BEAM_MAX 64      /* beams, picks */
 
 typedef struct sllm_gfx950_beam_desc {
     int32_t n_group, n_beam, n_vocab, n_pick, dtype;

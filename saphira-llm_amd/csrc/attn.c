@@ -1658,8 +1658,8 @@ int sllm_gfx950_beam_new(const sllm_gfx950_beam_desc *d, sllm_gfx950_beam **out)
     ATT_ON_DEVICE();
     if (out == NULL) return FAIL_ARG("beam_new: NULL out");
     *out = NULL;
-    if (d == NULL || bad_type(d->dtype) || d->n_group < 1 || d->n_beam < 1 || d->n_beam > (int32_t) BEAM_MAX_BEAM || d->n_vocab < 1 || d->n_vocab > 1 << 24 ||
-        d->n_pick < 1 || d->n_pick > (int32_t) BEAM_MAX_PICK || d->n_beam * d->n_pick > (int32_t) BEAM_MAX_LIST ||
+    if (d == NULL || bad_type(d->dtype) || d->n_group < 1 || d->n_beam < 1 || d->n_beam > SLLM_GFX950_BEAM_MAX || d->n_vocab < 1 || d->n_vocab > 1 << 24 ||
+        d->n_pick < 1 || d->n_pick > SLLM_GFX950_BEAM_MAX || d->n_beam * d->n_pick > (int32_t) BEAM_MAX_LIST ||
         (int64_t) d->n_pick > (int64_t) d->n_beam * d->n_vocab || (int64_t) d->n_group * d->n_beam > 1 << 20) {
         return FAIL_ARG("beam_new: type, groups, beams, vocabulary or picks outside what a plan takes");
     }

@@ -133,10 +133,8 @@ typedef struct att_read_args {
  * logits, `chunk` of them, and leaves its sum of exponentials and its best n_pick keys in order; the
  * second launch joins them, a group a workgroup.
  */
-#define BEAM_MAX_PICK  64u
-#define BEAM_MAX_BEAM  64u
 #define BEAM_MAX_LIST  2048u         /* n_beam * n_pick */
-#define BEAM_MAX_PARTS 64u           /* of a row: a lane each in the join */
+#define BEAM_MAX_PARTS 64u           /* of a row: a lane each in the join, as picks are in both */
 #define BEAM_JOIN_THREADS 512u
 #define BEAM_VALUES    8u            /* of a thread at a time */
 #define BEAM_TILE      (ATT_THREADS * BEAM_VALUES)
