@@ -153,7 +153,9 @@ int     sllm_gfx950_pages_compact(sllm_gfx950_pages *p, int32_t *n_moved);
  * act_dtype is the type of every row given or returned: the cache's, or f32
  * over an f16 cache (rounded to nearest by store; queries are not rounded), or
  * any of the three over 8 bits. Over 8 bits keys and values are what their codes
- * stand for, and queries and weights keep all their bits (f32), 16 (f16) or the 8 of bf16.
+ * stand for, queries keep all their bits, and weights 24 (f32) or 16 (f16, bf16); but the 8 of
+ * bf16 where more than 64 rows of bf16 see the same keys and there is work enough to go
+ * through them 128 at a time.
  *
  * A batch holds its pages until it is destroyed, whatever happens to its
  * sequences meanwhile; the next batch of a sequence that was truncated may

@@ -142,8 +142,14 @@ template <typename T, int D, bool KEYS> struct tile {
 // all for the same rows, and their results are joined in LDS; else each wave
 // has rows of its own and all share a tile. PAGED: keys are found by page. C: what a
 // cache of 8 bits holds, T what its values are turned into on their way to LDS or to the
-// products: bf16, which holds a code times its scale exactly. Queries and weights are then
-// sums of bf16 values, one for rows of bf16, two for f16 (16 bits), three for f32 (24).
+// products: bf16, which holds a code times its scale exactly. Queries are then sums of bf16
+// values, one for rows of bf16, two for f16 (all 11 bits), three for f32 (24), and weights
+// likewise; but of rows of bf16 with up to 64 a workgroup they are sums of two, 16 bits, which
+// leaves a result's own rounding (1.67e-3 of it on average; with 8 bits of a weight 2.0e-3 to 2.2e-3).
+// That costs nothing where memory bounds (8 sequences of up to 65536 positions 57.4 and
+// 57.5 us) and 4 to 7 % behind shared prefixes (64 sequences behind 4096 positions 24.6 and 25.7,
+// drafts of 5 27.0 and 28.8), but 22 % in 128 rows, which the products bound (4 times
+// 512 new positions 83.9 and 102.7 us): there weights have the 8 bits of the rows' type.
 template <typename A, typename T, int D, int NT, bool KEYS, bool PAGED, typename C = T>
 struct attention {
     typedef tile<T, D, KEYS> L;
@@ -151,7 +157,9 @@ struct attention {
     static constexpr bool HELD8 = !is_same<C, T>::value;
     static constexpr bool SPLIT = !HELD8 && !WIDE && sizeof(A) == 4;       // f32 rows against f16 keys
     static constexpr int PIECES = !HELD8 ? 1 : sizeof(A) == 4 ? 3 : is_f16<A>::value ? 2 : 1;
-    static constexpr int MORE = PIECES - 1 + SPLIT;              // values beside the first that a query or weight is the sum of
+    static constexpr int WEIGHT = HELD8 && PIECES == 1 && NT == 1 ? 2 : PIECES;
+    // values beside the first that a query, and that a weight is the sum of
+    static constexpr int MORE = PIECES - 1 + SPLIT, MOREW = WEIGHT - 1 + SPLIT;
     static constexpr int KT = L::KT;
     static constexpr int KS = KT / 16;                           // 16-key subtiles
     static constexpr int DT = D / 16;
@@ -268,13 +276,13 @@ struct attention {
         return min((int) it.key1, it.vis0 + (int) t);
     }
 
-    // x as a sum of PIECES bf16 values: cut off, so that none is over x where x is near f32's
+    // x as a sum of N (2, 3) bf16 values: cut off, so that none is over x where x is near f32's
     // end, and what is left rounded to the last
-    __device__ __forceinline__ static void pieces(float x, T (&p)[3]) {
+    template <int N> __device__ __forceinline__ static void pieces(float x, T (&p)[3]) {
         const float hi = __uint_as_float(__float_as_uint(x) & 0xffff0000u);
         p[0] = (T) hi;
         x -= hi;
-        if constexpr (PIECES > 2) {
+        if constexpr (N > 2) {
             const float mid = __uint_as_float(__float_as_uint(x) & 0xffff0000u);
             p[1] = (T) mid;
             p[2] = (T) (x - mid);
@@ -320,7 +328,7 @@ struct attention {
 #pragma unroll
                     for (int e = 0; e < 8; ++e) {
                         T p[3];
-                        pieces(x[e], p);
+                        pieces<PIECES>(x[e], p);
                         qf[nt][s][e] = p[0];
                         ql[nt][s][e] = p[1];
                         if constexpr (PIECES > 2) qm[nt][s][e] = p[2];
@@ -594,7 +602,7 @@ struct attention {
     // of p as it was rounded, so that weights still add up to 1: values that are all alike
     // come back as they are (they were 0.4 % off where bf16 rounded all weights one way).
     struct probs {
-        t8 p[WIDE ? 1 : NT], rest[MORE ? NT : 1], last[MORE > 1 ? NT : 1];
+        t8 p[WIDE ? 1 : NT], rest[MOREW ? NT : 1], last[MOREW > 1 ? NT : 1];
         f32x4 w[WIDE ? NT : 1];
     };
 
@@ -643,22 +651,22 @@ struct attention {
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
                     const float x = __builtin_amdgcn_exp2f(fmaf(s[ks][nt][i], c[nt], -m[nt]));
-                    if constexpr (WIDE || PIECES > 1) sum += x;
+                    if constexpr (WIDE || WEIGHT > 1) sum += x;
                     if constexpr (WIDE) {
                         p.w[nt][i] = x;
-                    } else if constexpr (PIECES > 1) {           // (16 or more bits of x: as good as x in the sum)
+                    } else if constexpr (WEIGHT > 1) {           // (16 or more bits of x: as good as x in the sum)
                         T y[3];
-                        pieces(x, y);
+                        pieces<WEIGHT>(x, y);
                         p.p[nt][4 * ks + i] = y[0];
                         p.rest[nt][4 * ks + i] = y[1];
-                        if constexpr (PIECES > 2) p.last[nt][4 * ks + i] = y[2];
+                        if constexpr (WEIGHT > 2) p.last[nt][4 * ks + i] = y[2];
                     } else {
                         p.p[nt][4 * ks + i] = (T) x;
                         if constexpr (SPLIT) p.rest[nt][4 * ks + i] = (T) (x - (float) p.p[nt][4 * ks + i]);
                     }
                 }
             }
-            if constexpr (!WIDE && PIECES == 1) {
+            if constexpr (!WIDE && WEIGHT == 1) {
 #pragma unroll
                 for (int e = 0; e < 8; e += 2) {
                     sum = add_two(p.p[nt][e], p.p[nt][e + 1], sum);
@@ -723,8 +731,8 @@ struct attention {
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt) {
                     o[dt][nt] = mfma(vf, p.p[nt], o[dt][nt]);
-                    if constexpr (MORE > 0) o[dt][nt] = mfma(vf, p.rest[nt], o[dt][nt]);
-                    if constexpr (MORE > 1) o[dt][nt] = mfma(vf, p.last[nt], o[dt][nt]);
+                    if constexpr (MOREW > 0) o[dt][nt] = mfma(vf, p.rest[nt], o[dt][nt]);
+                    if constexpr (MOREW > 1) o[dt][nt] = mfma(vf, p.last[nt], o[dt][nt]);
                 }
             }
         }
