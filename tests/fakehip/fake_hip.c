@@ -27,6 +27,9 @@
  *                                they wait, or free memory
  *   fakehip_launches()           kernels launched since the last fakehip_clear:
  *                                name:grid, a space behind each
+ *   fakehip_items(), fakehip_n_items()
+ *                                the work items (att_item) of the last launch of an
+ *                                attention kernel, valid while its batch or plan lives
  */
 #include <hip/hip_runtime_api.h>
 
@@ -34,6 +37,8 @@
 #include <stdio.h>
 #include <stdlib.h>
 #include <string.h>
+
+#include "attn_layout.h"
 
 #define FAKE_EXPORT __attribute__((visibility("default")))
 
@@ -48,6 +53,7 @@ static size_t   g_launches_len;
 static __thread int g_current;
 static int      g_capturing;
 static int      g_broken;
+static att_args g_attend;
 
 FAKE_EXPORT void fakehip_fail(const char *fn, int err, unsigned skip) {
     snprintf(g_fail_fn, sizeof g_fail_fn, "%s", fn);
@@ -63,6 +69,8 @@ FAKE_EXPORT void fakehip_current(int d) { g_current = d; }
 FAKE_EXPORT void fakehip_capture(int on) { g_capturing = on; }
 FAKE_EXPORT int  fakehip_broken(void) { return g_broken; }
 FAKE_EXPORT unsigned long fakehip_calls(void) { return g_calls; }
+FAKE_EXPORT const void *fakehip_items(void) { return g_attend.items; }
+FAKE_EXPORT uint32_t fakehip_n_items(void) { return g_attend.n_items; }
 
 static int inject(const char *fn) {
     ++g_calls;
@@ -208,6 +216,7 @@ hipError_t hipModuleLaunchKernel(hipFunction_t f, unsigned int gx, unsigned int 
     if (g_launches_len + strlen(name) + 13 <= sizeof g_launches) {
         g_launches_len += (size_t) snprintf(g_launches + g_launches_len, sizeof g_launches - g_launches_len, "%s:%u ", name, gx);
     }
+    if (strncmp(name, "sllm_k_attend_", 14) == 0) g_attend = *(const att_args *) args[0];
     if (strcmp(name, "sllm_k_host_done") == 0) {
         **(uint32_t **) args[0] = *(uint32_t *) args[1];
     } else if (strcmp(name, "sllm_k_quant_host") == 0) {
