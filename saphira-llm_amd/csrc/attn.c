@@ -802,13 +802,27 @@ static uint32_t seg_tiles(const segment *s, uint32_t group) {
 
 /*
  * 8 bits: where tiles of 128 rows have fewer keys than this a CU, they are made two of 64:
- * twice the workgroups, but each key is turned into bf16 twice as often. us, 128 rows / 64, bf16
- * rows over int8, 20 heads over 5 of 128: 64 sequences behind 4096 shared positions (160 keys a CU) 25.1 /
- * 24.5, 6000 (234) 29.4 / 28.4, 8000 (312) 32.5 / 32.7, 11000 (430) 35.0 / 40.1, 16000 43.4 / 50.7; 128
- * new positions behind 900 (70) 20.5 / 17.3, 4 times 512 behind 4000 88 / 112; drafts of 5 behind 1000, 32
- * heads over 8 (150) 30.2 / 26.6.
+ * twice the workgroups, but each key is turned into bf16 twice as often (and weights of bf16 rows are
+ * of 16 bits, not 8). us, 64 rows / 128, 64 sequences behind a shared prefix, 20 heads over 5, by keys a CU:
+ *
+ *                       160           195           234           273           312           371           430
+ *   bf16 128 int8   25.7 / 25.9   27.6 / 27.9   30.2 / 29.0   31.9 / 30.5   35.1 / 31.9   38.6 / 33.1   43.5 / 34.4
+ *   bf16 128 e4m3   24.0 / 25.2   25.5 / 27.1   27.7 / 28.2   29.2 / 29.4   31.6 / 30.3   34.8 / 31.5   39.1 / 32.8
+ *   f16  128 int8   27.0 / 29.6   28.8 / 32.6   31.7 / 34.5   33.3 / 36.5   36.9 / 38.3   40.6 / 40.6   45.6 / 42.9
+ *   f16  128 e4m3   25.4 / 28.2   27.0 / 31.2   29.6 / 32.8   30.6 / 34.4   33.5 / 36.6   36.9 / 38.2   41.3 / 40.2
+ *   bf16  64 int8   20.7 / 18.8   22.2 / 20.4   25.5 / 21.6   26.7 / 23.2   29.5 / 24.6   32.5 / 26.5   36.4 / 28.2
+ *   bf16  64 e4m3   18.7 / 17.5   19.9 / 19.4   22.3 / 20.3   23.5 / 21.7   25.6 / 22.7   27.9 / 24.2   31.0 / 25.7
+ *   f16   64 int8   21.3 / 20.8   22.8 / 22.5   26.1 / 24.0   27.5 / 25.9   30.5 / 27.4   33.4 / 29.7   37.5 / 31.8
+ *   f16   64 e4m3   20.1 / 19.8   21.4 / 21.4   24.1 / 22.7   25.4 / 24.2   27.9 / 25.5   30.4 / 27.4   34.0 / 29.3
+ *
+ * and of few keys, 128 new positions behind 900 (70 a CU) bf16 int8 18.1 / 20.6, 14.7 / 15.4 with heads of 64; drafts of 5
+ * behind 1000, 32 heads over 8 (150) 28.7 / 29.5 and 25.0 / 24.5, f16 30.3 / 36.7 and 25.8 / 27.3. int8 and e4m3 cross near
+ * enough to each other to have one border.
  */
-#define HELD8_HALF_KEYS 300u
+static uint32_t held8_half_keys(int32_t head_dim, int32_t act) {
+    if (head_dim <= 64) return act == SLLM_GFX950_F16 ? 170u : 130u;
+    return act == SLLM_GFX950_F16 ? 380u : 220u;
+}
 
 static uint32_t split_keys(const plan *x, uint32_t group, uint32_t n_head_kv, int many, uint32_t step) {
     uint64_t work = 0;
@@ -921,7 +935,7 @@ static int lay_out(sllm_gfx950_batch *b, plan *x, int32_t n, const int32_t *len0
         s->mode = mode_of(s->n_tok * group, p->d.dtype, b->act);
         if (s->mode == ATT_MANY) many += (uint64_t) seg_tiles(s, group) * (uint64_t) s->n_keys * kv;
     }
-    if (held8(p->d.dtype) && many < (uint64_t) sllm_shim_cu() * HELD8_HALF_KEYS) {
+    if (held8(p->d.dtype) && many < (uint64_t) sllm_shim_cu() * held8_half_keys(p->d.head_dim, b->act)) {
         for (int32_t i = 0; i < x->n_seg; ++i) if (x->seg[i].mode == ATT_MANY) x->seg[i].mode = ATT_HALF;
     }
     /* segments of each sequence, and those with one part alone */

@@ -7,7 +7,7 @@ MANY = {
     "four heads a KV head, the last tile's rows few": (64, 16, 128, 64, [1601], [101], 0),
     "a padded head": (60, 20, 80, 32, [1703], [97], 0),
     "a prompt from its start": (64, 16, 64, 32, [610, 30], [610, 30], 0),
-    "a shared prefix": (192, 12, 128, 64, [1 + 7 * (i % 5) for i in range(10)], [1] * 10, 4111),
+    "a shared prefix": (208, 13, 128, 64, [1 + 7 * (i % 5) for i in range(10)], [1] * 10, 4111),
     "a shared prefix, a narrow head": (192, 24, 64, 16, [5 + 11 * (i % 5) for i in range(14)], [1 + i % 2 for i in range(14)], 2500),
     "a group of three rows a token over a prefix": (72, 24, 96, 16, [200, 333, 90], [55, 60, 49], 1200),
 }
