@@ -350,6 +350,7 @@ static void copies_start(copies *c, const sllm_gfx950_pages *p) {
     c->a.row_bytes = p->row_bytes;
     c->a.n_blocks = (uint32_t) (p->page_bytes / p->block_bytes);
     c->a.scales = held8(p->d.dtype) ? (uint32_t) p->d.page_tokens * p->row_bytes : 0;
+    c->a.list = NULL;
     c->a.n_pairs = c->most = 0;
     c->st = SLLM_GFX950_OK;
 }
@@ -486,6 +487,37 @@ static int check_names(sllm_gfx950_pages *p, const int32_t *seqs, int32_t n, con
     return SLLM_GFX950_OK;
 }
 
+static int buffer_get(sllm_gfx950_pages *p, buffer *b, size_t dev_bytes, size_t pin_bytes);
+static void buffer_put(sllm_gfx950_pages *p, buffer *b);
+
+/* n copies in one launch, so that all are on their way or none: what a reorder writes may be
+ * pages that it takes back where it fails. (n under ATTN_MAX_SEQS, a grid's most in y.) */
+static int copies_at_once(sllm_gfx950_pages *p, const att_pair *pair, uint32_t n) {
+    copies c;
+    copies_start(&c, p);
+    if (n <= ATT_PAIRS) {
+        for (uint32_t i = 0; i < n; ++i) copies_add(&c, (int32_t) pair[i].src, (int32_t) pair[i].dst, (int32_t) pair[i].rows);
+        return copies_flush(&c);
+    }
+    buffer b;
+    int st = buffer_get(p, &b, n * sizeof *pair, n * sizeof *pair);
+    if (st != SLLM_GFX950_OK) return st;
+    memcpy(b.pin, pair, n * sizeof *pair);
+    hipError_t e = hipMemcpyAsync(b.dev, b.pin, n * sizeof *pair, hipMemcpyHostToDevice, sllm_shim_stream());
+    if (e == hipSuccess) e = hipEventRecord(b.sent, sllm_shim_stream());
+    if (e != hipSuccess) {
+        hipStreamSynchronize(sllm_shim_stream());
+        buffer_drop(&b);
+        return sllm_shim_hip_fail(e, "seq_reorder");
+    }
+    for (uint32_t i = 0; i < n; ++i) if (pair[i].rows > c.most) c.most = pair[i].rows;
+    c.a.list = (const att_pair *) b.dev;
+    c.a.n_pairs = n;
+    st = copies_flush(&c);
+    buffer_put(p, &b);
+    return st;
+}
+
 static void hold_page(sllm_gfx950_pages *p, int32_t page) {      /* (one that may be free) */
     if (p->refs[page]++ == 0 && p->holds[page] == 0) --p->n_free;
 }
@@ -509,6 +541,7 @@ int sllm_gfx950_seq_reorder(sllm_gfx950_pages *p, const int32_t *seqs, const int
         if (parent[i] < 0 || parent[i] >= n) return FAIL_ARG("seq_reorder: sequence %d of %d goes on from %d", i, n, parent[i]);
     }
     int32_t *work = malloc(((size_t) n * 3 + 1) * sizeof *work), *was = NULL;
+    att_pair *pairs = NULL;
     if (work == NULL) return FAIL_NOMEM("seq_reorder: %d sequences", n);
     int32_t *keeper = work, *len = work + n, *at = work + 2 * (size_t) n;
     pthread_mutex_lock(&p->mtx);
@@ -524,7 +557,9 @@ int sllm_gfx950_seq_reorder(sllm_gfx950_pages *p, const int32_t *seqs, const int
         for (int32_t i = n - 1; i >= 0; --i) if (keeper[parent[i]] != parent[i]) keeper[parent[i]] = i;     /* itself, or the first */
         for (int32_t i = 0; i < n; ++i) need += keeper[parent[i]] != i && (len[parent[i]] & (p->d.page_tokens - 1)) != 0;
         if (total > INT32_MAX) st = FAIL_ARG("seq_reorder: too many pages");
-        else if ((was = malloc((size_t) (total ? total : 1) * sizeof *was)) == NULL) st = FAIL_NOMEM("seq_reorder: %lld pages", (long long) total);
+        else if ((was = malloc((size_t) (total ? total : 1) * sizeof *was)) == NULL || (pairs = malloc((size_t) (need ? need : 1) * sizeof *pairs)) == NULL) {
+            st = FAIL_NOMEM("seq_reorder: %lld pages", (long long) total);
+        }
     }
     if (st == SLLM_GFX950_OK) {
         at[0] = 0;
@@ -545,8 +580,7 @@ int sllm_gfx950_seq_reorder(sllm_gfx950_pages *p, const int32_t *seqs, const int
         int32_t got = 0;
         if (need > p->n_free) st = FAIL_NOMEM("seq_reorder: %lld pages wanted, %d free", (long long) need, p->n_free);
         else {
-            copies c;
-            copies_start(&c, p);
+            uint32_t n_pairs = 0;
             for (; got < n; ++got) {
                 const int32_t q = parent[got], whole = len[q] >> p->page_shift, rows = len[q] & (p->d.page_tokens - 1);
                 sequence *s = &p->seq[seqs[got]];
@@ -556,10 +590,10 @@ int sllm_gfx950_seq_reorder(sllm_gfx950_pages *p, const int32_t *seqs, const int
                 if (s->n_pages > 0) memcpy(s->page, was + at[q], (size_t) s->n_pages * sizeof *was);
                 if (rows && keeper[q] != got) {
                     s->page[whole] = take_page(p);
-                    copies_add(&c, was[at[q] + whole], s->page[whole], rows);
+                    pairs[n_pairs++] = (att_pair) { (uint32_t) was[at[q] + whole], (uint32_t) s->page[whole], (uint32_t) rows };
                 }
             }
-            st = copies_flush(&c);
+            st = copies_at_once(p, pairs, n_pairs);
         }
         if (st != SLLM_GFX950_OK) {                      /* as it was */
             for (int32_t i = 0; i < got; ++i) {
@@ -580,6 +614,7 @@ int sllm_gfx950_seq_reorder(sllm_gfx950_pages *p, const int32_t *seqs, const int
     pthread_mutex_unlock(&p->mtx);
     free(work);
     free(was);
+    free(pairs);
     return st;
 }
 

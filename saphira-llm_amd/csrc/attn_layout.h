@@ -161,6 +161,7 @@ typedef struct att_copy_args {
     uint32_t  block_bytes, row_bytes, n_blocks, n_pairs;
     att_pair  pair[ATT_PAIRS];
     uint32_t  scales;                /* 8 bits: where a block's scale bytes start, of which rows are copied too */
+    const att_pair *list;            /* the pairs, where they are more than `pair` has room for */
 } att_copy_args;
 
 #define ATT_COPY_CHUNKS 1024u        /* 16-byte pieces a workgroup */

@@ -1,0 +1,48 @@
+"""Reorders of more sequences than one launch's arguments name copies for (sllm_gfx950_attn.h)
+on the GPU: what each then reads back."""
+import numpy as np
+import pytest
+import torch
+
+import held8_oracle as h8
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.mark.parametrize("dtype", ["float32", "int8"])
+@pytest.mark.parametrize("n", [320, 321, 322, 999])
+def test_many_sequences(amd, dev, dtype, n):
+    kv, d, page, layers = 2, 32, 16, 2
+    r = np.random.default_rng(n)
+    lens = [int(r.integers(1, 40)) for _ in range(n)]
+    pages = sum(-(-x // page) for x in lens)
+    c = amd.PagedCache(dev, layers, kv, d, page, 2 * pages + n, dtype)
+    ids = [c.new() for _ in range(n)]
+    b = c.batch(ids, lens, kv, "float32")
+    rows = [[torch.randn(sum(lens), kv, d) for _ in range(2)] for _ in range(layers)]
+    for layer in range(layers):
+        bufs = [dev.put(x.numpy()) for x in rows[layer]]
+        b.store(layer, bufs[0].ptr, bufs[1].ptr)
+        dev.sync()
+        for x in bufs:
+            x.free()
+    b.close()
+    hold = (lambda x: x) if dtype == "float32" else (lambda x: torch.from_numpy(h8.held(x.double().numpy(), dtype)).float())
+    held = [[torch.split(hold(x), lens) for x in layer] for layer in rows]
+    now = list(range(n))
+    for turn in range(3):
+        parent = [int(r.integers(0, n)) if turn < 2 else now.index(now[0]) for _ in range(n)]
+        c.reorder(ids, parent)
+        now = [now[p] for p in parent]
+        b = c.batch(ids, [0] * n, kv, "float32")
+        out = [dev.alloc(b.positions * kv * d * 4) for _ in range(2)]
+        for layer in range(layers):
+            b.read(layer, out[0].ptr, out[1].ptr)
+            dev.sync()
+            for i in range(2):
+                want = torch.cat([held[layer][i][s] for s in now])
+                assert torch.equal(torch.from_numpy(out[i].download(np.float32, want.numel())).view_as(want), want), (turn, layer, i)
+        b.close()
+        for x in out:
+            x.free()
+    c.close()
