@@ -1893,8 +1893,8 @@ template <typename T> struct beam_loads {
     }
 };
 
-// A part of a row of logits: the largest, the sum of exponentials relative to it, the best
-// keys. Its waves take turns at 64 * BEAM_VALUES logits. Of their first ones they tell each other
+// A part of a row of logits: a reference at most 1 below the largest, the sum of exponentials
+// relative to it, the best keys. Its waves take turns at 64 * BEAM_VALUES logits. Of their first ones they tell each other
 // what n_pick keys of the part are no smaller than, and from then on put down what is not below that
 // (128256 logits in four parts, 16 picks: about 100 of 32768), which is put in order at the end.
 //
@@ -1982,7 +1982,7 @@ template <typename T> __device__ __forceinline__ void beam_body(const att_beam_a
             }
 #pragma unroll
             for (uint32_t i = 0; i < BEAM_VALUES; ++i) top[u] = fmaxf(top[u], x[u][i]);  // (of NaN and a number, the number)
-            if (top[u] > m) {
+            if (top[u] > m + 1.0f) {                             // (else terms are at most e: rises that are small would add up their errors)
                 sum *= (double) exp_of(m - top[u]);
                 m = top[u];
             }

@@ -144,7 +144,7 @@ typedef struct att_beam_args {
     const int32_t *ended;            /* or NULL */
     float         *out;
     int32_t       *beam, *token;
-    double        *sums;             /* [row][chunk][2]: the largest logit, the sum of exponentials */
+    double        *sums;             /* [row][chunk][2]: a reference near the largest logit, the sum of exponentials relative to it */
     uint64_t      *keys;             /* [row][chunk][n_pick] */
     uint64_t       stride;           /* bytes */
     uint32_t       n_beam, n_vocab, n_pick, n_chunk, chunk, pad;
