@@ -209,9 +209,10 @@ int  sllm_gfx950_batch_attend(sllm_gfx950_batch *b, int32_t layer, const void *q
  *   PARTS   with turns = original * frequency / (2 pi): as it is from `fast` turns on,
  *           divided by factor below `slow`, and between them in proportion
  *
- * Angles are exact to 2^-30 of a turn at any position of 32 bits (of frequencies over a turn a
- * position to as many times that; over 2^20 radians they are refused); rows are computed in f32 and
- * rounded once.
+ * A position times a frequency is reduced to a part of a turn that is exact to 2^-30 of one at any
+ * position of 32 bits (of frequencies over a turn a position to as many times that; over 2^20
+ * radians they are refused). From there on f32: sine and cosine are off by at most 2^-22 beside
+ * that, and rows are rounded once.
  */
 enum { SLLM_GFX950_ROPE_HALVES, SLLM_GFX950_ROPE_PAIRS };
 enum { SLLM_GFX950_ROPE_PLAIN, SLLM_GFX950_ROPE_LINEAR, SLLM_GFX950_ROPE_NTK, SLLM_GFX950_ROPE_PARTS };

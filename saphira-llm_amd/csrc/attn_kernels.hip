@@ -1472,7 +1472,8 @@ namespace {
 
 // cos and sin of p / 2^32 turns: the quarter turn that p is nearest to, and the two series
 // on what is left, |x| <= pi / 4 (the first terms left out are x^13 / 13! and x^12 / 12!,
-// under 2^-32). p is exact to 2 of 2^-32 turns however far the position.
+// under 2^-32). p is exact to 2 of 2^-32 turns however far the position; what is left of it is
+// rounded to f32 (up to 2^-28 of a turn) and again by its product.
 __device__ __forceinline__ void cos_sin(uint32_t p, float &c, float &s) {
     const uint32_t quarter = (p + 0x20000000u) >> 30;
     const float x = (float) (int32_t) (p - (quarter << 30)) * 1.46291807926715968e-9f, x2 = x * x;      // 2 pi / 2^32
