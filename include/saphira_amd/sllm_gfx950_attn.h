@@ -121,7 +121,9 @@ int     sllm_gfx950_seq_truncate(sllm_gfx950_pages *p, int32_t seq, int32_t n_to
  * seqs[parent[i]] was (0 <= parent[i] < n), all at one time. Whole pages are shared; the
  * page that a sequence ends in is kept by itself, or else by the first that goes on from
  * it, and copied for each other, in pages that are free then. SLLM_GFX950_ERR_NOMEM where
- * these are too few, and nothing is changed.
+ * these are too few, and nothing is changed. It takes what has been stored so far: a store
+ * that comes later, through a batch made before, shows in whichever sequences hold its page then,
+ * the first that went on from it among them, and not in the copies.
  */
 int     sllm_gfx950_seq_reorder(sllm_gfx950_pages *p, const int32_t *seqs, const int32_t *parent, int32_t n);
 /* end n sequences: all of them, or none where one is unknown or named twice */

@@ -46,3 +46,41 @@ def test_many_sequences(amd, dev, dtype, n):
         for x in out:
             x.free()
     c.close()
+
+
+@pytest.mark.parametrize("dtype", ["float32", "int8"])
+@pytest.mark.parametrize("stays", [False, True])
+def test_a_store_through_a_batch_made_before(amd, dev, dtype, stays):
+    """It shows where its page went, whole pages to all and the last to one, and not in the
+    copies, which have what was stored when they were made."""
+    kv, d, page = 1, 32, 16
+    c = amd.PagedCache(dev, 1, kv, d, page, 40, dtype)
+    ids = [c.new() for _ in range(4)]
+    lens = [20, 3, 3, 3]
+    hold = (lambda x: x) if dtype == "float32" else (lambda x: torch.from_numpy(h8.held(x.double().numpy(), dtype)).float())
+
+    def store(b, x):
+        buf = dev.put(x.numpy())
+        b.store(0, buf.ptr, buf.ptr)
+        dev.sync()
+        buf.free()
+
+    first, second = torch.randn(sum(lens), kv, d), torch.randn(sum(lens), kv, d)
+    b = c.batch(ids, lens, kv, "float32")
+    store(b, first)
+    c.reorder(ids, [0, 0, 0, 0] if stays else [1, 0, 0, 0])      # goes on from sequence 0: itself and three, or three others
+    store(b, second)
+    b.close()
+    b = c.batch(ids, [0] * 4, kv, "float32")
+    out = [dev.alloc(b.positions * kv * d * 4) for _ in range(2)]
+    b.read(0, out[0].ptr, out[1].ptr)
+    dev.sync()
+    old, new = hold(first), hold(second)
+    kept = new[:20]
+    copied = torch.cat([new[:16], old[16:20]])
+    want = torch.cat([kept] + [copied] * 3) if stays else torch.cat([new[20:23], kept, copied, copied])
+    for x in out:
+        assert torch.equal(torch.from_numpy(x.download(np.float32, want.numel())).view_as(want), want)
+        x.free()
+    b.close()
+    c.close()
