@@ -237,7 +237,8 @@ void sllm_gfx950_rope_free(sllm_gfx950_rope *r);
 /*
  * Rows of q [n_rows][n_head][head_dim] and, or NULL, k [n_rows][n_head_kv][head_dim], row i
  * at position pos[i] (device memory; below 0 too), into q_out and k_out: where they come from
- * (same pointer and stride), or memory that overlaps nothing the call reads. Strides in
+ * (same pointer and stride), or memory that overlaps nothing the call reads (rows with different
+ * strides overlap where the memory from their first to their last does). Strides in
  * elements, multiples of 16 bytes, 0: packed. back: turned the other way, which is the
  * gradient of what the call did.
  */

@@ -1691,7 +1691,7 @@ struct sllm_gfx950_beam {
 /* A row's parts: as many as give every CU BEAM_GROUPS workgroups, of whole tiles, but no more than
  * the join has lanes. (us, 256 rows of 128256 at 2 / 4 / 8 / 16 of them: bf16, 16 picks 28.9 / 26.2 /
  * 30.5 / 30.8, 1 pick 24.5 / 23.2 / 26.6 / 27.2, 64 picks 59 / 56 / 52 / 45; f32 32.3 / 34.4 / 37.8 / 39.7;
- * 1024 rows of 32000 27.5 / 26.4 / 28.4 / 28.6.) */
+ * 1024 rows of 32000 27.5 / 26.4 / 28.4 / 28.6. One number for all: 64 picks of few rows would like more, f32 fewer.) */
 #define BEAM_GROUPS 4u
 
 static void beam_chunks(sllm_gfx950_beam *p) {

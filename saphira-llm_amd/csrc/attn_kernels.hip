@@ -1247,9 +1247,9 @@ __device__ __forceinline__ void paged_body(const att_args &a) {
 // there: for few rows right before the products, else once for a workgroup on the way to LDS. A
 // scale is a power of two, so nothing is rounded and no score or weight is multiplied by it. What
 // that costs the vector unit, 2.75 instructions a value of int8 and half of one of e4m3, memory hides
-// for few rows: 8 sequences of up to 65536 positions, e4m3 under bf16, 317 MB in 58.2 us with the join,
+// for few rows: 8 sequences of up to 65536 positions, e4m3 under bf16, 317 MB in 58.1 us with the join,
 // 5.4 TB/s (without the loads of scales it would be 56.4). Many rows are bound as over bf16: 64
-// sequences behind 4096 shared positions, int8, 23.5 us; one of 1101 positions, f32 rows, 9.2 us, two
+// sequences behind 4096 shared positions, int8, 24.8 us; one of 1101 positions, f32 rows, 9.3 us, two
 // launches. Two tiles of few rows on their way at a time: 57.9 us for 58.6, but 26.8 for 26.0 behind a shared
 // prefix. (Queries of f32 take three times the registers: no 32 rows a wave.)
 template <typename A, typename C, int D>
