@@ -96,3 +96,22 @@ def test_scores_a_step_apart(amd, dev, dtype):
 def test_many_beams_of_random_logits(amd, dev, dtype):
     check(amd, dev, normal(6, 8, 8, 32000) * 2.5, scores_of(7, 8, 8), 32, dtype)
     check(amd, dev, normal(8, 1, 4, 50001) / 64, scores_of(9, 1, 4), 16, dtype)
+
+
+@pytest.mark.parametrize("dtype", list(ora.TYPES))
+@pytest.mark.parametrize("groups,beams,vocab,picks", [(1 << 20, 1, 9, 3), (1 << 14, 64, 5, 32)])
+def test_as_many_rows_as_a_plan_takes(amd, dev, dtype, groups, beams, vocab, picks):
+    x = (normal(11, groups, beams, vocab) * 2).to(ora.TYPES[dtype])
+    scores = -torch.rand(groups, beams, generator=torch.Generator().manual_seed(12))
+    s = Select(amd, dev, x, scores.numpy(), None, picks, dtype)
+    s.run()
+    got, beam, token = (torch.from_numpy(y) for y in s.read())
+    s.close()
+    want = (scores.double()[..., None] + torch.log_softmax(x.double(), -1)).view(groups, -1)
+    mine = want.gather(1, beam.long() * vocab + token.long())
+    assert ((got.double() - mine).abs() <= 2.0 ** -17 + 2.0 ** -23 * (mine.abs() + 1)).all()
+    assert (got[:, 1:] <= got[:, :-1]).all()
+    best = want.topk(picks, 1).values                            # (in order, up to what logarithms are off by)
+    assert ((mine - best).abs() <= 2.0 ** -16).all()
+    at = (beam.long() * vocab + token.long()).sort(1).values
+    assert (at[:, 1:] != at[:, :-1]).all()

@@ -84,3 +84,28 @@ def test_a_store_through_a_batch_made_before(amd, dev, dtype, stays):
         x.free()
     b.close()
     c.close()
+
+
+def test_as_many_sequences_as_a_cache_holds(amd, dev):
+    """65536 beams that go on from one, in pages that the call frees."""
+    n, kv, d, page = 65536, 1, 16, 16
+    c = amd.PagedCache(dev, 1, kv, d, page, n, "int8")
+    ids = [c.new() for _ in range(n)]
+    b = c.batch(ids, [3] * n, kv, "float32")
+    rows = torch.randn(3 * n, kv, d)
+    buf = dev.put(rows.numpy())
+    b.store(0, buf.ptr, buf.ptr)
+    b.close()
+    c.reorder(ids, [77] * n)
+    assert c.in_use() == n
+    b = c.batch(ids, [0] * n, kv, "float32")
+    out = [dev.alloc(3 * n * kv * d * 4) for _ in range(2)]
+    b.read(0, out[0].ptr, out[1].ptr)
+    dev.sync()
+    want = torch.from_numpy(h8.held(rows[231:234].double().numpy(), "int8")).float().expand(n, 3, kv, d)
+    for x in out:
+        assert torch.equal(torch.from_numpy(x.download(np.float32, rows.numel())).view(n, 3, kv, d), want)
+        x.free()
+    b.close()
+    c.close()
+    buf.free()
