@@ -303,9 +303,10 @@ void sllm_gfx950_prompt_destroy(sllm_gfx950_prompt *p);
  * they are ordered by logit, between beams by that value, compared in 64 bits; what is alike by the
  * lower beam and the lower token. The sum's terms are of 32 bits: the logarithm is off by at most
  * 2^-24 (17.5 + 4.25 times how far a logit lies below the largest, on average by probability),
- * under 2^-17, and is the same bits for the same row wherever it lies; so beams nearer to
- * each other than that may come in either order. A NaN logit counts as -infinity. A beam whose score is not finite, or of
- * which a logit is +infinity or all are -infinity, has nothing but -infinity.
+ * under 2^-17, and is the same bits for the same row wherever in a plan's calls it lies; so beams
+ * nearer to each other than that may come in either order. A NaN logit counts as -infinity. A beam
+ * whose score is not finite, or of which a logit is +infinity or all are -infinity, has nothing
+ * but -infinity.
  *
  * At most 64 beams and 64 picks, n_beam * n_pick at most 2048 and n_pick at most n_beam * n_vocab;
  * n_vocab at most 2^24, n_group * n_beam at most 2^20. dtype is the logits' type.
